@@ -416,6 +416,38 @@ class StepSequenceAppend:
 
 
 @dataclasses.dataclass
+class StepSequenceRead:
+    """Logical steps start_index[b] .. + Ln of a cache as values (no counterpart in the reference): out [B, Ln, H, D] f32 or f16
+    from a cache of any dtype, contiguous, ring or paged. `lengths` i32 [B]: steps each request has (default: the cache's);
+    rows of other steps become zeros."""
+    out: int
+    cache: int
+    start_index: Optional[int] = None
+    lengths: Optional[int] = None
+    page_table: Optional[int] = None
+
+
+@dataclasses.dataclass
+class StepQKNormRopeAppend:
+    """RMSNorm of every query and key head, RoPE1D of both, append of K and V: q | k | v from one
+    [B, L, (h_q + 2 h_kv) * head_dim] matmul output (possibly a strided view), caches f16, q8_0 or q4_0, possibly rolling or
+    paged. q_gamma / k_gamma f32 [head_dim]; None: no norm."""
+    q_out: int
+    qkv: int
+    positions: int
+    end_index: int
+    k_cache: int
+    v_cache: int
+    base_frequency: float
+    q_gamma: Optional[int] = None
+    k_gamma: Optional[int] = None
+    eps: float = 1e-6
+    scale_factor: float = 1.0
+    rope_proportion: float = 1.0
+    page_table: Optional[int] = None
+
+
+@dataclasses.dataclass
 class StepGatherRows:
     """src/aion/runtime/executable.zig:155; q8_0 table dequantized on read."""
     out: int
@@ -492,6 +524,12 @@ class CudaSession:
             return {step.x}, {step.out}
         if isinstance(step, StepSequenceAppend):
             return {step.new_kv, step.end_index, step.cache} | img(step.page_table), {step.cache}
+        if isinstance(step, StepSequenceRead):
+            return {step.cache} | img(step.start_index) | img(step.lengths) | img(step.page_table), {step.out}
+        if isinstance(step, StepQKNormRopeAppend):
+            reads = {step.qkv, step.positions, step.end_index, step.k_cache, step.v_cache}
+            reads |= img(step.q_gamma) | img(step.k_gamma) | img(step.page_table)
+            return reads, {step.q_out, step.k_cache, step.v_cache}
         if isinstance(step, StepGatherRows):
             return {step.table, step.indices}, {step.out}
         if isinstance(step, StepArgMax):
@@ -610,6 +648,8 @@ class CudaSession:
             raise BackendError(capi.INVALID_ARGUMENT, "attention: q, k, v, out must be rank 4")
         if om.dtype != capi.DTYPE_F32:
             raise BackendError(capi.INVALID_ARGUMENT, "attention: out must be f32")
+        for m in (km, vm):
+            self._cache_axis(m, "attention")
         B, L, Hq, Dk = qm.shape
         _, T, Hkv, _ = km.shape
         Dv = vm.shape[3]
@@ -776,8 +816,9 @@ class CudaSession:
         cm, nm = st.meta(s.cache), st.meta(s.new_kv)
         im = self._need(s.end_index, capi.DTYPE_I32, "sequence_append.end_index")
         # src/aion/backend/cpu/exec/sequence_append.zig:25-37
-        if cm.rank != 4 or nm.rank != 4 or im.rank != 1 or cm.dtype != nm.dtype:
+        if cm.rank != 4 or nm.rank != 4 or im.rank != 1 or (cm.dtype != nm.dtype and cm.dtype not in BLOCK_BYTES):
             raise BackendError(capi.INVALID_ARGUMENT, "sequence_append: ranks / dtypes")
+        self._cache_axis(cm, "sequence_append")
         paged = s.page_table is not None
         if (not paged and cm.shape[0] != nm.shape[0]) or cm.shape[2] != nm.shape[2] or cm.shape[3] != nm.shape[3] or im.shape[0] != nm.shape[0]:
             raise BackendError(capi.INVALID_ARGUMENT, "sequence_append: shapes do not agree")
@@ -796,8 +837,78 @@ class CudaSession:
         rec = capi.SequenceAppend(cache=st.acquire_mut(s.cache).operand(), new_kv=st.acquire_const(s.new_kv).operand(),
                                   end_index=st.acquire_const(s.end_index).operand(), batch=B, t_cap=T, heads=H, head_dim=D,
                                   new_len=nm.shape[1], dtype=cm.dtype, rolling=1 if policy == "rolling" else 0,
-                                  page_table=table, page_tokens=page_tokens, pool_pages=pool_pages)
+                                  page_table=table, page_tokens=page_tokens, pool_pages=pool_pages, new_dtype=nm.dtype)
         _check(self._lib.aion_cuda_sequence_append(self.backend._h, C.byref(rec)))
+
+    @staticmethod
+    def _cache_axis(m: TensorMeta, what: str) -> None:
+        """A quantized cache [B, T, H, D] holds its blocks along D."""
+        if m.dtype in BLOCK_BYTES and m.quant_axis != m.rank - 1:
+            raise BackendError(capi.INVALID_ARGUMENT, f"{what}: a quantized cache is quantized along its last axis")
+
+    def _paging(self, cache: TensorMeta, table: Optional[int], batch: int, what: str) -> tuple:
+        """(requests, steps per request, {page_table, page_tokens, pool_pages}) of a cache, contiguous or paged."""
+        if table is None:
+            return cache.shape[0], cache.shape[1], {}
+        tm = self._need(table, capi.DTYPE_I32, f"{what}.page_table")
+        if tm.rank != 2 or tm.shape[0] != batch:
+            raise BackendError(capi.INVALID_ARGUMENT, f"{what}: page_table must be i32 [B, pages per request]")
+        return batch, tm.shape[1] * cache.shape[1], dict(page_table=self.store.acquire_const(table).operand(),
+                                                         page_tokens=cache.shape[1], pool_pages=cache.shape[0])
+
+    def _policy(self, tid: int, what: str) -> int:
+        policy = self.store.sequence_cache_policy_info(tid)
+        if policy == "growable":
+            raise BackendError(capi.UNSUPPORTED, f"{what}: growable caches are settled by the storage layer, not here")
+        return 1 if policy == "rolling" else 0
+
+    def _sequence_read(self, s: StepSequenceRead) -> None:
+        st = self.store
+        cm, om = st.meta(s.cache), st.meta(s.out)
+        if cm.rank != 4 or om.rank != 4 or tuple(cm.shape[2:]) != tuple(om.shape[2:]):
+            raise BackendError(capi.INVALID_ARGUMENT, "sequence_read: out [B, Ln, H, D], cache [B, T, H, D]")
+        self._cache_axis(cm, "sequence_read")
+        B, T, paging = self._paging(cm, s.page_table, om.shape[0], "sequence_read")
+        if B != om.shape[0]:
+            raise BackendError(capi.INVALID_ARGUMENT, "sequence_read: shapes do not agree")
+        ops = {}
+        for name, tid in (("start_index", s.start_index), ("lengths", s.lengths)):
+            if tid is not None:
+                if tuple(self._need(tid, capi.DTYPE_I32, f"sequence_read.{name}").shape) != (B,):
+                    raise BackendError(capi.INVALID_ARGUMENT, f"sequence_read: {name} must be i32 [B]")
+                ops[name] = st.acquire_const(tid).operand()
+        rec = capi.SequenceRead(out=st.acquire_mut(s.out).operand(), cache=st.acquire_const(s.cache).operand(), batch=B, t_cap=T,
+                                heads=cm.shape[2], head_dim=cm.shape[3], out_len=om.shape[1], dtype=cm.dtype, out_dtype=om.dtype,
+                                rolling=self._policy(s.cache, "sequence_read"), **ops, **paging)
+        _check(self._lib.aion_cuda_sequence_read(self.backend._h, C.byref(rec)))
+
+    def _qk_norm_rope_append(self, s: StepQKNormRopeAppend) -> None:
+        st, what = self.store, "qk_norm_rope_append"
+        qm, xm = self._need(s.q_out, capi.DTYPE_F32, f"{what}.q_out"), self._need(s.qkv, capi.DTYPE_F32, f"{what}.qkv")
+        pm, im = self._need(s.positions, capi.DTYPE_I32, f"{what}.positions"), self._need(s.end_index, capi.DTYPE_I32, f"{what}.end_index")
+        km, vm = st.meta(s.k_cache), st.meta(s.v_cache)
+        if qm.rank != 4 or km.rank != 4 or tuple(km.shape) != tuple(vm.shape) or tuple(pm.shape) != tuple(qm.shape[:2]):
+            raise BackendError(capi.INVALID_ARGUMENT, f"{what}: q_out [B, L, Hq, D], caches [B, T, Hkv, D], positions [B, L]")
+        for m in (km, vm):
+            self._cache_axis(m, what)
+        B, L, Hq, D = qm.shape
+        Hkv = km.shape[2]
+        Bc, T, paging = self._paging(km, s.page_table, B, what)
+        if Bc != B or km.shape[3] != D or tuple(im.shape) != (B,) or xm.shape[-1] != (Hq + 2 * Hkv) * D or int(np.prod(xm.shape[:-1])) != B * L:
+            raise BackendError(capi.INVALID_ARGUMENT, f"{what}: qkv must hold q | k | v per (b, l), end_index one step per request")
+        ops = {}
+        for name, tid in (("q_gamma", s.q_gamma), ("k_gamma", s.k_gamma)):
+            if tid is not None:
+                if tuple(self._need(tid, capi.DTYPE_F32, f"{what}.{name}").shape) != (D,):
+                    raise BackendError(capi.INVALID_ARGUMENT, f"{what}: {name} must be f32 [head_dim]")
+                ops[name] = st.acquire_const(tid).operand()
+        op = lambda t: st.acquire_const(t).operand()
+        rec = capi.QKNormRopeAppend(q_out=op(s.q_out), qkv=op(s.qkv), positions=op(s.positions), end_index=op(s.end_index),
+                                    k_cache=op(s.k_cache), v_cache=op(s.v_cache), batch=B, len=L, h_q=Hq, h_kv=Hkv, head_dim=D,
+                                    ld_qkv=xm.row_stride, t_cap=T, eps=s.eps, base_frequency=s.base_frequency,
+                                    scale_factor=s.scale_factor, proportion=s.rope_proportion, k_dtype=km.dtype, v_dtype=vm.dtype,
+                                    rolling=self._policy(s.k_cache, what), **ops, **paging)
+        _check(self._lib.aion_cuda_qk_norm_rope_append(self.backend._h, C.byref(rec)))
 
     def _gather_rows(self, s: StepGatherRows) -> None:
         st = self.store
@@ -829,7 +940,8 @@ class CudaSession:
 
     _GLUE = {StepRMSNormPair: "_rms_norm_pair", StepRopeKVAppend: "_rope_kv_append",
              StepRMSNorm: "_rms_norm", StepElemwiseBinary: "_elemwise", StepRoPE1D: "_rope", StepCast: "_cast",
-             StepSequenceAppend: "_sequence_append", StepGatherRows: "_gather_rows", StepArgMax: "_argmax"}
+             StepSequenceAppend: "_sequence_append", StepSequenceRead: "_sequence_read",
+             StepQKNormRopeAppend: "_qk_norm_rope_append", StepGatherRows: "_gather_rows", StepArgMax: "_argmax"}
 
 
 class RecordedProgram:

@@ -135,6 +135,24 @@ class SequenceAppend(C.Structure):
     _fields_ = [("cache", Operand), ("new_kv", Operand), ("end_index", Operand),
                 ("batch", C.c_uint64), ("t_cap", C.c_uint64), ("heads", C.c_uint64), ("head_dim", C.c_uint64),
                 ("new_len", C.c_uint64), ("dtype", C.c_uint32), ("rolling", C.c_uint32),
+                ("page_table", Operand), ("page_tokens", C.c_uint64), ("pool_pages", C.c_uint64),
+                ("new_dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class SequenceRead(C.Structure):
+    _fields_ = [("out", Operand), ("cache", Operand), ("start_index", Operand), ("lengths", Operand),
+                ("batch", C.c_uint64), ("t_cap", C.c_uint64), ("heads", C.c_uint64), ("head_dim", C.c_uint64),
+                ("out_len", C.c_uint64), ("dtype", C.c_uint32), ("out_dtype", C.c_uint32), ("rolling", C.c_uint32),
+                ("reserved", C.c_uint32), ("page_table", Operand), ("page_tokens", C.c_uint64), ("pool_pages", C.c_uint64)]
+
+
+class QKNormRopeAppend(C.Structure):
+    _fields_ = [("q_out", Operand), ("qkv", Operand), ("q_gamma", Operand), ("k_gamma", Operand), ("positions", Operand),
+                ("end_index", Operand), ("k_cache", Operand), ("v_cache", Operand),
+                ("batch", C.c_uint64), ("len", C.c_uint64), ("h_q", C.c_uint64), ("h_kv", C.c_uint64),
+                ("head_dim", C.c_uint64), ("ld_qkv", C.c_uint64), ("t_cap", C.c_uint64),
+                ("eps", C.c_float), ("base_frequency", C.c_float), ("scale_factor", C.c_float), ("proportion", C.c_float),
+                ("k_dtype", C.c_uint32), ("v_dtype", C.c_uint32), ("rolling", C.c_uint32), ("reserved", C.c_uint32),
                 ("page_table", Operand), ("page_tokens", C.c_uint64), ("pool_pages", C.c_uint64)]
 
 
@@ -189,6 +207,8 @@ SIGNATURES = {
     "aion_cuda_rope": (C.c_int32, [_DEV, C.POINTER(RoPE)]),
     "aion_cuda_cast": (C.c_int32, [_DEV, C.POINTER(Cast)]),
     "aion_cuda_sequence_append": (C.c_int32, [_DEV, C.POINTER(SequenceAppend)]),
+    "aion_cuda_sequence_read": (C.c_int32, [_DEV, C.POINTER(SequenceRead)]),
+    "aion_cuda_qk_norm_rope_append": (C.c_int32, [_DEV, C.POINTER(QKNormRopeAppend)]),
     "aion_cuda_gather_rows": (C.c_int32, [_DEV, C.POINTER(GatherRows)]),
     "aion_cuda_argmax": (C.c_int32, [_DEV, C.POINTER(ArgMax)]),
     "aion_cuda_rms_norm_pair": (C.c_int32, [_DEV, C.POINTER(RMSNormPair)]),

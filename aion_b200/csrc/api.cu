@@ -325,8 +325,11 @@ int32_t aion_cuda_attention(AionCudaDevice* dev, const AionCudaAttention* s) {
   // src/aion/backend/cpu/exec/attention.zig:1452-1500.
   if (!(s->scale > 0.0f) || !std::isfinite(s->scale)) return fail(AION_CUDA_INVALID_ARGUMENT, "attention: scale must be finite and positive");
   if (!std::isfinite(s->soft_cap) || s->soft_cap < 0.0f) return fail(AION_CUDA_INVALID_ARGUMENT, "attention: soft cap must be finite and >= 0");
-  for (uint32_t dt : {s->q_dtype, s->k_dtype, s->v_dtype})
-    if (dt != AION_CUDA_DTYPE_F16 && dt != AION_CUDA_DTYPE_F32) return fail(AION_CUDA_INVALID_ARGUMENT, "attention: q/k/v dtype %u", dt);
+  for (uint32_t dt : {s->q_dtype, s->k_dtype, s->v_dtype}) {
+    const bool block = dt == AION_CUDA_DTYPE_Q8_0 || dt == AION_CUDA_DTYPE_Q4_0;   // K / V of a quantized cache
+    if (dt != AION_CUDA_DTYPE_F16 && dt != AION_CUDA_DTYPE_F32 && !block) return fail(AION_CUDA_INVALID_ARGUMENT, "attention: q/k/v dtype %u", dt);
+  }
+  if (s->q_dtype != AION_CUDA_DTYPE_F16 && s->q_dtype != AION_CUDA_DTYPE_F32) return fail(AION_CUDA_INVALID_ARGUMENT, "attention: q dtype %u", s->q_dtype);
   if (s->h_kv == 0 || s->h_q == 0 || s->h_q % s->h_kv != 0)
     return fail(AION_CUDA_INVALID_ARGUMENT, "attention: %llu query heads over %llu kv heads", (unsigned long long)s->h_q,
                 (unsigned long long)s->h_kv);

@@ -29,9 +29,7 @@
 #include <cmath>
 #include <mutex>
 
-#include "act_image.cuh"
-#include "common.cuh"
-#include "ptx.cuh"
+#include "attention_device.cuh"
 
 namespace aion {
 
@@ -40,73 +38,6 @@ namespace {
 constexpr int KT = 64;              // keys per stage
 constexpr int CONSUMER_WARPS = 4;   // 16 keys each
 constexpr int THREADS = (CONSUMER_WARPS + 1) * 32;
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct AttnParams {
-  const void* q;
-  const void* k;
-  const void* v;
-  float* out;
-  const int32_t* positions;
-  const int32_t* lengths;
-  uint32_t B, L, Hq, Hkv, Dk, Dv, T;
-  uint32_t q_dtype, k_dtype, v_dtype;
-  uint32_t rolling;
-  uint32_t win_left, win_right, win_chunk;
-  float scale, soft_cap;
-  uint32_t splits;
-  uint32_t head_groups;  // ceil((Hq/Hkv) / 8)
-  uint32_t col_heads;    // query heads of a head group: min(Hq/Hkv, 8)
-  uint32_t pos_per_tile; // query positions sharing one 8-column MMA tile
-  uint32_t l_blocks;     // blocks of positions per request
-  const int32_t* page_table;  // [B][pages_per_request] page numbers, or null: K / V are [B, T, ...]
-  uint32_t page_tokens, pages_per_request, pool_pages;
-  float* partial;        // [unit][split][columns][Dv + 4]: sums, max, sum of weights, pad
-  int* tickets;          // [unit]
-  int* fault;
-  // Optional: the quantized image of `out` as [B*L, Hq*Dv] rows (act_image.cuh), for the matmul
-  // that consumes the attention output.
-  uint8_t* image;
-  ActImageLayout image_layout;
-  uint32_t image_dtype;
-  uint32_t wait_limit;   // polls a barrier wait makes before it gives up and reports FAULT_WAIT_EXPIRED
-  uint32_t drop_first;   // test hook: every CTA leaves out the copies of its first stage, so that wait runs out
-};
-
-struct KeyRange {
-  uint32_t lo, hi;
-  bool bad;
-};
-
-// Window and ring clipping of one query row; flags inputs the reference rejects.
-__device__ __forceinline__ KeyRange key_range(const AttnParams& p, uint32_t b, uint32_t l) {
-  KeyRange r{0, 0, false};
-  int64_t valid_end = p.T;
-  if (p.lengths) {
-    const int32_t e = p.lengths[b];
-    if (e < 0) { r.bad = true; return r; }
-    valid_end = e;
-  }
-  if (!p.rolling && valid_end > (int64_t)p.T) { r.bad = true; return r; }
-  int64_t q_pos = l;
-  if (p.positions) {
-    const int32_t qp = p.positions[(uint64_t)b * p.L + l];
-    if (qp < 0) { r.bad = true; return r; }
-    q_pos = qp;
-  }
-  const int64_t anchor = p.win_chunk > 0 ? (q_pos / p.win_chunk) * p.win_chunk : q_pos;
-  const int64_t span = p.win_chunk > 0 ? p.win_chunk : 1;
-  int64_t lo = anchor - min(anchor, (int64_t)p.win_left);
-  int64_t hi = min(valid_end, anchor + span + (int64_t)p.win_right);
-  if (p.rolling && valid_end > (int64_t)p.T) lo = max(lo, valid_end - (int64_t)p.T);
-  if (hi > lo) {
-    r.lo = (uint32_t)lo;
-    r.hi = (uint32_t)hi;
-  }
-  return r;
-}
-
-__device__ __forceinline__ float soft_cap_logit(float x, float cap) { return cap > 0.0f ? cap * tanhf(x / cap) : x; }
 
 // ------------------------------------------------------------------------------------
 // tensor-core decode kernel
@@ -121,23 +52,11 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, u
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
                : "r"(addr));
 }
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // Two shared-memory layouts of a K / V tile of KT rows:
 //  * tiled (the usual case): the tile arrives as D/64 TMA boxes of 64 columns x KT rows with
 //    the 128-byte swizzle, so 16-byte chunk c of row r sits in column block c/8 at
@@ -187,29 +106,6 @@ struct DecodeGeom {
 };
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(CONSUMER_WARPS * 32) : "memory"); }
-
-constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
-
-// The last step of one float4 of an output column: o / lsum (zeros for a column without keys), the store, and
-// the quantized image of the output. All 32 lanes of a warp call it together (a column that does not exist
-// passes on = false). Callers run it in a loop that is NOT unrolled: this code runs once per CTA, at the very
-// end, on the CTA every other one is waiting for, and run once it costs what fetching its instructions costs
-// (four columns spelled out side by side took 4 to 5 us, most of it in the quantizer).
-template <int D>
-__device__ __forceinline__ void finish_column(const AttnParams& p, float4 o, float lsum, bool on, bool has_keys, uint32_t col, uint32_t d4,
-                                              const uint32_t* col_row, const uint32_t* col_orow, const uint32_t* col_head, bool report) {
-  const bool good = lsum > 0.0f && isfinite(lsum);
-  const float inv = good ? __frcp_rn(lsum) : 0.0f;
-  float4 r = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-  if (!good) r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (!good && on && has_keys && report) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
-  if (on) *reinterpret_cast<float4*>(p.out + (uint64_t)col_row[col] * D + 4 * d4) = r;
-  if (p.image) {
-    const uint32_t irow = on ? col_orow[col] : 0, kb = on ? (col_head[col] * (D / 4) + d4) >> 3 : 0;
-    if (p.image_dtype == AION_CUDA_DTYPE_Q8_0) quantize_store_block_8lanes<AION_CUDA_DTYPE_Q8_0>(r, d4 & 7, on, p.image, p.image_layout, irow, kb);
-    else quantize_store_block_8lanes<AION_CUDA_DTYPE_Q4_0>(r, d4 & 7, on, p.image, p.image_layout, irow, kb);
-  }
-}
 
 template <int D, bool QF32, bool TILED, bool BLOCK, int NT>
 __global__ void __launch_bounds__(THREADS, 1) attn_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmap_k,
@@ -849,11 +745,19 @@ int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
   if (B > 0x7FFFFFFF || L > 0x7FFFFFFF || Hq > 65535 || Dk > 65535 || Dv > 65535 || T > 0x7FFFFFFF || B * L * Hq > 0x7FFFFFFF)
     return fail(AION_CUDA_UNSUPPORTED, "attention: a dimension is beyond what the kernels index");
   auto esz = [](uint32_t dt) { return dt == AION_CUDA_DTYPE_F32 ? 4u : 2u; };
+  auto is_quant = [](uint32_t dt) { return dt == AION_CUDA_DTYPE_Q8_0 || dt == AION_CUDA_DTYPE_Q4_0; };
+  // Bytes of `values` values of K or V (whole blocks where they are quantized).
+  auto kv_bytes = [&](uint32_t dt, uint64_t values) { return is_quant(dt) ? values / QK * block_bytes_of(dt) : values * esz(dt); };
+  const bool quant = is_quant(s->k_dtype);
+  if (quant != is_quant(s->v_dtype)) return fail(AION_CUDA_UNSUPPORTED, "attention: K and V are both quantized, or neither");
+  if (quant && (Dk % QK || Dv % QK)) return fail(AION_CUDA_UNSUPPORTED, "attention: quantized K / V need heads of whole 32-blocks, got %llu and %llu", (unsigned long long)Dk, (unsigned long long)Dv);
   const bool paged = s->page_table.handle != 0;
   const uint64_t page_tokens = s->page_tokens, pool_pages = s->pool_pages;
   uint64_t pages_per_request = 0;
   if (paged) {
-    if (page_tokens == 0 || page_tokens % KT != 0 || page_tokens > (1u << 20))
+    if (quant && (page_tokens == 0 || page_tokens > (1u << 20)))
+      return fail(AION_CUDA_INVALID_ARGUMENT, "attention: page_tokens %llu", (unsigned long long)page_tokens);
+    if (!quant && (page_tokens == 0 || page_tokens % KT != 0 || page_tokens > (1u << 20)))
       return fail(AION_CUDA_INVALID_ARGUMENT, "attention: page_tokens %llu must be a positive multiple of %d", (unsigned long long)page_tokens, KT);
     if (pool_pages == 0 || pool_pages * page_tokens > 0x7FFFFFFFull)
       return fail(AION_CUDA_INVALID_ARGUMENT, "attention: pool of %llu pages", (unsigned long long)pool_pages);
@@ -864,8 +768,10 @@ int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
   const uint8_t *q, *k, *v;
   float* out;
   if (int32_t st = resolve(s->q, B * L * Hq * Dk * esz(s->q_dtype), "attention.q", &q)) return st;
-  if (int32_t st = resolve(s->k, kv_rows * Hkv * Dk * esz(s->k_dtype), "attention.k", &k)) return st;
-  if (int32_t st = resolve(s->v, kv_rows * Hkv * Dv * esz(s->v_dtype), "attention.v", &v)) return st;
+  if (quant && (kv_rows > (1ull << 40) || Hkv * (Dk + Dv) > (1ull << 20)))
+    return fail(AION_CUDA_UNSUPPORTED, "attention: a dimension is beyond what the kernels index");
+  if (int32_t st = resolve(s->k, kv_bytes(s->k_dtype, kv_rows * Hkv * Dk), "attention.k", &k)) return st;
+  if (int32_t st = resolve(s->v, kv_bytes(s->v_dtype, kv_rows * Hkv * Dv), "attention.v", &v)) return st;
   if (int32_t st = resolve(s->out, B * L * Hq * Dv * sizeof(float), "attention.out", &out)) return st;
   p.q = q;
   p.k = k;
@@ -897,11 +803,14 @@ int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
   const bool f16kv = s->k_dtype == AION_CUDA_DTYPE_F16 && s->v_dtype == AION_CUDA_DTYPE_F16;
   const bool aligned = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
                        (reinterpret_cast<uintptr_t>(q) & 3) == 0;
+  if (quant && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 1 || reinterpret_cast<uintptr_t>(out) & 3 ||
+                reinterpret_cast<uintptr_t>(q) & (esz(s->q_dtype) - 1)))
+    return fail(AION_CUDA_INVALID_ARGUMENT, "attention: misaligned operand");
   const bool tensor_path = f16kv && aligned && Dk == Dv && (Dk == 64 || Dk == 128 || Dk == 256) && !(s->flags & AION_CUDA_ATTENTION_GENERIC);
-  if (paged && !tensor_path)
+  if (paged && !tensor_path && !quant)
     return fail(AION_CUDA_UNSUPPORTED, "attention: the page table is read by the f16 tensor-core kernel only (Dk = Dv in {64, 128, 256}, aligned operands)");
   if (s->image.handle) {
-    if (!tensor_path) return fail(AION_CUDA_UNSUPPORTED, "attention: the output image is written by the f16 tensor-core kernel only (Dk = Dv in {64, 128, 256}, aligned operands)");
+    if (!tensor_path && !quant) return fail(AION_CUDA_UNSUPPORTED, "attention: the output image is written by the f16 tensor-core kernel only (Dk = Dv in {64, 128, 256}, aligned operands)");
     if (s->image_dtype != AION_CUDA_DTYPE_Q8_0 && s->image_dtype != AION_CUDA_DTYPE_Q4_0)
       return fail(AION_CUDA_INVALID_ARGUMENT, "attention: image dtype %u", s->image_dtype);
     p.image_layout = act_image_layout(B * L, Hq * Dv / QK);
@@ -909,6 +818,7 @@ int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
     if (reinterpret_cast<uintptr_t>(p.image) & 15) return fail(AION_CUDA_INVALID_ARGUMENT, "attention.image: the image must be 16-byte aligned");
     p.image_dtype = s->image_dtype;
   }
+  if (quant) return attention_qcache_launch(dev, p);
   if (tensor_path) {
     const uint32_t group = p.Hq / p.Hkv;
     p.head_groups = (group + 7) / 8;

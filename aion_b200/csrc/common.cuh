@@ -246,6 +246,7 @@ struct GemmPlan {
   bool pair;   // pairs of CTAs (two-SM MMAs); tile_rows is then the pair's
 };
 bool gemm_tcgen05_plan(const AionCudaDevice* dev, const MatMulArgs& g, GemmPlan* out);
+int32_t append_quantized(AionCudaDevice* dev, const AionCudaSequenceAppend* s);
 int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s);
 int32_t peer_wait_launch(AionCudaDevice* dev, const uint32_t* flags, uint32_t* state, uint32_t world, uint32_t poll_limit);
 

@@ -769,6 +769,7 @@ int32_t aion_cuda_cast(AionCudaDevice* dev, const AionCudaCast* s) {
 
 int32_t aion_cuda_sequence_append(AionCudaDevice* dev, const AionCudaSequenceAppend* s) {
   if (!dev || !s) return fail(AION_CUDA_INVALID_ARGUMENT, "sequence_append: null argument");
+  if (s->dtype == AION_CUDA_DTYPE_Q8_0 || s->dtype == AION_CUDA_DTYPE_Q4_0) return append_quantized(dev, s);
   if (s->dtype != AION_CUDA_DTYPE_F16 && s->dtype != AION_CUDA_DTYPE_F32)
     return fail(AION_CUDA_INVALID_ARGUMENT, "sequence_append: cache dtype %u", s->dtype);
   if (s->batch == 0 || s->new_len == 0 || s->heads == 0 || s->head_dim == 0) return AION_CUDA_OK;

@@ -331,6 +331,12 @@ typedef struct AionCudaAttention {
   AionCudaOperand page_table;
   uint64_t pool_pages;
 } AionCudaAttention;
+/* Quantized K / V: k_dtype and v_dtype may be AION_CUDA_DTYPE_Q8_0 or AION_CUDA_DTYPE_Q4_0, each of
+ * its own (both quantized, or neither): the caches that aion_cuda_sequence_append and
+ * aion_cuda_qk_norm_rope_append write. Everything above holds for them (a page table may then have
+ * any positive page_tokens). Keys and values are used as code x scale, logits and sums are f32: the
+ * result is that of f32 attention over the dequantized cache. A page number outside the pool is
+ * reported like a bad length, and its keys are left out. */
 
 AION_CUDA_API int32_t aion_cuda_attention(AionCudaDevice* dev, const AionCudaAttention* step);
 
@@ -415,8 +421,39 @@ typedef struct AionCudaSequenceAppend {
    * outside the pool is reported like a bad index. */
   AionCudaOperand page_table;
   uint64_t page_tokens, pool_pages;
+  uint32_t new_dtype; /* quantized caches only: AION_CUDA_DTYPE_F32 | AION_CUDA_DTYPE_F16 of new_kv */
+  uint32_t reserved;
 } AionCudaSequenceAppend;
 AION_CUDA_API int32_t aion_cuda_sequence_append(AionCudaDevice* dev, const AionCudaSequenceAppend* step);
+
+/* Quantized caches. No counterpart in the reference, whose caches are f16 or f32. A cache of dtype
+ * AION_CUDA_DTYPE_Q8_0 or AION_CUDA_DTYPE_Q4_0 is [B, T, H, D] (a ring, or a pool of pages, alike)
+ * whose head rows are D / 32 consecutive blocks: a q8_0 cache takes 53 % of an f16 one's bytes, a
+ * q4_0 cache 28 %. D % 32 == 0, the cache 2-byte aligned.
+ *  - aion_cuda_sequence_append with such a dtype quantizes new_kv [B, Ln, H, D] (new_dtype) as it
+ *    is written: the blocks are those that aion_cuda_quantize makes of the rows. page_tokens may be
+ *    any positive number. An f16 or f32 cache ignores new_dtype: its rows have the cache's type.
+ *    Of more new rows than a ring holds, the last T stay.
+ *  - aion_cuda_sequence_read gives logical steps back as values:
+ *      out [B, out_len, H, D] (out_dtype f32 or f16), row t of request b = step start_index[b] + t.
+ *    lengths i32 [B] says how many logical steps each request has (absent: t_cap): steps
+ *    [0, lengths[b]) are read, of a ring the last t_cap of them; every other row of out becomes
+ *    zeros. start_index absent: 0. Caches of dtype f32, f16, q8_0 and q4_0; the values are
+ *    code x scale, exact in f32 (aion_cuda_dequantize) and rounded once to f16.
+ *    A negative start or length, a length beyond a plain or paged cache, or a page number outside
+ *    the pool is reported by the next aion_cuda_sync / aion_cuda_d2h; the rows it concerns become
+ *    zeros. Pages without a step that is read are not looked up. out must not overlap the cache. */
+typedef struct AionCudaSequenceRead AionCudaSequenceRead;
+struct AionCudaSequenceRead {
+  AionCudaOperand out, cache;
+  AionCudaOperand start_index; /* handle 0 = absent */
+  AionCudaOperand lengths;     /* handle 0 = absent */
+  uint64_t batch, t_cap, heads, head_dim, out_len;
+  uint32_t dtype, out_dtype, rolling, reserved;
+  AionCudaOperand page_table; /* handle 0 = absent; as in AionCudaSequenceAppend */
+  uint64_t page_tokens, pool_pages;
+};
+AION_CUDA_API int32_t aion_cuda_sequence_read(AionCudaDevice* dev, const AionCudaSequenceRead* step);
 
 /* `GatherRows` step from a q8_0 [table_rows, d] table (quant_axis 1, any block order) to
  * f32 [count, d] (aion src/aion/backend/cpu/exec/gather.zig:22-28, 57-87). Indices follow
@@ -474,6 +511,34 @@ typedef struct AionCudaRopeKVAppend {
   uint32_t rolling;
 } AionCudaRopeKVAppend;
 AION_CUDA_API int32_t aion_cuda_rope_kv_append(AionCudaDevice* dev, const AionCudaRopeKVAppend* step);
+
+/* RMSNorm of every query head and every key head, RoPE1D of both, and the append of K and V to
+ * their caches, which may be quantized and paged. qkv as in AionCudaRopeKVAppend.
+ *   y = (x * inv) * gamma, inv = 1 / sqrt(mean(x^2) + eps) over the head (the mean is taken in
+ *   64 bits); gamma f32 [head_dim], one for all query heads, one for all key heads.
+ *   q_gamma / k_gamma with handle 0: those heads are rotated without a norm.
+ *   q_out [B, L, h_q, head_dim] f32 = RoPE(norm(q))
+ *   k_cache / v_cache [B, t_cap, h_kv, head_dim] (or pools, one page_table for both) of k_dtype /
+ *   v_dtype, each f16, q8_0 or q4_0: rows end_index[b] + l receive RoPE(norm(k)) and v.
+ * Range rules, rolling and pages as in aion_cuda_sequence_append, except that q_out is written
+ * for every row. A head whose mean square is not finite is reported by the next aion_cuda_sync /
+ * aion_cuda_d2h (nothing of that head is written). q_out must not overlap qkv. Of more new rows
+ * than a ring holds, the last t_cap stay. head_dim even, at most 1024, a multiple of 32 for a
+ * quantized cache.
+ * Results equal RMSNorm, RoPE1D, Cast and SequenceAppend in sequence, up to the norm's statistic. */
+typedef struct AionCudaQKNormRopeAppend AionCudaQKNormRopeAppend;
+struct AionCudaQKNormRopeAppend {
+  AionCudaOperand q_out, qkv;
+  AionCudaOperand q_gamma, k_gamma; /* handle 0 = absent */
+  AionCudaOperand positions, end_index, k_cache, v_cache;
+  uint64_t batch, len, h_q, h_kv, head_dim, ld_qkv, t_cap;
+  float eps, base_frequency, scale_factor, proportion;
+  uint32_t k_dtype, v_dtype;
+  uint32_t rolling, reserved;
+  AionCudaOperand page_table; /* handle 0 = absent */
+  uint64_t page_tokens, pool_pages;
+};
+AION_CUDA_API int32_t aion_cuda_qk_norm_rope_append(AionCudaDevice* dev, const AionCudaQKNormRopeAppend* step);
 
 /* ---------------------------------------------------------------------------------
  * Block quantizer on the device. `quantizeBlocks` (aion src/aion/storage/quantize.zig:31-103)
