@@ -818,7 +818,7 @@ int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
     if (reinterpret_cast<uintptr_t>(p.image) & 15) return fail(AION_CUDA_INVALID_ARGUMENT, "attention.image: the image must be 16-byte aligned");
     p.image_dtype = s->image_dtype;
   }
-  if (quant) return attention_qcache_launch(dev, p);
+  if (quant) return attention_qcache_launch(dev, p, s->flags);
   if (tensor_path) {
     const uint32_t group = p.Hq / p.Hkv;
     p.head_groups = (group + 7) / 8;

@@ -92,7 +92,7 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 
 // K / V in q8_0 / q4_0 blocks (attention_qcache.cu).
-int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p);
+int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p, uint32_t flags);
 
 constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
 

@@ -6,6 +6,8 @@
 //   out[block] = sum_t softmax_t * s_t[block] * c_t[block]
 // over the keys [lo, hi) of the row's window; zeros for an empty range. The codes are exact in any float type
 // and the scales in f32, so only the f32 sums round: the result is f32 attention over the dequantized cache.
+#include <mutex>
+
 #include "attention_device.cuh"
 #include "cache_geom.cuh"
 
@@ -124,11 +126,686 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
   return AION_CUDA_OK;
 }
 
+// ------------------------------------------------------------------------------------
+// tensor-core kernel for few query columns (decode): head sizes 64, 128, 256
+// ------------------------------------------------------------------------------------
+// A CTA serves up to eight query columns of one kv head, a column being (query position, query head of the
+// group), and a slice of the context; its four warps walk tiles of 16 keys on their own, each with a private
+// ring of cp.async stages, so nothing in the loop waits for another warp.
+//
+//  * S^T[16 keys x 8] = C . Q^T on f16 m16n8k16: the codes are exact in f16, q is two f16 terms (22 bits, normed
+//    by the column's largest value), and the products of one block of 32 dimensions are scaled by the block's
+//    scale in f32. q4_0 codes enter as the subnormals n * 2^-24 that a nibble IS in the low bits of an f16 (one
+//    AND per two codes); their offset of 8 is the accumulator's initial value, -8 sum q.
+//  * The logits are transposed by movmatrix (two 16-bit halves each), so a lane holds one column's logits of the
+//    keys that it needs as the B operand of the second product.
+//  * O^T[D x 8] += V-codes^T . P'^T, P' = p * scale of (key, block) in f32, again two f16 terms. P' is scaled by
+//    a power of two that follows the largest V scale met so far: without it small V scales would push the terms
+//    into f16's subnormals. The accumulators are moved over when that power or a column's maximum grows.
+//  * The splits' partial sums meet in the last CTA of a unit to arrive (log-sum-exp), as in attention.cu.
+//
+// A lane reads a block pair's bytes where they lie: 2 x 18 (34) bytes are 9 (17) aligned words whose first and
+// middle ones hold the scales, and the order of the dimensions inside a block is free as long as Q's order is
+// the same. Rows are padded in shared memory to a pitch of 4 (mod 8) words, where no two lanes meet in a bank.
+constexpr int TK = 16;              // keys of a tile
+constexpr int WARPS = 4;
+constexpr int THREADS = WARPS * 32;
+constexpr int COLS = 8;
+
+template <int D, bool Q8>
+struct RowFmt {
+  static constexpr int BB = Q8 ? Q8_BYTES : Q4_BYTES;
+  static constexpr int BYTES = D / QK * BB;          // one head row
+  static constexpr int CHUNKS = Q8 ? 17 : 9;         // copies of CHUNK bytes
+  static constexpr int CHUNK = D / 16;
+  static constexpr int PITCH = Q8 ? (D == 64 ? 80 : D == 128 ? 144 : 272) : (D == 64 ? 48 : D == 128 ? 80 : 144);
+  static_assert(CHUNKS * CHUNK == BYTES && PITCH % CHUNK == 0 && PITCH >= BYTES && (PITCH / 4) % 8 == 4, "row layout");
+};
+
+template <int D, bool KQ8, bool VQ8>
+struct DecodeGeom {
+  using K = RowFmt<D, KQ8>;
+  using V = RowFmt<D, VQ8>;
+  static constexpr int STAGE = TK * (K::PITCH + V::PITCH);
+  // Two CTAs an SM for D = 256 (registers), three below: 100 / 66 KB of ring each.
+  static constexpr int NST_MAX = (D == 256 ? 92 : 60) * 1024 / (WARPS * STAGE);
+  static constexpr int NST = NST_MAX > 8 ? 8 : NST_MAX;
+  static constexpr int WS = COLS * D + 2 * COLS;     // floats of a warp's result: sums, maxima, weights
+  static constexpr int RING = WARPS * NST * STAGE;
+  static_assert(NST >= 2 && WARPS * WS * 4 <= RING, "ring");
+  static constexpr int OFF_VS = RING;                                  // f32 [warp][block][16 keys]: V scales
+  static constexpr int OFF_Q = OFF_VS + WARPS * (D / QK) * TK * 4;     // f32 [8][D]: q, normed
+  static constexpr int OFF_CI = OFF_Q + COLS * D * 4;                  // f32 [block][8]: -8 sum q
+  static constexpr int OFF_META = OFF_CI + D / QK * COLS * 4;          // per column: row, first key, key end, output row, head, factor
+  static constexpr int OFF_VALID = OFF_META + COLS * 24;               // per warp and stage: which keys are there
+  static constexpr int OFF_FLAGS = OFF_VALID + WARPS * NST * 4;
+  static constexpr int SMEM = OFF_FLAGS + 32;
+  static constexpr int MAX_SPLITS = 128;
+  static_assert(MAX_SPLITS * COLS * 8 + COLS * 4 <= RING, "factors of the merge");
+};
+
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool there) {
+  const int n = there ? BYTES : 0;   // nothing is read and zeros are written where the key is not there
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint32_t movm(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// D = A . B + C with a C of its own.
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                             float c0, float c1, float c2, float c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ float half_bits(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
+__device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// Two terms of f16 for a pair of f32 values: x = hi + lo to 22 bits.
+__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  *hi = *reinterpret_cast<const uint32_t*>(&h);
+  *lo = pack_half2(a - f.x, b - f.y);
+}
+
+// Which dimension of a block the lane index u (t of a key row's words) reaches with code i of its word(s).
+// K words: q4_0 one word of eight nibbles per lane t; q8_0 two words, u = t and t + 4, of four bytes.
+__host__ __device__ constexpr int pair_byte(bool q8, bool second, int u, int j) {
+  // byte j of word u of the block's codes; in a pair's first block word 0 is put together from the codes' first
+  // and last two bytes (they share words with the two scales)
+  const int n = q8 ? 32 : 16;
+  return second ? 4 * u + j : u ? 4 * u - 2 + j : j < 2 ? j : n - 4 + j;
+}
+
+// The A operand of 16 keys x 32 dimensions: two MMAs' worth, from the words of key rows g and g + 8.
+template <bool Q8>
+struct KFrag {
+  uint32_t a[2][4];
+  uint32_t scale_lo, scale_hi;   // f16 bits for keys g, g + 8
+};
+__device__ __forceinline__ void unpack_q4_subnormal(uint32_t w, uint32_t (&x)[4]) {
+  x[0] = w & 0x000F000Fu;        // n * 2^-24
+  x[1] = w & 0x00F000F0u;        // n * 2^-20
+  w >>= 8;
+  x[2] = w & 0x000F000Fu;
+  x[3] = w & 0x00F000F0u;
+}
+__device__ __forceinline__ void unpack_q8(uint32_t w, uint32_t* r0, uint32_t* r1) {
+  w ^= 0x80808080u;
+  // 0x6400 | u is 1024 + u: minus 1152 leaves the signed code, exactly
+  *r0 = h2_add(__byte_perm(w, 0x64646464u, 0x4140), 0xE480E480u);
+  *r1 = h2_add(__byte_perm(w, 0x64646464u, 0x4342), 0xE480E480u);
+}
+
+template <int D, bool KQ8, bool VQ8>
+__global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_kernel(const AttnParams p) {
+  using G = DecodeGeom<D, KQ8, VQ8>;
+  using KF = RowFmt<D, KQ8>;
+  using VF = RowFmt<D, VQ8>;
+  constexpr int NB = D / QK;          // blocks of a head row
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t sbase = ptx::smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+
+  // unit = (b, block of positions, hkv, head group); split = blockIdx.y
+  const uint32_t unit = blockIdx.x, split = blockIdx.y;
+  const uint32_t hg = unit % p.head_groups;
+  const uint32_t hkv = (unit / p.head_groups) % p.Hkv;
+  const uint32_t bl = unit / (p.head_groups * p.Hkv);
+  const uint32_t lb = p.l_blocks - 1 - bl % p.l_blocks, b = bl / p.l_blocks;
+  const uint32_t group = p.Hq / p.Hkv;
+  const uint32_t h0 = hkv * group + hg * 8;
+  const uint32_t nh = min(8u, group - hg * 8);
+  const uint32_t l0 = lb * p.pos_per_tile;
+
+  uint32_t* col_row = reinterpret_cast<uint32_t*>(smem + G::OFF_META);  // (b*L + l)*Hq + head, NO_ROW: padding
+  uint32_t* col_lo = col_row + COLS;
+  uint32_t* col_hi = col_lo + COLS;
+  uint32_t* col_orow = col_hi + COLS;
+  uint32_t* col_head = col_orow + COLS;
+  float* col_factor = reinterpret_cast<float*>(col_head + COLS);
+  float* qs = reinterpret_cast<float*>(smem + G::OFF_Q);
+  float* ci = reinterpret_cast<float*>(smem + G::OFF_CI);
+  int* flags = reinterpret_cast<int*>(smem + G::OFF_FLAGS);   // [0] bad inputs, [1] last CTA of the unit
+
+  if (tid == 0) flags[0] = 0;
+  __syncthreads();
+  ptx::pdl_launch_dependents();
+  ptx::pdl_wait();
+  if (tid < COLS) {
+    const uint32_t pl = tid / p.col_heads, hh = tid - pl * p.col_heads, l = l0 + pl;
+    uint32_t row = NO_ROW, lo = 0, hi = 0;
+    if (pl < p.pos_per_tile && hh < nh && l < p.L) {
+      const KeyRange kr = key_range(p, b, l);
+      if (kr.bad) flags[0] = 1;
+      row = (b * p.L + l) * p.Hq + h0 + hh;
+      lo = kr.lo, hi = kr.hi;
+    }
+    col_row[tid] = row, col_lo[tid] = lo, col_hi[tid] = hi;
+    col_orow[tid] = b * p.L + l, col_head[tid] = h0 + hh;
+  }
+  __syncthreads();
+  if (flags[0] && tid == 0) atomicExch(p.fault, FAULT_INVALID_ARGUMENT);
+  // The union of the columns' ranges, and what all of them see.
+  uint32_t u_lo = 0xFFFFFFFFu, u_hi = 0, all_lo = 0, all_hi = 0xFFFFFFFFu;
+#pragma unroll
+  for (int c = 0; c < COLS; c++) {
+    const uint32_t lo = col_lo[c], hi = col_hi[c];
+    if (hi > lo) u_lo = min(u_lo, lo), u_hi = max(u_hi, hi);
+    if (col_row[c] != NO_ROW) all_lo = max(all_lo, lo), all_hi = min(all_hi, hi);
+  }
+  u_lo = min(u_lo, u_hi);
+  uint32_t per = (u_hi - u_lo + p.splits - 1) / p.splits;
+  per = (per + TK - 1) / TK * TK;
+  const uint32_t my_lo = (uint32_t)min((uint64_t)u_hi, u_lo + (uint64_t)split * per);
+  const uint32_t my_hi = (uint32_t)min((uint64_t)u_hi, (uint64_t)my_lo + per);
+  const uint32_t tiles = (my_hi - my_lo + TK - 1) / TK;
+
+  // ---- the warp's copies: tile i of the CTA's slice, into stage (i / WARPS) % NST of its ring
+  CacheGeom geom = geom_of(p);
+  const uint32_t bq = p.page_table ? b : 0;
+  const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;
+  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + (row0 * p.Hkv + hkv) * KF::BYTES;
+  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + (row0 * p.Hkv + hkv) * VF::BYTES;
+  const uint32_t ring = sbase + warp * (G::NST * G::STAGE);
+  uint32_t* valid = reinterpret_cast<uint32_t*>(smem + G::OFF_VALID) + warp * G::NST;
+  // Row (below the request's first one, or in the pool) of this lane's key of a tile; its table entry is read a
+  // tile ahead of the copies.
+  auto find_row = [&](uint32_t tile, bool* there) -> uint32_t {
+    const uint32_t key = my_lo + tile * TK + (lane & 15);
+    *there = tile < tiles && key < my_hi;
+    if (!*there) return 0;
+    const int64_t r = cache_row(geom, bq, key);
+    if (r < 0) {
+      atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
+      *there = false;
+      return 0;
+    }
+    return (uint32_t)r;
+  };
+  auto issue = [&](uint32_t stage, uint32_t row, bool there) {
+    const uint32_t mask = __ballot_sync(FULL, there) & 0xFFFFu;
+    if (lane == 0) valid[stage] = mask;
+    const uint32_t dst = ring + stage * G::STAGE;
+#pragma unroll
+    for (int i = 0; i < (TK * KF::CHUNKS + 31) / 32; i++) {
+      const uint32_t idx = lane + 32 * i, key = idx / KF::CHUNKS, c = idx - key * KF::CHUNKS;
+      const uint32_t r = __shfl_sync(FULL, row, key & 15);
+      if (idx < TK * KF::CHUNKS)
+        cp_async<KF::CHUNK>(dst + key * KF::PITCH + c * KF::CHUNK, kbase + (uint64_t)r * (p.Hkv * KF::BYTES) + c * KF::CHUNK, (mask >> key) & 1);
+    }
+    const uint32_t vdst = dst + TK * KF::PITCH;
+#pragma unroll
+    for (int i = 0; i < (TK * VF::CHUNKS + 31) / 32; i++) {
+      const uint32_t idx = lane + 32 * i, key = idx / VF::CHUNKS, c = idx - key * VF::CHUNKS;
+      const uint32_t r = __shfl_sync(FULL, row, key & 15);
+      if (idx < TK * VF::CHUNKS)
+        cp_async<VF::CHUNK>(vdst + key * VF::PITCH + c * VF::CHUNK, vbase + (uint64_t)r * (p.Hkv * VF::BYTES) + c * VF::CHUNK, (mask >> key) & 1);
+    }
+  };
+  const uint32_t mine = tiles > (uint32_t)warp ? (tiles - warp + WARPS - 1) / WARPS : 0;   // tiles of this warp
+  bool next_there;
+  uint32_t next_row = find_row(warp, &next_there);
+#pragma unroll
+  for (int s = 0; s < G::NST - 1; s++) {
+    if ((uint32_t)s < mine) issue(s, next_row, next_there);
+    cp_commit();
+    if ((uint32_t)s < mine) next_row = find_row(warp + (s + 1) * WARPS, &next_there);
+  }
+
+  // ---- q: normed by the column's largest value to [2^13, 2^14), and the sums that offset q4_0 codes
+  for (int c = warp; c < COLS; c += WARPS) {
+    float v[D / 32], top = 0.0f;
+    const uint32_t row = col_row[c];
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      v[i] = 0.0f;
+      if (row != NO_ROW) {
+        const uint64_t at = (uint64_t)row * D + lane + 32 * i;
+        v[i] = p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at] : __half2float(static_cast<const __half*>(p.q)[at]);
+      }
+      top = fmaxf(top, fabsf(v[i]));
+    }
+    uint32_t e = __reduce_max_sync(FULL, __float_as_uint(top)) >> 23;     // biased exponent
+    if (e == 255) e = 127;                                                // not finite: the logits will not be either
+    e = max(e, 40u);                                                      // far below any logit that matters
+    const float up = __uint_as_float((127u + 13u + 127u - e) << 23);      // 2^(13 - (e - 127)), e >= 40
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) qs[c * D + lane + 32 * i] = v[i] * up;
+    if (lane == 0) col_factor[c] = p.scale * __uint_as_float((e - 13u) << 23);
+  }
+  __syncthreads();
+  // Q^T as the B operand: this lane's column g, the dimensions of word t. Where a q4_0 code enters times 16, q
+  // enters by 16 less.
+  uint32_t qh[D / 16][2], ql[D / 16][2];
+#pragma unroll
+  for (int blk = 0; blk < NB; blk++) {
+    float part = 0.0f;
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        float x[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          int dim;
+          if (KQ8) dim = pair_byte(true, blk & 1, t + 4 * m, 2 * r + h);
+          else dim = 2 * pair_byte(false, blk & 1, t, m + 2 * h) + r;      // nibbles (2m + r, 2m + r + 4): bytes m, m + 2
+          x[h] = qs[g * D + blk * QK + dim] * (!KQ8 && r ? 0.0625f : 1.0f);
+        }
+        uint32_t hi, lo;
+        split2(x[0], x[1], &hi, &lo);
+        qh[2 * blk + m][r] = hi, ql[2 * blk + m][r] = lo;
+        if (!KQ8) {
+          const float2 a = __half22float2(*reinterpret_cast<__half2*>(&hi)), c = __half22float2(*reinterpret_cast<__half2*>(&lo));
+          part += ((a.x + c.x) + (a.y + c.y)) * (r ? 16.0f : 1.0f);
+        }
+      }
+    if (!KQ8) {
+      part += __shfl_xor_sync(FULL, part, 1);
+      part += __shfl_xor_sync(FULL, part, 2);
+      if (warp == 0 && t == 0) ci[blk * COLS + g] = part * (-8.0f * 5.9604644775390625e-8f);   // -8 * 2^-24
+    }
+  }
+  if (!KQ8) __syncthreads();
+  const float f0 = col_factor[2 * t], f1 = col_factor[2 * t + 1];
+  const uint32_t lo_g = col_lo[g], hi_g = col_hi[g];
+
+  float acc[D / 16][4];
+#pragma unroll
+  for (int i = 0; i < D / 16; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[i][e] = 0.0f;
+  float m_run = -INFINITY, l_run = 0.0f;     // column g; l_run: this lane's keys only
+  uint32_t e_run = 0;                        // exponent field of the largest V scale so far
+  const uint32_t vs = sbase + G::OFF_VS + warp * (NB * TK * 4);
+
+  for (uint32_t i = 0; i < mine; i++) {
+    const uint32_t stage = i % G::NST;
+    {
+      const uint32_t ahead = i + G::NST - 1;
+      if (ahead < mine) {
+        issue(ahead % G::NST, next_row, next_there);
+        next_row = find_row(warp + (ahead + 1) * WARPS, &next_there);
+      }
+      cp_commit();
+    }
+    cp_wait<G::NST - 1>();
+    __syncwarp();
+    const uint32_t ks = ring + stage * G::STAGE, vst = ks + TK * KF::PITCH;
+    const uint32_t there = valid[stage];
+    const uint32_t key0 = my_lo + (warp + i * WARPS) * TK;
+
+    // V scales of the tile as f32, times 2^(29 - E) of the largest exponent so far
+    uint32_t sc[NB / 2], top = 0;
+#pragma unroll
+    for (int j = 0; j < NB / 2; j++) {
+      const uint32_t at = lane + 32 * j;     // (block, key)
+      sc[j] = lds16(vst + (at & 15) * VF::PITCH + (at >> 4) * VF::BB);
+      const uint32_t mag = sc[j] & 0x7FFFu;
+      if (mag < 0x7C00u) top = max(top, mag);
+    }
+    const uint32_t e_new = max(e_run, __reduce_max_sync(FULL, top) >> 10);
+    const float vmul = __uint_as_float((127u + 29u - e_new) << 23);
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < NB / 2; j++) {
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(vs + (lane + 32 * j) * 4), "f"(half_bits(sc[j]) * vmul) : "memory");
+      odd |= (sc[j] & 0x7FFFu) >= 0x7C00u;
+    }
+    odd = __any_sync(FULL, odd);             // an infinite or NaN scale: its keys must not reach columns that do not see them
+    __syncwarp();
+
+    // S^T of 16 keys x 8 columns
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int pr = 0; pr < NB / 2; pr++) {
+      uint32_t a[2][2][4];                   // [block of the pair][MMA][operand]
+      float sl[2], sh[2];                    // scales of keys g, g + 8
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const uint32_t row = ks + (g + 8 * half) * KF::PITCH + pr * 2 * KF::BB;
+        const uint32_t w0 = lds32(row);
+        if (KQ8) {
+          const uint32_t w8 = lds32(row + 32), wt = lds32(row + 4 * t), wu = lds32(row + 16 + 4 * t);
+          const uint32_t x0 = lds32(row + 36 + 4 * t), x1 = lds32(row + 52 + 4 * t);
+          const uint32_t first = t ? wt : __byte_perm(w0, w8, 0x5432);
+          unpack_q8(first, &a[0][0][half], &a[0][0][2 + half]);
+          unpack_q8(wu, &a[0][1][half], &a[0][1][2 + half]);
+          unpack_q8(x0, &a[1][0][half], &a[1][0][2 + half]);
+          unpack_q8(x1, &a[1][1][half], &a[1][1][2 + half]);
+          (half ? sh : sl)[0] = half_bits(w0 & 0xFFFFu), (half ? sh : sl)[1] = half_bits(w8 >> 16);
+        } else {
+          const uint32_t w4 = lds32(row + 16), wt = lds32(row + 4 * t), x0 = lds32(row + 20 + 4 * t);
+          const uint32_t first = t ? wt : __byte_perm(w0, w4, 0x5432);
+          uint32_t u[4];
+          unpack_q4_subnormal(first, u);
+          a[0][0][half] = u[0], a[0][0][2 + half] = u[1], a[0][1][half] = u[2], a[0][1][2 + half] = u[3];
+          unpack_q4_subnormal(x0, u);
+          a[1][0][half] = u[0], a[1][0][2 + half] = u[1], a[1][1][half] = u[2], a[1][1][2 + half] = u[3];
+          (half ? sh : sl)[0] = half_bits(w0 & 0xFFFFu), (half ? sh : sl)[1] = half_bits(w4 >> 16);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int blk = 2 * pr + k;
+        float c[4];
+        float2 init = make_float2(0.0f, 0.0f);
+        if (!KQ8) init = lds_f2(sbase + G::OFF_CI + (blk * COLS + 2 * t) * 4);
+        mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], qh[2 * blk][0], qh[2 * blk][1], init.x, init.y, init.x, init.y);
+        mma_f16(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], qh[2 * blk + 1][0], qh[2 * blk + 1][1]);
+        mma_f16(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], ql[2 * blk][0], ql[2 * blk][1]);
+        mma_f16(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], ql[2 * blk + 1][0], ql[2 * blk + 1][1]);
+        s[0] = fmaf(sl[k], c[0], s[0]);
+        s[1] = fmaf(sl[k], c[1], s[1]);
+        s[2] = fmaf(sh[k], c[2], s[2]);
+        s[3] = fmaf(sh[k], c[3], s[3]);
+      }
+    }
+    // logits, and their transpose: column g, keys 2t, 2t + 1, 2t + 8, 2t + 9
+    float y[4];
+    {
+      const float unit24 = KQ8 ? 1.0f : 16777216.0f;
+      s[0] = (s[0] * unit24) * f0, s[1] = (s[1] * unit24) * f1, s[2] = (s[2] * unit24) * f0, s[3] = (s[3] * unit24) * f1;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t u = __float_as_uint(s[2 * h]), w = __float_as_uint(s[2 * h + 1]);
+        const uint32_t low = movm(__byte_perm(u, w, 0x5410)), high = movm(__byte_perm(u, w, 0x7632));
+        y[2 * h] = __uint_as_float(__byte_perm(low, high, 0x5410));
+        y[2 * h + 1] = __uint_as_float(__byte_perm(low, high, 0x7632));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) y[k] = soft_cap_logit(y[k], p.soft_cap) * LOG2E;
+    if (there != 0xFFFFu || key0 < all_lo || key0 + TK > all_hi) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const uint32_t kk = 2 * t + (k & 1) + 8 * (k >> 1), key = key0 + kk;
+        if (!((there >> kk) & 1) || key < lo_g || key >= hi_g) y[k] = -INFINITY;
+      }
+    }
+    float m_new = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), m_run);
+    m_new = fmaxf(m_new, __shfl_xor_sync(FULL, m_new, 1));
+    m_new = fmaxf(m_new, __shfl_xor_sync(FULL, m_new, 2));
+    if (__any_sync(FULL, m_new > m_run) || e_new > e_run) {
+      const float alpha = m_new > m_run ? exp2f(m_run - m_new) : 1.0f;
+      l_run *= alpha;
+      const float down = __uint_as_float((127u + e_run - e_new) << 23);   // 2^(old - new)
+      const float a0 = __shfl_sync(FULL, alpha, 8 * t) * down, a1 = __shfl_sync(FULL, alpha, 8 * t + 4) * down;
+#pragma unroll
+      for (int j = 0; j < D / 16; j++) acc[j][0] *= a0, acc[j][1] *= a1, acc[j][2] *= a0, acc[j][3] *= a1;
+      m_run = m_new;
+      e_run = e_new;
+    }
+    const float m_safe = m_run == -INFINITY ? 0.0f : m_run;
+    float pr4[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) pr4[k] = exp2f(y[k] - m_safe);
+    l_run += (pr4[0] + pr4[1]) + (pr4[2] + pr4[3]);
+
+    // O^T += V^T . P'^T, block by block
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++) {
+      const float2 v0 = lds_f2(vs + (blk * TK + 2 * t) * 4), v1 = lds_f2(vs + (blk * TK + 2 * t + 8) * 4);
+      float w[4] = {pr4[0] * v0.x, pr4[1] * v0.y, pr4[2] * v1.x, pr4[3] * v1.y};
+      if (odd)
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = pr4[k] == 0.0f ? 0.0f : w[k];
+      uint32_t bh[2], blw[2];
+      split2(w[0], w[1], &bh[0], &blw[0]);
+      split2(w[2], w[3], &bh[1], &blw[1]);
+      uint32_t a[2][4];   // [row tile][operand]: rows g and g + 8, key pairs (2t, 2t + 1) and (2t + 8, 2t + 9)
+#pragma unroll
+      for (int kp = 0; kp < 2; kp++) {
+        const uint32_t row = vst + (2 * t + 8 * kp) * VF::PITCH;
+        if (VQ8) {
+          uint32_t x[2];
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const uint32_t at = row + h * VF::PITCH + (blk >> 1) * 2 * VF::BB;
+            if (blk & 1) x[h] = lds32(at + 36 + 4 * g);
+            else {
+              const uint32_t wg = lds32(at + 4 * g), w8 = lds32(at + 32);
+              x[h] = g ? wg : __byte_perm(wg, w8, 0x5432);
+            }
+            x[h] ^= 0x80808080u;
+          }
+          const uint32_t lo2 = __byte_perm(x[0], x[1], 0x5140), hi2 = __byte_perm(x[0], x[1], 0x7362);
+          a[0][2 * kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4140), 0xE480E480u);
+          a[0][2 * kp + 1] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4342), 0xE480E480u);
+          a[1][2 * kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4140), 0xE480E480u);
+          a[1][2 * kp + 1] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4342), 0xE480E480u);
+        } else {
+          const uint32_t at = row + blk * VF::BB + 2 + 2 * g;
+          uint32_t x = __byte_perm(lds16(at), lds16(at + VF::PITCH), 0x5410);
+          // 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n: both leave n - 8 exactly
+          a[0][2 * kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+          a[0][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+          x >>= 8;
+          a[1][2 * kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+          a[1][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        mma_f16(acc[2 * blk + m], a[m][0], a[m][1], a[m][2], a[m][3], bh[0], bh[1]);
+        mma_f16(acc[2 * blk + m], a[m][0], a[m][1], a[m][2], a[m][3], blw[0], blw[1]);
+      }
+    }
+    __syncwarp();   // the stage and the scales are free again
+  }
+  cp_wait<0>();
+
+  // ---- the four warps' sums meet
+  l_run += __shfl_xor_sync(FULL, l_run, 1);
+  l_run += __shfl_xor_sync(FULL, l_run, 2);
+  __syncthreads();
+  float* all = reinterpret_cast<float*>(smem);
+  {
+    float* mb = all + warp * G::WS;
+    // 2^(E - 29) in two exact steps: the product of the whole range would leave f32 for E = 0
+    const float back = __uint_as_float((127u + e_run - 29u) << 23);
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++)
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          const int dim = blk * QK + (VQ8 ? pair_byte(true, blk & 1, g, 2 * m + r) : 4 * g + 2 * m + r);
+          mb[(2 * t) * D + dim] = acc[2 * blk + m][2 * r] * back;
+          mb[(2 * t + 1) * D + dim] = acc[2 * blk + m][2 * r + 1] * back;
+        }
+    if (t == 0) mb[COLS * D + g] = m_run, mb[COLS * D + COLS + g] = l_run;
+  }
+  __syncthreads();
+  constexpr int C4 = COLS * D / 4 / THREADS;
+  constexpr int PP = D + 4;                   // a partial row: D sums, maximum, weight, pad
+  float* part = p.partial + ((uint64_t)unit * p.splits + split) * COLS * PP;
+  const bool direct = p.splits == 1;
+  const uint32_t d4 = tid % (D / 4);
+#pragma unroll 1
+  for (int c = 0; c < C4; c++) {
+    const uint32_t idx4 = tid + c * THREADS, col = idx4 / (D / 4);
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) M = fmaxf(M, all[w * G::WS + COLS * D + col]);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float lsum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      const float mw = all[w * G::WS + COLS * D + col];
+      const float f = mw == -INFINITY ? 0.0f : exp2f(mw - M);
+      const float4 x = *reinterpret_cast<const float4*>(all + w * G::WS + 4 * idx4);
+      o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
+      lsum += all[w * G::WS + COLS * D + COLS + col] * f;
+    }
+    const bool on = col_row[col] != NO_ROW;
+    if (direct) {
+      finish_column<D>(p, o, lsum, on, col_hi[col] > col_lo[col], col, d4, col_row, col_orow, col_head, !flags[0]);
+    } else if (on) {
+      *reinterpret_cast<float4*>(part + col * PP + 4 * d4) = o;
+      if (d4 == 0) *reinterpret_cast<float2*>(part + col * PP + D) = make_float2(M, lsum);
+    }
+  }
+  if (direct) return;
+  // ---- and the splits' in the last CTA of the unit
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    const int prev = atomicAdd(p.tickets + unit, 1), last = prev == (int)p.splits - 1;
+    if (last) p.tickets[unit] = 0;   // ready for the next launch
+    flags[1] = last;
+  }
+  __syncthreads();
+  if (!flags[1]) return;
+  __threadfence();
+  const float* pu = p.partial + (uint64_t)unit * p.splits * COLS * PP;
+  float* fac = all;                           // [8][splits]: maximum, then factor
+  float* wsum = fac + COLS * p.splits;
+  float* lsums = wsum + COLS * p.splits;
+  for (uint32_t idx = tid; idx < COLS * p.splits; idx += THREADS) {
+    const uint32_t c = idx / p.splits, s2 = idx - c * p.splits;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (col_row[c] != NO_ROW) ml = __ldcg(reinterpret_cast<const float2*>(pu + (size_t)(s2 * COLS + c) * PP + D));
+    fac[idx] = ml.x, wsum[idx] = ml.y;
+  }
+  __syncthreads();
+  for (uint32_t c = warp; c < COLS; c += WARPS) {
+    float M = -INFINITY, lsum = 0.0f;
+    for (uint32_t s2 = lane; s2 < p.splits; s2 += 32) M = fmaxf(M, fac[c * p.splits + s2]);
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, o));
+    for (uint32_t s2 = lane; s2 < p.splits; s2 += 32) {
+      const float ms = fac[c * p.splits + s2], f = ms == -INFINITY ? 0.0f : exp2f(ms - M);
+      fac[c * p.splits + s2] = f;
+      lsum += f > 0.0f || isnan(f) ? wsum[c * p.splits + s2] * f : 0.0f;
+    }
+    for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(FULL, lsum, o);
+    if (lane == 0) lsums[c] = lsum;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int c = 0; c < C4; c++) {
+    const uint32_t idx4 = tid + c * THREADS, col = idx4 / (D / 4);
+    const bool on = col_row[col] != NO_ROW;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (on) {
+      const float* src = pu + (size_t)col * PP + 4 * d4;
+      for (uint32_t s0 = 0; s0 < p.splits; s0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          v[k] = s0 + k < p.splits ? __ldcg(reinterpret_cast<const float4*>(src + (size_t)(s0 + k) * COLS * PP)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (s0 + k < p.splits) {
+            const float f = fac[col * p.splits + s0 + k];
+            o.x += v[k].x * f, o.y += v[k].y * f, o.z += v[k].z * f, o.w += v[k].w * f;
+          }
+      }
+    }
+    finish_column<D>(p, o, lsums[col], on, col_hi[col] > col_lo[col], col, d4, col_row, col_orow, col_head, !flags[0]);
+  }
+}
+
+template <int D, bool KQ8, bool VQ8>
+int32_t launch_decode(AionCudaDevice* dev, const AttnParams& p, uint32_t units) {
+  using G = DecodeGeom<D, KQ8, VQ8>;
+  auto kernel = attn_qcache_decode_kernel<D, KQ8, VQ8>;
+  {
+    static std::mutex mu;   // once per device and instantiation
+    static bool configured[64] = {};
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev->ordinal < 0 || dev->ordinal >= 64 || !configured[dev->ordinal]) {
+      AION_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+      if (dev->ordinal >= 0 && dev->ordinal < 64) configured[dev->ordinal] = true;
+    }
+  }
+  if (p.splits > (uint32_t)G::MAX_SPLITS) return fail(AION_CUDA_INTERNAL_ERROR, "attention: %u splits exceed the merge buffer", p.splits);
+  AION_CUDA_TRY(launch_pdl_main(kernel, dim3(units, p.splits), dim3(THREADS), G::SMEM, dev->stream, p));
+  return AION_CUDA_OK;
+}
+
 }  // namespace
 
-int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p) {
+int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p, uint32_t flags) {
   const bool kq8 = p.k_dtype == AION_CUDA_DTYPE_Q8_0, vq8 = p.v_dtype == AION_CUDA_DTYPE_Q8_0;
-  if (p.image) return fail(AION_CUDA_UNSUPPORTED, "attention: no output image over a quantized cache");
+  // The tensor-core kernel copies rows in pieces of D / 16 bytes and stores its output in 16 bytes.
+  const uintptr_t kv = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
+  const bool tensor = p.Dk == p.Dv && (p.Dk == 64 || p.Dk == 128 || p.Dk == 256) && (kv & (p.Dk / 16 - 1)) == 0 &&
+                      (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && !(flags & AION_CUDA_ATTENTION_GENERIC);
+  if (tensor) {
+    const uint32_t group = p.Hq / p.Hkv;
+    p.head_groups = (group + 7) / 8;
+    p.col_heads = group < 8 ? group : 8;
+    p.pos_per_tile = 8 / p.col_heads;
+    if (p.pos_per_tile > p.L) p.pos_per_tile = p.L;
+    p.l_blocks = (p.L + p.pos_per_tile - 1) / p.pos_per_tile;
+    const uint64_t units = (uint64_t)p.B * p.l_blocks * p.Hkv * p.head_groups;
+    if (units > 0x7FFFFFFF) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
+    // Splits: enough CTAs to fill the SMs once, none below one tile per warp.
+    uint64_t max_keys = p.T;
+    const uint64_t span = (uint64_t)(p.win_chunk ? p.win_chunk : 1) + p.win_left + p.win_right + p.pos_per_tile;
+    if (p.win_left != AION_CUDA_WINDOW_UNBOUNDED && p.win_right != AION_CUDA_WINDOW_UNBOUNDED && span < max_keys) max_keys = span;
+    const uint64_t resident = (uint64_t)dev->sm_count * (p.Dk == 256 ? 2 : 3);
+    uint64_t splits = resident / units, most = (max_keys + TK * WARPS - 1) / (TK * WARPS);
+    if (splits > most) splits = most;
+    if (splits > 128) splits = 128;
+    if (splits < 1) splits = 1;
+    if (dev->attn_split_override) splits = dev->attn_split_override > 128 ? 128 : dev->attn_split_override;
+    p.splits = (uint32_t)splits;
+    if (splits > 1) {
+      if (int32_t st = dev->reserve_scratch(units * splits * COLS * (p.Dk + 4) * sizeof(float))) return st;
+      if (int32_t st = dev->reserve_tickets(units)) return st;
+      p.partial = static_cast<float*>(dev->lane_scratch());
+      p.tickets = dev->lane_tickets();
+    }
+    const uint32_t u = (uint32_t)units;
+#define AION_QCACHE(D)                                                                                     \
+  if (kq8) return vq8 ? launch_decode<D, true, true>(dev, p, u) : launch_decode<D, true, false>(dev, p, u); \
+  return vq8 ? launch_decode<D, false, true>(dev, p, u) : launch_decode<D, false, false>(dev, p, u);
+    switch (p.Dk) {
+      case 64: AION_QCACHE(64)
+      case 128: AION_QCACHE(128)
+      default: AION_QCACHE(256)
+    }
+#undef AION_QCACHE
+  }
+  if (p.image) return fail(AION_CUDA_UNSUPPORTED, "attention: the output image is written by the tensor-core kernels only (Dk = Dv in {64, 128, 256}, aligned operands)");
   if (p.Dv > 32 * MAX_DV_PER_LANE || (p.Dk + ROW_WARPS * (p.Dv + 2)) * sizeof(float) > 48 * 1024)
     return fail(AION_CUDA_UNSUPPORTED, "attention: head dimensions %u / %u exceed the any-shape kernel", p.Dk, p.Dv);
   p.splits = 1;
