@@ -131,7 +131,9 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
 // ------------------------------------------------------------------------------------
 // A CTA serves up to eight query columns of one kv head, a column being (query position, query head of the
 // group), and a slice of the context; its four warps walk tiles of 16 keys on their own, each with a private
-// ring of cp.async stages, so nothing in the loop waits for another warp.
+// ring of stages, so nothing in the loop waits for another warp. A tile's rows arrive as one TMA box of K and one
+// of V (16 rows of the head's bytes, rounded out to 16-byte granules) where the rows of the cache begin on
+// 16-byte boundaries, pages and rings in multiples of 16 rows; else by cp.async in pieces of D / 16 bytes.
 //
 //  * S^T[16 keys x 8] = C . Q^T on f16 m16n8k16: the codes are exact in f16, q is two f16 terms (22 bits, normed
 //    by the column's largest value), and the products of one block of 32 dimensions are scaled by the block's
@@ -178,7 +180,8 @@ struct DecodeGeom {
   static constexpr int OFF_CI = OFF_Q + COLS * D * 4;                  // f32 [block][8]: -8 sum q
   static constexpr int OFF_META = OFF_CI + D / QK * COLS * 4;          // per column: row, first key, key end, output row, head, factor
   static constexpr int OFF_VALID = OFF_META + COLS * 24;               // per warp and stage: which keys are there
-  static constexpr int OFF_FLAGS = OFF_VALID + WARPS * NST * 4;
+  static constexpr int OFF_BARS = (OFF_VALID + WARPS * NST * 4 + 7) / 8 * 8;   // per warp and stage: the copies' barrier
+  static constexpr int OFF_FLAGS = OFF_BARS + WARPS * NST * 8;
   static constexpr int SMEM = OFF_FLAGS + 32;
   static constexpr int MAX_SPLITS = 128;
   static_assert(MAX_SPLITS * COLS * 8 + COLS * 4 <= RING, "factors of the merge");
@@ -234,12 +237,16 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-// Two terms of f16 for a pair of f32 values: x = hi + lo to 22 bits.
+// Two terms of f16 for a pair of f32 values: x = hi + lo to 22 bits. The remainder is taken by a subtraction that
+// reads the f16 term as it is (on the FMA pipe; a conversion back to f32 would go to the busier ALU pipe).
 __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
-  const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
-  *hi = *reinterpret_cast<const uint32_t*>(&h);
-  *lo = pack_half2(a - f.x, b - f.y);
+  const uint32_t h = pack_half2(a, b);
+  float na, nb;   // hi - x
+  asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %4;\n\t}"
+      : "=f"(na), "=f"(nb)
+      : "r"(h), "f"(a), "f"(b));
+  *hi = h;
+  *lo = pack_half2(-na, -nb);
 }
 
 // Which dimension of a block the lane index u (t of a key row's words) reaches with code i of its word(s).
@@ -271,8 +278,9 @@ __device__ __forceinline__ void unpack_q8(uint32_t w, uint32_t* r0, uint32_t* r1
   *r1 = h2_add(__byte_perm(w, 0x64646464u, 0x4342), 0xE480E480u);
 }
 
-template <int D, bool KQ8, bool VQ8>
-__global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_kernel(const AttnParams p) {
+template <int D, bool KQ8, bool VQ8, bool TMA>
+__global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmap_k,
+                                                                                       const __grid_constant__ CUtensorMap tmap_v) {
   using G = DecodeGeom<D, KQ8, VQ8>;
   using KF = RowFmt<D, KQ8>;
   using VF = RowFmt<D, VQ8>;
@@ -303,7 +311,12 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
   float* ci = reinterpret_cast<float*>(smem + G::OFF_CI);
   int* flags = reinterpret_cast<int*>(smem + G::OFF_FLAGS);   // [0] bad inputs, [1] last CTA of the unit
 
+  const uint32_t bars = sbase + G::OFF_BARS + warp * (G::NST * 8);
   if (tid == 0) flags[0] = 0;
+  if (TMA && lane == 0) {
+    for (int s = 0; s < G::NST; s++) ptx::mbar_init(bars + 8 * s, 1);
+    ptx::fence_barrier_init();
+  }
   __syncthreads();
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
@@ -330,62 +343,94 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
     if (col_row[c] != NO_ROW) all_lo = max(all_lo, lo), all_hi = min(all_hi, hi);
   }
   u_lo = min(u_lo, u_hi);
-  uint32_t per = (u_hi - u_lo + p.splits - 1) / p.splits;
+  // Slices begin on multiples of a tile, so that none straddles a page or a ring's end that is one.
+  const uint32_t base = u_lo / TK * TK;
+  uint32_t per = (u_hi - base + p.splits - 1) / p.splits;
   per = (per + TK - 1) / TK * TK;
-  const uint32_t my_lo = (uint32_t)min((uint64_t)u_hi, u_lo + (uint64_t)split * per);
+  const uint32_t my_lo = (uint32_t)min((uint64_t)u_hi, base + (uint64_t)split * per);
   const uint32_t my_hi = (uint32_t)min((uint64_t)u_hi, (uint64_t)my_lo + per);
   const uint32_t tiles = (my_hi - my_lo + TK - 1) / TK;
 
   // ---- the warp's copies: tile i of the CTA's slice, into stage (i / WARPS) % NST of its ring
-  CacheGeom geom = geom_of(p);
-  const uint32_t bq = p.page_table ? b : 0;
-  const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + (row0 * p.Hkv + hkv) * KF::BYTES;
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + (row0 * p.Hkv + hkv) * VF::BYTES;
+  const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;   // the request's first row, or the pool's
   const uint32_t ring = sbase + warp * (G::NST * G::STAGE);
   uint32_t* valid = reinterpret_cast<uint32_t*>(smem + G::OFF_VALID) + warp * G::NST;
-  // Row (below the request's first one, or in the pool) of this lane's key of a tile; its table entry is read a
-  // tile ahead of the copies.
-  auto find_row = [&](uint32_t tile, bool* there) -> uint32_t {
-    const uint32_t key = my_lo + tile * TK + (lane & 15);
-    *there = tile < tiles && key < my_hi;
-    if (!*there) return 0;
-    const int64_t r = cache_row(geom, bq, key);
-    if (r < 0) {
-      atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
-      *there = false;
-      return 0;
-    }
-    return (uint32_t)r;
+  // A box begins on a 16-byte boundary: the head's bytes are this far into each row.
+  const uint32_t kshift = TMA ? (hkv * KF::BYTES) & 15 : 0, vshift = TMA ? (hkv * VF::BYTES) & 15 : 0;
+  // Where a tile's rows lie. The page number is read a tile ahead of the copies and looked at only then.
+  struct Place {
+    int32_t page;      // raw entry of the page table; 0 where there is none
+    uint32_t in_page;  // row inside the page, or below row0
+    bool on;
   };
-  auto issue = [&](uint32_t stage, uint32_t row, bool there) {
-    const uint32_t mask = __ballot_sync(FULL, there) & 0xFFFFu;
-    if (lane == 0) valid[stage] = mask;
-    const uint32_t dst = ring + stage * G::STAGE;
-#pragma unroll
-    for (int i = 0; i < (TK * KF::CHUNKS + 31) / 32; i++) {
-      const uint32_t idx = lane + 32 * i, key = idx / KF::CHUNKS, c = idx - key * KF::CHUNKS;
-      const uint32_t r = __shfl_sync(FULL, row, key & 15);
-      if (idx < TK * KF::CHUNKS)
-        cp_async<KF::CHUNK>(dst + key * KF::PITCH + c * KF::CHUNK, kbase + (uint64_t)r * (p.Hkv * KF::BYTES) + c * KF::CHUNK, (mask >> key) & 1);
+  auto place = [&](uint32_t tile) -> Place {
+    const uint32_t key = my_lo + tile * TK + (TMA ? 0 : lane & 15);
+    Place at{0, 0, tile < tiles && key < my_hi};
+    if (at.on) {
+      if (p.page_table) {
+        const uint32_t pi = key / p.page_tokens;
+        at.page = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + pi);
+        at.in_page = key - pi * p.page_tokens;
+      } else {
+        at.in_page = p.rolling ? key % p.T : key;
+      }
     }
-    const uint32_t vdst = dst + TK * KF::PITCH;
+    return at;
+  };
+  auto issue = [&](uint32_t tile, uint32_t stage, const Place& at) {
+    bool there = at.on;
+    uint64_t row = at.in_page;
+    if (p.page_table) {
+      if (there && (at.page < 0 || (uint32_t)at.page >= p.pool_pages)) {
+        atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
+        there = false;
+      }
+      row += (uint64_t)(there ? at.page : 0) * p.page_tokens;
+    }
+    row += row0;
+    const uint32_t dst = ring + stage * G::STAGE, vdst = dst + TK * KF::PITCH;
+    if constexpr (TMA) {
+      if (lane == 0) {
+        valid[stage] = there ? 0xFFFFu : 0;
+        const uint32_t bar = bars + 8 * stage;
+        ptx::mbar_arrive_expect_tx(bar, there ? (uint32_t)G::STAGE : 0u);
+        if (there && !(p.drop_first && tile == (uint32_t)warp)) {
+          ptx::tma_load_2d(dst, &tmap_k, (int)((hkv * KF::BYTES) / 16 * 2), (int)row, bar);
+          ptx::tma_load_2d(vdst, &tmap_v, (int)((hkv * VF::BYTES) / 16 * 2), (int)row, bar);
+        }
+      }
+    } else {
+      const uint32_t mask = __ballot_sync(FULL, there) & 0xFFFFu;
+      if (lane == 0) valid[stage] = mask;
+      const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + hkv * KF::BYTES;
+      const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + hkv * VF::BYTES;
 #pragma unroll
-    for (int i = 0; i < (TK * VF::CHUNKS + 31) / 32; i++) {
-      const uint32_t idx = lane + 32 * i, key = idx / VF::CHUNKS, c = idx - key * VF::CHUNKS;
-      const uint32_t r = __shfl_sync(FULL, row, key & 15);
-      if (idx < TK * VF::CHUNKS)
-        cp_async<VF::CHUNK>(vdst + key * VF::PITCH + c * VF::CHUNK, vbase + (uint64_t)r * (p.Hkv * VF::BYTES) + c * VF::CHUNK, (mask >> key) & 1);
+      for (int i = 0; i < (TK * KF::CHUNKS + 31) / 32; i++) {
+        const uint32_t idx = lane + 32 * i, key = idx / KF::CHUNKS, c = idx - key * KF::CHUNKS;
+        const uint64_t r = __shfl_sync(FULL, row, key & 15);
+        if (idx < TK * KF::CHUNKS)
+          cp_async<KF::CHUNK>(dst + key * KF::PITCH + c * KF::CHUNK, kbase + r * (p.Hkv * KF::BYTES) + c * KF::CHUNK, (mask >> key) & 1);
+      }
+#pragma unroll
+      for (int i = 0; i < (TK * VF::CHUNKS + 31) / 32; i++) {
+        const uint32_t idx = lane + 32 * i, key = idx / VF::CHUNKS, c = idx - key * VF::CHUNKS;
+        const uint64_t r = __shfl_sync(FULL, row, key & 15);
+        if (idx < TK * VF::CHUNKS)
+          cp_async<VF::CHUNK>(vdst + key * VF::PITCH + c * VF::CHUNK, vbase + r * (p.Hkv * VF::BYTES) + c * VF::CHUNK, (mask >> key) & 1);
+      }
+      cp_commit();
     }
   };
-  const uint32_t mine = tiles > (uint32_t)warp ? (tiles - warp + WARPS - 1) / WARPS : 0;   // tiles of this warp
-  bool next_there;
-  uint32_t next_row = find_row(warp, &next_there);
+  uint32_t mine = tiles > (uint32_t)warp ? (tiles - warp + WARPS - 1) / WARPS : 0;   // tiles of this warp
+  Place next = place(warp);
 #pragma unroll
   for (int s = 0; s < G::NST - 1; s++) {
-    if ((uint32_t)s < mine) issue(s, next_row, next_there);
-    cp_commit();
-    if ((uint32_t)s < mine) next_row = find_row(warp + (s + 1) * WARPS, &next_there);
+    if ((uint32_t)s < mine) {
+      issue(warp + s * WARPS, s, next);
+      next = place(warp + (s + 1) * WARPS);
+    } else if (!TMA) {
+      cp_commit();
+    }
   }
 
   // ---- q: normed by the column's largest value to [2^13, 2^14), and the sums that offset q4_0 codes
@@ -457,19 +502,32 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
 
   for (uint32_t i = 0; i < mine; i++) {
     const uint32_t stage = i % G::NST;
-    {
-      const uint32_t ahead = i + G::NST - 1;
-      if (ahead < mine) {
-        issue(ahead % G::NST, next_row, next_there);
-        next_row = find_row(warp + (ahead + 1) * WARPS, &next_there);
-      }
+    const uint32_t ahead = i + G::NST - 1;
+    if (ahead < mine) {
+      issue(warp + ahead * WARPS, ahead % G::NST, next);
+      next = place(warp + (ahead + 1) * WARPS);
+    } else if (!TMA) {
       cp_commit();
     }
-    cp_wait<G::NST - 1>();
-    __syncwarp();
-    const uint32_t ks = ring + stage * G::STAGE, vst = ks + TK * KF::PITCH;
-    const uint32_t there = valid[stage];
+    if constexpr (TMA) {
+      __syncwarp();
+      const bool landed = ptx::mbar_wait_bounded(bars + 8 * stage, (i / G::NST) & 1, p.wait_limit);
+      if (!__all_sync(FULL, landed)) {
+        if (lane == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED);
+        // what is still under way lands before the ring is used for the merge
+        for (uint32_t j = i + 1; j < min(mine, i + (uint32_t)G::NST); j++) ptx::mbar_wait_bounded(bars + 8 * (j % G::NST), (j / G::NST) & 1, p.wait_limit);
+        break;
+      }
+    } else {
+      cp_wait<G::NST - 1>();
+      __syncwarp();
+    }
+    const uint32_t ks = ring + stage * G::STAGE + kshift, vst = ring + stage * G::STAGE + TK * KF::PITCH + vshift;
     const uint32_t key0 = my_lo + (warp + i * WARPS) * TK;
+    const uint32_t there = valid[stage];
+    // Some column does not see some row of the tile: what lies there (rows past the end, of other requests,
+    // whatever a page holds) must not reach it, not even as 0 x infinity.
+    const bool partial = there != 0xFFFFu || key0 < all_lo || key0 + TK > all_hi;
 
     // V scales of the tile as f32, times 2^(29 - E) of the largest exponent so far
     uint32_t sc[NB / 2], top = 0;
@@ -477,18 +535,18 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
     for (int j = 0; j < NB / 2; j++) {
       const uint32_t at = lane + 32 * j;     // (block, key)
       sc[j] = lds16(vst + (at & 15) * VF::PITCH + (at >> 4) * VF::BB);
-      const uint32_t mag = sc[j] & 0x7FFFu;
-      if (mag < 0x7C00u) top = max(top, mag);
+      const uint32_t mag = sc[j] & 0x7FFFu, key = key0 + (at & 15);
+      if (mag < 0x7C00u && (!partial || (key >= u_lo && key < u_hi))) top = max(top, mag);
     }
     const uint32_t e_new = max(e_run, __reduce_max_sync(FULL, top) >> 10);
     const float vmul = __uint_as_float((127u + 29u - e_new) << 23);
-    bool odd = false;
+    bool odd = partial;
 #pragma unroll
     for (int j = 0; j < NB / 2; j++) {
       asm volatile("st.shared.f32 [%0], %1;" ::"r"(vs + (lane + 32 * j) * 4), "f"(half_bits(sc[j]) * vmul) : "memory");
       odd |= (sc[j] & 0x7FFFu) >= 0x7C00u;
     }
-    odd = __any_sync(FULL, odd);             // an infinite or NaN scale: its keys must not reach columns that do not see them
+    odd = __any_sync(FULL, odd);             // or an infinite or NaN scale
     __syncwarp();
 
     // S^T of 16 keys x 8 columns
@@ -552,7 +610,7 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
     }
 #pragma unroll
     for (int k = 0; k < 4; k++) y[k] = soft_cap_logit(y[k], p.soft_cap) * LOG2E;
-    if (there != 0xFFFFu || key0 < all_lo || key0 + TK > all_hi) {
+    if (partial) {
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const uint32_t kk = 2 * t + (k & 1) + 8 * (k >> 1), key = key0 + kk;
@@ -621,15 +679,20 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
           a[1][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
         }
       }
+      // The tensor core cuts its sums off instead of rounding them, always to the same side: over thousands of
+      // keys that adds up. So each tile is summed from zero and added in f32.
 #pragma unroll
       for (int m = 0; m < 2; m++) {
-        mma_f16(acc[2 * blk + m], a[m][0], a[m][1], a[m][2], a[m][3], bh[0], bh[1]);
-        mma_f16(acc[2 * blk + m], a[m][0], a[m][1], a[m][2], a[m][3], blw[0], blw[1]);
+        float o[4];
+        mma_f16_from(o, a[m][0], a[m][1], a[m][2], a[m][3], blw[0], blw[1], 0.0f, 0.0f, 0.0f, 0.0f);
+        mma_f16(o, a[m][0], a[m][1], a[m][2], a[m][3], bh[0], bh[1]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[2 * blk + m][e] += o[e];
       }
     }
     __syncwarp();   // the stage and the scales are free again
   }
-  cp_wait<0>();
+  if (!TMA) cp_wait<0>();
 
   // ---- the four warps' sums meet
   l_run += __shfl_xor_sync(FULL, l_run, 1);
@@ -742,10 +805,10 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
   }
 }
 
-template <int D, bool KQ8, bool VQ8>
-int32_t launch_decode(AionCudaDevice* dev, const AttnParams& p, uint32_t units) {
+template <int D, bool KQ8, bool VQ8, bool TMA>
+int32_t launch_decode_as(AionCudaDevice* dev, const AttnParams& p, uint32_t units, const CUtensorMap& tk, const CUtensorMap& tv) {
   using G = DecodeGeom<D, KQ8, VQ8>;
-  auto kernel = attn_qcache_decode_kernel<D, KQ8, VQ8>;
+  auto kernel = attn_qcache_decode_kernel<D, KQ8, VQ8, TMA>;
   {
     static std::mutex mu;   // once per device and instantiation
     static bool configured[64] = {};
@@ -756,8 +819,29 @@ int32_t launch_decode(AionCudaDevice* dev, const AttnParams& p, uint32_t units) 
     }
   }
   if (p.splits > (uint32_t)G::MAX_SPLITS) return fail(AION_CUDA_INTERNAL_ERROR, "attention: %u splits exceed the merge buffer", p.splits);
-  AION_CUDA_TRY(launch_pdl_main(kernel, dim3(units, p.splits), dim3(THREADS), G::SMEM, dev->stream, p));
+  AION_CUDA_TRY(launch_pdl_main(kernel, dim3(units, p.splits), dim3(THREADS), G::SMEM, dev->stream, p, tk, tv));
   return AION_CUDA_OK;
+}
+
+template <int D, bool KQ8, bool VQ8>
+int32_t launch_decode(AionCudaDevice* dev, const AttnParams& p, uint32_t units) {
+  using KF = RowFmt<D, KQ8>;
+  using VF = RowFmt<D, VQ8>;
+  const uint64_t rows = p.page_table ? (uint64_t)p.pool_pages * p.page_tokens : (uint64_t)p.B * p.T;
+  const uint64_t kw = (uint64_t)p.Hkv * KF::BYTES, vw = (uint64_t)p.Hkv * VF::BYTES;
+  // Boxes: 16-byte aligned rows, tiles of 16 rows that lie together.
+  const bool boxes = ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | kw | vw) & 15) == 0 && rows < (1ull << 31) &&
+                     (!p.page_table || p.page_tokens % TK == 0) && (!p.rolling || p.T % TK == 0);
+  CUtensorMap tk{}, tv{};
+  if (!boxes) return launch_decode_as<D, KQ8, VQ8, false>(dev, p, units, tk, tv);
+  const CUtensorMap* m;
+  const uint64_t kd[2] = {kw, rows}, vd[2] = {vw, rows};
+  const uint32_t kbox[2] = {KF::PITCH, TK}, vbox[2] = {VF::PITCH, TK};
+  if (int32_t st = tensor_map_bytes(dev, p.k, 2, kd, &kw, kbox, &m)) return st;
+  tk = *m;
+  if (int32_t st = tensor_map_bytes(dev, p.v, 2, vd, &vw, vbox, &m)) return st;
+  tv = *m;
+  return launch_decode_as<D, KQ8, VQ8, true>(dev, p, units, tk, tv);
 }
 
 }  // namespace

@@ -663,3 +663,36 @@ def test_a_prompt_then_tokens_then_the_way_out(sess, kdt, vdt, layout):
         want, bound = ref.attention(q, k, v, F32, F32, scale=0.088, positions=pos - lo, lengths=[held] * B)
         check(store.read(to), want, bound)
         done += n
+
+
+def test_an_expired_wait_is_reported_and_the_device_stays_usable(sess, backend):
+    """The kernel's copy barriers time out instead of hanging: with the test hook every warp leaves out its first copy."""
+    s, store = sess
+    q, k, v = inputs([12], 2, 200, 1, 128, 1, 8, Q8, Q8)
+    q, k, v = q, np.repeat(k, 2, 2), np.repeat(v, 2, 2)      # two kv heads: rows on 16-byte boundaries
+    want, step = run_attention(sess, q, k, v, Q8, Q8, scale=0.1)
+    lib = backend._lib
+    assert lib.aion_cuda_debug_expire_waits(backend.handle, 1) == capi.OK
+    try:
+        s.execute([step])
+        with pytest.raises(BackendError) as e:
+            backend.sync()
+        assert e.value.name == "ExecutionFailed"
+    finally:
+        lib.aion_cuda_debug_expire_waits(backend.handle, 0)
+    s.execute([step])
+    assert np.array_equal(store.read(step.out), want)
+
+
+@pytest.mark.parametrize("layout,page,T", [("plain", 0, 96), ("rolling", 0, 96), ("rolling", 0, 90), ("paged", 32, 96), ("paged", 40, 96)])
+@pytest.mark.parametrize("H", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("kdt,vdt", [(Q8, Q4), (Q4, Q8)])
+def test_rows_on_and_off_sixteen_byte_boundaries(sess, layout, page, T, H, D, kdt, vdt):
+    """Head counts and sizes whose rows begin on 16-byte boundaries and others, whole and ragged rings and pages."""
+    B = 3
+    q, k, v = inputs([H, D, T], B, T, H, D, 1, 2 * H, kdt, vdt)
+    lens = [T + 37, T, 50] if layout == "rolling" else [T, 1, 50]
+    pos = np.array([[n - 1] for n in lens], dtype=np.int32)
+    got, _ = run_attention(sess, q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, layout=layout, page=page, window=AttentionWindow.causal())
+    check(got, *ref.attention(q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, rolling=layout == "rolling"))
