@@ -7,6 +7,7 @@
 // over the keys [lo, hi) of the row's window; zeros for an empty range. The codes are exact in any float type
 // and the scales in f32, so only the f32 sums round: the result is f32 attention over the dequantized cache.
 #include <mutex>
+#include <type_traits>
 
 #include "attention_device.cuh"
 #include "cache_geom.cuh"
@@ -169,39 +170,30 @@ struct DecodeGeom {
   using K = RowFmt<D, KQ8>;
   using V = RowFmt<D, VQ8>;
   static constexpr int STAGE = TK * (K::PITCH + V::PITCH);
-  // Two CTAs an SM for D = 256 (registers), three below: 100 / 66 KB of ring each.
-  static constexpr int NST_MAX = (D == 256 ? 92 : 60) * 1024 / (WARPS * STAGE);
-  static constexpr int NST = NST_MAX > 8 ? 8 : NST_MAX;
+  // CTAs an SM: two for D = 256 (registers), three below. STAGES_FIT: what their shares of shared memory hold.
+  static constexpr int CTAS = D == 256 ? 2 : 3;
+  static constexpr int STAGES_FIT = (D == 256 ? 95 : 63) * 1024 / (WARPS * STAGE);
+  static constexpr int NST = STAGES_FIT > 8 ? 8 : STAGES_FIT;
+  // Tiles that an iteration takes together (the softmax, the waits and the f32 additions are paid once for them):
+  // two where the ring then still holds two more.
+  static constexpr int TPI = NST >= 4 ? 2 : 1;
+  static constexpr int AHEAD = NST - TPI;            // tiles under way while an iteration computes
   static constexpr int WS = COLS * D + 2 * COLS;     // floats of a warp's result: sums, maxima, weights
   static constexpr int RING = WARPS * NST * STAGE;
   static_assert(NST >= 2 && WARPS * WS * 4 <= RING, "ring");
-  static constexpr int OFF_VS = RING;                                  // f32 [warp][block][16 keys]: V scales
-  static constexpr int OFF_Q = OFF_VS + WARPS * (D / QK) * TK * 4;     // f32 [8][D]: q, normed
-  static constexpr int OFF_CI = OFF_Q + COLS * D * 4;                  // f32 [block][8]: -8 sum q
-  static constexpr int OFF_META = OFF_CI + D / QK * COLS * 4;          // per column: row, first key, key end, output row, head, factor
-  static constexpr int OFF_VALID = OFF_META + COLS * 24;               // per warp and stage: which keys are there
-  static constexpr int OFF_BARS = (OFF_VALID + WARPS * NST * 4 + 7) / 8 * 8;   // per warp and stage: the copies' barrier
+  static constexpr int OFF_VS = RING;                                        // f32 [warp][block][keys of an iteration]: V scales
+  static constexpr int OFF_Q = OFF_VS + WARPS * (D / QK) * TK * TPI * 4;     // uint4 [D / 16][32]: Q fragments; first f32 [8][D]: q
+  static constexpr int OFF_CI = OFF_Q + COLS * D * 4;                        // f32 [block][8]: -8 sum q
+  static constexpr int OFF_META = OFF_CI + D / QK * COLS * 4;                // per column: row, first key, key end, output row, head, factor
+  static constexpr int OFF_VALID = OFF_META + COLS * 24;                     // per warp and stage: which keys are there
+  static constexpr int OFF_BARS = (OFF_VALID + WARPS * NST * 4 + 7) / 8 * 8; // per warp and stage: the copies' barrier
   static constexpr int OFF_FLAGS = OFF_BARS + WARPS * NST * 8;
   static constexpr int SMEM = OFF_FLAGS + 32;
+  static_assert(CTAS * (SMEM + 1024) <= 227 * 1024, "shared memory of an SM");
   static constexpr int MAX_SPLITS = 128;
   static_assert(MAX_SPLITS * COLS * 8 + COLS * 4 <= RING, "factors of the merge");
 };
 
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ float2 lds_f2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
-  return v;
-}
 template <int BYTES>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool there) {
   const int n = there ? BYTES : 0;   // nothing is read and zeros are written where the key is not there
@@ -221,10 +213,14 @@ __device__ __forceinline__ uint32_t movm(uint32_t a) {
 // D = A . B + C with a C of its own.
 __device__ __forceinline__ void mma_f16_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                                              float c0, float c1, float c2, float c3) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ float ex2(float x) {   // 2^x to 2 units in the last place; 0 for -infinity
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ float half_bits(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
 __device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
@@ -258,12 +254,6 @@ __host__ __device__ constexpr int pair_byte(bool q8, bool second, int u, int j) 
   return second ? 4 * u + j : u ? 4 * u - 2 + j : j < 2 ? j : n - 4 + j;
 }
 
-// The A operand of 16 keys x 32 dimensions: two MMAs' worth, from the words of key rows g and g + 8.
-template <bool Q8>
-struct KFrag {
-  uint32_t a[2][4];
-  uint32_t scale_lo, scale_hi;   // f16 bits for keys g, g + 8
-};
 __device__ __forceinline__ void unpack_q4_subnormal(uint32_t w, uint32_t (&x)[4]) {
   x[0] = w & 0x000F000Fu;        // n * 2^-24
   x[1] = w & 0x00F000F0u;        // n * 2^-20
@@ -279,7 +269,7 @@ __device__ __forceinline__ void unpack_q8(uint32_t w, uint32_t* r0, uint32_t* r1
 }
 
 template <int D, bool KQ8, bool VQ8, bool TMA>
-__global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmap_k,
+__global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_qcache_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmap_k,
                                                                                        const __grid_constant__ CUtensorMap tmap_v) {
   using G = DecodeGeom<D, KQ8, VQ8>;
   using KF = RowFmt<D, KQ8>;
@@ -287,6 +277,9 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
   constexpr int NB = D / QK;          // blocks of a head row
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sbase = ptx::smem_u32(smem);
+  auto lds32 = [&](uint32_t at) { return *reinterpret_cast<const uint32_t*>(smem + at); };
+  auto lds16 = [&](uint32_t at) { return (uint32_t)*reinterpret_cast<const uint16_t*>(smem + at); };
+  auto lds_f2 = [&](uint32_t at) { return *reinterpret_cast<const float2*>(smem + at); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
 
@@ -320,6 +313,19 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
   __syncthreads();
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
+  // This warp's two columns of q are on their way while the ranges are worked out.
+  float qv[COLS / WARPS][D / 32];
+#pragma unroll
+  for (int j = 0; j < COLS / WARPS; j++) {
+    const uint32_t c = warp + j * WARPS, pl = c / p.col_heads, hh = c - pl * p.col_heads, l = l0 + pl;
+    const bool on = pl < p.pos_per_tile && hh < nh && l < p.L;
+    const uint64_t at = ((uint64_t)(b * p.L + l) * p.Hq + h0 + hh) * D + lane;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      qv[j][i] = 0.0f;
+      if (on) qv[j][i] = p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at + 32 * i] : __half2float(static_cast<const __half*>(p.q)[at + 32 * i]);
+    }
+  }
   if (tid < COLS) {
     const uint32_t pl = tid / p.col_heads, hh = tid - pl * p.col_heads, l = l0 + pl;
     uint32_t row = NO_ROW, lo = 0, hi = 0;
@@ -351,9 +357,9 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
   const uint32_t my_hi = (uint32_t)min((uint64_t)u_hi, (uint64_t)my_lo + per);
   const uint32_t tiles = (my_hi - my_lo + TK - 1) / TK;
 
-  // ---- the warp's copies: tile i of the CTA's slice, into stage (i / WARPS) % NST of its ring
+  // ---- the warp's copies. Its n-th tile is one of TPI neighbours; the warps take such groups in turn.
   const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;   // the request's first row, or the pool's
-  const uint32_t ring = sbase + warp * (G::NST * G::STAGE);
+  const uint32_t ring = warp * (G::NST * G::STAGE);   // offsets into shared memory
   uint32_t* valid = reinterpret_cast<uint32_t*>(smem + G::OFF_VALID) + warp * G::NST;
   // A box begins on a 16-byte boundary: the head's bytes are this far into each row.
   const uint32_t kshift = TMA ? (hkv * KF::BYTES) & 15 : 0, vshift = TMA ? (hkv * VF::BYTES) & 15 : 0;
@@ -363,21 +369,30 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
     uint32_t in_page;  // row inside the page, or below row0
     bool on;
   };
-  auto place = [&](uint32_t tile) -> Place {
-    const uint32_t key = my_lo + tile * TK + (TMA ? 0 : lane & 15);
+  auto tile_of = [&](uint32_t n) { return ((n / G::TPI) * WARPS + warp) * G::TPI + n % G::TPI; };
+  // (The page of the next tile is found by counting on from the last one: a division costs as much as a block of keys.)
+  uint32_t page_index = 0, page_key = 0;   // page of the last tile that was placed, and its first key
+  if (p.page_table) {
+    const uint32_t key = my_lo + tile_of(0) * TK + (TMA ? 0 : lane & 15);
+    page_index = key / p.page_tokens;
+    page_key = page_index * p.page_tokens;
+  }
+  auto place = [&](uint32_t n) -> Place {
+    const uint32_t tile = tile_of(n), key = my_lo + tile * TK + (TMA ? 0 : lane & 15);
     Place at{0, 0, tile < tiles && key < my_hi};
     if (at.on) {
       if (p.page_table) {
-        const uint32_t pi = key / p.page_tokens;
-        at.page = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + pi);
-        at.in_page = key - pi * p.page_tokens;
+        while (key - page_key >= p.page_tokens) page_index++, page_key += p.page_tokens;
+        at.page = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + page_index);
+        at.in_page = key - page_key;
       } else {
         at.in_page = p.rolling ? key % p.T : key;
       }
     }
     return at;
   };
-  auto issue = [&](uint32_t tile, uint32_t stage, const Place& at) {
+  auto issue = [&](uint32_t n, const Place& at) {
+    const uint32_t stage = n % G::NST;
     bool there = at.on;
     uint64_t row = at.in_page;
     if (p.page_table) {
@@ -388,13 +403,13 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
       row += (uint64_t)(there ? at.page : 0) * p.page_tokens;
     }
     row += row0;
-    const uint32_t dst = ring + stage * G::STAGE, vdst = dst + TK * KF::PITCH;
+    const uint32_t dst = sbase + ring + stage * G::STAGE, vdst = dst + TK * KF::PITCH;
     if constexpr (TMA) {
       if (lane == 0) {
         valid[stage] = there ? 0xFFFFu : 0;
         const uint32_t bar = bars + 8 * stage;
         ptx::mbar_arrive_expect_tx(bar, there ? (uint32_t)G::STAGE : 0u);
-        if (there && !(p.drop_first && tile == (uint32_t)warp)) {
+        if (there && !(p.drop_first && n == 0)) {
           ptx::tma_load_2d(dst, &tmap_k, (int)((hkv * KF::BYTES) / 16 * 2), (int)row, bar);
           ptx::tma_load_2d(vdst, &tmap_v, (int)((hkv * VF::BYTES) / 16 * 2), (int)row, bar);
         }
@@ -421,74 +436,90 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
       cp_commit();
     }
   };
-  uint32_t mine = tiles > (uint32_t)warp ? (tiles - warp + WARPS - 1) / WARPS : 0;   // tiles of this warp
-  Place next = place(warp);
+  const uint32_t groups = (tiles + G::TPI - 1) / G::TPI;
+  const uint32_t iters = groups > (uint32_t)warp ? (groups - warp + WARPS - 1) / WARPS : 0;
+  const uint32_t mine = iters * G::TPI;   // the last of them may lie behind the end: no key of it is there
+  Place next = place(0);
 #pragma unroll
-  for (int s = 0; s < G::NST - 1; s++) {
-    if ((uint32_t)s < mine) {
-      issue(warp + s * WARPS, s, next);
-      next = place(warp + (s + 1) * WARPS);
+  for (int n = 0; n < G::AHEAD; n++) {
+    if ((uint32_t)n < mine) {
+      issue(n, next);
+      next = place(n + 1);
     } else if (!TMA) {
       cp_commit();
     }
   }
 
   // ---- q: normed by the column's largest value to [2^13, 2^14), and the sums that offset q4_0 codes
-  for (int c = warp; c < COLS; c += WARPS) {
-    float v[D / 32], top = 0.0f;
-    const uint32_t row = col_row[c];
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-      v[i] = 0.0f;
-      if (row != NO_ROW) {
-        const uint64_t at = (uint64_t)row * D + lane + 32 * i;
-        v[i] = p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at] : __half2float(static_cast<const __half*>(p.q)[at]);
-      }
-      top = fmaxf(top, fabsf(v[i]));
-    }
+  for (int j = 0; j < COLS / WARPS; j++) {
+    const int c = warp + j * WARPS;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) top = fmaxf(top, fabsf(qv[j][i]));
     uint32_t e = __reduce_max_sync(FULL, __float_as_uint(top)) >> 23;     // biased exponent
     if (e == 255) e = 127;                                                // not finite: the logits will not be either
     e = max(e, 40u);                                                      // far below any logit that matters
     const float up = __uint_as_float((127u + 13u + 127u - e) << 23);      // 2^(13 - (e - 127)), e >= 40
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) qs[c * D + lane + 32 * i] = v[i] * up;
+    for (int i = 0; i < D / 32; i++) qs[c * D + lane + 32 * i] = qv[j][i] * up;
     if (lane == 0) col_factor[c] = p.scale * __uint_as_float((e - 13u) << 23);
   }
   __syncthreads();
   // Q^T as the B operand: this lane's column g, the dimensions of word t. Where a q4_0 code enters times 16, q
   // enters by 16 less.
-  uint32_t qh[D / 16][2], ql[D / 16][2];
+  // Every warp makes a part of the fragments for all.
+  uint4 made[NB / WARPS > 0 ? NB / WARPS : 1][2];
 #pragma unroll
-  for (int blk = 0; blk < NB; blk++) {
-    float part = 0.0f;
+  for (int j = 0; j < (NB + WARPS - 1) / WARPS; j++) {
+    const int blk = warp + j * WARPS;
+    if (blk < NB) {
+      float part = 0.0f;
 #pragma unroll
-    for (int m = 0; m < 2; m++)
+      for (int m = 0; m < 2; m++) {
+        uint32_t hl[2][2];
 #pragma unroll
-      for (int r = 0; r < 2; r++) {
-        float x[2];
+        for (int r = 0; r < 2; r++) {
+          float x[2];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          int dim;
-          if (KQ8) dim = pair_byte(true, blk & 1, t + 4 * m, 2 * r + h);
-          else dim = 2 * pair_byte(false, blk & 1, t, m + 2 * h) + r;      // nibbles (2m + r, 2m + r + 4): bytes m, m + 2
-          x[h] = qs[g * D + blk * QK + dim] * (!KQ8 && r ? 0.0625f : 1.0f);
+          for (int h = 0; h < 2; h++) {
+            int dim;
+            if (KQ8) dim = pair_byte(true, blk & 1, t + 4 * m, 2 * r + h);
+            else dim = 2 * pair_byte(false, blk & 1, t, m + 2 * h) + r;      // nibbles (2m + r, 2m + r + 4): bytes m, m + 2
+            x[h] = qs[g * D + blk * QK + dim] * (!KQ8 && r ? 0.0625f : 1.0f);
+          }
+          split2(x[0], x[1], &hl[0][r], &hl[1][r]);
+          if (!KQ8) {
+            const float2 a = __half22float2(*reinterpret_cast<__half2*>(&hl[0][r])), c = __half22float2(*reinterpret_cast<__half2*>(&hl[1][r]));
+            part += ((a.x + c.x) + (a.y + c.y)) * (r ? 16.0f : 1.0f);
+          }
         }
-        uint32_t hi, lo;
-        split2(x[0], x[1], &hi, &lo);
-        qh[2 * blk + m][r] = hi, ql[2 * blk + m][r] = lo;
-        if (!KQ8) {
-          const float2 a = __half22float2(*reinterpret_cast<__half2*>(&hi)), c = __half22float2(*reinterpret_cast<__half2*>(&lo));
-          part += ((a.x + c.x) + (a.y + c.y)) * (r ? 16.0f : 1.0f);
-        }
+        made[j][m] = make_uint4(hl[0][0], hl[0][1], hl[1][0], hl[1][1]);
       }
-    if (!KQ8) {
-      part += __shfl_xor_sync(FULL, part, 1);
-      part += __shfl_xor_sync(FULL, part, 2);
-      if (warp == 0 && t == 0) ci[blk * COLS + g] = part * (-8.0f * 5.9604644775390625e-8f);   // -8 * 2^-24
+      if (!KQ8) {
+        part += __shfl_xor_sync(FULL, part, 1);
+        part += __shfl_xor_sync(FULL, part, 2);
+        if (t == 0) ci[blk * COLS + g] = part * (-8.0f * 5.9604644775390625e-8f);   // -8 * 2^-24
+      }
     }
   }
-  if (!KQ8) __syncthreads();
-  const float f0 = col_factor[2 * t], f1 = col_factor[2 * t + 1];
+  __syncthreads();   // q has been read: the fragments take its place
+  uint4* qfrag = reinterpret_cast<uint4*>(smem + G::OFF_Q);
+#pragma unroll
+  for (int j = 0; j < (NB + WARPS - 1) / WARPS; j++) {
+    const int blk = warp + j * WARPS;
+    if (blk < NB) qfrag[(2 * blk) * 32 + lane] = made[j][0], qfrag[(2 * blk + 1) * 32 + lane] = made[j][1];
+  }
+  __syncthreads();
+  uint32_t qh[D / 16][2], ql[D / 16][2];
+#pragma unroll
+  for (int i = 0; i < D / 16; i++) {
+    const uint4 f = qfrag[i * 32 + lane];
+    qh[i][0] = f.x, qh[i][1] = f.y, ql[i][0] = f.z, ql[i][1] = f.w;
+  }
+  // With a soft cap the logits are wanted first; else they go straight to base 2.
+  const float to_base2 = p.soft_cap > 0.0f ? 1.0f : LOG2E;
+  const float f0 = col_factor[2 * t] * to_base2, f1 = col_factor[2 * t + 1] * to_base2;
   const uint32_t lo_g = col_lo[g], hi_g = col_hi[g];
 
   float acc[D / 16][4];
@@ -498,199 +529,226 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
     for (int e = 0; e < 4; e++) acc[i][e] = 0.0f;
   float m_run = -INFINITY, l_run = 0.0f;     // column g; l_run: this lane's keys only
   uint32_t e_run = 0;                        // exponent field of the largest V scale so far
-  const uint32_t vs = sbase + G::OFF_VS + warp * (NB * TK * 4);
+  constexpr int TPI = G::TPI, KI = TK * TPI;     // keys of an iteration
+  const uint32_t vs = G::OFF_VS + warp * (NB * KI * 4);
+  const uint32_t first_sel = t ? 0x3210u : 0x5432u, first_sel_v = g ? 0x3210u : 0x5432u;
 
-  for (uint32_t i = 0; i < mine; i++) {
-    const uint32_t stage = i % G::NST;
-    const uint32_t ahead = i + G::NST - 1;
-    if (ahead < mine) {
-      issue(warp + ahead * WARPS, ahead % G::NST, next);
-      next = place(warp + (ahead + 1) * WARPS);
-    } else if (!TMA) {
-      cp_commit();
+  for (uint32_t it = 0; it < iters; it++) {
+    // ---- the tiles of this iteration; those AHEAD of it set out
+#pragma unroll
+    for (int j = 0; j < TPI; j++) {
+      const uint32_t n = it * TPI + G::AHEAD + j;
+      if (n < mine) {
+        issue(n, next);
+        next = place(n + 1);
+      } else if (!TMA) {
+        cp_commit();
+      }
     }
     if constexpr (TMA) {
       __syncwarp();
-      const bool landed = ptx::mbar_wait_bounded(bars + 8 * stage, (i / G::NST) & 1, p.wait_limit);
+      bool landed = true;
+#pragma unroll
+      for (int j = 0; j < TPI; j++) {
+        const uint32_t n = it * TPI + j;
+        landed = landed && ptx::mbar_wait_bounded(bars + 8 * (n % G::NST), (n / G::NST) & 1, p.wait_limit);
+      }
       if (!__all_sync(FULL, landed)) {
         if (lane == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED);
         // what is still under way lands before the ring is used for the merge
-        for (uint32_t j = i + 1; j < min(mine, i + (uint32_t)G::NST); j++) ptx::mbar_wait_bounded(bars + 8 * (j % G::NST), (j / G::NST) & 1, p.wait_limit);
+        for (uint32_t n = it * TPI; n < min(mine, it * TPI + (uint32_t)G::NST); n++) ptx::mbar_wait_bounded(bars + 8 * (n % G::NST), (n / G::NST) & 1, p.wait_limit);
         break;
       }
     } else {
-      cp_wait<G::NST - 1>();
+      cp_wait<G::AHEAD>();
       __syncwarp();
     }
-    const uint32_t ks = ring + stage * G::STAGE + kshift, vst = ring + stage * G::STAGE + TK * KF::PITCH + vshift;
-    const uint32_t key0 = my_lo + (warp + i * WARPS) * TK;
-    const uint32_t there = valid[stage];
-    // Some column does not see some row of the tile: what lies there (rows past the end, of other requests,
-    // whatever a page holds) must not reach it, not even as 0 x infinity.
-    const bool partial = there != 0xFFFFu || key0 < all_lo || key0 + TK > all_hi;
-
-    // V scales of the tile as f32, times 2^(29 - E) of the largest exponent so far
-    uint32_t sc[NB / 2], top = 0;
+    const uint32_t key0 = my_lo + tile_of(it * TPI) * TK;
+    uint32_t at[TPI], there = 0;   // offset of a tile's K rows; which keys are there
 #pragma unroll
-    for (int j = 0; j < NB / 2; j++) {
-      const uint32_t at = lane + 32 * j;     // (block, key)
-      sc[j] = lds16(vst + (at & 15) * VF::PITCH + (at >> 4) * VF::BB);
-      const uint32_t mag = sc[j] & 0x7FFFu, key = key0 + (at & 15);
-      if (mag < 0x7C00u && (!partial || (key >= u_lo && key < u_hi))) top = max(top, mag);
+    for (int j = 0; j < TPI; j++) {
+      const uint32_t stage = (it * TPI + j) % G::NST;
+      at[j] = ring + stage * G::STAGE;
+      there |= valid[stage] << (TK * j);
+    }
+    // Some column does not see some row of the tiles: what lies there (rows past the end, of other requests,
+    // whatever a page holds) must not reach it, not even as 0 x infinity.
+    const bool partial = there != (TPI == 2 ? 0xFFFFFFFFu : 0xFFFFu) || key0 < all_lo || key0 + KI > all_hi;
+
+    // ---- V scales as f32, times 2^(29 - E) of the largest exponent so far
+    uint32_t sc[NB * KI / 32], top = 0;
+#pragma unroll
+    for (int j = 0; j < NB * KI / 32; j++) {
+      const uint32_t e = lane + 32 * j, blk = e / KI, k = e % KI;
+      sc[j] = lds16(at[TPI == 2 ? (k >> 4) : 0] + TK * KF::PITCH + vshift + (k & 15) * VF::PITCH + blk * VF::BB);
+      const uint32_t mag = sc[j] & 0x7FFFu, key = key0 + k;
+      if (mag < 0x7C00u && (!partial || (((there >> k) & 1) && key >= u_lo && key < u_hi))) top = max(top, mag);   // keys that some column sees
     }
     const uint32_t e_new = max(e_run, __reduce_max_sync(FULL, top) >> 10);
     const float vmul = __uint_as_float((127u + 29u - e_new) << 23);
     bool odd = partial;
 #pragma unroll
-    for (int j = 0; j < NB / 2; j++) {
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(vs + (lane + 32 * j) * 4), "f"(half_bits(sc[j]) * vmul) : "memory");
+    for (int j = 0; j < NB * KI / 32; j++) {
+      *reinterpret_cast<float*>(smem + vs + (lane + 32 * j) * 4) = half_bits(sc[j]) * vmul;
       odd |= (sc[j] & 0x7FFFu) >= 0x7C00u;
     }
     odd = __any_sync(FULL, odd);             // or an infinite or NaN scale
     __syncwarp();
 
-    // S^T of 16 keys x 8 columns
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // ---- S^T: 16 keys x 8 columns for each tile
+    float s[TPI][4];
+#pragma unroll
+    for (int j = 0; j < TPI; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
 #pragma unroll
     for (int pr = 0; pr < NB / 2; pr++) {
-      uint32_t a[2][2][4];                   // [block of the pair][MMA][operand]
-      float sl[2], sh[2];                    // scales of keys g, g + 8
+      float2 init[2];
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const uint32_t row = ks + (g + 8 * half) * KF::PITCH + pr * 2 * KF::BB;
-        const uint32_t w0 = lds32(row);
-        if (KQ8) {
-          const uint32_t w8 = lds32(row + 32), wt = lds32(row + 4 * t), wu = lds32(row + 16 + 4 * t);
-          const uint32_t x0 = lds32(row + 36 + 4 * t), x1 = lds32(row + 52 + 4 * t);
-          const uint32_t first = t ? wt : __byte_perm(w0, w8, 0x5432);
-          unpack_q8(first, &a[0][0][half], &a[0][0][2 + half]);
-          unpack_q8(wu, &a[0][1][half], &a[0][1][2 + half]);
-          unpack_q8(x0, &a[1][0][half], &a[1][0][2 + half]);
-          unpack_q8(x1, &a[1][1][half], &a[1][1][2 + half]);
-          (half ? sh : sl)[0] = half_bits(w0 & 0xFFFFu), (half ? sh : sl)[1] = half_bits(w8 >> 16);
-        } else {
-          const uint32_t w4 = lds32(row + 16), wt = lds32(row + 4 * t), x0 = lds32(row + 20 + 4 * t);
-          const uint32_t first = t ? wt : __byte_perm(w0, w4, 0x5432);
-          uint32_t u[4];
-          unpack_q4_subnormal(first, u);
-          a[0][0][half] = u[0], a[0][0][2 + half] = u[1], a[0][1][half] = u[2], a[0][1][2 + half] = u[3];
-          unpack_q4_subnormal(x0, u);
-          a[1][0][half] = u[0], a[1][0][2 + half] = u[1], a[1][1][half] = u[2], a[1][1][2 + half] = u[3];
-          (half ? sh : sl)[0] = half_bits(w0 & 0xFFFFu), (half ? sh : sl)[1] = half_bits(w4 >> 16);
+      for (int k = 0; k < 2; k++) init[k] = KQ8 ? make_float2(0.0f, 0.0f) : lds_f2(G::OFF_CI + ((2 * pr + k) * COLS + 2 * t) * 4);
+#pragma unroll
+      for (int j = 0; j < TPI; j++) {
+        uint32_t a[2][2][4];                   // [block of the pair][MMA][operand]
+        float sl[2], sh[2];                    // scales of keys g, g + 8
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const uint32_t row = at[j] + kshift + (g + 8 * half) * KF::PITCH + pr * 2 * KF::BB;
+          const uint32_t w0 = lds32(row), wm = lds32(row + (KQ8 ? 32 : 16)), wt = lds32(row + 4 * t);
+          const uint32_t first = __byte_perm(wt, wm, first_sel);
+          if (KQ8) {
+            unpack_q8(first, &a[0][0][half], &a[0][0][2 + half]);
+            unpack_q8(lds32(row + 16 + 4 * t), &a[0][1][half], &a[0][1][2 + half]);
+            unpack_q8(lds32(row + 36 + 4 * t), &a[1][0][half], &a[1][0][2 + half]);
+            unpack_q8(lds32(row + 52 + 4 * t), &a[1][1][half], &a[1][1][2 + half]);
+          } else {
+            uint32_t u[4];
+            unpack_q4_subnormal(first, u);
+            a[0][0][half] = u[0], a[0][0][2 + half] = u[1], a[0][1][half] = u[2], a[0][1][2 + half] = u[3];
+            unpack_q4_subnormal(lds32(row + 20 + 4 * t), u);
+            a[1][0][half] = u[0], a[1][0][2 + half] = u[1], a[1][1][half] = u[2], a[1][1][2 + half] = u[3];
+          }
+          (half ? sh : sl)[0] = half_bits(w0 & 0xFFFFu), (half ? sh : sl)[1] = half_bits(wm >> 16);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const int q = 2 * (2 * pr + k);
+          float c[4];
+          mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], ql[q][0], ql[q][1], init[k].x, init[k].y, init[k].x, init[k].y);
+          mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], ql[q + 1][0], ql[q + 1][1], c[0], c[1], c[2], c[3]);
+          mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], qh[q][0], qh[q][1], c[0], c[1], c[2], c[3]);
+          mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], qh[q + 1][0], qh[q + 1][1], c[0], c[1], c[2], c[3]);
+          s[j][0] = fmaf(sl[k], c[0], s[j][0]);
+          s[j][1] = fmaf(sl[k], c[1], s[j][1]);
+          s[j][2] = fmaf(sh[k], c[2], s[j][2]);
+          s[j][3] = fmaf(sh[k], c[3], s[j][3]);
         }
       }
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const int blk = 2 * pr + k;
-        float c[4];
-        float2 init = make_float2(0.0f, 0.0f);
-        if (!KQ8) init = lds_f2(sbase + G::OFF_CI + (blk * COLS + 2 * t) * 4);
-        mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], qh[2 * blk][0], qh[2 * blk][1], init.x, init.y, init.x, init.y);
-        mma_f16(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], qh[2 * blk + 1][0], qh[2 * blk + 1][1]);
-        mma_f16(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], ql[2 * blk][0], ql[2 * blk][1]);
-        mma_f16(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], ql[2 * blk + 1][0], ql[2 * blk + 1][1]);
-        s[0] = fmaf(sl[k], c[0], s[0]);
-        s[1] = fmaf(sl[k], c[1], s[1]);
-        s[2] = fmaf(sh[k], c[2], s[2]);
-        s[3] = fmaf(sh[k], c[3], s[3]);
-      }
     }
-    // logits, and their transpose: column g, keys 2t, 2t + 1, 2t + 8, 2t + 9
-    float y[4];
-    {
-      const float unit24 = KQ8 ? 1.0f : 16777216.0f;
-      s[0] = (s[0] * unit24) * f0, s[1] = (s[1] * unit24) * f1, s[2] = (s[2] * unit24) * f0, s[3] = (s[3] * unit24) * f1;
+    // ---- logits, and their transpose: column g, keys 2t, 2t + 1, 2t + 8, 2t + 9 of each tile
+    float y[4 * TPI];
+#pragma unroll
+    for (int j = 0; j < TPI; j++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const uint32_t u = __float_as_uint(s[2 * h]), w = __float_as_uint(s[2 * h + 1]);
+        float x0 = s[j][2 * h], x1 = s[j][2 * h + 1];
+        if (!KQ8) x0 *= 16777216.0f, x1 *= 16777216.0f;   // the codes' 2^24
+        const uint32_t u = __float_as_uint(x0 * f0), w = __float_as_uint(x1 * f1);
         const uint32_t low = movm(__byte_perm(u, w, 0x5410)), high = movm(__byte_perm(u, w, 0x7632));
-        y[2 * h] = __uint_as_float(__byte_perm(low, high, 0x5410));
-        y[2 * h + 1] = __uint_as_float(__byte_perm(low, high, 0x7632));
+        y[4 * j + 2 * h] = __uint_as_float(__byte_perm(low, high, 0x5410));
+        y[4 * j + 2 * h + 1] = __uint_as_float(__byte_perm(low, high, 0x7632));
       }
-    }
+    if (p.soft_cap > 0.0f)
 #pragma unroll
-    for (int k = 0; k < 4; k++) y[k] = soft_cap_logit(y[k], p.soft_cap) * LOG2E;
+      for (int k = 0; k < 4 * TPI; k++) y[k] = soft_cap_logit(y[k], p.soft_cap) * LOG2E;
     if (partial) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
+      for (int k = 0; k < 4 * TPI; k++) {
         const uint32_t kk = 2 * t + (k & 1) + 8 * (k >> 1), key = key0 + kk;
         if (!((there >> kk) & 1) || key < lo_g || key >= hi_g) y[k] = -INFINITY;
       }
     }
-    float m_new = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), m_run);
+    float m_new = m_run;
+#pragma unroll
+    for (int k = 0; k < 4 * TPI; k++) m_new = fmaxf(m_new, y[k]);
     m_new = fmaxf(m_new, __shfl_xor_sync(FULL, m_new, 1));
     m_new = fmaxf(m_new, __shfl_xor_sync(FULL, m_new, 2));
-    if (__any_sync(FULL, m_new > m_run) || e_new > e_run) {
-      const float alpha = m_new > m_run ? exp2f(m_run - m_new) : 1.0f;
+    if (__any_sync(FULL, m_new > m_run || e_new > e_run)) {
+      const float alpha = m_new > m_run ? ex2(m_run - m_new) : 1.0f;
       l_run *= alpha;
       const float down = __uint_as_float((127u + e_run - e_new) << 23);   // 2^(old - new)
       const float a0 = __shfl_sync(FULL, alpha, 8 * t) * down, a1 = __shfl_sync(FULL, alpha, 8 * t + 4) * down;
 #pragma unroll
-      for (int j = 0; j < D / 16; j++) acc[j][0] *= a0, acc[j][1] *= a1, acc[j][2] *= a0, acc[j][3] *= a1;
+      for (int i = 0; i < D / 16; i++) acc[i][0] *= a0, acc[i][1] *= a1, acc[i][2] *= a0, acc[i][3] *= a1;
       m_run = m_new;
       e_run = e_new;
     }
     const float m_safe = m_run == -INFINITY ? 0.0f : m_run;
-    float pr4[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) pr4[k] = exp2f(y[k] - m_safe);
-    l_run += (pr4[0] + pr4[1]) + (pr4[2] + pr4[3]);
+    for (int k = 0; k < 4 * TPI; k++) {
+      y[k] = ex2(y[k] - m_safe);
+      l_run += y[k];
+    }
 
-    // O^T += V^T . P'^T, block by block
+    // ---- O^T += V^T . P'^T, block by block. (Two copies of the loop: one without the selections, and without a
+    // branch that would keep the blocks' instructions apart.)
+    auto add_values = [&](auto select) {
 #pragma unroll
-    for (int blk = 0; blk < NB; blk++) {
-      const float2 v0 = lds_f2(vs + (blk * TK + 2 * t) * 4), v1 = lds_f2(vs + (blk * TK + 2 * t + 8) * 4);
-      float w[4] = {pr4[0] * v0.x, pr4[1] * v0.y, pr4[2] * v1.x, pr4[3] * v1.y};
-      if (odd)
+      for (int blk = 0; blk < NB; blk++) {
+        uint32_t bh[TPI][2], blw[TPI][2];
+        uint32_t a[TPI][2][4];   // [tile][row tile][operand]: rows g and g + 8, key pairs (2t, 2t + 1) and (2t + 8, 2t + 9)
 #pragma unroll
-        for (int k = 0; k < 4; k++) w[k] = pr4[k] == 0.0f ? 0.0f : w[k];
-      uint32_t bh[2], blw[2];
-      split2(w[0], w[1], &bh[0], &blw[0]);
-      split2(w[2], w[3], &bh[1], &blw[1]);
-      uint32_t a[2][4];   // [row tile][operand]: rows g and g + 8, key pairs (2t, 2t + 1) and (2t + 8, 2t + 9)
+        for (int j = 0; j < TPI; j++) {
 #pragma unroll
-      for (int kp = 0; kp < 2; kp++) {
-        const uint32_t row = vst + (2 * t + 8 * kp) * VF::PITCH;
-        if (VQ8) {
-          uint32_t x[2];
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const uint32_t at = row + h * VF::PITCH + (blk >> 1) * 2 * VF::BB;
-            if (blk & 1) x[h] = lds32(at + 36 + 4 * g);
-            else {
-              const uint32_t wg = lds32(at + 4 * g), w8 = lds32(at + 32);
-              x[h] = g ? wg : __byte_perm(wg, w8, 0x5432);
+          for (int kp = 0; kp < 2; kp++) {
+            const float2 v = lds_f2(vs + (blk * KI + j * TK + 2 * t + 8 * kp) * 4);
+            float w0 = y[4 * j + 2 * kp] * v.x, w1 = y[4 * j + 2 * kp + 1] * v.y;
+            if constexpr (decltype(select)::value) {
+              if (y[4 * j + 2 * kp] == 0.0f) w0 = 0.0f;
+              if (y[4 * j + 2 * kp + 1] == 0.0f) w1 = 0.0f;
             }
-            x[h] ^= 0x80808080u;
+            split2(w0, w1, &bh[j][kp], &blw[j][kp]);
+            const uint32_t row = at[j] + TK * KF::PITCH + vshift + (2 * t + 8 * kp) * VF::PITCH;
+            if (VQ8) {
+              uint32_t x[2];
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                const uint32_t pos = row + h * VF::PITCH + (blk >> 1) * 2 * VF::BB;
+                if (blk & 1) x[h] = lds32(pos + 36 + 4 * g);
+                else x[h] = __byte_perm(lds32(pos + 4 * g), lds32(pos + 32), first_sel_v);
+                x[h] ^= 0x80808080u;
+              }
+              const uint32_t lo2 = __byte_perm(x[0], x[1], 0x5140), hi2 = __byte_perm(x[0], x[1], 0x7362);
+              a[j][0][2 * kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4140), 0xE480E480u);
+              a[j][0][2 * kp + 1] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4342), 0xE480E480u);
+              a[j][1][2 * kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4140), 0xE480E480u);
+              a[j][1][2 * kp + 1] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4342), 0xE480E480u);
+            } else {
+              const uint32_t pos = row + blk * VF::BB + 2 + 2 * g;
+              uint32_t x = __byte_perm(lds16(pos), lds16(pos + VF::PITCH), 0x5410);
+              // 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n: both leave n - 8 exactly
+              a[j][0][2 * kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+              a[j][0][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+              x >>= 8;
+              a[j][1][2 * kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+              a[j][1][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+            }
           }
-          const uint32_t lo2 = __byte_perm(x[0], x[1], 0x5140), hi2 = __byte_perm(x[0], x[1], 0x7362);
-          a[0][2 * kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4140), 0xE480E480u);
-          a[0][2 * kp + 1] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4342), 0xE480E480u);
-          a[1][2 * kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4140), 0xE480E480u);
-          a[1][2 * kp + 1] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4342), 0xE480E480u);
-        } else {
-          const uint32_t at = row + blk * VF::BB + 2 + 2 * g;
-          uint32_t x = __byte_perm(lds16(at), lds16(at + VF::PITCH), 0x5410);
-          // 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n: both leave n - 8 exactly
-          a[0][2 * kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
-          a[0][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
-          x >>= 8;
-          a[1][2 * kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
-          a[1][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+        }
+        // The tensor core cuts its sums off instead of rounding them, always to the same side: over thousands of
+        // keys that adds up. So an iteration is summed from zero and added in f32.
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < TPI; j++) mma_f16_from(o, a[j][m][0], a[j][m][1], a[j][m][2], a[j][m][3], blw[j][0], blw[j][1], o[0], o[1], o[2], o[3]);
+#pragma unroll
+          for (int j = 0; j < TPI; j++) mma_f16_from(o, a[j][m][0], a[j][m][1], a[j][m][2], a[j][m][3], bh[j][0], bh[j][1], o[0], o[1], o[2], o[3]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[2 * blk + m][e] += o[e];
         }
       }
-      // The tensor core cuts its sums off instead of rounding them, always to the same side: over thousands of
-      // keys that adds up. So each tile is summed from zero and added in f32.
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-        float o[4];
-        mma_f16_from(o, a[m][0], a[m][1], a[m][2], a[m][3], blw[0], blw[1], 0.0f, 0.0f, 0.0f, 0.0f);
-        mma_f16(o, a[m][0], a[m][1], a[m][2], a[m][3], bh[0], bh[1]);
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[2 * blk + m][e] += o[e];
-      }
-    }
-    __syncwarp();   // the stage and the scales are free again
+    };
+    if (odd) add_values(std::true_type{});
+    else add_values(std::false_type{});
+    __syncwarp();   // the stages and the scales are free again
   }
   if (!TMA) cp_wait<0>();
 
@@ -781,27 +839,36 @@ __global__ void __launch_bounds__(THREADS, D == 256 ? 2 : 3) attn_qcache_decode_
     if (lane == 0) lsums[c] = lsum;
   }
   __syncthreads();
-#pragma unroll 1
-  for (int c = 0; c < C4; c++) {
-    const uint32_t idx4 = tid + c * THREADS, col = idx4 / (D / 4);
-    const bool on = col_row[col] != NO_ROW;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (on) {
-      const float* src = pu + (size_t)col * PP + 4 * d4;
-      for (uint32_t s0 = 0; s0 < p.splits; s0 += 8) {
-        float4 v[8];
+  // Every load of a thread's columns for four splits is on its way before the first is used: the trip to L2 is
+  // what this costs.
+  float4 o[C4];
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-          v[k] = s0 + k < p.splits ? __ldcg(reinterpret_cast<const float4*>(src + (size_t)(s0 + k) * COLS * PP)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int c = 0; c < C4; c++) o[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  constexpr int SI = 16 / C4;
+  for (uint32_t s0 = 0; s0 < p.splits; s0 += SI) {
+    float4 v[C4][SI];
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-          if (s0 + k < p.splits) {
-            const float f = fac[col * p.splits + s0 + k];
-            o.x += v[k].x * f, o.y += v[k].y * f, o.z += v[k].z * f, o.w += v[k].w * f;
-          }
+    for (int c = 0; c < C4; c++) {
+      const uint32_t col = (tid + c * THREADS) / (D / 4);
+#pragma unroll
+      for (int k = 0; k < SI; k++)
+        v[c][k] = s0 + k < p.splits && col_row[col] != NO_ROW ? __ldcg(reinterpret_cast<const float4*>(pu + ((size_t)(s0 + k) * COLS + col) * PP + 4 * d4))
+                                                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int c = 0; c < C4; c++) {
+      const uint32_t col = (tid + c * THREADS) / (D / 4);
+#pragma unroll
+      for (int k = 0; k < SI; k++) {
+        const float f = s0 + k < p.splits ? fac[col * p.splits + s0 + k] : 0.0f;
+        o[c].x += v[c][k].x * f, o[c].y += v[c][k].y * f, o[c].z += v[c][k].z * f, o[c].w += v[c][k].w * f;
       }
     }
-    finish_column<D>(p, o, lsums[col], on, col_hi[col] > col_lo[col], col, d4, col_row, col_orow, col_head, !flags[0]);
+  }
+#pragma unroll
+  for (int c = 0; c < C4; c++) {
+    const uint32_t col = (tid + c * THREADS) / (D / 4);
+    finish_column<D>(p, o[c], lsums[col], col_row[col] != NO_ROW, col_hi[col] > col_lo[col], col, d4, col_row, col_orow, col_head, !flags[0]);
   }
 }
 
@@ -865,8 +932,8 @@ int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p, uint32_t fla
     uint64_t max_keys = p.T;
     const uint64_t span = (uint64_t)(p.win_chunk ? p.win_chunk : 1) + p.win_left + p.win_right + p.pos_per_tile;
     if (p.win_left != AION_CUDA_WINDOW_UNBOUNDED && p.win_right != AION_CUDA_WINDOW_UNBOUNDED && span < max_keys) max_keys = span;
-    const uint64_t resident = (uint64_t)dev->sm_count * (p.Dk == 256 ? 2 : 3);
-    uint64_t splits = resident / units, most = (max_keys + TK * WARPS - 1) / (TK * WARPS);
+    const uint64_t resident = (uint64_t)dev->sm_count * (p.Dk == 256 ? 2 : 3);   // DecodeGeom::CTAS
+    uint64_t splits = resident / units, most = (max_keys + TK * WARPS - 1) / (TK * WARPS);   // a split is a tile per warp at least
     if (splits > most) splits = most;
     if (splits > 128) splits = 128;
     if (splits < 1) splits = 1;
