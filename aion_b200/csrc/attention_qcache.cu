@@ -6,8 +6,8 @@
 //   out[block] = sum_t softmax_t * s_t[block] * c_t[block]
 // over the keys [lo, hi) of the row's window; zeros for an empty range. The codes are exact in any float type
 // and the scales in f32, so only the f32 sums round: the result is f32 attention over the dequantized cache.
+#include <cstdlib>
 #include <mutex>
-#include <type_traits>
 
 #include "attention_device.cuh"
 #include "cache_geom.cuh"
@@ -134,7 +134,7 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
 // group), and a slice of the context; its four warps walk tiles of 16 keys on their own, each with a private
 // ring of stages, so nothing in the loop waits for another warp. A tile's rows arrive as one TMA box of K and one
 // of V (16 rows of the head's bytes, rounded out to 16-byte granules) where the rows of the cache begin on
-// 16-byte boundaries, pages and rings in multiples of 16 rows; else by cp.async in pieces of D / 16 bytes.
+// 16-byte boundaries, else by cp.async in pieces of D / 16 bytes.
 //
 //  * S^T[16 keys x 8] = C . Q^T on f16 m16n8k16: the codes are exact in f16, q is two f16 terms (22 bits, normed
 //    by the column's largest value), and the products of one block of 32 dimensions are scaled by the block's
@@ -145,7 +145,12 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
 //  * O^T[D x 8] += V-codes^T . P'^T, P' = p * scale of (key, block) in f32, again two f16 terms. P' is scaled by
 //    a power of two that follows the largest V scale met so far: without it small V scales would push the terms
 //    into f16's subnormals. The accumulators are moved over when that power or a column's maximum grows.
-//  * The splits' partial sums meet in the last CTA of a unit to arrive (log-sum-exp), as in attention.cu.
+//  * The context of a unit (one kv head's columns) is cut over clusters of up to eight CTAs. A cluster's sums meet
+//    through distributed shared memory, every CTA adding up its share of the outputs; only units that several
+//    clusters work on leave partial sums in global memory, for the last of them to arrive. (With one ticket per
+//    CTA instead, that one CTA's trips to L2 cost 7 us of a 1024-key decode's 14.)
+//  * With fewer units than the GPU holds CTAs, the clusters are dealt out in proportion to the keys that each
+//    unit has: every CTA works out the same table from the lengths and finds its place in it.
 //
 // A lane reads a block pair's bytes where they lie: 2 x 18 (34) bytes are 9 (17) aligned words whose first and
 // middle ones hold the scales, and the order of the dimensions inside a block is free as long as Q's order is
@@ -183,16 +188,78 @@ struct DecodeGeom {
   static_assert(NST >= 2 && WARPS * WS * 4 <= RING, "ring");
   static constexpr int OFF_VS = RING;                                        // f32 [warp][block][keys of an iteration]: V scales
   static constexpr int OFF_Q = OFF_VS + WARPS * (D / QK) * TK * TPI * 4;     // uint4 [D / 16][32]: Q fragments; first f32 [8][D]: q
-  static constexpr int OFF_CI = OFF_Q + COLS * D * 4;                        // f32 [block][8]: -8 sum q
-  static constexpr int OFF_META = OFF_CI + D / QK * COLS * 4;                // per column: row, first key, key end, output row, head, factor
-  static constexpr int OFF_VALID = OFF_META + COLS * 24;                     // per warp and stage: which keys are there
-  static constexpr int OFF_BARS = (OFF_VALID + WARPS * NST * 4 + 7) / 8 * 8; // per warp and stage: the copies' barrier
+  static constexpr int OFF_CI = OFF_Q + COLS * D * 4;                        // float4 [block][4]: -8 sum q of columns 2t, 2t + 1, twice
+  static constexpr int OFF_META = OFF_CI + D / QK * COLS * 8;                // per column: row, first key, key end, output row, head, factor
+  static constexpr int OFF_VALID = OFF_META + COLS * 24;                     // per warp and stage: which keys are there, the first of them
+  static constexpr int OFF_BARS = OFF_VALID + WARPS * NST * 8;               // per warp and stage: the copies' barrier
   static constexpr int OFF_FLAGS = OFF_BARS + WARPS * NST * 8;
   static constexpr int SMEM = OFF_FLAGS + 32;
   static_assert(CTAS * (SMEM + 1024) <= 227 * 1024, "shared memory of an SM");
-  static constexpr int MAX_SPLITS = 128;
-  static_assert(MAX_SPLITS * COLS * 8 + COLS * 4 <= RING, "factors of the merge");
+  static constexpr int OFF_RES = WARPS * WS * 4;     // f32 [8][D], maxima, weights: the CTA's result, in the drained ring
+  static_assert(OFF_RES % 16 == 0 && OFF_RES + WS * 4 <= RING, "room for the result");
+  static constexpr int MAX_ROW_UNITS = COLS * D;     // tile counts that fit where q will lie
 };
+
+// How the units are dealt to the clusters.
+struct DecodeGrid {
+  uint32_t cluster;      // CTAs of a cluster
+  uint32_t clusters;     // launched
+  uint32_t row_units;    // (request, block of positions) pairs
+  uint32_t per_row;      // units of each: kv heads x head groups
+  uint32_t least;        // tiles that a cluster takes at least, where there are as many
+  uint32_t dealt;        // 1: in proportion to the keys; 0: cluster c is unit c
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_cluster_f(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+
+// Tiles are cut so that none straddles a page or the end of a ring: a segment (a page, a lap of the ring, or the
+// whole contiguous cache) is cut into tiles of TK keys, the last of which may be shorter.
+struct TileSpace {
+  uint32_t seg_len, per_seg;
+};
+__device__ __forceinline__ TileSpace tile_space(const AttnParams& p) {
+  const uint32_t len = p.page_table ? p.page_tokens : p.rolling ? p.T : 0x7FFFFFFFu;
+  return TileSpace{len, len / TK + (len % TK != 0)};
+}
+__device__ __forceinline__ uint32_t tile_at(const TileSpace& ts, uint32_t key) {
+  const uint32_t seg = key / ts.seg_len;
+  return seg * ts.per_seg + (key - seg * ts.seg_len) / TK;
+}
+// Tiles [first, end) hold the keys that the columns of (request b, positions from l0 on) see together.
+struct TileRange {
+  uint32_t first, end;
+};
+__device__ __forceinline__ TileRange tiles_of_keys(const TileSpace& ts, uint32_t lo, uint32_t hi) {
+  if (hi <= lo) return TileRange{0, 0};
+  return TileRange{tile_at(ts, lo), tile_at(ts, hi - 1) + 1};
+}
+__device__ __forceinline__ uint32_t count_tiles(const AttnParams& p, const TileSpace& ts, uint32_t b, uint32_t l0) {
+  uint32_t lo = 0xFFFFFFFFu, hi = 0;
+  for (uint32_t l = l0; l < min(p.L, l0 + p.pos_per_tile); l++) {
+    const KeyRange r = key_range(p, b, l);
+    if (r.hi > r.lo) lo = min(lo, r.lo), hi = max(hi, r.hi);
+  }
+  const TileRange t = tiles_of_keys(ts, lo, hi);
+  return t.end - t.first;
+}
 
 template <int BYTES>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool there) {
@@ -233,16 +300,16 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-// Two terms of f16 for a pair of f32 values: x = hi + lo to 22 bits. The remainder is taken by a subtraction that
-// reads the f16 term as it is (on the FMA pipe; a conversion back to f32 would go to the busier ALU pipe).
+// Two terms of f16 for a pair of f32 values: x = hi + lo to 22 bits. The remainder is taken by an operation that
+// reads the f16 term as it is (times -1) (on the FMA pipe; a conversion back to f32 would go to the busier ALU pipe).
 __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
   const uint32_t h = pack_half2(a, b);
-  float na, nb;   // hi - x
-  asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %4;\n\t}"
-      : "=f"(na), "=f"(nb)
+  float la, lb;   // x - hi
+  asm("{.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xBC00;\n\tfma.rn.f32.f16 %0, l, m, %3;\n\tfma.rn.f32.f16 %1, h, m, %4;\n\t}"
+      : "=f"(la), "=f"(lb)
       : "r"(h), "f"(a), "f"(b));
   *hi = h;
-  *lo = pack_half2(-na, -nb);
+  *lo = pack_half2(la, lb);
 }
 
 // Which dimension of a block the lane index u (t of a key row's words) reaches with code i of its word(s).
@@ -269,8 +336,8 @@ __device__ __forceinline__ void unpack_q8(uint32_t w, uint32_t* r0, uint32_t* r1
 }
 
 template <int D, bool KQ8, bool VQ8, bool TMA>
-__global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_qcache_decode_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tmap_k,
-                                                                                       const __grid_constant__ CUtensorMap tmap_v) {
+__global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_qcache_decode_kernel(
+    const AttnParams p, const DecodeGrid dg, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v) {
   using G = DecodeGeom<D, KQ8, VQ8>;
   using KF = RowFmt<D, KQ8>;
   using VF = RowFmt<D, VQ8>;
@@ -283,17 +350,6 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
 
-  // unit = (b, block of positions, hkv, head group); split = blockIdx.y
-  const uint32_t unit = blockIdx.x, split = blockIdx.y;
-  const uint32_t hg = unit % p.head_groups;
-  const uint32_t hkv = (unit / p.head_groups) % p.Hkv;
-  const uint32_t bl = unit / (p.head_groups * p.Hkv);
-  const uint32_t lb = p.l_blocks - 1 - bl % p.l_blocks, b = bl / p.l_blocks;
-  const uint32_t group = p.Hq / p.Hkv;
-  const uint32_t h0 = hkv * group + hg * 8;
-  const uint32_t nh = min(8u, group - hg * 8);
-  const uint32_t l0 = lb * p.pos_per_tile;
-
   uint32_t* col_row = reinterpret_cast<uint32_t*>(smem + G::OFF_META);  // (b*L + l)*Hq + head, NO_ROW: padding
   uint32_t* col_lo = col_row + COLS;
   uint32_t* col_hi = col_lo + COLS;
@@ -302,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   float* col_factor = reinterpret_cast<float*>(col_head + COLS);
   float* qs = reinterpret_cast<float*>(smem + G::OFF_Q);
   float* ci = reinterpret_cast<float*>(smem + G::OFF_CI);
-  int* flags = reinterpret_cast<int*>(smem + G::OFF_FLAGS);   // [0] bad inputs, [1] last CTA of the unit
+  int* flags = reinterpret_cast<int*>(smem + G::OFF_FLAGS);   // [0] bad inputs, [1] last cluster of the unit
 
   const uint32_t bars = sbase + G::OFF_BARS + warp * (G::NST * 8);
   if (tid == 0) flags[0] = 0;
@@ -313,6 +369,76 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   __syncthreads();
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
+  const TileSpace ts = tile_space(p);
+  // ---- this cluster's unit, and its place among the unit's clusters
+  const uint32_t cluster = blockIdx.x / dg.cluster, rank = blockIdx.x - cluster * dg.cluster;
+  uint32_t row_unit = cluster / dg.per_row, in_row = cluster - row_unit * dg.per_row, split = 0, nsplit = 1;
+  if (dg.dealt) {
+    uint32_t* tiles_of = reinterpret_cast<uint32_t*>(smem + G::OFF_Q);
+    for (uint32_t r = tid; r < dg.row_units; r += THREADS) {
+      const uint32_t rb = r / p.l_blocks;
+      tiles_of[r] = count_tiles(p, ts, rb, (r - rb * p.l_blocks) * p.pos_per_tile);
+    }
+    __syncthreads();
+    uint32_t sum = 0;
+    for (uint32_t r = lane; r < dg.row_units; r += 32) sum += tiles_of[r];
+    sum = __reduce_add_sync(FULL, sum);
+    // The smallest quota of tiles, to a few parts in a hundred, for which no more clusters are wanted than there are.
+    // (sum ceil(t / quota) <= sum t / quota + units, so the first upper end is one.)
+    const uint32_t units = dg.row_units * dg.per_row, spare = dg.clusters - units;
+    auto wanted = [&](uint32_t quota) {
+      uint32_t n = 0;
+      for (uint32_t r = lane; r < dg.row_units; r += 32) n += max(1u, (tiles_of[r] + quota - 1) / quota);
+      return __reduce_add_sync(FULL, n) * dg.per_row;
+    };
+    uint32_t quota = 0x7FFFFFFFu;
+    if (spare) {
+      const uint64_t all = (uint64_t)sum * dg.per_row;
+      uint32_t low = (uint32_t)min((uint64_t)0x3FFFFFFFu, all / dg.clusters);
+      quota = (uint32_t)min((uint64_t)0x3FFFFFFFu, (all + spare - 1) / spare) + 1;
+      for (int i = 0; i < 4; i++) {
+        const uint32_t mid = low + (quota - low) / 2;
+        if (mid && wanted(mid) <= dg.clusters) quota = mid;
+        else low = mid;
+      }
+      quota = max(dg.least, quota);
+    }
+    uint32_t before = 0;   // clusters of the row units before this batch of 32
+    bool found = false;
+    for (uint32_t r0 = 0; r0 < dg.row_units; r0 += 32) {
+      const uint32_t r = r0 + lane;
+      const uint32_t n = r < dg.row_units ? max(1u, (tiles_of[r] + quota - 1) / quota) : 0;
+      uint32_t upto = n * dg.per_row;   // inclusive sum over the lanes
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(FULL, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const uint32_t end = before + upto, mine = __ballot_sync(FULL, cluster < end);
+      if (mine && !found) {   // the first lane whose clusters reach beyond this one's number
+        const int owner = __ffs(mine) - 1;
+        const uint32_t start = __shfl_sync(FULL, end - n * dg.per_row, owner);
+        nsplit = __shfl_sync(FULL, n, owner);
+        row_unit = r0 + owner;
+        in_row = (cluster - start) / nsplit;
+        split = (cluster - start) - in_row * nsplit;
+        found = true;
+        break;
+      }
+      before = __shfl_sync(FULL, end, 31);
+    }
+    if (!found) return;    // no unit wants this cluster: all of it leaves
+    __syncthreads();       // the counts have been read, q may take their place
+  }
+  const uint32_t hkv = in_row / p.head_groups, hg = in_row - hkv * p.head_groups;
+  const uint32_t b = row_unit / p.l_blocks;
+  // (Later positions see more keys under a causal window: where units queue, the long ones begin first.)
+  const uint32_t lb = dg.dealt ? row_unit - b * p.l_blocks : p.l_blocks - 1 - (row_unit - b * p.l_blocks);
+  const uint32_t unit = row_unit * dg.per_row + in_row;
+  const uint32_t group = p.Hq / p.Hkv;
+  const uint32_t h0 = hkv * group + hg * 8;
+  const uint32_t nh = min(8u, group - hg * 8);
+  const uint32_t l0 = lb * p.pos_per_tile;
   // This warp's two columns of q are on their way while the ranges are worked out.
   float qv[COLS / WARPS][D / 32];
 #pragma unroll
@@ -349,89 +475,65 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     if (col_row[c] != NO_ROW) all_lo = max(all_lo, lo), all_hi = min(all_hi, hi);
   }
   u_lo = min(u_lo, u_hi);
-  // Slices begin on multiples of a tile, so that none straddles a page or a ring's end that is one.
-  const uint32_t base = u_lo / TK * TK;
-  uint32_t per = (u_hi - base + p.splits - 1) / p.splits;
-  per = (per + TK - 1) / TK * TK;
-  const uint32_t my_lo = (uint32_t)min((uint64_t)u_hi, base + (uint64_t)split * per);
-  const uint32_t my_hi = (uint32_t)min((uint64_t)u_hi, (uint64_t)my_lo + per);
-  const uint32_t tiles = (my_hi - my_lo + TK - 1) / TK;
+  const TileRange whole = tiles_of_keys(ts, u_lo, u_hi);
+  const uint32_t parts = nsplit * dg.cluster, per = (whole.end - whole.first + parts - 1) / parts;
+  const uint32_t my_first = (uint32_t)min((uint64_t)whole.end, whole.first + (uint64_t)(split * dg.cluster + rank) * per);
+  const uint32_t tiles = min(whole.end - my_first, per);
 
   // ---- the warp's copies. Its n-th tile is one of TPI neighbours; the warps take such groups in turn.
   const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;   // the request's first row, or the pool's
   const uint32_t ring = warp * (G::NST * G::STAGE);   // offsets into shared memory
-  uint32_t* valid = reinterpret_cast<uint32_t*>(smem + G::OFF_VALID) + warp * G::NST;
+  uint2* valid = reinterpret_cast<uint2*>(smem + G::OFF_VALID) + warp * G::NST;   // per stage: which keys are there, the first key
   // A box begins on a 16-byte boundary: the head's bytes are this far into each row.
   const uint32_t kshift = TMA ? (hkv * KF::BYTES) & 15 : 0, vshift = TMA ? (hkv * VF::BYTES) & 15 : 0;
-  // Where a tile's rows lie. The page number is read a tile ahead of the copies and looked at only then.
-  struct Place {
-    int32_t page;      // raw entry of the page table; 0 where there is none
-    uint32_t in_page;  // row inside the page, or below row0
-    bool on;
-  };
   auto tile_of = [&](uint32_t n) { return ((n / G::TPI) * WARPS + warp) * G::TPI + n % G::TPI; };
-  // (The page of the next tile is found by counting on from the last one: a division costs as much as a block of keys.)
-  uint32_t page_index = 0, page_key = 0;   // page of the last tile that was placed, and its first key
-  if (p.page_table) {
-    const uint32_t key = my_lo + tile_of(0) * TK + (TMA ? 0 : lane & 15);
-    page_index = key / p.page_tokens;
-    page_key = page_index * p.page_tokens;
-  }
-  auto place = [&](uint32_t n) -> Place {
-    const uint32_t tile = tile_of(n), key = my_lo + tile * TK + (TMA ? 0 : lane & 15);
-    Place at{0, 0, tile < tiles && key < my_hi};
-    if (at.on) {
-      if (p.page_table) {
-        while (key - page_key >= p.page_tokens) page_index++, page_key += p.page_tokens;
-        at.page = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + page_index);
-        at.in_page = key - page_key;
-      } else {
-        at.in_page = p.rolling ? key % p.T : key;
-      }
-    }
-    return at;
+  // Where a tile lies: its segment, counted on from the last tile's (a division costs as much as a block of keys),
+  // and the raw entry of the page table, which is read a tile ahead of the copies and looked at only then.
+  uint32_t seg = (my_first + tile_of(0)) / ts.per_seg, in_seg = my_first + tile_of(0) - seg * ts.per_seg, last_n = 0;
+  int32_t next_page = 0;
+  auto place = [&](uint32_t n) {
+    in_seg += tile_of(n) - tile_of(last_n);
+    last_n = n;
+    while (in_seg >= ts.per_seg) in_seg -= ts.per_seg, seg++;
+    if (p.page_table && tile_of(n) < tiles) next_page = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + seg);
   };
-  auto issue = [&](uint32_t n, const Place& at) {
+  auto issue = [&](uint32_t n) {
     const uint32_t stage = n % G::NST;
-    bool there = at.on;
-    uint64_t row = at.in_page;
+    uint32_t count = tile_of(n) < tiles ? min((uint32_t)TK, ts.seg_len - in_seg * TK) : 0;   // keys of the tile
+    uint64_t row = count ? row0 + in_seg * TK : 0;
     if (p.page_table) {
-      if (there && (at.page < 0 || (uint32_t)at.page >= p.pool_pages)) {
-        atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
-        there = false;
+      if (count && (next_page < 0 || (uint32_t)next_page >= p.pool_pages)) {
+        if (lane == 0) atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
+        count = 0;
       }
-      row += (uint64_t)(there ? at.page : 0) * p.page_tokens;
+      row += (uint64_t)(count ? next_page : 0) * p.page_tokens;
     }
-    row += row0;
+    if (lane == 0) valid[stage] = make_uint2((1u << count) - 1, seg * ts.seg_len + in_seg * TK);
     const uint32_t dst = sbase + ring + stage * G::STAGE, vdst = dst + TK * KF::PITCH;
     if constexpr (TMA) {
       if (lane == 0) {
-        valid[stage] = there ? 0xFFFFu : 0;
         const uint32_t bar = bars + 8 * stage;
-        ptx::mbar_arrive_expect_tx(bar, there ? (uint32_t)G::STAGE : 0u);
-        if (there && !(p.drop_first && n == 0)) {
+        ptx::mbar_arrive_expect_tx(bar, count ? (uint32_t)G::STAGE : 0u);
+        if (count && !(p.drop_first && n == 0)) {
           ptx::tma_load_2d(dst, &tmap_k, (int)((hkv * KF::BYTES) / 16 * 2), (int)row, bar);
           ptx::tma_load_2d(vdst, &tmap_v, (int)((hkv * VF::BYTES) / 16 * 2), (int)row, bar);
         }
       }
     } else {
-      const uint32_t mask = __ballot_sync(FULL, there) & 0xFFFFu;
-      if (lane == 0) valid[stage] = mask;
-      const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + hkv * KF::BYTES;
-      const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + hkv * VF::BYTES;
+      const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + (row * p.Hkv + hkv) * KF::BYTES;
+      const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + (row * p.Hkv + hkv) * VF::BYTES;
+      // Where the key is not there the address is the first row's, and nothing is read from it.
 #pragma unroll
       for (int i = 0; i < (TK * KF::CHUNKS + 31) / 32; i++) {
         const uint32_t idx = lane + 32 * i, key = idx / KF::CHUNKS, c = idx - key * KF::CHUNKS;
-        const uint64_t r = __shfl_sync(FULL, row, key & 15);
         if (idx < TK * KF::CHUNKS)
-          cp_async<KF::CHUNK>(dst + key * KF::PITCH + c * KF::CHUNK, kbase + r * (p.Hkv * KF::BYTES) + c * KF::CHUNK, (mask >> key) & 1);
+          cp_async<KF::CHUNK>(dst + key * KF::PITCH + c * KF::CHUNK, kbase + (key < count ? (uint64_t)key * (p.Hkv * KF::BYTES) + c * KF::CHUNK : 0), key < count);
       }
 #pragma unroll
       for (int i = 0; i < (TK * VF::CHUNKS + 31) / 32; i++) {
         const uint32_t idx = lane + 32 * i, key = idx / VF::CHUNKS, c = idx - key * VF::CHUNKS;
-        const uint64_t r = __shfl_sync(FULL, row, key & 15);
         if (idx < TK * VF::CHUNKS)
-          cp_async<VF::CHUNK>(vdst + key * VF::PITCH + c * VF::CHUNK, vbase + r * (p.Hkv * VF::BYTES) + c * VF::CHUNK, (mask >> key) & 1);
+          cp_async<VF::CHUNK>(vdst + key * VF::PITCH + c * VF::CHUNK, vbase + (key < count ? (uint64_t)key * (p.Hkv * VF::BYTES) + c * VF::CHUNK : 0), key < count);
       }
       cp_commit();
     }
@@ -439,12 +541,12 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   const uint32_t groups = (tiles + G::TPI - 1) / G::TPI;
   const uint32_t iters = groups > (uint32_t)warp ? (groups - warp + WARPS - 1) / WARPS : 0;
   const uint32_t mine = iters * G::TPI;   // the last of them may lie behind the end: no key of it is there
-  Place next = place(0);
+  place(0);
 #pragma unroll
   for (int n = 0; n < G::AHEAD; n++) {
     if ((uint32_t)n < mine) {
-      issue(n, next);
-      next = place(n + 1);
+      issue(n);
+      place(n + 1);
     } else if (!TMA) {
       cp_commit();
     }
@@ -499,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
       if (!KQ8) {
         part += __shfl_xor_sync(FULL, part, 1);
         part += __shfl_xor_sync(FULL, part, 2);
-        if (t == 0) ci[blk * COLS + g] = part * (-8.0f * 5.9604644775390625e-8f);   // -8 * 2^-24
+        if (t == 0) ci[blk * 2 * COLS + g / 2 * 4 + g % 2] = ci[blk * 2 * COLS + g / 2 * 4 + g % 2 + 2] = part * (-8.0f * 5.9604644775390625e-8f);   // -8 * 2^-24
       }
     }
   }
@@ -539,8 +641,8 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     for (int j = 0; j < TPI; j++) {
       const uint32_t n = it * TPI + G::AHEAD + j;
       if (n < mine) {
-        issue(n, next);
-        next = place(n + 1);
+        issue(n);
+        place(n + 1);
       } else if (!TMA) {
         cp_commit();
       }
@@ -563,36 +665,40 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
       cp_wait<G::AHEAD>();
       __syncwarp();
     }
-    const uint32_t key0 = my_lo + tile_of(it * TPI) * TK;
-    uint32_t at[TPI], there = 0;   // offset of a tile's K rows; which keys are there
+    uint32_t at[TPI], key0[TPI], there = 0;   // offset of a tile's K rows, its first key; which keys are there
+    // Some column does not see some row of the tiles: what lies there (rows past the end, of other requests,
+    // whatever a page holds) must not reach it, not even as 0 x infinity.
+    bool partial = false;
 #pragma unroll
     for (int j = 0; j < TPI; j++) {
       const uint32_t stage = (it * TPI + j) % G::NST;
+      const uint2 v = valid[stage];
       at[j] = ring + stage * G::STAGE;
-      there |= valid[stage] << (TK * j);
+      key0[j] = v.y;
+      there |= v.x << (TK * j);
+      partial |= v.x != 0xFFFFu || v.y < all_lo || v.y + TK > all_hi;
     }
-    // Some column does not see some row of the tiles: what lies there (rows past the end, of other requests,
-    // whatever a page holds) must not reach it, not even as 0 x infinity.
-    const bool partial = there != (TPI == 2 ? 0xFFFFFFFFu : 0xFFFFu) || key0 < all_lo || key0 + KI > all_hi;
 
-    // ---- V scales as f32, times 2^(29 - E) of the largest exponent so far
+    // ---- V scales as f32, times 2^(29 - E) of the largest exponent so far. One that is not finite becomes 0 here and
+    // makes the sums that it belongs to NaN below.
     uint32_t sc[NB * KI / 32], top = 0;
+    bool weird = false;
 #pragma unroll
     for (int j = 0; j < NB * KI / 32; j++) {
       const uint32_t e = lane + 32 * j, blk = e / KI, k = e % KI;
       sc[j] = lds16(at[TPI == 2 ? (k >> 4) : 0] + TK * KF::PITCH + vshift + (k & 15) * VF::PITCH + blk * VF::BB);
-      const uint32_t mag = sc[j] & 0x7FFFu, key = key0 + k;
-      if (mag < 0x7C00u && (!partial || (((there >> k) & 1) && key >= u_lo && key < u_hi))) top = max(top, mag);   // keys that some column sees
+      if (partial) {   // only keys that some column sees
+        const uint32_t key = key0[TPI == 2 ? (k >> 4) : 0] + (k & 15);
+        if (!((there >> k) & 1) || key < u_lo || key >= u_hi) sc[j] = 0;
+      }
+      if ((sc[j] & 0x7FFFu) >= 0x7C00u) sc[j] = 0, weird = true;
+      top = max(top, sc[j] & 0x7FFFu);
     }
     const uint32_t e_new = max(e_run, __reduce_max_sync(FULL, top) >> 10);
     const float vmul = __uint_as_float((127u + 29u - e_new) << 23);
-    bool odd = partial;
 #pragma unroll
-    for (int j = 0; j < NB * KI / 32; j++) {
-      *reinterpret_cast<float*>(smem + vs + (lane + 32 * j) * 4) = half_bits(sc[j]) * vmul;
-      odd |= (sc[j] & 0x7FFFu) >= 0x7C00u;
-    }
-    odd = __any_sync(FULL, odd);             // or an infinite or NaN scale
+    for (int j = 0; j < NB * KI / 32; j++) *reinterpret_cast<float*>(smem + vs + (lane + 32 * j) * 4) = half_bits(sc[j]) * vmul;
+    weird = __any_sync(FULL, weird);
     __syncwarp();
 
     // ---- S^T: 16 keys x 8 columns for each tile
@@ -601,9 +707,9 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     for (int j = 0; j < TPI; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
 #pragma unroll
     for (int pr = 0; pr < NB / 2; pr++) {
-      float2 init[2];
+      float4 init[2];
 #pragma unroll
-      for (int k = 0; k < 2; k++) init[k] = KQ8 ? make_float2(0.0f, 0.0f) : lds_f2(G::OFF_CI + ((2 * pr + k) * COLS + 2 * t) * 4);
+      for (int k = 0; k < 2; k++) init[k] = KQ8 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(ci + (2 * pr + k) * 2 * COLS + 4 * t);
 #pragma unroll
       for (int j = 0; j < TPI; j++) {
         uint32_t a[2][2][4];                   // [block of the pair][MMA][operand]
@@ -631,7 +737,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
         for (int k = 0; k < 2; k++) {
           const int q = 2 * (2 * pr + k);
           float c[4];
-          mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], ql[q][0], ql[q][1], init[k].x, init[k].y, init[k].x, init[k].y);
+          mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], ql[q][0], ql[q][1], init[k].x, init[k].y, init[k].z, init[k].w);
           mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], ql[q + 1][0], ql[q + 1][1], c[0], c[1], c[2], c[3]);
           mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], qh[q][0], qh[q][1], c[0], c[1], c[2], c[3]);
           mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], qh[q + 1][0], qh[q + 1][1], c[0], c[1], c[2], c[3]);
@@ -661,7 +767,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     if (partial) {
 #pragma unroll
       for (int k = 0; k < 4 * TPI; k++) {
-        const uint32_t kk = 2 * t + (k & 1) + 8 * (k >> 1), key = key0 + kk;
+        const uint32_t kk = 2 * t + (k & 1) + 8 * (k >> 1), key = key0[k >> 2] + (kk & 15);
         if (!((there >> kk) & 1) || key < lo_g || key >= hi_g) y[k] = -INFINITY;
       }
     }
@@ -687,9 +793,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
       l_run += y[k];
     }
 
-    // ---- O^T += V^T . P'^T, block by block. (Two copies of the loop: one without the selections, and without a
-    // branch that would keep the blocks' instructions apart.)
-    auto add_values = [&](auto select) {
+    // ---- O^T += V^T . P'^T, block by block
 #pragma unroll
       for (int blk = 0; blk < NB; blk++) {
         uint32_t bh[TPI][2], blw[TPI][2];
@@ -699,11 +803,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
 #pragma unroll
           for (int kp = 0; kp < 2; kp++) {
             const float2 v = lds_f2(vs + (blk * KI + j * TK + 2 * t + 8 * kp) * 4);
-            float w0 = y[4 * j + 2 * kp] * v.x, w1 = y[4 * j + 2 * kp + 1] * v.y;
-            if constexpr (decltype(select)::value) {
-              if (y[4 * j + 2 * kp] == 0.0f) w0 = 0.0f;
-              if (y[4 * j + 2 * kp + 1] == 0.0f) w1 = 0.0f;
-            }
+            const float w0 = y[4 * j + 2 * kp] * v.x, w1 = y[4 * j + 2 * kp + 1] * v.y;
             split2(w0, w1, &bh[j][kp], &blw[j][kp]);
             const uint32_t row = at[j] + TK * KF::PITCH + vshift + (2 * t + 8 * kp) * VF::PITCH;
             if (VQ8) {
@@ -745,9 +845,22 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
           for (int e = 0; e < 4; e++) acc[2 * blk + m][e] += o[e];
         }
       }
-    };
-    if (odd) add_values(std::true_type{});
-    else add_values(std::false_type{});
+    if (weird) {
+#pragma unroll
+      for (int blk = 0; blk < NB; blk++) {
+        bool met = false;   // column g gives weight to a key whose scale of this block is not finite
+#pragma unroll
+        for (int k = 0; k < 4 * TPI; k++) {
+          const uint32_t kk = 2 * t + (k & 1) + 8 * ((k >> 1) & 1);
+          const uint32_t bits = lds16(at[k >> 2] + TK * KF::PITCH + vshift + kk * VF::PITCH + blk * VF::BB) & 0x7FFFu;
+          met |= bits >= 0x7C00u && y[k] > 0.0f;
+        }
+        const uint32_t who = __ballot_sync(FULL, met);
+        const float n0 = (who >> (8 * t)) & 15 ? NAN : 0.0f, n1 = (who >> (8 * t + 4)) & 15 ? NAN : 0.0f;
+#pragma unroll
+        for (int m = 0; m < 2; m++) acc[2 * blk + m][0] += n0, acc[2 * blk + m][1] += n1, acc[2 * blk + m][2] += n0, acc[2 * blk + m][3] += n1;
+      }
+    }
     __syncwarp();   // the stages and the scales are free again
   }
   if (!TMA) cp_wait<0>();
@@ -775,13 +888,11 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   }
   __syncthreads();
   constexpr int C4 = COLS * D / 4 / THREADS;
-  constexpr int PP = D + 4;                   // a partial row: D sums, maximum, weight, pad
-  float* part = p.partial + ((uint64_t)unit * p.splits + split) * COLS * PP;
-  const bool direct = p.splits == 1;
-  const uint32_t d4 = tid % (D / 4);
+  float* res = reinterpret_cast<float*>(smem + G::OFF_RES);   // [8][D], then maxima and weights
+  const bool direct = nsplit * dg.cluster == 1;
 #pragma unroll 1
   for (int c = 0; c < C4; c++) {
-    const uint32_t idx4 = tid + c * THREADS, col = idx4 / (D / 4);
+    const uint32_t idx4 = tid + c * THREADS, col = idx4 / (D / 4), d4 = idx4 % (D / 4);
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WARPS; w++) M = fmaxf(M, all[w * G::WS + COLS * D + col]);
@@ -790,117 +901,190 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
 #pragma unroll
     for (int w = 0; w < WARPS; w++) {
       const float mw = all[w * G::WS + COLS * D + col];
-      const float f = mw == -INFINITY ? 0.0f : exp2f(mw - M);
+      const float f = mw == -INFINITY ? 0.0f : ex2(mw - M);
       const float4 x = *reinterpret_cast<const float4*>(all + w * G::WS + 4 * idx4);
       o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
       lsum += all[w * G::WS + COLS * D + COLS + col] * f;
     }
-    const bool on = col_row[col] != NO_ROW;
     if (direct) {
+      finish_column<D>(p, o, lsum, col_row[col] != NO_ROW, col_hi[col] > col_lo[col], col, d4, col_row, col_orow, col_head, !flags[0]);
+    } else {
+      *reinterpret_cast<float4*>(res + 4 * idx4) = o;
+      if (d4 == 0) res[COLS * D + col] = M, res[COLS * D + COLS + col] = lsum;
+    }
+  }
+  if (direct) return;
+  // ---- the cluster's: every CTA adds up its share of the outputs over all of them
+  cluster_sync();
+  constexpr int PP = D + 4;                   // a partial row: D sums, maximum, weight, pad
+  const uint32_t share = COLS * D / 4 / dg.cluster;
+  const uint32_t res_addr = sbase + G::OFF_RES;
+  float* part = p.partial + (uint64_t)cluster * COLS * PP;
+#pragma unroll 1
+  for (uint32_t i = tid; i < (share + 31) / 32 * 32; i += THREADS) {   // whole warps: the image is made by eight lanes together
+    const bool on4 = i < share;
+    const uint32_t idx4 = rank * share + (on4 ? i : 0), col = idx4 / (D / 4), d4 = idx4 % (D / 4);
+    const bool on = on4 && col_row[col] != NO_ROW;
+    float m[8], l[8], M = -INFINITY, lsum = 0.0f;
+    float4 v[8], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      m[k] = -INFINITY, l[k] = 0.0f, v[k] = o;
+      if (k < (int)dg.cluster) {
+        const uint32_t a = cluster_addr(res_addr, k);
+        m[k] = ld_cluster_f(a + (COLS * D + col) * 4);
+        l[k] = ld_cluster_f(a + (COLS * D + COLS + col) * 4);
+        v[k] = ld_cluster_f4(a + 16 * idx4);
+      }
+      M = fmaxf(M, m[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float f = m[k] == -INFINITY ? 0.0f : ex2(m[k] - M);
+      o.x += v[k].x * f, o.y += v[k].y * f, o.z += v[k].z * f, o.w += v[k].w * f;
+      lsum += l[k] * f;
+    }
+    if (nsplit == 1) {
       finish_column<D>(p, o, lsum, on, col_hi[col] > col_lo[col], col, d4, col_row, col_orow, col_head, !flags[0]);
     } else if (on) {
       *reinterpret_cast<float4*>(part + col * PP + 4 * d4) = o;
       if (d4 == 0) *reinterpret_cast<float2*>(part + col * PP + D) = make_float2(M, lsum);
     }
   }
-  if (direct) return;
-  // ---- and the splits' in the last CTA of the unit
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    const int prev = atomicAdd(p.tickets + unit, 1), last = prev == (int)p.splits - 1;
+  if (nsplit > 1) __threadfence();
+  cluster_sync();   // no CTA leaves, or looks for the others' sums, before all have read and written
+  if (nsplit == 1) return;
+  // ---- and the clusters' in the last of them to arrive
+  if (rank == 0 && tid == 0) {
+    __threadfence();
+    const int prev = atomicAdd(p.tickets + unit, 1), last = prev == (int)nsplit - 1;
     if (last) p.tickets[unit] = 0;   // ready for the next launch
-    flags[1] = last;
+    for (uint32_t k = 0; k < dg.cluster; k++) st_cluster_u32(cluster_addr(sbase + G::OFF_FLAGS + 4, k), last);
   }
-  __syncthreads();
+  cluster_sync();
   if (!flags[1]) return;
   __threadfence();
-  const float* pu = p.partial + (uint64_t)unit * p.splits * COLS * PP;
-  float* fac = all;                           // [8][splits]: maximum, then factor
-  float* wsum = fac + COLS * p.splits;
-  float* lsums = wsum + COLS * p.splits;
-  for (uint32_t idx = tid; idx < COLS * p.splits; idx += THREADS) {
-    const uint32_t c = idx / p.splits, s2 = idx - c * p.splits;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (col_row[c] != NO_ROW) ml = __ldcg(reinterpret_cast<const float2*>(pu + (size_t)(s2 * COLS + c) * PP + D));
-    fac[idx] = ml.x, wsum[idx] = ml.y;
-  }
-  __syncthreads();
-  for (uint32_t c = warp; c < COLS; c += WARPS) {
+  const float* pu = p.partial + (uint64_t)(cluster - split) * COLS * PP;
+#pragma unroll 1
+  for (uint32_t i = tid; i < (share + 31) / 32 * 32; i += THREADS) {
+    const bool on4 = i < share;
+    const uint32_t idx4 = rank * share + (on4 ? i : 0), col = idx4 / (D / 4), d4 = idx4 % (D / 4);
+    const bool on = on4 && col_row[col] != NO_ROW;
     float M = -INFINITY, lsum = 0.0f;
-    for (uint32_t s2 = lane; s2 < p.splits; s2 += 32) M = fmaxf(M, fac[c * p.splits + s2]);
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, o));
-    for (uint32_t s2 = lane; s2 < p.splits; s2 += 32) {
-      const float ms = fac[c * p.splits + s2], f = ms == -INFINITY ? 0.0f : exp2f(ms - M);
-      fac[c * p.splits + s2] = f;
-      lsum += f > 0.0f || isnan(f) ? wsum[c * p.splits + s2] * f : 0.0f;
-    }
-    for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(FULL, lsum, o);
-    if (lane == 0) lsums[c] = lsum;
-  }
-  __syncthreads();
-  // Every load of a thread's columns for four splits is on its way before the first is used: the trip to L2 is
-  // what this costs.
-  float4 o[C4];
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t s0 = 0; s0 < nsplit; s0 += 8) {   // the loads of eight partial sums are under way together
+      float2 ml[8];
+      float4 v[8];
+      float top = M;
 #pragma unroll
-  for (int c = 0; c < C4; c++) o[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  constexpr int SI = 16 / C4;
-  for (uint32_t s0 = 0; s0 < p.splits; s0 += SI) {
-    float4 v[C4][SI];
+      for (int k = 0; k < 8; k++) {
+        ml[k] = make_float2(-INFINITY, 0.0f), v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (on && s0 + k < nsplit) {
+          const float* src = pu + ((uint64_t)(s0 + k) * COLS + col) * PP;
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(src + D));
+          v[k] = __ldcg(reinterpret_cast<const float4*>(src + 4 * d4));
+        }
+      }
 #pragma unroll
-    for (int c = 0; c < C4; c++) {
-      const uint32_t col = (tid + c * THREADS) / (D / 4);
+      for (int k = 0; k < 8; k++) top = fmaxf(top, ml[k].x);
+      const float keep = M == -INFINITY ? 0.0f : ex2(M - top);
+      o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep, lsum *= keep;
+      M = top;
 #pragma unroll
-      for (int k = 0; k < SI; k++)
-        v[c][k] = s0 + k < p.splits && col_row[col] != NO_ROW ? __ldcg(reinterpret_cast<const float4*>(pu + ((size_t)(s0 + k) * COLS + col) * PP + 4 * d4))
-                                                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-#pragma unroll
-    for (int c = 0; c < C4; c++) {
-      const uint32_t col = (tid + c * THREADS) / (D / 4);
-#pragma unroll
-      for (int k = 0; k < SI; k++) {
-        const float f = s0 + k < p.splits ? fac[col * p.splits + s0 + k] : 0.0f;
-        o[c].x += v[c][k].x * f, o[c].y += v[c][k].y * f, o[c].z += v[c][k].z * f, o[c].w += v[c][k].w * f;
+      for (int k = 0; k < 8; k++) {
+        const float f = ml[k].x == -INFINITY ? 0.0f : ex2(ml[k].x - M);
+        o.x += v[k].x * f, o.y += v[k].y * f, o.z += v[k].z * f, o.w += v[k].w * f;
+        lsum += ml[k].y * f;
       }
     }
-  }
-#pragma unroll
-  for (int c = 0; c < C4; c++) {
-    const uint32_t col = (tid + c * THREADS) / (D / 4);
-    finish_column<D>(p, o[c], lsums[col], col_row[col] != NO_ROW, col_hi[col] > col_lo[col], col, d4, col_row, col_orow, col_head, !flags[0]);
+    finish_column<D>(p, o, lsum, on, col_hi[col] > col_lo[col], col, d4, col_row, col_orow, col_head, !flags[0]);
   }
 }
 
 template <int D, bool KQ8, bool VQ8, bool TMA>
-int32_t launch_decode_as(AionCudaDevice* dev, const AttnParams& p, uint32_t units, const CUtensorMap& tk, const CUtensorMap& tv) {
+int32_t launch_decode_as(AionCudaDevice* dev, AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, uint64_t max_keys) {
   using G = DecodeGeom<D, KQ8, VQ8>;
   auto kernel = attn_qcache_decode_kernel<D, KQ8, VQ8, TMA>;
+  // Clusters of 1, 2, 4 and 8 CTAs that the device holds at once; worked out once per device and instantiation.
+  uint32_t resident[4];
   {
-    static std::mutex mu;   // once per device and instantiation
-    static bool configured[64] = {};
+    static std::mutex mu;
+    static uint32_t held[64][4] = {};
     std::lock_guard<std::mutex> lock(mu);
-    if (dev->ordinal < 0 || dev->ordinal >= 64 || !configured[dev->ordinal]) {
+    if (dev->ordinal < 0 || dev->ordinal >= 64) return fail(AION_CUDA_UNSUPPORTED, "attention: device %d", dev->ordinal);
+    if (!held[dev->ordinal][0]) {
       AION_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
-      if (dev->ordinal >= 0 && dev->ordinal < 64) configured[dev->ordinal] = true;
+      prefer_max_shared(reinterpret_cast<const void*>(kernel));
+      for (int i = 3; i >= 0; i--) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(8);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = G::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1u << i, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        AION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+        held[dev->ordinal][i] = n > 0 ? (uint32_t)n : 1u;
+      }
     }
+    for (int i = 0; i < 4; i++) resident[i] = held[dev->ordinal][i];
   }
-  if (p.splits > (uint32_t)G::MAX_SPLITS) return fail(AION_CUDA_INTERNAL_ERROR, "attention: %u splits exceed the merge buffer", p.splits);
-  AION_CUDA_TRY(launch_pdl_main(kernel, dim3(units, p.splits), dim3(THREADS), G::SMEM, dev->stream, p, tk, tv));
+  DecodeGrid dg{};
+  dg.row_units = p.B * p.l_blocks;
+  dg.per_row = p.Hkv * p.head_groups;
+  const uint64_t units = (uint64_t)dg.row_units * dg.per_row;
+  // A cluster's CTAs add up their sums cheaply (2.5 us), so a unit gets as large a cluster as leaves every unit one and
+  // every warp a tile. Where a warp has 16 tiles and more (30 us) it pays to deal smaller clusters out by the keys that
+  // each unit has, although the table (3 us) and partial sums in global memory (4 us) come on top: 6 requests of
+  // 25 941 to 65 536 keys take 194 us with a cluster of eight each, 152 us dealt; 64 of 512 to 2048 keys 24 and 27 us.
+  const uint64_t tiles = (max_keys + TK - 1) / TK, per_warp = tiles * units / ((uint64_t)resident[0] * WARPS);
+  const bool deal = per_warp >= 16 && units > 1;
+  const uint64_t each = deal ? (per_warp >= 32 ? 8 : 4) : 1;   // clusters a unit, so that the shares come out even
+  int lg = 0;
+  while (lg < 3 && each * units <= resident[lg + 1] && tiles >= ((uint64_t)WARPS << (lg + 1))) lg++;
+  if (dev->attn_split_override) for (lg = 0; lg < 3 && (2u << lg) <= dev->attn_split_override; lg++) {}
+  dg.cluster = 1u << lg;
+  // A single unit with more keys than one cluster should walk (four tiles a warp) takes several as well.
+  dg.least = dg.cluster * WARPS * 4;
+  dg.dealt = (deal || units == 1) && units < resident[lg] && dg.row_units <= (uint32_t)G::MAX_ROW_UNITS && tiles > dg.least;
+  dg.clusters = dg.dealt ? resident[lg] : (uint32_t)units;
+  if (dg.dealt) {
+    if (int32_t st = dev->reserve_scratch((size_t)dg.clusters * COLS * (D + 4) * sizeof(float))) return st;
+    if (int32_t st = dev->reserve_tickets(units)) return st;
+    p.partial = static_cast<float*>(dev->lane_scratch());
+    p.tickets = dev->lane_tickets();
+  }
+  if ((uint64_t)dg.clusters * dg.cluster > 0x7FFFFFFFull) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(dg.clusters * dg.cluster);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = G::SMEM;
+  cfg.stream = dev->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = dg.cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  static const bool no_pdl_main = std::getenv("AION_CUDA_NO_PDL_MAIN") != nullptr;  // tuning only
+  cfg.numAttrs = no_pdl_main ? 1 : 2;
+  AION_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, dg, tk, tv));
   return AION_CUDA_OK;
 }
 
 template <int D, bool KQ8, bool VQ8>
-int32_t launch_decode(AionCudaDevice* dev, const AttnParams& p, uint32_t units) {
+int32_t launch_decode(AionCudaDevice* dev, AttnParams& p, uint64_t max_keys) {
   using KF = RowFmt<D, KQ8>;
   using VF = RowFmt<D, VQ8>;
   const uint64_t rows = p.page_table ? (uint64_t)p.pool_pages * p.page_tokens : (uint64_t)p.B * p.T;
   const uint64_t kw = (uint64_t)p.Hkv * KF::BYTES, vw = (uint64_t)p.Hkv * VF::BYTES;
-  // Boxes: 16-byte aligned rows, tiles of 16 rows that lie together.
-  const bool boxes = ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | kw | vw) & 15) == 0 && rows < (1ull << 31) &&
-                     (!p.page_table || p.page_tokens % TK == 0) && (!p.rolling || p.T % TK == 0);
+  // Boxes need rows that begin on 16-byte boundaries.
+  const bool boxes = ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | kw | vw) & 15) == 0 && rows < (1ull << 31);
   CUtensorMap tk{}, tv{};
-  if (!boxes) return launch_decode_as<D, KQ8, VQ8, false>(dev, p, units, tk, tv);
+  if (!boxes) return launch_decode_as<D, KQ8, VQ8, false>(dev, p, tk, tv, max_keys);
   const CUtensorMap* m;
   const uint64_t kd[2] = {kw, rows}, vd[2] = {vw, rows};
   const uint32_t kbox[2] = {KF::PITCH, TK}, vbox[2] = {VF::PITCH, TK};
@@ -908,7 +1092,7 @@ int32_t launch_decode(AionCudaDevice* dev, const AttnParams& p, uint32_t units) 
   tk = *m;
   if (int32_t st = tensor_map_bytes(dev, p.v, 2, vd, &vw, vbox, &m)) return st;
   tv = *m;
-  return launch_decode_as<D, KQ8, VQ8, true>(dev, p, units, tk, tv);
+  return launch_decode_as<D, KQ8, VQ8, true>(dev, p, tk, tv, max_keys);
 }
 
 }  // namespace
@@ -928,27 +1112,13 @@ int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p, uint32_t fla
     p.l_blocks = (p.L + p.pos_per_tile - 1) / p.pos_per_tile;
     const uint64_t units = (uint64_t)p.B * p.l_blocks * p.Hkv * p.head_groups;
     if (units > 0x7FFFFFFF) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
-    // Splits: enough CTAs to fill the SMs once, none below one tile per warp.
+    // Upper bound of the keys of a unit.
     uint64_t max_keys = p.T;
     const uint64_t span = (uint64_t)(p.win_chunk ? p.win_chunk : 1) + p.win_left + p.win_right + p.pos_per_tile;
     if (p.win_left != AION_CUDA_WINDOW_UNBOUNDED && p.win_right != AION_CUDA_WINDOW_UNBOUNDED && span < max_keys) max_keys = span;
-    const uint64_t resident = (uint64_t)dev->sm_count * (p.Dk == 256 ? 2 : 3);   // DecodeGeom::CTAS
-    uint64_t splits = resident / units, most = (max_keys + TK * WARPS - 1) / (TK * WARPS);   // a split is a tile per warp at least
-    if (splits > most) splits = most;
-    if (splits > 128) splits = 128;
-    if (splits < 1) splits = 1;
-    if (dev->attn_split_override) splits = dev->attn_split_override > 128 ? 128 : dev->attn_split_override;
-    p.splits = (uint32_t)splits;
-    if (splits > 1) {
-      if (int32_t st = dev->reserve_scratch(units * splits * COLS * (p.Dk + 4) * sizeof(float))) return st;
-      if (int32_t st = dev->reserve_tickets(units)) return st;
-      p.partial = static_cast<float*>(dev->lane_scratch());
-      p.tickets = dev->lane_tickets();
-    }
-    const uint32_t u = (uint32_t)units;
 #define AION_QCACHE(D)                                                                                     \
-  if (kq8) return vq8 ? launch_decode<D, true, true>(dev, p, u) : launch_decode<D, true, false>(dev, p, u); \
-  return vq8 ? launch_decode<D, false, true>(dev, p, u) : launch_decode<D, false, false>(dev, p, u);
+  if (kq8) return vq8 ? launch_decode<D, true, true>(dev, p, max_keys) : launch_decode<D, true, false>(dev, p, max_keys); \
+  return vq8 ? launch_decode<D, false, true>(dev, p, max_keys) : launch_decode<D, false, false>(dev, p, max_keys);
     switch (p.Dk) {
       case 64: AION_QCACHE(64)
       case 128: AION_QCACHE(128)
