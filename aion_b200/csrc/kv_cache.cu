@@ -5,6 +5,7 @@
 // 16 bytes of nibbles). The codes are those of aion_cuda_quantize, so this file is compiled without FMA
 // contraction too. All three steps move each byte once and compute little: HBM bounds the large ones, the
 // launch and one trip to memory the small ones.
+#include <algorithm>
 #include <cmath>
 
 #include "cache_geom.cuh"
@@ -65,37 +66,79 @@ __device__ __forceinline__ void store_block_part(uint8_t* dst, uint32_t i, uint3
   }
 }
 
-// ---- append: eight lanes per block, blocks of all new rows in order -----------------------------
-template <int DT, typename T>
-__global__ void __launch_bounds__(256) append_quantized_kernel(uint8_t* __restrict__ cache, const T* __restrict__ rows,
+// ---- append: a warp per piece of a new row, eight lanes per block ------------------------------------
+// Four consecutive values as f32; VEC: the address is a multiple of their size.
+template <bool VEC>
+__device__ __forceinline__ void load_4(const float* p, float (&v)[4]) {
+  if (VEC) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = p[j];
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void load_4(const __half* p, float (&v)[4]) {
+  if (VEC) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = __half2float(p[j]);
+  }
+}
+
+// A piece is 16 blocks of a row (four of each lane group): where the row goes is worked out once for them, and their
+// loads are under way together.
+constexpr int PIECE = 16;
+
+template <int DT, typename T, bool VEC>
+__global__ void __launch_bounds__(128) append_quantized_kernel(uint8_t* __restrict__ cache, const T* __restrict__ rows,
                                                                const int32_t* __restrict__ end_index, CacheGeom g, uint32_t new_len,
-                                                               uint32_t blocks_per_row, uint64_t nblocks, int* fault) {
+                                                               uint32_t blocks_per_row, uint32_t pieces_per_row, uint32_t pieces, int* fault) {
   constexpr int BB = DT == AION_CUDA_DTYPE_Q8_0 ? Q8_BYTES : Q4_BYTES;
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
-  const uint32_t i = threadIdx.x & 7;
-  const uint64_t step = (uint64_t)gridDim.x * (blockDim.x / 8);
-  const uint64_t first = blockIdx.x * (uint64_t)(blockDim.x / 8) + threadIdx.x / 8;
-  for (uint64_t base = first & ~3ull; base < nblocks; base += step) {   // the four groups of a warp leave together
-    const uint64_t blk = base + (first & 3);
-    const bool on = blk < nblocks;
-    const uint64_t r = on ? blk / blocks_per_row : 0;
-    const uint32_t in_row = on ? (uint32_t)(blk - r * blocks_per_row) : 0;
-    const uint32_t b = (uint32_t)(r / new_len), t = (uint32_t)(r - (uint64_t)b * new_len);
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (on)
+  const uint32_t lane = threadIdx.x & 31, i = lane & 7, warps = gridDim.x * (blockDim.x / 32);
+  for (uint32_t piece = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; piece < pieces; piece += warps) {
+    const uint32_t r = piece / pieces_per_row, first = (piece - r * pieces_per_row) * PIECE + lane / 8;
+    const uint32_t b = r / new_len, t = r - b * new_len;
+    float v[PIECE / 4][4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) v[j] = (float)rows[blk * QK + 4 * i + j];
+    for (int k = 0; k < PIECE / 4; k++) {
+      const uint32_t blk = first + 4 * k;
+      if (blk < blocks_per_row) load_4<VEC>(rows + ((uint64_t)r * blocks_per_row + blk) * QK + 4 * i, v[k]);
+      else v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.0f;
+    }
     bool bad = false;
-    const int64_t row = on ? append_row(g, b, end_index[b], t, new_len, &bad) : -1;
-    if (bad && i == 0) atomicCAS(fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
-    uint16_t scale;
-    const uint32_t codes = quantize_4<DT>(v, &scale);
-    if (row >= 0) store_block_part<DT>(cache + ((uint64_t)row * blocks_per_row + in_row) * BB, i, codes, scale);
+    const int64_t row = append_row(g, b, end_index[b], t, new_len, &bad);
+    if (bad && lane == 0) atomicCAS(fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
+    if (row < 0) continue;   // the same for the whole warp
+    uint8_t* dst = cache + (uint64_t)row * blocks_per_row * BB;
+#pragma unroll
+    for (int k = 0; k < PIECE / 4; k++) {
+      const uint32_t blk = first + 4 * k;
+      uint16_t scale;
+      const uint32_t codes = quantize_4<DT>(v[k], &scale);
+      if (blk < blocks_per_row) store_block_part<DT>(dst + blk * BB, i, codes, scale);
+    }
   }
 }
 
 // ---- read: values of logical steps -----------------------------------------------------------------
+// The row that holds step start[b] + t, negative: none, and zeros are read.
+__device__ __forceinline__ int64_t read_row(const CacheGeom& g, const int32_t* start, const int32_t* lengths, uint32_t b, uint32_t t, bool* bad) {
+  const ReadSpan s = read_span(g, start, lengths, b);
+  *bad = s.bad;
+  const uint64_t step = (uint64_t)(start && !s.bad ? start[b] : 0) + t;
+  if (step < s.lo || step >= s.hi) return -1;
+  const int64_t row = cache_row(g, b, (uint32_t)step);
+  *bad = row < 0;
+  return row;
+}
+
 template <typename O>
 __device__ __forceinline__ O as_out(float v) { return (O)v; }
 template <>
@@ -116,7 +159,7 @@ __device__ __forceinline__ float row_value(const uint8_t* p, uint32_t e) {
   return __fmul_rn((float)q, scale);
 }
 
-// One thread per value.
+// One thread per value: rows of any size at any address.
 template <int DT, typename O>
 __global__ void __launch_bounds__(256) sequence_read_kernel(O* __restrict__ out, const uint8_t* __restrict__ cache,
                                                             const int32_t* __restrict__ start, const int32_t* __restrict__ lengths,
@@ -128,17 +171,105 @@ __global__ void __launch_bounds__(256) sequence_read_kernel(O* __restrict__ out,
     const uint64_t r = i / row_values;
     const uint32_t e = (uint32_t)(i - r * row_values);
     const uint32_t b = (uint32_t)(r / out_len), t = (uint32_t)(r - (uint64_t)b * out_len);
-    const ReadSpan s = read_span(g, start, lengths, b);
-    const uint64_t step = (uint64_t)(start && !s.bad ? start[b] : 0) + t;
-    bool bad = s.bad;
-    float v = 0.0f;
-    if (step >= s.lo && step < s.hi) {
-      const int64_t row = cache_row(g, b, (uint32_t)step);
-      if (row < 0) bad = true;
-      else v = row_value<DT>(cache + (uint64_t)row * row_bytes, e);
-    }
+    bool bad;
+    const int64_t row = read_row(g, start, lengths, b, t, &bad);
+    const float v = row >= 0 ? row_value<DT>(cache + (uint64_t)row * row_bytes, e) : 0.0f;
     if (bad) atomicCAS(fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
     out[i] = as_out<O>(v);
+  }
+}
+
+// Eight consecutive values of a stored row as f32; e is a multiple of 8, of rows that hold whole eights.
+template <int DT>
+struct Raw8 {
+  uint32_t w[DT == AION_CUDA_DTYPE_F32 ? 8 : DT == AION_CUDA_DTYPE_F16 ? 4 : DT == AION_CUDA_DTYPE_Q8_0 ? 3 : 2];
+  __device__ __forceinline__ void load(const uint8_t* row, uint32_t e) {
+    if constexpr (DT == AION_CUDA_DTYPE_F32) {
+      const uint4 a = *reinterpret_cast<const uint4*>(row + 4ull * e), b = *reinterpret_cast<const uint4*>(row + 4ull * e + 16);
+      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    } else if constexpr (DT == AION_CUDA_DTYPE_F16) {
+      const uint4 a = *reinterpret_cast<const uint4*>(row + 2ull * e);
+      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    } else {
+      // Blocks lie on 2-byte boundaries only.
+      constexpr bool Q8 = DT == AION_CUDA_DTYPE_Q8_0;
+      const uint16_t* blk = reinterpret_cast<const uint16_t*>(row + (uint64_t)(e / QK) * (Q8 ? Q8_BYTES : Q4_BYTES));
+      const uint32_t j = e % QK / 8;
+      w[0] = blk[0];
+      if (Q8) {
+        w[1] = blk[1 + 4 * j] | (uint32_t)blk[2 + 4 * j] << 16;
+        w[2] = blk[3 + 4 * j] | (uint32_t)blk[4 + 4 * j] << 16;
+      } else {
+        w[1] = blk[1 + 2 * j] | (uint32_t)blk[2 + 2 * j] << 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint32_t& x : w) x = 0;
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      if constexpr (DT == AION_CUDA_DTYPE_F32) v[k] = __uint_as_float(w[k]);
+      else if constexpr (DT == AION_CUDA_DTYPE_F16) v[k] = __half2float(__ushort_as_half((unsigned short)(w[k / 2] >> (16 * (k & 1)))));
+      else {
+        const float scale = __half2float(__ushort_as_half((unsigned short)w[0]));
+        int q;
+        if constexpr (DT == AION_CUDA_DTYPE_Q8_0) q = (int)(w[1 + k / 4] << (24 - 8 * (k & 3))) >> 24;
+        else q = (int)((w[1] >> (4 * k)) & 15) - 8;
+        v[k] = __fmul_rn((float)q, scale);
+      }
+    }
+  }
+};
+__device__ __forceinline__ void store_8(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store_8(__half* p, const float (&v)[8]) {
+  __half2 h[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+
+// A warp per piece of a row, eight values per lane and step: where the row lies is worked out once for a piece, and
+// the loads of its four steps are under way together.
+constexpr int READ_STEPS = 4;
+
+template <int DT, typename O>
+__global__ void __launch_bounds__(128) sequence_read8_kernel(O* __restrict__ out, const uint8_t* __restrict__ cache,
+                                                             const int32_t* __restrict__ start, const int32_t* __restrict__ lengths,
+                                                             CacheGeom g, uint32_t out_len, uint32_t row_eights, uint64_t row_bytes,
+                                                             uint32_t pieces_per_row, uint32_t pieces, int* fault) {
+  ptx::pdl_launch_dependents();
+  ptx::pdl_wait();
+  const uint32_t lane = threadIdx.x & 31, warps = gridDim.x * (blockDim.x / 32);
+  for (uint32_t piece = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; piece < pieces; piece += warps) {
+    const uint32_t r = piece / pieces_per_row, first = (piece - r * pieces_per_row) * (32 * READ_STEPS) + lane;
+    const uint32_t b = r / out_len, t = r - b * out_len;
+    bool bad;
+    const int64_t row = read_row(g, start, lengths, b, t, &bad);
+    if (bad && lane == 0) atomicCAS(fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
+    const uint8_t* src = cache + (uint64_t)(row < 0 ? 0 : row) * row_bytes;
+    Raw8<DT> raw[READ_STEPS];
+#pragma unroll
+    for (int k = 0; k < READ_STEPS; k++) {
+      raw[k].zero();
+      if (row >= 0 && first + 32 * k < row_eights) raw[k].load(src, 8 * (first + 32 * k));
+    }
+#pragma unroll
+    for (int k = 0; k < READ_STEPS; k++)
+      if (first + 32 * k < row_eights) {
+        float v[8];
+        raw[k].values(v);
+        // a row that is not held: zeros, not minus zeros (0 x -8)
+        if (row < 0)
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] = 0.0f;
+        store_8(out + ((uint64_t)r * row_eights + first + 32 * k) * 8, v);
+      }
   }
 }
 
@@ -251,6 +382,146 @@ __global__ void __launch_bounds__(NR_THREADS) qk_norm_rope_append_kernel(const N
   }
 }
 
+// The same for heads of 64, 128 and 256: D / 8 lanes hold a head, each of them the values 4j .. 4j + 3 of its first half
+// and of its second half (the pairs that rotate together; eight lanes hold a block). A CTA takes ROWS rows at a time:
+// first their angles, one per thread and pair, into shared memory, then the heads.
+constexpr int NRF_THREADS = 256;
+
+__device__ __forceinline__ void store_4(uint32_t dtype, uint8_t* cache, uint64_t head_index, uint32_t d, uint32_t at, const float (&v)[4], bool on) {
+  if (dtype == AION_CUDA_DTYPE_F16) {
+    const __half2 h[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
+    if (on) *reinterpret_cast<uint2*>(cache + (head_index * d + at) * 2) = *reinterpret_cast<const uint2*>(h);
+    return;
+  }
+  const uint64_t blk = head_index * (d / QK) + at / QK;
+  uint16_t scale;
+  if (dtype == AION_CUDA_DTYPE_Q8_0) {
+    const uint32_t codes = quantize_4<AION_CUDA_DTYPE_Q8_0>(v, &scale);
+    if (on) store_block_part<AION_CUDA_DTYPE_Q8_0>(cache + blk * Q8_BYTES, (at / 4) & 7, codes, scale);
+  } else {
+    const uint32_t codes = quantize_4<AION_CUDA_DTYPE_Q4_0>(v, &scale);
+    if (on) store_block_part<AION_CUDA_DTYPE_Q4_0>(cache + blk * Q4_BYTES, (at / 4) & 7, codes, scale);
+  }
+}
+
+// 1 / sqrt(x) of a double to the last bits of a float: the f32 estimate, two steps of Newton's iteration in f64.
+__device__ __forceinline__ float inverse_root(double x) {
+  if (!(x > 1e-30 && x < 1e30)) return (float)(1.0 / sqrt(x));
+  double y = (double)rsqrtf((float)x);
+  const double h = 0.5 * x;
+  y = y * (1.5 - h * y * y);
+  y = y * (1.5 - h * y * y);
+  return (float)y;
+}
+
+template <int D, int ROWS>
+__global__ void __launch_bounds__(NRF_THREADS) qk_norm_rope_append_lanes_kernel(const NormRopeParams p, uint32_t rows) {
+  constexpr int LPH = D / 8, HPW = 32 / LPH, HALF = D / 2;
+  __shared__ float cs[ROWS][HALF], sn[ROWS][HALF];
+  __shared__ int64_t dst_row[ROWS];
+  ptx::pdl_launch_dependents();
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane % LPH;
+  // Frequency of this thread's pair by repeated f32 multiplies, as the RoPE step builds it (each thread keeps one pair).
+  static_assert(NRF_THREADS % HALF == 0, "a pair per thread");
+  const uint32_t pair = tid % HALF;
+  float freq = p.scale_factor;
+  for (uint32_t k = 0; k < pair; k++) freq *= p.step;
+  ptx::pdl_wait();
+  float qg[8], kg[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const uint32_t at = 4 * j + (k & 3) + (k >> 2) * HALF;
+    qg[k] = p.q_gamma ? p.q_gamma[at] : 1.0f;
+    kg[k] = p.k_gamma ? p.k_gamma[at] : 1.0f;
+  }
+  const uint32_t slots = p.h_q + 2 * p.h_kv, per_row = (slots + HPW - 1) / HPW;   // heads; warps' loads of them
+  for (uint32_t row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
+#pragma unroll
+    for (int r = 0; r < (ROWS * HALF + NRF_THREADS - 1) / NRF_THREADS; r++) {
+      const uint32_t rr = r * (NRF_THREADS / HALF) + tid / HALF;
+      if (rr < ROWS && row0 + rr < rows) {
+        float c = 1.0f, s = 0.0f;
+        if (pair < p.rope_pairs) {
+          double sd, cd;
+          sincos((double)((float)p.positions[row0 + rr] * freq), &sd, &cd);
+          c = (float)cd, s = (float)sd;
+        }
+        cs[rr][pair] = c, sn[rr][pair] = s;
+      }
+    }
+    if (tid < ROWS && row0 + tid < rows) {
+      const uint32_t row = row0 + tid, b = row / p.len, l = row - b * p.len;
+      bool bad;
+      dst_row[tid] = append_row(p.geom, b, p.end_index[b], l, p.len, &bad);
+      if (bad) atomicCAS(p.fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
+    }
+    __syncthreads();
+    const uint32_t work = min((uint32_t)ROWS, rows - row0) * per_row;
+    for (uint32_t w = warp; w < work; w += NRF_THREADS / 32) {
+      const uint32_t rr = w / per_row, h = (w - rr * per_row) * HPW + lane / LPH;
+      const bool on = h < slots, is_q = h < p.h_q, is_v = h >= p.h_q + p.h_kv;
+      const uint64_t row = row0 + rr;
+      float x[2][4];
+      const float* src = p.qkv + row * p.ld + (uint64_t)(on ? h : 0) * D + 4 * j;
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const float4 a = *reinterpret_cast<const float4*>(src + half * HALF);
+        x[half][0] = a.x, x[half][1] = a.y, x[half][2] = a.z, x[half][3] = a.w;
+      }
+      bool good = on;
+      if (p.q_gamma || p.k_gamma) {   // (every lane takes part in the shuffles)
+        // The sum of squares is taken in 64 bits (each square is exact there): its f32 root does not depend on
+        // the order of the sum, so a code on a border does not either.
+        double ss = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) ss += (double)x[k >> 2][k & 3] * (double)x[k >> 2][k & 3];
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
+        if (!is_v && (is_q ? p.q_gamma : p.k_gamma)) {
+          const double ms = ss * (1.0 / D) + (double)p.eps;   // D is a power of two
+          if (!(ms > 0.0) || isinf(ms)) {
+            if (on && j == 0) atomicCAS(p.fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
+            good = false;
+          }
+          const float inv = inverse_root(ms);
+#pragma unroll
+          for (int k = 0; k < 8; k++) x[k >> 2][k & 3] = (x[k >> 2][k & 3] * inv) * (is_q ? qg[k] : kg[k]);
+        }
+      }
+      if (!is_v) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t pr = 4 * j + k;
+          if (pr < p.rope_pairs) {
+            const float c = cs[rr][pr], s = sn[rr][pr], a = x[0][k], b2 = x[1][k];
+            x[0][k] = a * c - b2 * s;
+            x[1][k] = a * s + b2 * c;
+          }
+        }
+      }
+      const int64_t dst = dst_row[rr];
+      // All lanes go through the quantizer of each kind that the warp has: its maxima are taken by shuffles.
+      const uint32_t hk = is_v ? h - p.h_q - p.h_kv : h - p.h_q;
+      const bool to_k = good && on && !is_q && !is_v && dst >= 0, to_v = on && is_v && dst >= 0;
+      if (is_q && good) {
+        float* qo = p.q_out + (row * p.h_q + h) * D + 4 * j;
+#pragma unroll
+        for (int half = 0; half < 2; half++) *reinterpret_cast<float4*>(qo + half * HALF) = make_float4(x[half][0], x[half][1], x[half][2], x[half][3]);
+      }
+      const uint64_t head = (uint64_t)(dst < 0 ? 0 : dst) * p.h_kv + hk;
+      if (__any_sync(FULL, to_k)) {
+        store_4(p.k_dtype, p.k_cache, head, D, 4 * j, x[0], to_k);
+        store_4(p.k_dtype, p.k_cache, head, D, HALF + 4 * j, x[1], to_k);
+      }
+      if (__any_sync(FULL, to_v)) {
+        store_4(p.v_dtype, p.v_cache, head, D, 4 * j, x[0], to_v);
+        store_4(p.v_dtype, p.v_cache, head, D, HALF + 4 * j, x[1], to_v);
+      }
+    }
+    __syncthreads();   // the angles may be overwritten
+  }
+}
+
 // ---- host side ---------------------------------------------------------------------------------------
 bool quantized(uint32_t dt) { return dt == AION_CUDA_DTYPE_Q8_0 || dt == AION_CUDA_DTYPE_Q4_0; }
 
@@ -286,36 +557,49 @@ unsigned blocks_for(const AionCudaDevice* dev, uint64_t items, unsigned per_bloc
   return (unsigned)(want < cap ? want : cap);
 }
 
+template <int DT, typename T>
+int32_t launch_append_as(AionCudaDevice* dev, const AionCudaSequenceAppend* s, uint8_t* cache, const T* rows, const int32_t* idx, const CacheGeom& g) {
+  const uint64_t bpr = s->heads * s->head_dim / QK, ppr = ceil_div(bpr, (uint64_t)PIECE), pieces = s->batch * s->new_len * ppr;
+  if (pieces > 0x7FFFFFFFull) return fail(AION_CUDA_UNSUPPORTED, "sequence_append: too many rows for one launch");
+  const bool vec = (reinterpret_cast<uintptr_t>(rows) & (4 * sizeof(T) - 1)) == 0;
+  AION_CUDA_TRY(launch_pdl(vec ? append_quantized_kernel<DT, T, true> : append_quantized_kernel<DT, T, false>, dim3(blocks_for(dev, pieces, 4)), dim3(128), 0,
+                           dev->stream, cache, rows, idx, g, (uint32_t)s->new_len, (uint32_t)bpr, (uint32_t)ppr, (uint32_t)pieces, dev->fault_dev));
+  return AION_CUDA_OK;
+}
+
 template <typename T>
 int32_t launch_append(AionCudaDevice* dev, const AionCudaSequenceAppend* s, uint8_t* cache, const T* rows, const int32_t* idx, const CacheGeom& g) {
-  const uint64_t bpr = s->heads * s->head_dim / QK, nblocks = s->batch * s->new_len * bpr;
-  const dim3 grid(blocks_for(dev, nblocks, 256 / 8)), block(256);
-  if (s->dtype == AION_CUDA_DTYPE_Q8_0)
-    AION_CUDA_TRY(launch_pdl(append_quantized_kernel<AION_CUDA_DTYPE_Q8_0, T>, grid, block, 0, dev->stream, cache, rows, idx, g, (uint32_t)s->new_len,
-                             (uint32_t)bpr, nblocks, dev->fault_dev));
-  else
-    AION_CUDA_TRY(launch_pdl(append_quantized_kernel<AION_CUDA_DTYPE_Q4_0, T>, grid, block, 0, dev->stream, cache, rows, idx, g, (uint32_t)s->new_len,
-                             (uint32_t)bpr, nblocks, dev->fault_dev));
+  if (s->dtype == AION_CUDA_DTYPE_Q8_0) return launch_append_as<AION_CUDA_DTYPE_Q8_0, T>(dev, s, cache, rows, idx, g);
+  return launch_append_as<AION_CUDA_DTYPE_Q4_0, T>(dev, s, cache, rows, idx, g);
+}
+
+template <int DT, typename O>
+int32_t launch_read_as(AionCudaDevice* dev, const AionCudaSequenceRead* s, O* out, const uint8_t* cache, const int32_t* start, const int32_t* lengths,
+                       const CacheGeom& g) {
+  const uint64_t row_values = s->heads * s->head_dim, count = s->batch * s->out_len * row_values;
+  const uint64_t row_bytes = cache_bytes(s->dtype, row_values);
+  // Eight values at a time where rows are whole eights on 16-byte boundaries (of a quantized cache: of out alone).
+  const uint64_t ppr = ceil_div(row_values / 8, (uint64_t)(32 * READ_STEPS)), pieces = s->batch * s->out_len * ppr;
+  const uintptr_t addr = reinterpret_cast<uintptr_t>(out) | (quantized(s->dtype) ? 0 : reinterpret_cast<uintptr_t>(cache) | row_bytes);
+  if (row_values % 8 == 0 && (addr & 15) == 0 && pieces <= 0x7FFFFFFFull) {
+    AION_CUDA_TRY(launch_pdl(sequence_read8_kernel<DT, O>, dim3(blocks_for(dev, pieces, 4)), dim3(128), 0, dev->stream, out, cache, start, lengths, g,
+                             (uint32_t)s->out_len, (uint32_t)(row_values / 8), row_bytes, (uint32_t)ppr, (uint32_t)pieces, dev->fault_dev));
+  } else {
+    AION_CUDA_TRY(launch_pdl(sequence_read_kernel<DT, O>, dim3(blocks_for(dev, count, 256)), dim3(256), 0, dev->stream, out, cache, start, lengths, g,
+                             (uint32_t)s->out_len, (uint32_t)row_values, row_bytes, count, dev->fault_dev));
+  }
   return AION_CUDA_OK;
 }
 
 template <typename O>
 int32_t launch_read(AionCudaDevice* dev, const AionCudaSequenceRead* s, O* out, const uint8_t* cache, const int32_t* start, const int32_t* lengths,
                     const CacheGeom& g) {
-  const uint64_t row_values = s->heads * s->head_dim, count = s->batch * s->out_len * row_values;
-  const uint64_t row_bytes = cache_bytes(s->dtype, row_values);
-  const dim3 grid(blocks_for(dev, count, 256)), block(256);
-#define AION_READ(DT)                                                                                                          \
-  AION_CUDA_TRY(launch_pdl(sequence_read_kernel<DT, O>, grid, block, 0, dev->stream, out, cache, start, lengths, g, (uint32_t)s->out_len, \
-                           (uint32_t)row_values, row_bytes, count, dev->fault_dev))
   switch (s->dtype) {
-    case AION_CUDA_DTYPE_F32: AION_READ(AION_CUDA_DTYPE_F32); break;
-    case AION_CUDA_DTYPE_F16: AION_READ(AION_CUDA_DTYPE_F16); break;
-    case AION_CUDA_DTYPE_Q8_0: AION_READ(AION_CUDA_DTYPE_Q8_0); break;
-    default: AION_READ(AION_CUDA_DTYPE_Q4_0); break;
+    case AION_CUDA_DTYPE_F32: return launch_read_as<AION_CUDA_DTYPE_F32>(dev, s, out, cache, start, lengths, g);
+    case AION_CUDA_DTYPE_F16: return launch_read_as<AION_CUDA_DTYPE_F16>(dev, s, out, cache, start, lengths, g);
+    case AION_CUDA_DTYPE_Q8_0: return launch_read_as<AION_CUDA_DTYPE_Q8_0>(dev, s, out, cache, start, lengths, g);
+    default: return launch_read_as<AION_CUDA_DTYPE_Q4_0>(dev, s, out, cache, start, lengths, g);
   }
-#undef AION_READ
-  return AION_CUDA_OK;
 }
 
 }  // namespace
@@ -436,6 +720,24 @@ int32_t aion_cuda_qk_norm_rope_append(AionCudaDevice* dev, const AionCudaQKNormR
   p.scale_factor = s->scale_factor, p.eps = s->eps;
   p.k_dtype = s->k_dtype, p.v_dtype = s->v_dtype;
   p.fault = dev->fault_dev;
+  // Heads of 64, 128 and 256 at addresses of 16 bytes (8 in an f16 cache): eight values a lane. Four rows a CTA while
+  // the rows fill the SMs four times over that way, one below.
+  uintptr_t at16 = reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.qkv) | (ld * 4), at8 = 0;
+  if (s->k_dtype == AION_CUDA_DTYPE_F16) at8 |= reinterpret_cast<uintptr_t>(p.k_cache);
+  if (s->v_dtype == AION_CUDA_DTYPE_F16) at8 |= reinterpret_cast<uintptr_t>(p.v_cache);
+  if ((d == 64 || d == 128 || d == 256) && (at16 & 15) == 0 && (at8 & 7) == 0) {
+    const uint64_t sms = (uint64_t)dev->sm_count;
+    const bool four = rows >= 16 * sms;
+    const unsigned grid = (unsigned)std::min<uint64_t>(four ? (rows + 3) / 4 : rows, sms * 8);
+#define AION_NRF(DD)                                                                                                                        \
+    AION_CUDA_TRY(launch_pdl(four ? qk_norm_rope_append_lanes_kernel<DD, 4> : qk_norm_rope_append_lanes_kernel<DD, 1>, dim3(grid), dim3(NRF_THREADS), 0, \
+                             dev->stream, p, (uint32_t)rows))
+    if (d == 64) AION_NRF(64);
+    else if (d == 128) AION_NRF(128);
+    else AION_NRF(256);
+#undef AION_NRF
+    return AION_CUDA_OK;
+  }
   const size_t smem = (d + NR_WARPS * d) * sizeof(float);
   AION_CUDA_TRY(launch_pdl(qk_norm_rope_append_kernel, dim3((unsigned)rows), dim3(NR_THREADS), smem, dev->stream, p));
   return AION_CUDA_OK;
