@@ -20,8 +20,12 @@ namespace {
 constexpr uint32_t FULL = 0xFFFFFFFFu;
 
 // ---- the block quantizer, eight lanes to a block ------------------------------------------------
+// Nearest whole number, halves away from zero, as the int conversion of roundf: the sum is cut off towards zero, so
+// 0.5 minus an ulp stays below one. (One operation on the conversion unit instead of roundf's two.) NaN gives 0.
+__device__ __forceinline__ int round_away(float r) { return __float2int_rz(__fadd_rz(r, copysignf(0.5f, r))); }
+
 // Lane i of eight (i = lane & 7) holds values 4i .. 4i + 3 of a block. Returns the block's f16 scale and this
-// lane's codes: q8_0 four bytes, q4_0 four nibbles. Operation for operation the block quantizer of quant.cu.
+// lane's codes: q8_0 four bytes, q4_0 four nibbles. The same numbers as the block quantizer of quant.cu.
 // All lanes of a warp call it together.
 template <int DT>
 __device__ __forceinline__ uint32_t quantize_4(const float (&v)[4], uint16_t* scale_bits) {
@@ -35,18 +39,34 @@ __device__ __forceinline__ uint32_t quantize_4(const float (&v)[4], uint16_t* sc
     const __half sh = __float2half_rn(scale);
     *scale_bits = __half_as_ushort(sh);
     const float eff = __half2float(sh);
-    const float inv = (amax == 0.0f || eff == 0.0f) ? 0.0f : __fdiv_rn(1.0f, eff);
+    const float inv = (amax == 0.0f || eff == 0.0f) ? 0.0f : __frcp_rn(eff);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const int q = max(-128, min(127, (int)roundf(__fmul_rn(v[j], inv))));
+      const int q = max(-128, min(127, round_away(__fmul_rn(v[j], inv))));
       codes |= ((uint32_t)q & 0xFFu) << (8 * j);
     }
   } else {
     const float scale = amax == 0.0f ? 1.0f : __fdiv_rn(amax, 7.0f);
     *scale_bits = __half_as_ushort(__float2half_rn(scale));
+    float r[4];
+    if (scale > 1e-30f && scale < 1e30f) {
+      // Correctly rounded quotients by one divisor: its correctly rounded reciprocal y, q = v y, and twice
+      // q + (v - scale q) y with fused products (P. Markstein, Computation of elementary functions on the IBM RISC
+      // System/6000, 1990). The remainders are exact but where the quotient is far below one half.
+      const float y = __frcp_rn(scale);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        float q = __fmul_rn(v[j], y);
+        q = __fmaf_rn(__fmaf_rn(-scale, q, v[j]), y, q);
+        r[j] = __fmaf_rn(__fmaf_rn(-scale, q, v[j]), y, q);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) r[j] = __fdiv_rn(v[j], scale);
+    }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const int q = max(-8, min(7, (int)roundf(__fdiv_rn(v[j], scale)))) + 8;
+      const int q = max(-8, min(7, round_away(r[j]))) + 8;
       codes |= (uint32_t)q << (4 * j);
     }
   }
@@ -383,9 +403,11 @@ __global__ void __launch_bounds__(NR_THREADS) qk_norm_rope_append_kernel(const N
 }
 
 // The same for heads of 64, 128 and 256: D / 8 lanes hold a head, each of them the values 4j .. 4j + 3 of its first half
-// and of its second half (the pairs that rotate together; eight lanes hold a block). A CTA takes ROWS rows at a time:
-// first their angles, one per thread and pair, into shared memory, then the heads.
-constexpr int NRF_THREADS = 256;
+// and of its second half (the pairs that rotate together; eight lanes hold a block). The warps' loads of all rows, 256
+// values each, are cut into equal runs, one per resident warp: a warp works out a row's angles, a few a lane, keeps them
+// in registers while it walks the row's heads, and has the next load's values on their way.
+constexpr int NRF_THREADS = 128;
+constexpr int NRF_CTAS = 6;   // an SM: 80 registers a thread (5 CTAs, 6 and, with spills, 8: 139, 134 and 147 us for 16000 rows of 16 heads of 256)
 
 __device__ __forceinline__ void store_4(uint32_t dtype, uint8_t* cache, uint64_t head_index, uint32_t d, uint32_t at, const float (&v)[4], bool on) {
   if (dtype == AION_CUDA_DTYPE_F16) {
@@ -414,18 +436,17 @@ __device__ __forceinline__ float inverse_root(double x) {
   return (float)y;
 }
 
-template <int D, int ROWS>
-__global__ void __launch_bounds__(NRF_THREADS) qk_norm_rope_append_lanes_kernel(const NormRopeParams p, uint32_t rows) {
-  constexpr int LPH = D / 8, HPW = 32 / LPH, HALF = D / 2;
-  __shared__ float cs[ROWS][HALF], sn[ROWS][HALF];
-  __shared__ int64_t dst_row[ROWS];
+template <int D>
+__global__ void __launch_bounds__(NRF_THREADS, NRF_CTAS) qk_norm_rope_append_lanes_kernel(const NormRopeParams p, uint32_t total, uint32_t run) {
+  constexpr int LPH = D / 8, HPW = 32 / LPH, HALF = D / 2, PPL = D / 64;   // lanes a head, heads a load, pairs a lane works out
   ptx::pdl_launch_dependents();
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane % LPH;
-  // Frequency of this thread's pair by repeated f32 multiplies, as the RoPE step builds it (each thread keeps one pair).
-  static_assert(NRF_THREADS % HALF == 0, "a pair per thread");
-  const uint32_t pair = tid % HALF;
-  float freq = p.scale_factor;
-  for (uint32_t k = 0; k < pair; k++) freq *= p.step;
+  const uint32_t lane = threadIdx.x & 31, j = lane % LPH;
+  // Frequencies of this lane's pairs by repeated f32 multiplies, as the RoPE step builds them.
+  float freq[PPL];
+  freq[0] = p.scale_factor;
+  for (uint32_t k = 0; k < lane * PPL; k++) freq[0] *= p.step;
+#pragma unroll
+  for (int k = 1; k < PPL; k++) freq[k] = freq[k - 1] * p.step;
   ptx::pdl_wait();
   float qg[8], kg[8];
 #pragma unroll
@@ -434,42 +455,51 @@ __global__ void __launch_bounds__(NRF_THREADS) qk_norm_rope_append_lanes_kernel(
     qg[k] = p.q_gamma ? p.q_gamma[at] : 1.0f;
     kg[k] = p.k_gamma ? p.k_gamma[at] : 1.0f;
   }
-  const uint32_t slots = p.h_q + 2 * p.h_kv, per_row = (slots + HPW - 1) / HPW;   // heads; warps' loads of them
-  for (uint32_t row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
+  const bool norms = p.q_gamma || p.k_gamma;
+  const uint32_t slots = p.h_q + 2 * p.h_kv, loads = (slots + HPW - 1) / HPW;   // heads of a row, and the warp's loads of them
+  const uint64_t begin = (uint64_t)run * (blockIdx.x * (NRF_THREADS / 32) + threadIdx.x / 32);
+  if (begin >= total) return;
+  uint32_t left = min(run, total - (uint32_t)begin), row = (uint32_t)begin / loads, n = (uint32_t)begin - row * loads;
+  float4 ahead[2];
+  auto load = [&](uint32_t r, uint32_t k) {
+    const uint32_t h = min(k * HPW + lane / LPH, slots - 1);
+    const float* src = p.qkv + (uint64_t)r * p.ld + h * D + 4 * j;
+    ahead[0] = *reinterpret_cast<const float4*>(src);
+    ahead[1] = *reinterpret_cast<const float4*>(src + HALF);
+  };
+  load(row, n);
+  while (left > 0) {
+    const uint32_t b = row / p.len, l = row - b * p.len;
+    bool bad;
+    const int64_t dst = append_row(p.geom, b, p.end_index[b], l, p.len, &bad);
+    if (bad && lane == 0) atomicCAS(p.fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
+    // the angles of pairs 4j .. 4j + 3
+    float cs[4], sn[4];
+    {
+      const float pos = (float)p.positions[row];
+      float c[PPL], s[PPL];
 #pragma unroll
-    for (int r = 0; r < (ROWS * HALF + NRF_THREADS - 1) / NRF_THREADS; r++) {
-      const uint32_t rr = r * (NRF_THREADS / HALF) + tid / HALF;
-      if (rr < ROWS && row0 + rr < rows) {
-        float c = 1.0f, s = 0.0f;
-        if (pair < p.rope_pairs) {
+      for (int k = 0; k < PPL; k++) {
+        c[k] = 1.0f, s[k] = 0.0f;
+        if (lane * PPL + k < p.rope_pairs) {
           double sd, cd;
-          sincos((double)((float)p.positions[row0 + rr] * freq), &sd, &cd);
-          c = (float)cd, s = (float)sd;
+          sincos((double)(pos * freq[k]), &sd, &cd);
+          c[k] = (float)cd, s[k] = (float)sd;
         }
-        cs[rr][pair] = c, sn[rr][pair] = s;
       }
-    }
-    if (tid < ROWS && row0 + tid < rows) {
-      const uint32_t row = row0 + tid, b = row / p.len, l = row - b * p.len;
-      bool bad;
-      dst_row[tid] = append_row(p.geom, b, p.end_index[b], l, p.len, &bad);
-      if (bad) atomicCAS(p.fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
-    }
-    __syncthreads();
-    const uint32_t work = min((uint32_t)ROWS, rows - row0) * per_row;
-    for (uint32_t w = warp; w < work; w += NRF_THREADS / 32) {
-      const uint32_t rr = w / per_row, h = (w - rr * per_row) * HPW + lane / LPH;
-      const bool on = h < slots, is_q = h < p.h_q, is_v = h >= p.h_q + p.h_kv;
-      const uint64_t row = row0 + rr;
-      float x[2][4];
-      const float* src = p.qkv + row * p.ld + (uint64_t)(on ? h : 0) * D + 4 * j;
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
-        const float4 a = *reinterpret_cast<const float4*>(src + half * HALF);
-        x[half][0] = a.x, x[half][1] = a.y, x[half][2] = a.z, x[half][3] = a.w;
+      for (int k = 0; k < 4; k++) {
+        cs[k] = PPL == 4 ? c[k % PPL] : __shfl_sync(FULL, c[k % PPL], (4 * j + k) / PPL);
+        sn[k] = PPL == 4 ? s[k % PPL] : __shfl_sync(FULL, s[k % PPL], (4 * j + k) / PPL);
       }
+    }
+    for (; n < loads && left > 0; n++, left--) {
+      float x[2][4] = {{ahead[0].x, ahead[0].y, ahead[0].z, ahead[0].w}, {ahead[1].x, ahead[1].y, ahead[1].z, ahead[1].w}};
+      if (left > 1) load(n + 1 < loads ? row : row + 1, n + 1 < loads ? n + 1 : 0);
+      const uint32_t h = n * HPW + lane / LPH;
+      const bool on = h < slots, is_q = h < p.h_q, is_v = h >= p.h_q + p.h_kv;
       bool good = on;
-      if (p.q_gamma || p.k_gamma) {   // (every lane takes part in the shuffles)
+      if (norms && n * HPW < p.h_q + p.h_kv) {   // (every lane takes part in the shuffles)
         // The sum of squares is taken in 64 bits (each square is exact there): its f32 root does not depend on
         // the order of the sum, so a code on a border does not either.
         double ss = 0.0;
@@ -491,34 +521,32 @@ __global__ void __launch_bounds__(NRF_THREADS) qk_norm_rope_append_lanes_kernel(
       if (!is_v) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const uint32_t pr = 4 * j + k;
-          if (pr < p.rope_pairs) {
-            const float c = cs[rr][pr], s = sn[rr][pr], a = x[0][k], b2 = x[1][k];
-            x[0][k] = a * c - b2 * s;
-            x[1][k] = a * s + b2 * c;
-          }
+          const float a = x[0][k], b2 = x[1][k];
+          const bool turn = 4 * j + k < p.rope_pairs;
+          x[0][k] = turn ? a * cs[k] - b2 * sn[k] : a;
+          x[1][k] = turn ? a * sn[k] + b2 * cs[k] : b2;
         }
       }
-      const int64_t dst = dst_row[rr];
-      // All lanes go through the quantizer of each kind that the warp has: its maxima are taken by shuffles.
-      const uint32_t hk = is_v ? h - p.h_q - p.h_kv : h - p.h_q;
-      const bool to_k = good && on && !is_q && !is_v && dst >= 0, to_v = on && is_v && dst >= 0;
       if (is_q && good) {
-        float* qo = p.q_out + (row * p.h_q + h) * D + 4 * j;
-#pragma unroll
-        for (int half = 0; half < 2; half++) *reinterpret_cast<float4*>(qo + half * HALF) = make_float4(x[half][0], x[half][1], x[half][2], x[half][3]);
+        float* qo = p.q_out + ((uint64_t)row * p.h_q + h) * D + 4 * j;
+        *reinterpret_cast<float4*>(qo) = make_float4(x[0][0], x[0][1], x[0][2], x[0][3]);
+        *reinterpret_cast<float4*>(qo + HALF) = make_float4(x[1][0], x[1][1], x[1][2], x[1][3]);
       }
-      const uint64_t head = (uint64_t)(dst < 0 ? 0 : dst) * p.h_kv + hk;
-      if (__any_sync(FULL, to_k)) {
+      // All lanes go through the quantizer of each cache that the warp has heads for: its maxima are taken by shuffles.
+      if ((n + 1) * HPW > p.h_q && n * HPW < p.h_q + p.h_kv) {
+        const bool to_k = good && !is_q && !is_v && dst >= 0;
+        const uint64_t head = (uint64_t)(dst < 0 ? 0 : dst) * p.h_kv + (h - p.h_q);
         store_4(p.k_dtype, p.k_cache, head, D, 4 * j, x[0], to_k);
         store_4(p.k_dtype, p.k_cache, head, D, HALF + 4 * j, x[1], to_k);
       }
-      if (__any_sync(FULL, to_v)) {
+      if ((n + 1) * HPW > p.h_q + p.h_kv) {
+        const bool to_v = on && is_v && dst >= 0;
+        const uint64_t head = (uint64_t)(dst < 0 ? 0 : dst) * p.h_kv + (h - p.h_q - p.h_kv);
         store_4(p.v_dtype, p.v_cache, head, D, 4 * j, x[0], to_v);
         store_4(p.v_dtype, p.v_cache, head, D, HALF + 4 * j, x[1], to_v);
       }
     }
-    __syncthreads();   // the angles may be overwritten
+    row++, n = 0;
   }
 }
 
@@ -720,23 +748,22 @@ int32_t aion_cuda_qk_norm_rope_append(AionCudaDevice* dev, const AionCudaQKNormR
   p.scale_factor = s->scale_factor, p.eps = s->eps;
   p.k_dtype = s->k_dtype, p.v_dtype = s->v_dtype;
   p.fault = dev->fault_dev;
-  // Heads of 64, 128 and 256 at addresses of 16 bytes (8 in an f16 cache): eight values a lane. Four rows a CTA while
-  // the rows fill the SMs four times over that way, one below.
+  // Heads of 64, 128 and 256 at addresses of 16 bytes (8 in an f16 cache): eight values a lane.
   uintptr_t at16 = reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.qkv) | (ld * 4), at8 = 0;
   if (s->k_dtype == AION_CUDA_DTYPE_F16) at8 |= reinterpret_cast<uintptr_t>(p.k_cache);
   if (s->v_dtype == AION_CUDA_DTYPE_F16) at8 |= reinterpret_cast<uintptr_t>(p.v_cache);
   if ((d == 64 || d == 128 || d == 256) && (at16 & 15) == 0 && (at8 & 7) == 0) {
-    const uint64_t sms = (uint64_t)dev->sm_count;
-    const bool four = rows >= 16 * sms;
-    const unsigned grid = (unsigned)std::min<uint64_t>(four ? (rows + 3) / 4 : rows, sms * 8);
-#define AION_NRF(DD)                                                                                                                        \
-    AION_CUDA_TRY(launch_pdl(four ? qk_norm_rope_append_lanes_kernel<DD, 4> : qk_norm_rope_append_lanes_kernel<DD, 1>, dim3(grid), dim3(NRF_THREADS), 0, \
-                             dev->stream, p, (uint32_t)rows))
-    if (d == 64) AION_NRF(64);
-    else if (d == 128) AION_NRF(128);
-    else AION_NRF(256);
+    const uint64_t total = rows * ceil_div(s->h_q + 2 * s->h_kv, 256 / d), resident = (uint64_t)dev->sm_count * NRF_CTAS * (NRF_THREADS / 32);
+    const uint64_t run = ceil_div(total, resident);
+    if (total <= 0x7FFFFFFFull) {
+      const dim3 grid((unsigned)ceil_div(ceil_div(total, run), (uint64_t)(NRF_THREADS / 32))), block(NRF_THREADS);
+#define AION_NRF(DD) AION_CUDA_TRY(launch_pdl(qk_norm_rope_append_lanes_kernel<DD>, grid, block, 0, dev->stream, p, (uint32_t)total, (uint32_t)run))
+      if (d == 64) AION_NRF(64);
+      else if (d == 128) AION_NRF(128);
+      else AION_NRF(256);
 #undef AION_NRF
-    return AION_CUDA_OK;
+      return AION_CUDA_OK;
+    }
   }
   const size_t smem = (d + NR_WARPS * d) * sizeof(float);
   AION_CUDA_TRY(launch_pdl(qk_norm_rope_append_kernel, dim3((unsigned)rows), dim3(NR_THREADS), smem, dev->stream, p));
