@@ -24,6 +24,15 @@ constexpr uint32_t FULL = 0xFFFFFFFFu;
 // 0.5 minus an ulp stays below one. (One operation on the conversion unit instead of roundf's two.) NaN gives 0.
 __device__ __forceinline__ int round_away(float r) { return __float2int_rz(__fadd_rz(r, copysignf(0.5f, r))); }
 
+// v / s correctly rounded, for a divisor that many values share: y is its correctly rounded reciprocal, and the quotient
+// v y is corrected twice by q + (v - s q) y with fused products (P. Markstein, Computation of elementary functions on
+// the IBM RISC System/6000, 1990). The remainders are exact but where the quotient is far below one half.
+__device__ __forceinline__ float quotient(float v, float s, float y) {
+  float q = __fmul_rn(v, y);
+  q = __fmaf_rn(__fmaf_rn(-s, q, v), y, q);
+  return __fmaf_rn(__fmaf_rn(-s, q, v), y, q);
+}
+
 // Lane i of eight (i = lane & 7) holds values 4i .. 4i + 3 of a block. Returns the block's f16 scale and this
 // lane's codes: q8_0 four bytes, q4_0 four nibbles. The same numbers as the block quantizer of quant.cu.
 // All lanes of a warp call it together.
@@ -34,41 +43,39 @@ __device__ __forceinline__ uint32_t quantize_4(const float (&v)[4], uint16_t* sc
   amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
   amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 4));
   uint32_t codes = 0;
+  // Scales far from f32's ends, and from f16's lower one: every quotient is within half a code of the range, and none
+  // has to be cut off.
+  const bool plain = amax > 1e-2f && amax < 1e30f;
   if (DT == AION_CUDA_DTYPE_Q8_0) {
-    const float scale = amax == 0.0f ? 1.0f : __fdiv_rn(amax, 127.0f);
+    float scale = 1.0f;
+    if (plain) scale = quotient(amax, 127.0f, 1.0f / 127.0f);
+    else if (amax != 0.0f) scale = __fdiv_rn(amax, 127.0f);
     const __half sh = __float2half_rn(scale);
     *scale_bits = __half_as_ushort(sh);
     const float eff = __half2float(sh);
     const float inv = (amax == 0.0f || eff == 0.0f) ? 0.0f : __frcp_rn(eff);
+    int q[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int q = max(-128, min(127, round_away(__fmul_rn(v[j], inv))));
-      codes |= ((uint32_t)q & 0xFFu) << (8 * j);
-    }
+    for (int j = 0; j < 4; j++) q[j] = round_away(__fmul_rn(v[j], inv));
+    if (!plain)
+#pragma unroll
+      for (int j = 0; j < 4; j++) q[j] = max(-128, min(127, q[j]));
+    codes = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
   } else {
-    const float scale = amax == 0.0f ? 1.0f : __fdiv_rn(amax, 7.0f);
-    *scale_bits = __half_as_ushort(__float2half_rn(scale));
-    float r[4];
-    if (scale > 1e-30f && scale < 1e30f) {
-      // Correctly rounded quotients by one divisor: its correctly rounded reciprocal y, q = v y, and twice
-      // q + (v - scale q) y with fused products (P. Markstein, Computation of elementary functions on the IBM RISC
-      // System/6000, 1990). The remainders are exact but where the quotient is far below one half.
-      const float y = __frcp_rn(scale);
+    int q[4];
+    if (plain) {
+      const float scale = quotient(amax, 7.0f, 1.0f / 7.0f), y = __frcp_rn(scale);
+      *scale_bits = __half_as_ushort(__float2half_rn(scale));
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        float q = __fmul_rn(v[j], y);
-        q = __fmaf_rn(__fmaf_rn(-scale, q, v[j]), y, q);
-        r[j] = __fmaf_rn(__fmaf_rn(-scale, q, v[j]), y, q);
-      }
+      for (int j = 0; j < 4; j++) q[j] = round_away(quotient(v[j], scale, y));
     } else {
+      const float scale = amax == 0.0f ? 1.0f : __fdiv_rn(amax, 7.0f);
+      *scale_bits = __half_as_ushort(__float2half_rn(scale));
 #pragma unroll
-      for (int j = 0; j < 4; j++) r[j] = __fdiv_rn(v[j], scale);
+      for (int j = 0; j < 4; j++) q[j] = max(-8, min(7, round_away(__fdiv_rn(v[j], scale))));
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int q = max(-8, min(7, round_away(r[j]))) + 8;
-      codes |= (uint32_t)q << (4 * j);
-    }
+    for (int j = 0; j < 4; j++) codes += (uint32_t)(q[j] + 8) << (4 * j);
   }
   return codes;
 }
@@ -409,20 +416,20 @@ __global__ void __launch_bounds__(NR_THREADS) qk_norm_rope_append_kernel(const N
 constexpr int NRF_THREADS = 128;
 constexpr int NRF_CTAS = 6;   // an SM: 80 registers a thread (5 CTAs, 6 and, with spills, 8: 139, 134 and 147 us for 16000 rows of 16 heads of 256)
 
-__device__ __forceinline__ void store_4(uint32_t dtype, uint8_t* cache, uint64_t head_index, uint32_t d, uint32_t at, const float (&v)[4], bool on) {
+// A lane's four values into a head: `dst` is where they belong in an f16 cache, or their block in a quantized one.
+__device__ __forceinline__ void store_4(uint32_t dtype, uint8_t* dst, uint32_t i, const float (&v)[4], bool on) {
   if (dtype == AION_CUDA_DTYPE_F16) {
     const __half2 h[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
-    if (on) *reinterpret_cast<uint2*>(cache + (head_index * d + at) * 2) = *reinterpret_cast<const uint2*>(h);
+    if (on) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
     return;
   }
-  const uint64_t blk = head_index * (d / QK) + at / QK;
   uint16_t scale;
   if (dtype == AION_CUDA_DTYPE_Q8_0) {
     const uint32_t codes = quantize_4<AION_CUDA_DTYPE_Q8_0>(v, &scale);
-    if (on) store_block_part<AION_CUDA_DTYPE_Q8_0>(cache + blk * Q8_BYTES, (at / 4) & 7, codes, scale);
+    if (on) store_block_part<AION_CUDA_DTYPE_Q8_0>(dst, i, codes, scale);
   } else {
     const uint32_t codes = quantize_4<AION_CUDA_DTYPE_Q4_0>(v, &scale);
-    if (on) store_block_part<AION_CUDA_DTYPE_Q4_0>(cache + blk * Q4_BYTES, (at / 4) & 7, codes, scale);
+    if (on) store_block_part<AION_CUDA_DTYPE_Q4_0>(dst, i, codes, scale);
   }
 }
 
@@ -448,14 +455,12 @@ __global__ void __launch_bounds__(NRF_THREADS, NRF_CTAS) qk_norm_rope_append_lan
 #pragma unroll
   for (int k = 1; k < PPL; k++) freq[k] = freq[k - 1] * p.step;
   ptx::pdl_wait();
-  float qg[8], kg[8];
-#pragma unroll
-  for (int k = 0; k < 8; k++) {
-    const uint32_t at = 4 * j + (k & 3) + (k >> 2) * HALF;
-    qg[k] = p.q_gamma ? p.q_gamma[at] : 1.0f;
-    kg[k] = p.k_gamma ? p.k_gamma[at] : 1.0f;
-  }
   const bool norms = p.q_gamma || p.k_gamma;
+  // Bytes of a head in each cache, and where this lane's values of its first and second half lie in it.
+  auto size_of = [](uint32_t dt, uint32_t values) {
+    return dt == AION_CUDA_DTYPE_F16 ? values * 2 : values / QK * (dt == AION_CUDA_DTYPE_Q8_0 ? Q8_BYTES : Q4_BYTES);
+  };
+  const uint32_t k_head = size_of(p.k_dtype, D), k_at = size_of(p.k_dtype, 4 * j), v_head = size_of(p.v_dtype, D), v_at = size_of(p.v_dtype, 4 * j);
   const uint32_t slots = p.h_q + 2 * p.h_kv, loads = (slots + HPW - 1) / HPW;   // heads of a row, and the warp's loads of them
   const uint64_t begin = (uint64_t)run * (blockIdx.x * (NRF_THREADS / 32) + threadIdx.x / 32);
   if (begin >= total) return;
@@ -473,6 +478,8 @@ __global__ void __launch_bounds__(NRF_THREADS, NRF_CTAS) qk_norm_rope_append_lan
     bool bad;
     const int64_t dst = append_row(p.geom, b, p.end_index[b], l, p.len, &bad);
     if (bad && lane == 0) atomicCAS(p.fault, FAULT_NONE, FAULT_INVALID_ARGUMENT);
+    uint8_t* const k_row = p.k_cache + (uint64_t)(dst < 0 ? 0 : dst) * p.h_kv * k_head + k_at;
+    uint8_t* const v_row = p.v_cache + (uint64_t)(dst < 0 ? 0 : dst) * p.h_kv * v_head + v_at;
     // the angles of pairs 4j .. 4j + 3
     float cs[4], sn[4];
     {
@@ -514,8 +521,9 @@ __global__ void __launch_bounds__(NRF_THREADS, NRF_CTAS) qk_norm_rope_append_lan
             good = false;
           }
           const float inv = inverse_root(ms);
+          const float* gamma = (is_q ? p.q_gamma : p.k_gamma) + 4 * j;   // (a kilobyte that stays in L1)
 #pragma unroll
-          for (int k = 0; k < 8; k++) x[k >> 2][k & 3] = (x[k >> 2][k & 3] * inv) * (is_q ? qg[k] : kg[k]);
+          for (int k = 0; k < 8; k++) x[k >> 2][k & 3] = (x[k >> 2][k & 3] * inv) * __ldg(gamma + (k & 3) + (k >> 2) * HALF);
         }
       }
       if (!is_v) {
@@ -535,15 +543,15 @@ __global__ void __launch_bounds__(NRF_THREADS, NRF_CTAS) qk_norm_rope_append_lan
       // All lanes go through the quantizer of each cache that the warp has heads for: its maxima are taken by shuffles.
       if ((n + 1) * HPW > p.h_q && n * HPW < p.h_q + p.h_kv) {
         const bool to_k = good && !is_q && !is_v && dst >= 0;
-        const uint64_t head = (uint64_t)(dst < 0 ? 0 : dst) * p.h_kv + (h - p.h_q);
-        store_4(p.k_dtype, p.k_cache, head, D, 4 * j, x[0], to_k);
-        store_4(p.k_dtype, p.k_cache, head, D, HALF + 4 * j, x[1], to_k);
+        uint8_t* at = k_row + (to_k ? h - p.h_q : 0) * k_head;
+        store_4(p.k_dtype, at, j & 7, x[0], to_k);
+        store_4(p.k_dtype, at + k_head / 2, j & 7, x[1], to_k);
       }
       if ((n + 1) * HPW > p.h_q + p.h_kv) {
         const bool to_v = on && is_v && dst >= 0;
-        const uint64_t head = (uint64_t)(dst < 0 ? 0 : dst) * p.h_kv + (h - p.h_q - p.h_kv);
-        store_4(p.v_dtype, p.v_cache, head, D, 4 * j, x[0], to_v);
-        store_4(p.v_dtype, p.v_cache, head, D, HALF + 4 * j, x[1], to_v);
+        uint8_t* at = v_row + (to_v ? h - p.h_q - p.h_kv : 0) * v_head;
+        store_4(p.v_dtype, at, j & 7, x[0], to_v);
+        store_4(p.v_dtype, at + v_head / 2, j & 7, x[1], to_v);
       }
     }
     row++, n = 0;

@@ -696,3 +696,23 @@ def test_rows_on_and_off_sixteen_byte_boundaries(sess, layout, page, T, H, D, kd
     pos = np.array([[n - 1] for n in lens], dtype=np.int32)
     got, _ = run_attention(sess, q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, layout=layout, page=page, window=AttentionWindow.causal())
     check(got, *ref.attention(q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, rolling=layout == "rolling"))
+
+
+@pytest.mark.parametrize("dtype", [Q8, Q4], ids=["q8", "q4"])
+def test_append_rounds_every_quotient_as_the_quantizer_does(sess, dtype):
+    """Values on and beside the borders between codes, for many scales: every byte is the quantizer's."""
+    from aion_b200.backend import quantize
+    s, store = sess
+    rng = np.random.default_rng(41)
+    n = 20000
+    top = (np.exp(rng.uniform(-6, 6, (n, 1))) * (1 + rng.integers(0, 2, (n, 1)))).astype(np.float32)
+    levels = 127 if dtype == Q8 else 7
+    scale = (top / np.float32(levels)).astype(np.float32)
+    near = (rng.integers(-levels, levels, (n, 31)) + 0.5) * (scale.astype(np.float16).astype(np.float32) if dtype == Q8 else scale)
+    near = near.astype(np.float32)
+    near = (near.view(np.int32) + rng.integers(-2, 3, (n, 31), dtype=np.int32)).view(np.float32)   # up to two ulps off the border
+    rows = np.concatenate([top, np.clip(near, -top, top)], 1).astype(np.float32)
+    zeros = np.zeros((1, n, 1, 32 // 32 * (34 if dtype == Q8 else 18)), np.uint8)
+    tc = put_cache(store, zeros, dtype, 32)
+    s.execute([StepSequenceAppend(cache=tc, new_kv=put(store, rows.reshape(1, n, 1, 32), F32), end_index=put(store, np.zeros(1, np.int32), I32))])
+    assert np.array_equal(store.read(tc).view(np.uint8).reshape(-1), quantize(s.backend, dtype, rows, 1))
