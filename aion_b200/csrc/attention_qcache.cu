@@ -9,14 +9,14 @@
 #include <cstdlib>
 #include <mutex>
 
-#include "attention_device.cuh"
+#include "attention_qcache.cuh"
 #include "cache_geom.cuh"
 
 namespace aion {
 
 namespace {
 
-constexpr uint32_t FULL = 0xFFFFFFFFu;
+using namespace qcache;
 
 __device__ __forceinline__ CacheGeom geom_of(const AttnParams& p) {
   return CacheGeom{p.page_table, p.T, p.page_tokens, p.pages_per_request, p.pool_pages, p.rolling};
@@ -155,20 +155,9 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
 // A lane reads a block pair's bytes where they lie: 2 x 18 (34) bytes are 9 (17) aligned words whose first and
 // middle ones hold the scales, and the order of the dimensions inside a block is free as long as Q's order is
 // the same. Rows are padded in shared memory to a pitch of 4 (mod 8) words, where no two lanes meet in a bank.
-constexpr int TK = 16;              // keys of a tile
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int COLS = 8;
-
-template <int D, bool Q8>
-struct RowFmt {
-  static constexpr int BB = Q8 ? Q8_BYTES : Q4_BYTES;
-  static constexpr int BYTES = D / QK * BB;          // one head row
-  static constexpr int CHUNKS = Q8 ? 17 : 9;         // copies of CHUNK bytes
-  static constexpr int CHUNK = D / 16;
-  static constexpr int PITCH = Q8 ? (D == 64 ? 80 : D == 128 ? 144 : 272) : (D == 64 ? 48 : D == 128 ? 80 : 144);
-  static_assert(CHUNKS * CHUNK == BYTES && PITCH % CHUNK == 0 && PITCH >= BYTES && (PITCH / 4) % 8 == 4, "row layout");
-};
 
 template <int D, bool KQ8, bool VQ8>
 struct DecodeGeom {
@@ -210,47 +199,6 @@ struct DecodeGrid {
   uint32_t dealt;        // 1: in proportion to the keys; 0: cluster c is unit c
 };
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  return a;
-}
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t a) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ float ld_cluster_f(uint32_t a) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_cluster_u32(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
-
-// Tiles are cut so that none straddles a page or the end of a ring: a segment (a page, a lap of the ring, or the
-// whole contiguous cache) is cut into tiles of TK keys, the last of which may be shorter.
-struct TileSpace {
-  uint32_t seg_len, per_seg;
-};
-__device__ __forceinline__ TileSpace tile_space(const AttnParams& p) {
-  const uint32_t len = p.page_table ? p.page_tokens : p.rolling ? p.T : 0x7FFFFFFFu;
-  return TileSpace{len, len / TK + (len % TK != 0)};
-}
-__device__ __forceinline__ uint32_t tile_at(const TileSpace& ts, uint32_t key) {
-  const uint32_t seg = key / ts.seg_len;
-  return seg * ts.per_seg + (key - seg * ts.seg_len) / TK;
-}
-// Tiles [first, end) hold the keys that the columns of (request b, positions from l0 on) see together.
-struct TileRange {
-  uint32_t first, end;
-};
-__device__ __forceinline__ TileRange tiles_of_keys(const TileSpace& ts, uint32_t lo, uint32_t hi) {
-  if (hi <= lo) return TileRange{0, 0};
-  return TileRange{tile_at(ts, lo), tile_at(ts, hi - 1) + 1};
-}
 __device__ __forceinline__ uint32_t count_tiles(const AttnParams& p, const TileSpace& ts, uint32_t b, uint32_t l0) {
   uint32_t lo = 0xFFFFFFFFu, hi = 0;
   for (uint32_t l = l0; l < min(p.L, l0 + p.pos_per_tile); l++) {
@@ -272,69 +220,6 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool the
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint32_t movm(uint32_t a) {
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
-}
-// D = A . B + C with a C of its own.
-__device__ __forceinline__ void mma_f16_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
-                                             float c0, float c1, float c2, float c3) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
-}
-__device__ __forceinline__ float ex2(float x) {   // 2^x to 2 units in the last place; 0 for -infinity
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float half_bits(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
-__device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// Two terms of f16 for a pair of f32 values: x = hi + lo to 22 bits. The remainder is taken by an operation that
-// reads the f16 term as it is (times -1) (on the FMA pipe; a conversion back to f32 would go to the busier ALU pipe).
-__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
-  const uint32_t h = pack_half2(a, b);
-  float la, lb;   // x - hi
-  asm("{.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xBC00;\n\tfma.rn.f32.f16 %0, l, m, %3;\n\tfma.rn.f32.f16 %1, h, m, %4;\n\t}"
-      : "=f"(la), "=f"(lb)
-      : "r"(h), "f"(a), "f"(b));
-  *hi = h;
-  *lo = pack_half2(la, lb);
-}
-
-// Which dimension of a block the lane index u (t of a key row's words) reaches with code i of its word(s).
-// K words: q4_0 one word of eight nibbles per lane t; q8_0 two words, u = t and t + 4, of four bytes.
-__host__ __device__ constexpr int pair_byte(bool q8, bool second, int u, int j) {
-  // byte j of word u of the block's codes; in a pair's first block word 0 is put together from the codes' first
-  // and last two bytes (they share words with the two scales)
-  const int n = q8 ? 32 : 16;
-  return second ? 4 * u + j : u ? 4 * u - 2 + j : j < 2 ? j : n - 4 + j;
-}
-
-__device__ __forceinline__ void unpack_q4_subnormal(uint32_t w, uint32_t (&x)[4]) {
-  x[0] = w & 0x000F000Fu;        // n * 2^-24
-  x[1] = w & 0x00F000F0u;        // n * 2^-20
-  w >>= 8;
-  x[2] = w & 0x000F000Fu;
-  x[3] = w & 0x00F000F0u;
-}
-__device__ __forceinline__ void unpack_q8(uint32_t w, uint32_t* r0, uint32_t* r1) {
-  w ^= 0x80808080u;
-  // 0x6400 | u is 1024 + u: minus 1152 leaves the signed code, exactly
-  *r0 = h2_add(__byte_perm(w, 0x64646464u, 0x4140), 0xE480E480u);
-  *r1 = h2_add(__byte_perm(w, 0x64646464u, 0x4342), 0xE480E480u);
-}
-
 template <int D, bool KQ8, bool VQ8, bool TMA>
 __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_qcache_decode_kernel(
     const AttnParams p, const DecodeGrid dg, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v) {
@@ -1076,7 +961,7 @@ int32_t launch_decode_as(AionCudaDevice* dev, AttnParams& p, const CUtensorMap& 
 }
 
 template <int D, bool KQ8, bool VQ8>
-int32_t launch_decode(AionCudaDevice* dev, AttnParams& p, uint64_t max_keys) {
+int32_t launch_decode(AionCudaDevice* dev, AttnParams& p, uint64_t max_keys, bool rows_kernel) {
   using KF = RowFmt<D, KQ8>;
   using VF = RowFmt<D, VQ8>;
   const uint64_t rows = p.page_table ? (uint64_t)p.pool_pages * p.page_tokens : (uint64_t)p.B * p.T;
@@ -1092,6 +977,7 @@ int32_t launch_decode(AionCudaDevice* dev, AttnParams& p, uint64_t max_keys) {
   tk = *m;
   if (int32_t st = tensor_map_bytes(dev, p.v, 2, vd, &vw, vbox, &m)) return st;
   tv = *m;
+  if (rows_kernel) return attention_qcache_rows(dev, p, tk, tv, max_keys);
   return launch_decode_as<D, KQ8, VQ8, true>(dev, p, tk, tv, max_keys);
 }
 
@@ -1112,13 +998,16 @@ int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p, uint32_t fla
     p.l_blocks = (p.L + p.pos_per_tile - 1) / p.pos_per_tile;
     const uint64_t units = (uint64_t)p.B * p.l_blocks * p.Hkv * p.head_groups;
     if (units > 0x7FFFFFFF) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
+    // Many rows per kv head: the kernel that streams the keys once for 128 of them.
+    const bool rows_kernel = !p.image && p.L > 1 && !(flags & AION_CUDA_ATTENTION_ROW_UNITS) &&
+                             ((flags & AION_CUDA_ATTENTION_BLOCKS) || p.L * group > 32);
     // Upper bound of the keys of a unit.
     uint64_t max_keys = p.T;
     const uint64_t span = (uint64_t)(p.win_chunk ? p.win_chunk : 1) + p.win_left + p.win_right + p.pos_per_tile;
     if (p.win_left != AION_CUDA_WINDOW_UNBOUNDED && p.win_right != AION_CUDA_WINDOW_UNBOUNDED && span < max_keys) max_keys = span;
 #define AION_QCACHE(D)                                                                                     \
-  if (kq8) return vq8 ? launch_decode<D, true, true>(dev, p, max_keys) : launch_decode<D, true, false>(dev, p, max_keys); \
-  return vq8 ? launch_decode<D, false, true>(dev, p, max_keys) : launch_decode<D, false, false>(dev, p, max_keys);
+  if (kq8) return vq8 ? launch_decode<D, true, true>(dev, p, max_keys, rows_kernel) : launch_decode<D, true, false>(dev, p, max_keys, rows_kernel); \
+  return vq8 ? launch_decode<D, false, true>(dev, p, max_keys, rows_kernel) : launch_decode<D, false, false>(dev, p, max_keys, rows_kernel);
     switch (p.Dk) {
       case 64: AION_QCACHE(64)
       case 128: AION_QCACHE(128)

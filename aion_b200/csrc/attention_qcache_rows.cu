@@ -1,0 +1,616 @@
+// `Attention` over a quantized KV cache for many query rows (prompts, several new rows per request): a CTA holds up to 128
+// rows of one kv head, a row being (query position, query head of the group), sixteen to a warp, and streams the keys once
+// for all of them.
+//
+//  * S[16 x 64] = Q . C^T and O[16 x D] += P' . V-codes on f16 m16n8k16 with the codes as exact f16 integers (see
+//    attention_qcache.cu): q and P' = p * (V scale) are two f16 terms each, so the tensor pipe does 8 * rows * keys * D
+//    operations for the 4 that f32 attention counts, and half its rate is the ceiling. Dequantized operands for tcgen05
+//    would need two terms of K and V as well (three products each), and 128 x 256 queries in two terms fill the shared
+//    memory that their tiles would need.
+//  * The logits' fragment is the second product's A operand as it stands; only the scale of (key, block) is multiplied in
+//    per block of 32 dimensions, before the split into two terms.
+//  * Every warp unpacks the fragments it needs from the raw blocks in shared memory: that costs about as many issue slots
+//    as the MMAs they feed leave over, and no traffic.
+//  * Stages of 64 keys arrive as TMA boxes of 16 rows, one stage ahead; their scales are turned into f32 once for the CTA.
+//  * A context too long for the few CTAs of a short prompt is cut over a cluster, whose CTAs add up their sums through
+//    distributed shared memory.
+#include <cstdlib>
+#include <mutex>
+
+#include "attention_qcache.cuh"
+
+namespace aion {
+
+namespace {
+
+using namespace qcache;
+
+constexpr int RW = 8;                 // warps
+constexpr int RTHREADS = RW * 32;
+constexpr int ROWS = RW * 16;
+constexpr int SUBS = 4;               // tiles of a stage
+constexpr int SK = SUBS * TK;         // keys of a stage
+
+struct RowsGrid {
+  uint32_t cluster;      // CTAs that share a unit's keys
+  uint32_t row_blocks;   // blocks of ROWS rows per (request, kv head)
+  uint32_t rows;         // L * query heads of the group
+};
+
+template <int D, bool KQ8, bool VQ8>
+struct RowsGeom {
+  using K = RowFmt<D, KQ8>;
+  using V = RowFmt<D, VQ8>;
+  static constexpr int NB = D / QK;
+  static constexpr int TILE = TK * (K::PITCH + V::PITCH);
+  static constexpr int STAGE = SUBS * TILE;
+  static constexpr int OFF_QF = 2 * STAGE;                       // uint4 [warp][D / 16][hi, lo][32]; at the end f32 [ROWS][D]
+  static constexpr int QF_BYTES = RW * (D / 16) * 2 * 512;
+  static constexpr int OFF_KS = OFF_QF + QF_BYTES;               // f32 [block][64]: K scales of the stage
+  static constexpr int OFF_VS = OFF_KS + NB * SK * 4;            // f32 [block][64]: V scales, times 2^(29 - E)
+  static constexpr int OFF_CI = OFF_VS + NB * SK * 4;            // f32 [warp][block][16]: -8 sum q; at the end maxima and weights [2][ROWS]
+  static constexpr int CI_BYTES = RW * NB * 16 * 4 > 2 * ROWS * 4 ? RW * NB * 16 * 4 : 2 * ROWS * 4;
+  static constexpr int OFF_VALID = OFF_CI + CI_BYTES;            // uint2 [2][SUBS]: which keys are there, the first of them
+  static constexpr int OFF_BARS = OFF_VALID + 2 * SUBS * 8;
+  static constexpr int OFF_FLAGS = OFF_BARS + 16;                // bad inputs, gave up, largest V scale, odd stage, first key, key end
+  static constexpr int SMEM = OFF_FLAGS + 32;
+  static_assert(QF_BYTES == ROWS * D * 4 && SMEM <= 227 * 1024, "shared memory");
+};
+
+template <int D, bool KQ8, bool VQ8>
+__global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const AttnParams p, const RowsGrid rg, const __grid_constant__ CUtensorMap tmap_k,
+                                                                      const __grid_constant__ CUtensorMap tmap_v) {
+  using G = RowsGeom<D, KQ8, VQ8>;
+  using KF = RowFmt<D, KQ8>;
+  using VF = RowFmt<D, VQ8>;
+  constexpr int NB = G::NB;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t sbase = ptx::smem_u32(smem);
+  auto lds32 = [&](uint32_t at) { return *reinterpret_cast<const uint32_t*>(smem + at); };
+  auto lds16 = [&](uint32_t at) { return (uint32_t)*reinterpret_cast<const uint16_t*>(smem + at); };
+  auto lds_f2 = [&](uint32_t at) { return *reinterpret_cast<const float2*>(smem + at); };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t bars = sbase + G::OFF_BARS;
+  uint32_t* flags = reinterpret_cast<uint32_t*>(smem + G::OFF_FLAGS);
+  uint2* valid = reinterpret_cast<uint2*>(smem + G::OFF_VALID);
+
+  if (tid == 0) {
+    ptx::mbar_init(bars, 1);
+    ptx::mbar_init(bars + 8, 1);
+    flags[0] = flags[1] = flags[2] = flags[3] = flags[5] = 0;
+    flags[4] = 0xFFFFFFFFu;
+    ptx::fence_barrier_init();
+  }
+  __syncthreads();
+  ptx::pdl_launch_dependents();
+  ptx::pdl_wait();
+
+  // unit = (b, block of rows, kv head), blocks last first (they see most keys under a causal window); rank: its slice of the keys
+  const uint32_t unit = blockIdx.x / rg.cluster, rank = blockIdx.x - unit * rg.cluster;
+  const uint32_t hkv = unit % p.Hkv, bl = unit / p.Hkv, b = bl / rg.row_blocks, rb = rg.row_blocks - 1 - (bl - b * rg.row_blocks);
+  const uint32_t group = p.Hq / p.Hkv;
+  // Row r of the block: position and head of it, its row of q and out seen as [B * L * Hq, D]; NO_ROW beyond the last.
+  auto row_of = [&](uint32_t r, uint32_t* l) -> uint32_t {
+    const uint32_t i = rb * ROWS + r;
+    *l = i / group;
+    return i < rg.rows ? (b * p.L + *l) * p.Hq + hkv * group + (i - *l * group) : NO_ROW;
+  };
+  uint32_t my_row[2], lo[2], hi[2];   // rows g and g + 8 of the warp
+  bool bad = false;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    uint32_t l;
+    my_row[h] = row_of(warp * 16 + g + 8 * h, &l);
+    lo[h] = hi[h] = 0;
+    if (my_row[h] != NO_ROW) {
+      const KeyRange kr = key_range(p, b, l);
+      bad |= kr.bad;
+      lo[h] = kr.lo, hi[h] = kr.hi;
+    }
+  }
+  if (bad) flags[0] = 1;
+  // What some row of the warp sees, and what all of its rows see.
+  uint32_t w_lo = 0xFFFFFFFFu, w_hi = 0, w_all_lo = 0, w_all_hi = 0xFFFFFFFFu;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    if (hi[h] > lo[h]) w_lo = min(w_lo, lo[h]), w_hi = max(w_hi, hi[h]);
+    if (my_row[h] != NO_ROW) w_all_lo = max(w_all_lo, lo[h]), w_all_hi = min(w_all_hi, hi[h]);
+  }
+  w_lo = __reduce_min_sync(FULL, w_lo), w_hi = __reduce_max_sync(FULL, w_hi);
+  w_all_lo = __reduce_max_sync(FULL, w_all_lo), w_all_hi = __reduce_min_sync(FULL, w_all_hi);
+  if (lane == 0 && w_hi > 0) atomicMin(flags + 4, w_lo), atomicMax(flags + 5, w_hi);
+  __syncthreads();
+  if (flags[0] && tid == 0) atomicExch(p.fault, FAULT_INVALID_ARGUMENT);
+  const uint32_t u_hi = flags[5], u_lo = min(flags[4], u_hi);
+  const TileSpace ts = tile_space(p);
+  const TileRange whole = tiles_of_keys(ts, u_lo, u_hi);
+  uint32_t per = (whole.end - whole.first + rg.cluster - 1) / rg.cluster;
+  per = (per + SUBS - 1) / SUBS * SUBS;
+  const uint32_t my_first = (uint32_t)min((uint64_t)whole.end, whole.first + (uint64_t)rank * per);
+  const uint32_t tiles = min(whole.end - my_first, per), stages = (tiles + SUBS - 1) / SUBS;
+
+  // ---- thread 0 brings the stages; the page numbers of the next one are read a stage ahead
+  const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;
+  const uint32_t kshift = (hkv * KF::BYTES) & 15, vshift = (hkv * VF::BYTES) & 15;
+  uint32_t seg = my_first / ts.per_seg, in_seg = my_first - seg * ts.per_seg;
+  struct Place {
+    uint32_t seg, in_seg;
+    int32_t page;
+  } next[SUBS];
+  auto place = [&](uint32_t stage) {
+#pragma unroll
+    for (int s = 0; s < SUBS; s++) {
+      next[s] = Place{seg, in_seg, 0};
+      if (p.page_table && stage * SUBS + s < tiles) next[s].page = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + seg);
+      if (++in_seg >= ts.per_seg) in_seg = 0, seg++;
+    }
+  };
+  auto issue = [&](uint32_t stage) {
+    const uint32_t st = stage & 1, bar = bars + 8 * st, dst = sbase + st * G::STAGE;
+    uint32_t count[SUBS], bytes = 0;
+    uint64_t row[SUBS];
+#pragma unroll
+    for (int s = 0; s < SUBS; s++) {
+      count[s] = stage * SUBS + s < tiles ? min((uint32_t)TK, ts.seg_len - next[s].in_seg * TK) : 0;
+      row[s] = row0 + next[s].in_seg * TK;
+      if (p.page_table) {
+        if (count[s] && (next[s].page < 0 || (uint32_t)next[s].page >= p.pool_pages)) {
+          atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
+          count[s] = 0;
+        }
+        row[s] += (uint64_t)(count[s] ? next[s].page : 0) * p.page_tokens;
+      }
+      valid[st * SUBS + s] = make_uint2((1u << count[s]) - 1, next[s].seg * ts.seg_len + next[s].in_seg * TK);
+      if (count[s]) bytes += G::TILE;
+    }
+    ptx::mbar_arrive_expect_tx(bar, bytes);
+    if (p.drop_first && stage == 0) return;
+#pragma unroll
+    for (int s = 0; s < SUBS; s++)
+      if (count[s]) {
+        ptx::tma_load_2d(dst + s * G::TILE, &tmap_k, (int)((hkv * KF::BYTES) / 16 * 2), (int)row[s], bar);
+        ptx::tma_load_2d(dst + s * G::TILE + TK * KF::PITCH, &tmap_v, (int)((hkv * VF::BYTES) / 16 * 2), (int)row[s], bar);
+      }
+  };
+  if (tid == 0 && stages) {
+    place(0);
+    issue(0);
+    place(1);
+  }
+
+  // ---- q as the A operand: rows g and g + 8, two terms, normed by the row's largest value to [2^13, 2^14)
+  const uint32_t qf = G::OFF_QF + warp * ((D / 16) * 1024) + lane * 16;
+  float factor[2];
+  {
+    float up[2] = {0.0f, 0.0f};
+#pragma unroll 1
+    for (int r = 0; r < 16; r++) {
+      uint32_t l;
+      const uint32_t row = row_of(warp * 16 + r, &l);
+      float top = 0.0f;
+      if (row != NO_ROW)
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+          const uint64_t at = (uint64_t)row * D + lane + 32 * i;
+          top = fmaxf(top, fabsf(p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at] : __half2float(static_cast<const __half*>(p.q)[at])));
+        }
+      uint32_t e = __reduce_max_sync(FULL, __float_as_uint(top)) >> 23;
+      if (e == 255) e = 127;
+      e = max(e, 40u);
+      if ((r & 7) == g) {
+        const float to_base2 = p.soft_cap > 0.0f ? 1.0f : LOG2E;
+        (r < 8 ? up[0] : up[1]) = __uint_as_float((127u + 13u + 127u - e) << 23);
+        (r < 8 ? factor[0] : factor[1]) = p.scale * __uint_as_float((e - 13u) << 23) * to_base2;
+      }
+    }
+#pragma unroll 1
+    for (int blk = 0; blk < NB; blk++) {
+      float part[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        uint32_t h4[4], l4[4];
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+          for (int half = 0; half < 2; half++) {   // operand order: (row g, r 0), (row g + 8, r 0), (row g, r 1), (row g + 8, r 1)
+            float x[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const int dim = KQ8 ? pair_byte(true, blk & 1, t + 4 * m, 2 * r + h) : 2 * pair_byte(false, blk & 1, t, m + 2 * h) + r;
+              x[h] = 0.0f;
+              if (my_row[half] != NO_ROW) {
+                const uint64_t at = (uint64_t)my_row[half] * D + blk * QK + dim;
+                x[h] = p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at] : __half2float(static_cast<const __half*>(p.q)[at]);
+              }
+              x[h] = x[h] * up[half] * (!KQ8 && r ? 0.0625f : 1.0f);
+            }
+            split2(x[0], x[1], &h4[2 * r + half], &l4[2 * r + half]);
+            if (!KQ8) {
+              const float2 a = __half22float2(*reinterpret_cast<__half2*>(&h4[2 * r + half])), c = __half22float2(*reinterpret_cast<__half2*>(&l4[2 * r + half]));
+              part[half] += ((a.x + c.x) + (a.y + c.y)) * (r ? 16.0f : 1.0f);
+            }
+          }
+        *reinterpret_cast<uint4*>(smem + qf + (2 * blk + m) * 1024) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+        *reinterpret_cast<uint4*>(smem + qf + (2 * blk + m) * 1024 + 512) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+      }
+      if (!KQ8) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          part[half] += __shfl_xor_sync(FULL, part[half], 1);
+          part[half] += __shfl_xor_sync(FULL, part[half], 2);
+          if (t == 0) *reinterpret_cast<float*>(smem + G::OFF_CI + ((warp * NB + blk) * 16 + g + 8 * half) * 4) = part[half] * (-8.0f * 5.9604644775390625e-8f);
+        }
+      }
+    }
+  }
+  __syncwarp();
+
+  float acc[NB][4][4];   // [block][8 dimensions][row g: 2, row g + 8: 2]
+#pragma unroll
+  for (int i = 0; i < NB; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[i][j][e] = 0.0f;
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
+  uint32_t e_run = 0;
+  const uint32_t first_sel = t ? 0x3210u : 0x5432u, first_sel_v = g ? 0x3210u : 0x5432u;
+
+  for (uint32_t it = 0; it < stages; it++) {
+    const uint32_t st = it & 1, ring = st * G::STAGE;
+    if (!ptx::mbar_wait_bounded(bars + 8 * st, (it >> 1) & 1, p.wait_limit)) flags[1] = 1;
+    // ---- this thread's part of the stage's scales
+    constexpr int PER = (NB * SK + RTHREADS - 1) / RTHREADS;
+    uint32_t ksc[PER], vsc[PER], top = 0;
+    bool weird = false;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const uint32_t e = tid + RTHREADS * j, blk = e / SK, k = e % SK, at = ring + (k / TK) * G::TILE;
+      ksc[j] = vsc[j] = 0;
+      if (NB * SK % RTHREADS && e >= NB * SK) break;
+      ksc[j] = lds16(at + kshift + (k % TK) * KF::PITCH + blk * KF::BB);
+      vsc[j] = lds16(at + TK * KF::PITCH + vshift + (k % TK) * VF::PITCH + blk * VF::BB);
+      const uint2 v = valid[st * SUBS + k / TK];
+      const uint32_t key = v.y + k % TK;
+      if (!((v.x >> (k % TK)) & 1) || key < u_lo || key >= u_hi) vsc[j] = 0;   // no row sees it
+      if ((vsc[j] & 0x7FFFu) >= 0x7C00u) vsc[j] = 0, weird = true;
+      top = max(top, vsc[j] & 0x7FFFu);
+    }
+    top = __reduce_max_sync(FULL, top);
+    if (lane == 0) atomicMax(flags + 2, top);
+    if (weird) flags[3] = it + 1;
+    __syncthreads();
+    // Every warp has finished the last stage: its place is free for the next.
+    if (tid == 0 && it + 1 < stages && !flags[1]) {
+      issue(it + 1);
+      place(it + 2);
+    }
+    if (flags[1]) {
+      if (tid == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED);
+      ptx::mbar_wait_bounded(bars + 8 * st, (it >> 1) & 1, p.wait_limit);
+      break;
+    }
+    const uint32_t e_new = flags[2] >> 10;   // the largest exponent so far
+    const float vmul = __uint_as_float((127u + 29u - e_new) << 23);
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      if (NB * SK % RTHREADS && tid + RTHREADS * j >= NB * SK) break;
+      *reinterpret_cast<float*>(smem + G::OFF_KS + (tid + RTHREADS * j) * 4) = half_bits(ksc[j]);
+      *reinterpret_cast<float*>(smem + G::OFF_VS + (tid + RTHREADS * j) * 4) = half_bits(vsc[j]) * vmul;
+    }
+    weird = flags[3] == it + 1;
+    // Does some row of this warp see a key of the stage, and do all of them see all?
+    bool some = false, partial = false;
+    uint32_t key0[SUBS], there[SUBS];
+#pragma unroll
+    for (int s = 0; s < SUBS; s++) {
+      const uint2 v = valid[st * SUBS + s];
+      there[s] = v.x, key0[s] = v.y;
+      some |= v.x && v.y < w_hi && v.y + TK > w_lo;
+      partial |= v.x != 0xFFFFu || v.y < w_all_lo || v.y + TK > w_all_hi;
+    }
+    __syncthreads();
+    if (!some) continue;
+
+    // ---- S: rows g and g + 8, keys 8n + 2t and 8n + 2t + 1
+    float s[SK / 8][4];
+#pragma unroll
+    for (int n = 0; n < SK / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+    const uint32_t krow = ring + kshift + g * KF::PITCH;
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++) {
+      uint4 qh[2], ql[2];
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        qh[m] = *reinterpret_cast<const uint4*>(smem + qf + (2 * blk + m) * 1024);
+        ql[m] = *reinterpret_cast<const uint4*>(smem + qf + (2 * blk + m) * 1024 + 512);
+      }
+      float ci[2] = {0.0f, 0.0f};
+      if (!KQ8)
+#pragma unroll
+        for (int half = 0; half < 2; half++) ci[half] = *reinterpret_cast<const float*>(smem + G::OFF_CI + ((warp * NB + blk) * 16 + g + 8 * half) * 4);
+#pragma unroll
+      for (int n = 0; n < SK / 8; n++) {
+        const uint32_t row = krow + (n >> 1) * G::TILE + (n & 1) * 8 * KF::PITCH + (blk >> 1) * 2 * KF::BB;
+        uint32_t b[2][2];
+        if (KQ8) {
+          if (blk & 1) {
+            unpack_q8(lds32(row + 36 + 4 * t), &b[0][0], &b[0][1]);
+            unpack_q8(lds32(row + 52 + 4 * t), &b[1][0], &b[1][1]);
+          } else {
+            unpack_q8(__byte_perm(lds32(row + 4 * t), lds32(row + 32), first_sel), &b[0][0], &b[0][1]);
+            unpack_q8(lds32(row + 16 + 4 * t), &b[1][0], &b[1][1]);
+          }
+        } else {
+          uint32_t u[4];
+          unpack_q4_subnormal(blk & 1 ? lds32(row + 20 + 4 * t) : __byte_perm(lds32(row + 4 * t), lds32(row + 16), first_sel), u);
+          b[0][0] = u[0], b[0][1] = u[1], b[1][0] = u[2], b[1][1] = u[3];
+        }
+        float c[4];
+        mma_f16_from(c, ql[0].x, ql[0].y, ql[0].z, ql[0].w, b[0][0], b[0][1], ci[0], ci[0], ci[1], ci[1]);
+        mma_f16_from(c, ql[1].x, ql[1].y, ql[1].z, ql[1].w, b[1][0], b[1][1], c[0], c[1], c[2], c[3]);
+        mma_f16_from(c, qh[0].x, qh[0].y, qh[0].z, qh[0].w, b[0][0], b[0][1], c[0], c[1], c[2], c[3]);
+        mma_f16_from(c, qh[1].x, qh[1].y, qh[1].z, qh[1].w, b[1][0], b[1][1], c[0], c[1], c[2], c[3]);
+        const float2 sc = lds_f2(G::OFF_KS + (blk * SK + 8 * n + 2 * t) * 4);
+        s[n][0] = fmaf(sc.x, c[0], s[n][0]);
+        s[n][1] = fmaf(sc.y, c[1], s[n][1]);
+        s[n][2] = fmaf(sc.x, c[2], s[n][2]);
+        s[n][3] = fmaf(sc.y, c[3], s[n][3]);
+      }
+    }
+    // ---- softmax
+    float m_new[2] = {m_run[0], m_run[1]};
+#pragma unroll
+    for (int n = 0; n < SK / 8; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float y = s[n][e];
+        if (!KQ8) y *= 16777216.0f;   // the codes' 2^24
+        y *= factor[e >> 1];
+        if (p.soft_cap > 0.0f) y = soft_cap_logit(y, p.soft_cap) * LOG2E;
+        if (partial) {
+          const uint32_t k = (n & 1) * 8 + 2 * t + (e & 1), key = key0[n >> 1] + k;
+          if (!((there[n >> 1] >> k) & 1) || key < lo[e >> 1] || key >= hi[e >> 1]) y = -INFINITY;
+        }
+        s[n][e] = y;
+        m_new[e >> 1] = fmaxf(m_new[e >> 1], y);
+      }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      m_new[h] = fmaxf(m_new[h], __shfl_xor_sync(FULL, m_new[h], 1));
+      m_new[h] = fmaxf(m_new[h], __shfl_xor_sync(FULL, m_new[h], 2));
+    }
+    if (__any_sync(FULL, m_new[0] > m_run[0] || m_new[1] > m_run[1] || e_new > e_run)) {
+      const float down = __uint_as_float((127u + e_run - e_new) << 23);
+      float a[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        a[h] = m_new[h] > m_run[h] ? ex2(m_run[h] - m_new[h]) : 1.0f;
+        l_run[h] *= a[h];
+        a[h] *= down;
+        m_run[h] = m_new[h];
+      }
+      e_run = e_new;
+#pragma unroll
+      for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j][0] *= a[0], acc[i][j][1] *= a[0], acc[i][j][2] *= a[1], acc[i][j][3] *= a[1];
+    }
+    const float safe[2] = {m_run[0] == -INFINITY ? 0.0f : m_run[0], m_run[1] == -INFINITY ? 0.0f : m_run[1]};
+#pragma unroll
+    for (int n = 0; n < SK / 8; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        s[n][e] = ex2(s[n][e] - safe[e >> 1]);
+        l_run[e >> 1] += s[n][e];
+      }
+
+    // ---- O += P' . V
+    const uint32_t vrow = ring + TK * KF::PITCH + vshift + 2 * t * VF::PITCH;
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++) {
+      // (Summed from zero and added in f32: the tensor core cuts its sums off to one side.)
+      float o[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < SUBS; j++) {
+        uint32_t ah[4], al[4], bf[4][2];
+#pragma unroll
+        for (int kp = 0; kp < 2; kp++) {
+          const float2 v = lds_f2(G::OFF_VS + (blk * SK + TK * j + 2 * t + 8 * kp) * 4);
+          split2(s[2 * j + kp][0] * v.x, s[2 * j + kp][1] * v.y, &ah[2 * kp], &al[2 * kp]);
+          split2(s[2 * j + kp][2] * v.x, s[2 * j + kp][3] * v.y, &ah[2 * kp + 1], &al[2 * kp + 1]);
+          const uint32_t row = vrow + j * G::TILE + 8 * kp * VF::PITCH;
+          if (VQ8) {
+            uint32_t x[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const uint32_t pos = row + h * VF::PITCH + (blk >> 1) * 2 * VF::BB;
+              if (blk & 1) x[h] = lds32(pos + 36 + 4 * g);
+              else x[h] = __byte_perm(lds32(pos + 4 * g), lds32(pos + 32), first_sel_v);
+              x[h] ^= 0x80808080u;
+            }
+            const uint32_t lo2 = __byte_perm(x[0], x[1], 0x5140), hi2 = __byte_perm(x[0], x[1], 0x7362);
+            bf[0][kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4140), 0xE480E480u);
+            bf[1][kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4342), 0xE480E480u);
+            bf[2][kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4140), 0xE480E480u);
+            bf[3][kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4342), 0xE480E480u);
+          } else {
+            const uint32_t pos = row + blk * VF::BB + 2 + 2 * g;
+            uint32_t x = __byte_perm(lds16(pos), lds16(pos + VF::PITCH), 0x5410);
+            bf[0][kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+            bf[1][kp] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+            x >>= 8;
+            bf[2][kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+            bf[3][kp] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) mma_f16_from(o[i], al[0], al[1], al[2], al[3], bf[i][0], bf[i][1], o[i][0], o[i][1], o[i][2], o[i][3]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) mma_f16_from(o[i], ah[0], ah[1], ah[2], ah[3], bf[i][0], bf[i][1], o[i][0], o[i][1], o[i][2], o[i][3]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[blk][i][e] += o[i][e];
+    }
+    if (weird) {   // a V scale that is not finite: NaN where a row gives weight to its key
+#pragma unroll
+      for (int blk = 0; blk < NB; blk++) {
+        bool met[2] = {false, false};
+#pragma unroll
+        for (int n = 0; n < SK / 8; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const uint32_t k = (n & 1) * 8 + 2 * t + (e & 1);
+            const uint32_t bits = lds16(ring + (n >> 1) * G::TILE + TK * KF::PITCH + vshift + k * VF::PITCH + blk * VF::BB) & 0x7FFFu;
+            met[e >> 1] |= bits >= 0x7C00u && s[n][e] > 0.0f;
+          }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t who = __ballot_sync(FULL, met[h]);
+          const float add = (who >> (4 * g)) & 15 ? NAN : 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[blk][i][2 * h] += add, acc[blk][i][2 * h + 1] += add;
+        }
+      }
+    }
+  }
+
+  // ---- the rows' sums: straight out, or through shared memory to the cluster's others
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    l_run[h] += __shfl_xor_sync(FULL, l_run[h], 1);
+    l_run[h] += __shfl_xor_sync(FULL, l_run[h], 2);
+  }
+  const float back = __uint_as_float((127u + e_run - 29u) << 23);
+  const bool report = !flags[0] && !flags[1];
+  float* res = reinterpret_cast<float*>(smem + G::OFF_QF);
+  float* stats = reinterpret_cast<float*>(smem + G::OFF_CI);   // maxima, then weights
+  if (rg.cluster > 1) __syncthreads();   // every warp is done with its queries
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const uint32_t r = warp * 16 + g + 8 * h;
+    const bool good = l_run[h] > 0.0f && isfinite(l_run[h]);
+    float mul = back;
+    float* dst = res + r * D;
+    if (rg.cluster == 1) {
+      if (my_row[h] == NO_ROW) continue;
+      if (!good && hi[h] > lo[h] && report) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
+      mul = good ? back * __frcp_rn(l_run[h]) : 0.0f;
+      dst = p.out + (uint64_t)my_row[h] * D;
+    } else if (t == 0) {
+      stats[r] = m_run[h], stats[ROWS + r] = l_run[h];
+    }
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++)
+#pragma unroll
+      for (int c = 0; c < 2; c++) {   // dimensions of the column group 2t + c
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = rg.cluster == 1 && !good ? 0.0f : acc[blk][i][2 * h + c] * mul;
+        float* at = dst + blk * QK;
+        if (VQ8) {
+          const int d0 = pair_byte(true, blk & 1, 2 * t + c, 0), d2 = pair_byte(true, blk & 1, 2 * t + c, 2);
+          *reinterpret_cast<float2*>(at + d0) = make_float2(v[0], v[1]);
+          *reinterpret_cast<float2*>(at + d2) = make_float2(v[2], v[3]);
+        } else {
+          *reinterpret_cast<float4*>(at + 4 * (2 * t + c)) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+  }
+  if (rg.cluster == 1) return;
+  cluster_sync();
+  const uint32_t share = ROWS / rg.cluster, res_addr = sbase + G::OFF_QF, stats_addr = sbase + G::OFF_CI;
+  for (uint32_t i = tid; i < share * (D / 4); i += RTHREADS) {
+    const uint32_t r = rank * share + i / (D / 4), d4 = i % (D / 4);
+    uint32_t l;
+    const uint32_t row = row_of(r, &l);
+    if (row == NO_ROW) continue;
+    float m[8], w[8], M = -INFINITY, lsum = 0.0f;
+    float4 v[8], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      m[k] = -INFINITY, w[k] = 0.0f, v[k] = o;
+      if (k < (int)rg.cluster) {
+        const uint32_t a = cluster_addr(stats_addr, k);
+        m[k] = ld_cluster_f(a + 4 * r), w[k] = ld_cluster_f(a + 4 * (ROWS + r));
+        v[k] = ld_cluster_f4(cluster_addr(res_addr, k) + (r * D + 4 * d4) * 4);
+      }
+      M = fmaxf(M, m[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float f = m[k] == -INFINITY ? 0.0f : ex2(m[k] - M);
+      o.x += v[k].x * f, o.y += v[k].y * f, o.z += v[k].z * f, o.w += v[k].w * f;
+      lsum += w[k] * f;
+    }
+    const bool good = lsum > 0.0f && isfinite(lsum);
+    if (!good && d4 == 0 && report) {
+      const KeyRange kr = key_range(p, b, l);
+      if (kr.hi > kr.lo) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
+    }
+    const float inv = good ? __frcp_rn(lsum) : 0.0f;
+    *reinterpret_cast<float4*>(p.out + (uint64_t)row * D + 4 * d4) = good ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  cluster_sync();   // no CTA leaves before the others have read its sums
+}
+
+template <int D, bool KQ8, bool VQ8>
+int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, uint64_t max_keys) {
+  using G = RowsGeom<D, KQ8, VQ8>;
+  auto kernel = attn_qcache_rows_kernel<D, KQ8, VQ8>;
+  {
+    static std::mutex mu;   // once per device and instantiation
+    static bool configured[64] = {};
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev->ordinal < 0 || dev->ordinal >= 64 || !configured[dev->ordinal]) {
+      AION_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+      prefer_max_shared(reinterpret_cast<const void*>(kernel));
+      if (dev->ordinal >= 0 && dev->ordinal < 64) configured[dev->ordinal] = true;
+    }
+  }
+  RowsGrid rg{};
+  rg.rows = p.L * (p.Hq / p.Hkv);
+  rg.row_blocks = (rg.rows + ROWS - 1) / ROWS;
+  const uint64_t units = (uint64_t)p.B * rg.row_blocks * p.Hkv;
+  // One CTA an SM: a unit's keys are cut over as many as leave no SM without one, four stages each at least.
+  rg.cluster = 1;
+  while (rg.cluster < 8 && units * rg.cluster * 2 <= (uint64_t)dev->sm_count && max_keys >= (uint64_t)rg.cluster * 2 * 4 * SK) rg.cluster *= 2;
+  if (units * rg.cluster > 0x7FFFFFFFull) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(units * rg.cluster));
+  cfg.blockDim = dim3(RTHREADS);
+  cfg.dynamicSmemBytes = G::SMEM;
+  cfg.stream = dev->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = rg.cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  static const bool no_pdl_main = std::getenv("AION_CUDA_NO_PDL_MAIN") != nullptr;  // tuning only
+  cfg.numAttrs = no_pdl_main ? 1 : 2;
+  AION_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, rg, tk, tv));
+  return AION_CUDA_OK;
+}
+
+}  // namespace
+
+int32_t attention_qcache_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, uint64_t max_keys) {
+  const bool kq8 = p.k_dtype == AION_CUDA_DTYPE_Q8_0, vq8 = p.v_dtype == AION_CUDA_DTYPE_Q8_0;
+#define AION_QROWS(D)                                                                                                                  \
+  if (kq8) return vq8 ? launch_rows<D, true, true>(dev, p, tk, tv, max_keys) : launch_rows<D, true, false>(dev, p, tk, tv, max_keys); \
+  return vq8 ? launch_rows<D, false, true>(dev, p, tk, tv, max_keys) : launch_rows<D, false, false>(dev, p, tk, tv, max_keys);
+  switch (p.Dk) {
+    case 64: AION_QROWS(64)
+    case 128: AION_QROWS(128)
+    default: AION_QROWS(256)
+  }
+#undef AION_QROWS
+}
+
+}  // namespace aion

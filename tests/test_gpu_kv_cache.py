@@ -716,3 +716,69 @@ def test_append_rounds_every_quotient_as_the_quantizer_does(sess, dtype):
     tc = put_cache(store, zeros, dtype, 32)
     s.execute([StepSequenceAppend(cache=tc, new_kv=put(store, rows.reshape(1, n, 1, 32), F32), end_index=put(store, np.zeros(1, np.int32), I32))])
     assert np.array_equal(store.read(tc).view(np.uint8).reshape(-1), quantize(s.backend, dtype, rows, 1))
+
+
+FORCED = [capi.ATTENTION_ROW_UNITS, capi.ATTENTION_BLOCKS, capi.ATTENTION_GENERIC]
+
+
+@pytest.mark.parametrize("flags", FORCED, ids=["columns", "rows", "any"])
+@pytest.mark.parametrize("L,Hq,H,D", [(2, 8, 2, 256), (9, 14, 2, 64), (33, 8, 4, 128), (130, 2, 2, 64), (50, 6, 2, 256)])
+@pytest.mark.parametrize("layout,page", [("plain", 0), ("paged", 24), ("rolling", 0)])
+@pytest.mark.parametrize("kdt,vdt", ALL, ids=[f"{NAMES[a]}{NAMES[b]}" for a, b in ALL])
+def test_each_kernel_on_several_rows(sess, flags, L, Hq, H, D, layout, page, kdt, vdt):
+    """Causal rows with a window, in every layout, by each of the three kernels."""
+    B, T = 2, 300
+    q, k, v = inputs([L, D, kdt], B, T, H, D, L, Hq, kdt, vdt)
+    lens = [711, 300] if layout == "rolling" else [300, 137]
+    pos = np.array([[n - L + i for i in range(L)] for n in lens], dtype=np.int32)
+    got, _ = run_attention(sess, q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, layout=layout, page=page,
+                           window=AttentionWindow(left=150, right=0), cap=25.0, flags=flags)
+    check(got, *ref.attention(q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, rolling=layout == "rolling", left=150, cap=25.0))
+
+
+@pytest.mark.parametrize("flags", [capi.ATTENTION_ROW_UNITS, capi.ATTENTION_BLOCKS], ids=["columns", "rows"])
+@pytest.mark.parametrize("L,T,kdt,vdt", [(7, 1400, Q8, Q4), (20, 1500, Q4, Q4), (3, 1100, Q8, Q8)])
+def test_long_contexts_cut_over_clusters(sess, flags, L, T, kdt, vdt):
+    """Few rows over many keys: the context is shared by the CTAs of a cluster, and one request has nothing."""
+    B, H, D, Hq = 3, 1, 128, 4
+    q, k, v = inputs([L, T], B, T, H, D, L, Hq, kdt, vdt)
+    lens = [T, 0, T // 3]
+    pos = np.array([[max(0, n - L) + i for i in range(L)] for n in lens], dtype=np.int32)
+    got, _ = run_attention(sess, q, k, v, kdt, vdt, scale=0.1, positions=pos, lengths=lens, window=AttentionWindow.causal(), flags=flags)
+    check(got, *ref.attention(q, k, v, kdt, vdt, scale=0.1, positions=pos, lengths=lens))
+    assert not got[1].any()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("flags", [capi.ATTENTION_ROW_UNITS, capi.ATTENTION_BLOCKS], ids=["columns", "rows"])
+def test_a_scale_that_is_not_finite_spoils_its_own_block(sess, bad, flags):
+    """A V scale of NaN or infinity: the rows that see its key have NaN or infinities in the block's 32 dimensions, and their true
+    values in the others; rows that do not see it are clean."""
+    B, T, H, L, D = 1, 90, 1, 12, 128
+    q, k, v = inputs([5], B, T, H, D, L, 4, Q8, Q4)
+    pos = np.arange(70, 70 + L, dtype=np.int32)[None]
+    kw = dict(scale=0.1, positions=pos, lengths=[T])
+    want, bound = ref.attention(q, k, v, Q8, Q4, **kw)
+    v.reshape(B, T, H, 4, 18)[0, 75, 0, 2, :2] = np.frombuffer(np.float16(bad).tobytes(), np.uint8)
+    got, _ = run_attention(sess, q, k, v, Q8, Q4, window=AttentionWindow.causal(), flags=flags, **kw)
+    clean = np.ones(got.shape, bool)
+    clean[:, 5:, :, 64:96] = False
+    assert not np.isfinite(got[~clean]).any()
+    assert (np.abs(got - want)[clean] <= bound[clean]).all()
+
+
+def test_an_expired_wait_in_the_rows_kernel_is_reported(sess, backend):
+    s, store = sess
+    q, k, v = inputs([13], 1, 200, 2, 128, 40, 4, Q8, Q8)
+    want, step = run_attention(sess, q, k, v, Q8, Q8, scale=0.1, flags=capi.ATTENTION_BLOCKS)
+    lib = backend._lib
+    assert lib.aion_cuda_debug_expire_waits(backend.handle, 1) == capi.OK
+    try:
+        s.execute([step])
+        with pytest.raises(BackendError) as e:
+            backend.sync()
+        assert e.value.name == "ExecutionFailed"
+    finally:
+        lib.aion_cuda_debug_expire_waits(backend.handle, 0)
+    s.execute([step])
+    assert np.array_equal(store.read(step.out), want)
