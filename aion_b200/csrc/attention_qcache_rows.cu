@@ -9,9 +9,11 @@
 //    memory that their tiles would need.
 //  * The logits' fragment is the second product's A operand as it stands; only the scale of (key, block) is multiplied in
 //    per block of 32 dimensions, before the split into two terms.
-//  * Every warp unpacks the fragments it needs from the raw blocks in shared memory: that costs about as many issue slots
-//    as the MMAs they feed leave over, and no traffic.
-//  * Stages of 64 keys arrive as TMA boxes of 16 rows, one stage ahead; their scales are turned into f32 once for the CTA.
+//  * Four warps turn the raw blocks into fragments of f16 codes, in the order in which the MMAs' lanes take them, and the
+//    scales into f32; eight warps consume them, sixteen rows each. (With every warp unpacking for itself a tensor
+//    instruction came with eight others, and the 1024-row chunk that takes XXX us took 721.) Two buffers of 32 keys lie
+//    between the two sides; raw tiles arrive as TMA boxes of 16 rows. The consumers hold 216 registers, the unpacking
+//    warps 72.
 //  * A context too long for the few CTAs of a short prompt is cut over a cluster, whose CTAs add up their sums through
 //    distributed shared memory.
 #include <cstdlib>
@@ -25,11 +27,14 @@ namespace {
 
 using namespace qcache;
 
-constexpr int RW = 8;                 // warps
-constexpr int RTHREADS = RW * 32;
+constexpr int RW = 8;                 // consumer warps
+constexpr int PW = 4;                 // unpacking warps
+constexpr int RTHREADS = (RW + PW) * 32;
 constexpr int ROWS = RW * 16;
-constexpr int SUBS = 4;               // tiles of a stage
+constexpr int SUBS = 2;               // tiles of a stage
 constexpr int SK = SUBS * TK;         // keys of a stage
+constexpr int CONSUMER_REGS = 216, UNPACK_REGS = 72;
+static_assert(CONSUMER_REGS * RW * 32 + UNPACK_REGS * PW * 32 <= 168 * RTHREADS, "the registers that the block is launched with");
 
 struct RowsGrid {
   uint32_t cluster;      // CTAs that share a unit's keys
@@ -44,18 +49,26 @@ struct RowsGeom {
   static constexpr int NB = D / QK;
   static constexpr int TILE = TK * (K::PITCH + V::PITCH);
   static constexpr int STAGE = SUBS * TILE;
-  static constexpr int OFF_QF = 2 * STAGE;                       // uint4 [warp][D / 16][hi, lo][32]; at the end f32 [ROWS][D]
+  static constexpr int RAWS = D == 256 ? 1 : 2;                  // raw stages
+  static constexpr int KFRAG = NB * (SK / 8) * 512, VFRAG = NB * SUBS * 1024, FRAG = KFRAG + VFRAG;
+  static constexpr int OFF_QF = 0;                               // uint4 [warp][D / 16][hi, lo][32]; at the end f32 [ROWS][D]
   static constexpr int QF_BYTES = RW * (D / 16) * 2 * 512;
-  static constexpr int OFF_KS = OFF_QF + QF_BYTES;               // f32 [block][64]: K scales of the stage
-  static constexpr int OFF_VS = OFF_KS + NB * SK * 4;            // f32 [block][64]: V scales, times 2^(29 - E)
-  static constexpr int OFF_CI = OFF_VS + NB * SK * 4;            // f32 [warp][block][16]: -8 sum q; at the end maxima and weights [2][ROWS]
-  static constexpr int CI_BYTES = RW * NB * 16 * 4 > 2 * ROWS * 4 ? RW * NB * 16 * 4 : 2 * ROWS * 4;
-  static constexpr int OFF_VALID = OFF_CI + CI_BYTES;            // uint2 [2][SUBS]: which keys are there, the first of them
-  static constexpr int OFF_BARS = OFF_VALID + 2 * SUBS * 8;
-  static constexpr int OFF_FLAGS = OFF_BARS + 16;                // bad inputs, gave up, largest V scale, odd stage, first key, key end
+  static constexpr int OFF_FRAG = OFF_QF + QF_BYTES;             // uint4 [2][K: block, 8 keys][32], [V: block, 16 keys, half][32]
+  static constexpr int OFF_RAW = OFF_FRAG + 2 * FRAG;
+  static constexpr int OFF_KS = OFF_RAW + RAWS * STAGE;          // f32 [2][block][32]: K scales
+  static constexpr int OFF_VS = OFF_KS + 2 * NB * SK * 4;        // f32 [2][block][32]: V scales, times 2^(29 - E)
+  static constexpr int OFF_CI = OFF_VS + 2 * NB * SK * 4;        // f32 [warp][block][16]: -8 sum q
+  static constexpr int OFF_STATS = OFF_CI + RW * NB * 16 * 4;    // f32 [2][ROWS]: the rows' maxima and weights, for the cluster
+  static constexpr int OFF_ODD = OFF_STATS + 2 * ROWS * 4;       // u32 [2][block]: keys whose V scale is not finite
+  static constexpr int OFF_RVALID = OFF_ODD + 2 * NB * 4;        // uint2 [RAWS][SUBS]: which keys are there, the first of them
+  static constexpr int OFF_VALID = OFF_RVALID + RAWS * SUBS * 8; // the same for the fragments [2][SUBS], then [2] {exponent, any odd}
+  static constexpr int OFF_BARS = OFF_VALID + 2 * SUBS * 8 + 2 * 8;   // raw full [2], fragments full [2], empty [2]
+  static constexpr int OFF_FLAGS = OFF_BARS + 6 * 8;             // bad inputs, gave up, largest V scale, -, first key, key end
   static constexpr int SMEM = OFF_FLAGS + 32;
-  static_assert(QF_BYTES == ROWS * D * 4 && SMEM <= 227 * 1024, "shared memory");
+  static_assert(QF_BYTES == ROWS * D * 4 && OFF_RAW % 128 == 0 && SMEM <= 227 * 1024, "shared memory");
 };
+
+__device__ __forceinline__ void unpackers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory"); }
 
 template <int D, bool KQ8, bool VQ8>
 __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const AttnParams p, const RowsGrid rg, const __grid_constant__ CUtensorMap tmap_k,
@@ -71,13 +84,20 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   auto lds_f2 = [&](uint32_t at) { return *reinterpret_cast<const float2*>(smem + at); };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  const uint32_t bars = sbase + G::OFF_BARS;
-  uint32_t* flags = reinterpret_cast<uint32_t*>(smem + G::OFF_FLAGS);
-  uint2* valid = reinterpret_cast<uint2*>(smem + G::OFF_VALID);
+  const uint32_t raw_full = sbase + G::OFF_BARS, frag_full = raw_full + 16, frag_empty = raw_full + 32;
+  volatile uint32_t* flags = reinterpret_cast<uint32_t*>(smem + G::OFF_FLAGS);
+  uint2* raw_valid = reinterpret_cast<uint2*>(smem + G::OFF_RVALID);
+  uint2* valid = reinterpret_cast<uint2*>(smem + G::OFF_VALID);       // [2][SUBS]
+  uint2* summary = valid + 2 * SUBS;                                  // [2]
+  uint32_t* odd = reinterpret_cast<uint32_t*>(smem + G::OFF_ODD);     // [2][NB]
+  const bool consumer = warp < RW;
 
   if (tid == 0) {
-    ptx::mbar_init(bars, 1);
-    ptx::mbar_init(bars + 8, 1);
+    for (int s = 0; s < 2; s++) {
+      ptx::mbar_init(raw_full + 8 * s, 1);
+      ptx::mbar_init(frag_full + 8 * s, PW);
+      ptx::mbar_init(frag_empty + 8 * s, RW);
+    }
     flags[0] = flags[1] = flags[2] = flags[3] = flags[5] = 0;
     flags[4] = 0xFFFFFFFFu;
     ptx::fence_barrier_init();
@@ -101,7 +121,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
 #pragma unroll
   for (int h = 0; h < 2; h++) {
     uint32_t l;
-    my_row[h] = row_of(warp * 16 + g + 8 * h, &l);
+    my_row[h] = consumer ? row_of(warp * 16 + g + 8 * h, &l) : NO_ROW;
     lo[h] = hi[h] = 0;
     if (my_row[h] != NO_ROW) {
       const KeyRange kr = key_range(p, b, l);
@@ -119,7 +139,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   }
   w_lo = __reduce_min_sync(FULL, w_lo), w_hi = __reduce_max_sync(FULL, w_hi);
   w_all_lo = __reduce_max_sync(FULL, w_all_lo), w_all_hi = __reduce_min_sync(FULL, w_all_hi);
-  if (lane == 0 && w_hi > 0) atomicMin(flags + 4, w_lo), atomicMax(flags + 5, w_hi);
+  if (lane == 0 && w_hi > 0) atomicMin(const_cast<uint32_t*>(flags) + 4, w_lo), atomicMax(const_cast<uint32_t*>(flags) + 5, w_hi);
   __syncthreads();
   if (flags[0] && tid == 0) atomicExch(p.fault, FAULT_INVALID_ARGUMENT);
   const uint32_t u_hi = flags[5], u_lo = min(flags[4], u_hi);
@@ -130,55 +150,162 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   const uint32_t my_first = (uint32_t)min((uint64_t)whole.end, whole.first + (uint64_t)rank * per);
   const uint32_t tiles = min(whole.end - my_first, per), stages = (tiles + SUBS - 1) / SUBS;
 
-  // ---- thread 0 brings the stages; the page numbers of the next one are read a stage ahead
-  const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;
-  const uint32_t kshift = (hkv * KF::BYTES) & 15, vshift = (hkv * VF::BYTES) & 15;
-  uint32_t seg = my_first / ts.per_seg, in_seg = my_first - seg * ts.per_seg;
-  struct Place {
-    uint32_t seg, in_seg;
-    int32_t page;
-  } next[SUBS];
-  auto place = [&](uint32_t stage) {
-#pragma unroll
-    for (int s = 0; s < SUBS; s++) {
-      next[s] = Place{seg, in_seg, 0};
-      if (p.page_table && stage * SUBS + s < tiles) next[s].page = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + seg);
-      if (++in_seg >= ts.per_seg) in_seg = 0, seg++;
-    }
-  };
-  auto issue = [&](uint32_t stage) {
-    const uint32_t st = stage & 1, bar = bars + 8 * st, dst = sbase + st * G::STAGE;
-    uint32_t count[SUBS], bytes = 0;
-    uint64_t row[SUBS];
-#pragma unroll
-    for (int s = 0; s < SUBS; s++) {
-      count[s] = stage * SUBS + s < tiles ? min((uint32_t)TK, ts.seg_len - next[s].in_seg * TK) : 0;
-      row[s] = row0 + next[s].in_seg * TK;
-      if (p.page_table) {
-        if (count[s] && (next[s].page < 0 || (uint32_t)next[s].page >= p.pool_pages)) {
-          atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
-          count[s] = 0;
-        }
-        row[s] += (uint64_t)(count[s] ? next[s].page : 0) * p.page_tokens;
-      }
-      valid[st * SUBS + s] = make_uint2((1u << count[s]) - 1, next[s].seg * ts.seg_len + next[s].in_seg * TK);
-      if (count[s]) bytes += G::TILE;
-    }
-    ptx::mbar_arrive_expect_tx(bar, bytes);
-    if (p.drop_first && stage == 0) return;
-#pragma unroll
-    for (int s = 0; s < SUBS; s++)
-      if (count[s]) {
-        ptx::tma_load_2d(dst + s * G::TILE, &tmap_k, (int)((hkv * KF::BYTES) / 16 * 2), (int)row[s], bar);
-        ptx::tma_load_2d(dst + s * G::TILE + TK * KF::PITCH, &tmap_v, (int)((hkv * VF::BYTES) / 16 * 2), (int)row[s], bar);
-      }
-  };
-  if (tid == 0 && stages) {
-    place(0);
-    issue(0);
-    place(1);
-  }
+  float acc[NB][4][4];   // [block][8 dimensions][row g: 2, row g + 8: 2]
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
+  uint32_t e_run = 0;
 
+  if (!consumer) {
+    // ================ raw blocks to fragments ================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(UNPACK_REGS));
+    const int ptid = tid - RW * 32, pwarp = warp - RW;
+    const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;
+    const uint32_t kshift = (hkv * KF::BYTES) & 15, vshift = (hkv * VF::BYTES) & 15;
+    // The first of these threads brings the raw stages; the page numbers of the next one are read a stage ahead.
+    uint32_t seg = my_first / ts.per_seg, in_seg = my_first - seg * ts.per_seg;
+    uint32_t next_seg[SUBS], next_in[SUBS];
+    int32_t next_page[SUBS];
+    auto place = [&](uint32_t stage) {
+#pragma unroll
+      for (int s = 0; s < SUBS; s++) {
+        next_seg[s] = seg, next_in[s] = in_seg, next_page[s] = 0;
+        if (p.page_table && stage * SUBS + s < tiles) next_page[s] = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + seg);
+        if (++in_seg >= ts.per_seg) in_seg = 0, seg++;
+      }
+    };
+    auto issue = [&](uint32_t stage) {
+      const uint32_t st = stage % G::RAWS, bar = raw_full + 8 * st, dst = sbase + G::OFF_RAW + st * G::STAGE;
+      uint32_t count[SUBS], bytes = 0;
+      uint64_t row[SUBS];
+#pragma unroll
+      for (int s = 0; s < SUBS; s++) {
+        count[s] = stage * SUBS + s < tiles ? min((uint32_t)TK, ts.seg_len - next_in[s] * TK) : 0;
+        row[s] = row0 + next_in[s] * TK;
+        if (p.page_table) {
+          if (count[s] && (next_page[s] < 0 || (uint32_t)next_page[s] >= p.pool_pages)) {
+            atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
+            count[s] = 0;
+          }
+          row[s] += (uint64_t)(count[s] ? next_page[s] : 0) * p.page_tokens;
+        }
+        raw_valid[st * SUBS + s] = make_uint2((1u << count[s]) - 1, next_seg[s] * ts.seg_len + next_in[s] * TK);
+        if (count[s]) bytes += G::TILE;
+      }
+      ptx::mbar_arrive_expect_tx(bar, bytes);
+      if (p.drop_first && stage == 0) return;
+#pragma unroll
+      for (int s = 0; s < SUBS; s++)
+        if (count[s]) {
+          ptx::tma_load_2d(dst + s * G::TILE, &tmap_k, (int)((hkv * KF::BYTES) / 16 * 2), (int)row[s], bar);
+          ptx::tma_load_2d(dst + s * G::TILE + TK * KF::PITCH, &tmap_v, (int)((hkv * VF::BYTES) / 16 * 2), (int)row[s], bar);
+        }
+    };
+    if (ptid == 0)
+      for (uint32_t s = 0; s < min(stages, (uint32_t)G::RAWS); s++) place(s), issue(s);
+    if (ptid == 0) place(G::RAWS);
+    const uint32_t first_sel = t ? 0x3210u : 0x5432u, first_sel_v = g ? 0x3210u : 0x5432u;
+    for (uint32_t it = 0; it < stages; it++) {
+      const uint32_t buf = it & 1, raw = G::OFF_RAW + (it % G::RAWS) * G::STAGE, frag = G::OFF_FRAG + buf * G::FRAG + lane * 16;
+      bool ok = ptx::mbar_wait_bounded(raw_full + 8 * (it % G::RAWS), (it / G::RAWS) & 1, p.wait_limit);
+      if (it >= 2) ok = ptx::mbar_wait_bounded(frag_empty + 8 * buf, (it / 2 - 1) & 1, p.wait_limit) && ok;
+      if (!ok) flags[1] = 1;
+      // ---- scales
+      constexpr int PER = (NB * SK + PW * 32 - 1) / (PW * 32);
+      uint32_t vsc[PER], top = 0;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        const uint32_t blk = pwarp + PW * j;   // a warp takes the 32 keys of a block
+        vsc[j] = 0;
+        if (blk >= NB) break;
+        const uint32_t at = raw + (lane / TK) * G::TILE;
+        const float ks = half_bits(lds16(at + kshift + (lane % TK) * KF::PITCH + blk * KF::BB));
+        *reinterpret_cast<float*>(smem + G::OFF_KS + ((buf * NB + blk) * SK + lane) * 4) = ks;
+        vsc[j] = lds16(at + TK * KF::PITCH + vshift + (lane % TK) * VF::PITCH + blk * VF::BB);
+        const uint2 v = raw_valid[(it % G::RAWS) * SUBS + lane / TK];
+        const uint32_t key = v.y + lane % TK;
+        if (!((v.x >> (lane % TK)) & 1) || key < u_lo || key >= u_hi) vsc[j] = 0;   // no row sees it
+        const uint32_t not_finite = __ballot_sync(FULL, (vsc[j] & 0x7FFFu) >= 0x7C00u);
+        if ((vsc[j] & 0x7FFFu) >= 0x7C00u) vsc[j] = 0;
+        if (lane == 0) odd[buf * NB + blk] = not_finite;
+        top = max(top, vsc[j] & 0x7FFFu);
+      }
+      top = __reduce_max_sync(FULL, top);
+      if (lane == 0) atomicMax(const_cast<uint32_t*>(flags) + 2, top);
+      unpackers_sync();
+      if (flags[1]) {
+        if (ptid == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED);
+        for (uint32_t s = it; s < min(stages, it + G::RAWS); s++) ptx::mbar_wait_bounded(raw_full + 8 * (s % G::RAWS), (s / G::RAWS) & 1, p.wait_limit);
+        break;
+      }
+      const uint32_t e_new = flags[2] >> 10;   // the largest exponent so far
+      const float vmul = __uint_as_float((127u + 29u - e_new) << 23);
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        const uint32_t blk = pwarp + PW * j;
+        if (blk < NB) *reinterpret_cast<float*>(smem + G::OFF_VS + ((buf * NB + blk) * SK + lane) * 4) = half_bits(vsc[j]) * vmul;
+      }
+      if (ptid == 0) {
+        uint32_t any = 0;
+        for (int i = 0; i < NB; i++) any |= odd[buf * NB + i];
+        summary[buf] = make_uint2(e_new, any);
+        for (int s = 0; s < SUBS; s++) valid[buf * SUBS + s] = raw_valid[(it % G::RAWS) * SUBS + s];
+      }
+      // ---- K: the B operand of 8 keys x 32 dimensions
+      for (int n = pwarp; n < NB * (SK / 8); n += PW) {
+        const uint32_t blk = n / (SK / 8), k = n % (SK / 8);
+        const uint32_t row = raw + kshift + (k >> 1) * G::TILE + ((k & 1) * 8 + g) * KF::PITCH + (blk >> 1) * 2 * KF::BB;
+        uint32_t f[4];
+        if (KQ8) {
+          const uint32_t w0 = blk & 1 ? lds32(row + 36 + 4 * t) : __byte_perm(lds32(row + 4 * t), lds32(row + 32), first_sel);
+          unpack_q8(w0, &f[0], &f[1]);
+          unpack_q8(lds32(row + (blk & 1 ? 52 : 16) + 4 * t), &f[2], &f[3]);
+        } else {
+          unpack_q4_subnormal(blk & 1 ? lds32(row + 20 + 4 * t) : __byte_perm(lds32(row + 4 * t), lds32(row + 16), first_sel), f);
+        }
+        *reinterpret_cast<uint4*>(smem + frag + n * 512) = make_uint4(f[0], f[1], f[2], f[3]);
+      }
+      // ---- V: the B operand of 16 keys x 32 dimensions
+      for (int n = pwarp; n < NB * SUBS; n += PW) {
+        const uint32_t blk = n / SUBS, j = n % SUBS;
+        uint32_t f[4][2];
+#pragma unroll
+        for (int kp = 0; kp < 2; kp++) {
+          const uint32_t row = raw + j * G::TILE + TK * KF::PITCH + vshift + (2 * t + 8 * kp) * VF::PITCH;
+          if (VQ8) {
+            uint32_t x[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const uint32_t pos = row + h * VF::PITCH + (blk >> 1) * 2 * VF::BB;
+              x[h] = (blk & 1 ? lds32(pos + 36 + 4 * g) : __byte_perm(lds32(pos + 4 * g), lds32(pos + 32), first_sel_v)) ^ 0x80808080u;
+            }
+            const uint32_t lo2 = __byte_perm(x[0], x[1], 0x5140), hi2 = __byte_perm(x[0], x[1], 0x7362);
+            f[0][kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4140), 0xE480E480u);
+            f[1][kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4342), 0xE480E480u);
+            f[2][kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4140), 0xE480E480u);
+            f[3][kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4342), 0xE480E480u);
+          } else {
+            const uint32_t pos = row + blk * VF::BB + 2 + 2 * g;
+            uint32_t x = __byte_perm(lds16(pos), lds16(pos + VF::PITCH), 0x5410);
+            f[0][kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+            f[1][kp] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+            x >>= 8;
+            f[2][kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+            f[3][kp] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+          }
+        }
+        *reinterpret_cast<uint4*>(smem + frag + G::KFRAG + n * 1024) = make_uint4(f[0][0], f[0][1], f[1][0], f[1][1]);
+        *reinterpret_cast<uint4*>(smem + frag + G::KFRAG + n * 1024 + 512) = make_uint4(f[2][0], f[2][1], f[3][0], f[3][1]);
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(frag_full + 8 * buf);
+      unpackers_sync();   // the raw stage has been read
+      if (ptid == 0 && it + G::RAWS < stages) {
+        issue(it + G::RAWS);
+        place(it + G::RAWS + 1);
+      }
+    }
+  } else {
+  // ================ consumers ================
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CONSUMER_REGS));
   // ---- q as the A operand: rows g and g + 8, two terms, normed by the row's largest value to [2^13, 2^14)
   const uint32_t qf = G::OFF_QF + warp * ((D / 16) * 1024) + lane * 16;
   float factor[2];
@@ -246,78 +373,36 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   }
   __syncwarp();
 
-  float acc[NB][4][4];   // [block][8 dimensions][row g: 2, row g + 8: 2]
 #pragma unroll
   for (int i = 0; i < NB; i++)
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
       for (int e = 0; e < 4; e++) acc[i][j][e] = 0.0f;
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
-  uint32_t e_run = 0;
-  const uint32_t first_sel = t ? 0x3210u : 0x5432u, first_sel_v = g ? 0x3210u : 0x5432u;
 
   for (uint32_t it = 0; it < stages; it++) {
-    const uint32_t st = it & 1, ring = st * G::STAGE;
-    if (!ptx::mbar_wait_bounded(bars + 8 * st, (it >> 1) & 1, p.wait_limit)) flags[1] = 1;
-    // ---- this thread's part of the stage's scales
-    constexpr int PER = (NB * SK + RTHREADS - 1) / RTHREADS;
-    uint32_t ksc[PER], vsc[PER], top = 0;
-    bool weird = false;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      const uint32_t e = tid + RTHREADS * j, blk = e / SK, k = e % SK, at = ring + (k / TK) * G::TILE;
-      ksc[j] = vsc[j] = 0;
-      if (NB * SK % RTHREADS && e >= NB * SK) break;
-      ksc[j] = lds16(at + kshift + (k % TK) * KF::PITCH + blk * KF::BB);
-      vsc[j] = lds16(at + TK * KF::PITCH + vshift + (k % TK) * VF::PITCH + blk * VF::BB);
-      const uint2 v = valid[st * SUBS + k / TK];
-      const uint32_t key = v.y + k % TK;
-      if (!((v.x >> (k % TK)) & 1) || key < u_lo || key >= u_hi) vsc[j] = 0;   // no row sees it
-      if ((vsc[j] & 0x7FFFu) >= 0x7C00u) vsc[j] = 0, weird = true;
-      top = max(top, vsc[j] & 0x7FFFu);
-    }
-    top = __reduce_max_sync(FULL, top);
-    if (lane == 0) atomicMax(flags + 2, top);
-    if (weird) flags[3] = it + 1;
-    __syncthreads();
-    // Every warp has finished the last stage: its place is free for the next.
-    if (tid == 0 && it + 1 < stages && !flags[1]) {
-      issue(it + 1);
-      place(it + 2);
-    }
-    if (flags[1]) {
-      if (tid == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED);
-      ptx::mbar_wait_bounded(bars + 8 * st, (it >> 1) & 1, p.wait_limit);
+    const uint32_t buf = it & 1, frag = G::OFF_FRAG + buf * G::FRAG + lane * 16;
+    if (!__all_sync(FULL, ptx::mbar_wait_bounded(frag_full + 8 * buf, (it >> 1) & 1, p.wait_limit))) {
+      if (lane == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED), flags[1] = 1;
       break;
     }
-    const uint32_t e_new = flags[2] >> 10;   // the largest exponent so far
-    const float vmul = __uint_as_float((127u + 29u - e_new) << 23);
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      if (NB * SK % RTHREADS && tid + RTHREADS * j >= NB * SK) break;
-      *reinterpret_cast<float*>(smem + G::OFF_KS + (tid + RTHREADS * j) * 4) = half_bits(ksc[j]);
-      *reinterpret_cast<float*>(smem + G::OFF_VS + (tid + RTHREADS * j) * 4) = half_bits(vsc[j]) * vmul;
-    }
-    weird = flags[3] == it + 1;
+    const uint32_t e_new = summary[buf].x, any_odd = summary[buf].y;
     // Does some row of this warp see a key of the stage, and do all of them see all?
     bool some = false, partial = false;
     uint32_t key0[SUBS], there[SUBS];
 #pragma unroll
     for (int s = 0; s < SUBS; s++) {
-      const uint2 v = valid[st * SUBS + s];
+      const uint2 v = valid[buf * SUBS + s];
       there[s] = v.x, key0[s] = v.y;
       some |= v.x && v.y < w_hi && v.y + TK > w_lo;
       partial |= v.x != 0xFFFFu || v.y < w_all_lo || v.y + TK > w_all_hi;
     }
-    __syncthreads();
-    if (!some) continue;
+    if (some) {
 
     // ---- S: rows g and g + 8, keys 8n + 2t and 8n + 2t + 1
     float s[SK / 8][4];
 #pragma unroll
     for (int n = 0; n < SK / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-    const uint32_t krow = ring + kshift + g * KF::PITCH;
 #pragma unroll
     for (int blk = 0; blk < NB; blk++) {
       uint4 qh[2], ql[2];
@@ -332,27 +417,13 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         for (int half = 0; half < 2; half++) ci[half] = *reinterpret_cast<const float*>(smem + G::OFF_CI + ((warp * NB + blk) * 16 + g + 8 * half) * 4);
 #pragma unroll
       for (int n = 0; n < SK / 8; n++) {
-        const uint32_t row = krow + (n >> 1) * G::TILE + (n & 1) * 8 * KF::PITCH + (blk >> 1) * 2 * KF::BB;
-        uint32_t b[2][2];
-        if (KQ8) {
-          if (blk & 1) {
-            unpack_q8(lds32(row + 36 + 4 * t), &b[0][0], &b[0][1]);
-            unpack_q8(lds32(row + 52 + 4 * t), &b[1][0], &b[1][1]);
-          } else {
-            unpack_q8(__byte_perm(lds32(row + 4 * t), lds32(row + 32), first_sel), &b[0][0], &b[0][1]);
-            unpack_q8(lds32(row + 16 + 4 * t), &b[1][0], &b[1][1]);
-          }
-        } else {
-          uint32_t u[4];
-          unpack_q4_subnormal(blk & 1 ? lds32(row + 20 + 4 * t) : __byte_perm(lds32(row + 4 * t), lds32(row + 16), first_sel), u);
-          b[0][0] = u[0], b[0][1] = u[1], b[1][0] = u[2], b[1][1] = u[3];
-        }
+        const uint4 f = *reinterpret_cast<const uint4*>(smem + frag + (blk * (SK / 8) + n) * 512);
         float c[4];
-        mma_f16_from(c, ql[0].x, ql[0].y, ql[0].z, ql[0].w, b[0][0], b[0][1], ci[0], ci[0], ci[1], ci[1]);
-        mma_f16_from(c, ql[1].x, ql[1].y, ql[1].z, ql[1].w, b[1][0], b[1][1], c[0], c[1], c[2], c[3]);
-        mma_f16_from(c, qh[0].x, qh[0].y, qh[0].z, qh[0].w, b[0][0], b[0][1], c[0], c[1], c[2], c[3]);
-        mma_f16_from(c, qh[1].x, qh[1].y, qh[1].z, qh[1].w, b[1][0], b[1][1], c[0], c[1], c[2], c[3]);
-        const float2 sc = lds_f2(G::OFF_KS + (blk * SK + 8 * n + 2 * t) * 4);
+        mma_f16_from(c, ql[0].x, ql[0].y, ql[0].z, ql[0].w, f.x, f.y, ci[0], ci[0], ci[1], ci[1]);
+        mma_f16_from(c, ql[1].x, ql[1].y, ql[1].z, ql[1].w, f.z, f.w, c[0], c[1], c[2], c[3]);
+        mma_f16_from(c, qh[0].x, qh[0].y, qh[0].z, qh[0].w, f.x, f.y, c[0], c[1], c[2], c[3]);
+        mma_f16_from(c, qh[1].x, qh[1].y, qh[1].z, qh[1].w, f.z, f.w, c[0], c[1], c[2], c[3]);
+        const float2 sc = lds_f2(G::OFF_KS + ((buf * NB + blk) * SK + 8 * n + 2 * t) * 4);
         s[n][0] = fmaf(sc.x, c[0], s[n][0]);
         s[n][1] = fmaf(sc.y, c[1], s[n][1]);
         s[n][2] = fmaf(sc.x, c[2], s[n][2]);
@@ -407,7 +478,6 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       }
 
     // ---- O += P' . V
-    const uint32_t vrow = ring + TK * KF::PITCH + vshift + 2 * t * VF::PITCH;
 #pragma unroll
     for (int blk = 0; blk < NB; blk++) {
       // (Summed from zero and added in f32: the tensor core cuts its sums off to one side.)
@@ -416,37 +486,16 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       for (int i = 0; i < 4; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll
       for (int j = 0; j < SUBS; j++) {
-        uint32_t ah[4], al[4], bf[4][2];
+        uint32_t ah[4], al[4];
 #pragma unroll
         for (int kp = 0; kp < 2; kp++) {
-          const float2 v = lds_f2(G::OFF_VS + (blk * SK + TK * j + 2 * t + 8 * kp) * 4);
+          const float2 v = lds_f2(G::OFF_VS + ((buf * NB + blk) * SK + TK * j + 2 * t + 8 * kp) * 4);
           split2(s[2 * j + kp][0] * v.x, s[2 * j + kp][1] * v.y, &ah[2 * kp], &al[2 * kp]);
           split2(s[2 * j + kp][2] * v.x, s[2 * j + kp][3] * v.y, &ah[2 * kp + 1], &al[2 * kp + 1]);
-          const uint32_t row = vrow + j * G::TILE + 8 * kp * VF::PITCH;
-          if (VQ8) {
-            uint32_t x[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const uint32_t pos = row + h * VF::PITCH + (blk >> 1) * 2 * VF::BB;
-              if (blk & 1) x[h] = lds32(pos + 36 + 4 * g);
-              else x[h] = __byte_perm(lds32(pos + 4 * g), lds32(pos + 32), first_sel_v);
-              x[h] ^= 0x80808080u;
-            }
-            const uint32_t lo2 = __byte_perm(x[0], x[1], 0x5140), hi2 = __byte_perm(x[0], x[1], 0x7362);
-            bf[0][kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4140), 0xE480E480u);
-            bf[1][kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4342), 0xE480E480u);
-            bf[2][kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4140), 0xE480E480u);
-            bf[3][kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4342), 0xE480E480u);
-          } else {
-            const uint32_t pos = row + blk * VF::BB + 2 + 2 * g;
-            uint32_t x = __byte_perm(lds16(pos), lds16(pos + VF::PITCH), 0x5410);
-            bf[0][kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
-            bf[1][kp] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
-            x >>= 8;
-            bf[2][kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
-            bf[3][kp] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
-          }
         }
+        const uint4 f0 = *reinterpret_cast<const uint4*>(smem + frag + G::KFRAG + (blk * SUBS + j) * 1024);
+        const uint4 f1 = *reinterpret_cast<const uint4*>(smem + frag + G::KFRAG + (blk * SUBS + j) * 1024 + 512);
+        const uint32_t bf[4][2] = {{f0.x, f0.y}, {f0.z, f0.w}, {f1.x, f1.y}, {f1.z, f1.w}};
 #pragma unroll
         for (int i = 0; i < 4; i++) mma_f16_from(o[i], al[0], al[1], al[2], al[3], bf[i][0], bf[i][1], o[i][0], o[i][1], o[i][2], o[i][3]);
 #pragma unroll
@@ -457,18 +506,15 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[blk][i][e] += o[i][e];
     }
-    if (weird) {   // a V scale that is not finite: NaN where a row gives weight to its key
+    if (any_odd) {   // a V scale that is not finite: NaN where a row gives weight to its key
 #pragma unroll
       for (int blk = 0; blk < NB; blk++) {
+        const uint32_t which = odd[buf * NB + blk];
         bool met[2] = {false, false};
 #pragma unroll
         for (int n = 0; n < SK / 8; n++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const uint32_t k = (n & 1) * 8 + 2 * t + (e & 1);
-            const uint32_t bits = lds16(ring + (n >> 1) * G::TILE + TK * KF::PITCH + vshift + k * VF::PITCH + blk * VF::BB) & 0x7FFFu;
-            met[e >> 1] |= bits >= 0x7C00u && s[n][e] > 0.0f;
-          }
+          for (int e = 0; e < 4; e++) met[e >> 1] |= ((which >> (8 * n + 2 * t + (e & 1))) & 1) && s[n][e] > 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           const uint32_t who = __ballot_sync(FULL, met[h]);
@@ -478,6 +524,9 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         }
       }
     }
+    }
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(frag_empty + 8 * buf);   // the fragments have been read
   }
 
   // ---- the rows' sums: straight out, or through shared memory to the cluster's others
@@ -489,8 +538,8 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   const float back = __uint_as_float((127u + e_run - 29u) << 23);
   const bool report = !flags[0] && !flags[1];
   float* res = reinterpret_cast<float*>(smem + G::OFF_QF);
-  float* stats = reinterpret_cast<float*>(smem + G::OFF_CI);   // maxima, then weights
-  if (rg.cluster > 1) __syncthreads();   // every warp is done with its queries
+  float* stats = reinterpret_cast<float*>(smem + G::OFF_STATS);
+  __syncwarp();   // (a warp's sums take the place of its own queries)
 #pragma unroll
   for (int h = 0; h < 2; h++) {
     const uint32_t r = warp * 16 + g + 8 * h;
@@ -522,9 +571,11 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         }
       }
   }
+  }   // consumers
   if (rg.cluster == 1) return;
+  const bool report = !flags[0] && !flags[1];
   cluster_sync();
-  const uint32_t share = ROWS / rg.cluster, res_addr = sbase + G::OFF_QF, stats_addr = sbase + G::OFF_CI;
+  const uint32_t share = ROWS / rg.cluster, res_addr = sbase + G::OFF_QF, stats_addr = sbase + G::OFF_STATS;
   for (uint32_t i = tid; i < share * (D / 4); i += RTHREADS) {
     const uint32_t r = rank * share + i / (D / 4), d4 = i % (D / 4);
     uint32_t l;
