@@ -415,19 +415,27 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       if (!KQ8)
 #pragma unroll
         for (int half = 0; half < 2; half++) ci[half] = *reinterpret_cast<const float*>(smem + G::OFF_CI + ((warp * NB + blk) * 16 + g + 8 * half) * 4);
+      // (Step by step over all keys: neighbouring MMAs are independent.)
+      uint4 f[SK / 8];
+      float c[SK / 8][4];
 #pragma unroll
       for (int n = 0; n < SK / 8; n++) {
-        const uint4 f = *reinterpret_cast<const uint4*>(smem + frag + (blk * (SK / 8) + n) * 512);
-        float c[4];
-        mma_f16_from(c, ql[0].x, ql[0].y, ql[0].z, ql[0].w, f.x, f.y, ci[0], ci[0], ci[1], ci[1]);
-        mma_f16_from(c, ql[1].x, ql[1].y, ql[1].z, ql[1].w, f.z, f.w, c[0], c[1], c[2], c[3]);
-        mma_f16_from(c, qh[0].x, qh[0].y, qh[0].z, qh[0].w, f.x, f.y, c[0], c[1], c[2], c[3]);
-        mma_f16_from(c, qh[1].x, qh[1].y, qh[1].z, qh[1].w, f.z, f.w, c[0], c[1], c[2], c[3]);
+        f[n] = *reinterpret_cast<const uint4*>(smem + frag + (blk * (SK / 8) + n) * 512);
+        mma_f16_from(c[n], ql[0].x, ql[0].y, ql[0].z, ql[0].w, f[n].x, f[n].y, ci[0], ci[0], ci[1], ci[1]);
+      }
+#pragma unroll
+      for (int n = 0; n < SK / 8; n++) mma_f16_from(c[n], ql[1].x, ql[1].y, ql[1].z, ql[1].w, f[n].z, f[n].w, c[n][0], c[n][1], c[n][2], c[n][3]);
+#pragma unroll
+      for (int n = 0; n < SK / 8; n++) mma_f16_from(c[n], qh[0].x, qh[0].y, qh[0].z, qh[0].w, f[n].x, f[n].y, c[n][0], c[n][1], c[n][2], c[n][3]);
+#pragma unroll
+      for (int n = 0; n < SK / 8; n++) mma_f16_from(c[n], qh[1].x, qh[1].y, qh[1].z, qh[1].w, f[n].z, f[n].w, c[n][0], c[n][1], c[n][2], c[n][3]);
+#pragma unroll
+      for (int n = 0; n < SK / 8; n++) {
         const float2 sc = lds_f2(G::OFF_KS + ((buf * NB + blk) * SK + 8 * n + 2 * t) * 4);
-        s[n][0] = fmaf(sc.x, c[0], s[n][0]);
-        s[n][1] = fmaf(sc.y, c[1], s[n][1]);
-        s[n][2] = fmaf(sc.x, c[2], s[n][2]);
-        s[n][3] = fmaf(sc.y, c[3], s[n][3]);
+        s[n][0] = fmaf(sc.x, c[n][0], s[n][0]);
+        s[n][1] = fmaf(sc.y, c[n][1], s[n][1]);
+        s[n][2] = fmaf(sc.x, c[n][2], s[n][2]);
+        s[n][3] = fmaf(sc.y, c[n][3], s[n][3]);
       }
     }
     // ---- softmax
