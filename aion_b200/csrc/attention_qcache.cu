@@ -498,12 +498,6 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     if (blk < NB) qfrag[(2 * blk) * 32 + lane] = made[j][0], qfrag[(2 * blk + 1) * 32 + lane] = made[j][1];
   }
   __syncthreads();
-  uint32_t qh[D / 16][2], ql[D / 16][2];
-#pragma unroll
-  for (int i = 0; i < D / 16; i++) {
-    const uint4 f = qfrag[i * 32 + lane];
-    qh[i][0] = f.x, qh[i][1] = f.y, ql[i][0] = f.z, ql[i][1] = f.w;
-  }
   // With a soft cap the logits are wanted first; else they go straight to base 2.
   const float to_base2 = p.soft_cap > 0.0f ? 1.0f : LOG2E;
   const float f0 = col_factor[2 * t] * to_base2, f1 = col_factor[2 * t + 1] * to_base2;
@@ -592,6 +586,12 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     for (int j = 0; j < TPI; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
 #pragma unroll
     for (int pr = 0; pr < NB / 2; pr++) {
+      uint32_t qh[4][2], ql[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint4 f = qfrag[(4 * pr + i) * 32 + lane];
+        qh[i][0] = f.x, qh[i][1] = f.y, ql[i][0] = f.z, ql[i][1] = f.w;
+      }
       float4 init[2];
 #pragma unroll
       for (int k = 0; k < 2; k++) init[k] = KQ8 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(ci + (2 * pr + k) * 2 * COLS + 4 * t);
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
         }
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-          const int q = 2 * (2 * pr + k);
+          const int q = 2 * k;
           float c[4];
           mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], ql[q][0], ql[q][1], init[k].x, init[k].y, init[k].z, init[k].w);
           mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], ql[q + 1][0], ql[q + 1][1], c[0], c[1], c[2], c[3]);
@@ -688,8 +688,8 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
 #pragma unroll
           for (int kp = 0; kp < 2; kp++) {
             const float2 v = lds_f2(vs + (blk * KI + j * TK + 2 * t + 8 * kp) * 4);
-            const float w0 = y[4 * j + 2 * kp] * v.x, w1 = y[4 * j + 2 * kp + 1] * v.y;
-            split2(w0, w1, &bh[j][kp], &blw[j][kp]);
+            const float2 w = mul2(make_float2(y[4 * j + 2 * kp], y[4 * j + 2 * kp + 1]), v);
+            split2(w.x, w.y, &bh[j][kp], &blw[j][kp]);
             const uint32_t row = at[j] + TK * KF::PITCH + vshift + (2 * t + 8 * kp) * VF::PITCH;
             if (VQ8) {
               uint32_t x[2];
@@ -726,8 +726,8 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
           for (int j = 0; j < TPI; j++) mma_f16_from(o, a[j][m][0], a[j][m][1], a[j][m][2], a[j][m][3], blw[j][0], blw[j][1], o[0], o[1], o[2], o[3]);
 #pragma unroll
           for (int j = 0; j < TPI; j++) mma_f16_from(o, a[j][m][0], a[j][m][1], a[j][m][2], a[j][m][3], bh[j][0], bh[j][1], o[0], o[1], o[2], o[3]);
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[2 * blk + m][e] += o[e];
+          add2(acc[2 * blk + m][0], acc[2 * blk + m][1], o[0], o[1]);
+          add2(acc[2 * blk + m][2], acc[2 * blk + m][3], o[2], o[3]);
         }
       }
     if (weird) {

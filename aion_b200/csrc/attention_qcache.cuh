@@ -101,6 +101,20 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
   *lo = pack_half2(la, lb);
 }
 
+// Two f32 products or sums in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&d);
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  const float2 u = make_float2(x, y), v = make_float2(a, b);
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<const uint64_t*>(&u)), "l"(*reinterpret_cast<const uint64_t*>(&v)));
+  const float2 r = *reinterpret_cast<const float2*>(&d);
+  x = r.x, y = r.y;
+}
+
 // Which dimension of a block the lane index u (t of a key row's words) reaches with code i of its word(s).
 // K words: q4_0 one word of eight nibbles per lane t; q8_0 two words, u = t and t + 4, of four bytes.
 __host__ __device__ constexpr int pair_byte(bool q8, bool second, int u, int j) {

@@ -498,8 +498,9 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
 #pragma unroll
         for (int kp = 0; kp < 2; kp++) {
           const float2 v = lds_f2(G::OFF_VS + ((buf * NB + blk) * SK + TK * j + 2 * t + 8 * kp) * 4);
-          split2(s[2 * j + kp][0] * v.x, s[2 * j + kp][1] * v.y, &ah[2 * kp], &al[2 * kp]);
-          split2(s[2 * j + kp][2] * v.x, s[2 * j + kp][3] * v.y, &ah[2 * kp + 1], &al[2 * kp + 1]);
+          const float2 w0 = mul2(make_float2(s[2 * j + kp][0], s[2 * j + kp][1]), v), w1 = mul2(make_float2(s[2 * j + kp][2], s[2 * j + kp][3]), v);
+          split2(w0.x, w0.y, &ah[2 * kp], &al[2 * kp]);
+          split2(w1.x, w1.y, &ah[2 * kp + 1], &al[2 * kp + 1]);
         }
         const uint4 f0 = *reinterpret_cast<const uint4*>(smem + frag + G::KFRAG + (blk * SUBS + j) * 1024);
         const uint4 f1 = *reinterpret_cast<const uint4*>(smem + frag + G::KFRAG + (blk * SUBS + j) * 1024 + 512);
@@ -511,8 +512,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       }
 #pragma unroll
       for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[blk][i][e] += o[i][e];
+        add2(acc[blk][i][0], acc[blk][i][1], o[i][0], o[i][1]), add2(acc[blk][i][2], acc[blk][i][3], o[i][2], o[i][3]);
     }
     if (any_odd) {   // a V scale that is not finite: NaN where a row gives weight to its key
 #pragma unroll
