@@ -5,8 +5,9 @@ to the benchmark's dense core: per layer
 
     x_norm = RMSNorm(x)
     q, k, v = MatMul(x_norm, Wq | Wk | Wv)              q4_0 [K/32][N] weights
+    q, k    = RMSNorm(q | k) per head                   (qk_norm only)
     q, k    = RoPE1D(q | k, positions)
-    K, V    = SequenceAppend(cache, Cast(k | v -> f16), write_index)
+    K, V    = SequenceAppend(cache, Cast(k | v -> f16), write_index)    (f16, or quantized as it is appended)
     a       = Attention(q, K, V, positions, visible_end, scale, causal)
     x       = x + RMSNorm(MatMul(a, Wo))                 (RMSNorm with residual)
     h       = RMSNorm(x)
@@ -38,7 +39,7 @@ import numpy as np
 from . import capi
 from .backend import (AttentionWindow, Chunk, CudaBackend, CudaSession, DeviceStore, StepArgMax, StepAttention, StepCast,
                       StepElemwiseBinary, StepGatherRows, StepMatMul, StepRMSNorm, StepRMSNormPair, StepRoPE1D,
-                      StepRopeKVAppend, StepSequenceAppend, TensorMeta, _check, act_image_meta)
+                      StepRopeKVAppend, StepSequenceAppend, StepQKNormRopeAppend, TensorMeta, _check, act_image_meta)
 
 F32, F16, I32, Q4, Q8 = capi.DTYPE_F32, capi.DTYPE_F16, capi.DTYPE_I32, capi.DTYPE_Q4_0, capi.DTYPE_Q8_0
 
@@ -56,6 +57,16 @@ class DecoderConfig:
     eps: float = 1e-6
     rope_base: float = 10000.0
     weight_dtype: int = Q4
+    # KV cache: f16, or q8_0 / q4_0 blocks (53 % and 28 % of its bytes); K and V each of their own type.
+    k_dtype: int = F16
+    v_dtype: int = F16
+    # RMSNorm of every query and key head (gamma = 1) before the rotation.
+    qk_norm: bool = False
+
+    @property
+    def plain_cache(self) -> bool:
+        """f16 caches and heads without a norm: `StepRopeKVAppend`; else `StepQKNormRopeAppend`."""
+        return self.k_dtype == F16 and self.v_dtype == F16 and not self.qk_norm
 
     @property
     def q_width(self) -> int:
@@ -81,7 +92,8 @@ class DecoderConfig:
         return self.weights_per_step() // 32 * bb
 
     def kv_bytes_per_request_step(self) -> int:
-        return self.layers * 2 * self.ctx * self.kv_width * 2
+        row = sum(self.kv_width // 32 * (18 if dt == Q4 else 34) if dt in (Q4, Q8) else 2 * self.kv_width for dt in (self.k_dtype, self.v_dtype))
+        return self.layers * self.ctx * row
 
 
 def quantize_on_device(backend: CudaBackend, dtype: int, src: capi.Operand, shape: tuple, quant_axis: int, dst: capi.Operand) -> None:
@@ -193,14 +205,16 @@ class SyntheticDecoder:
 
     def _build_state(self) -> None:
         cfg, st, R = self.cfg, self.store, self.requests
+        self.head_beta = st.add(TensorMeta(F32, (cfg.head_dim,)), np.zeros(cfg.head_dim, np.float32)) if cfg.qk_norm else None
+        self.head_gamma = st.add(TensorMeta(F32, (cfg.head_dim,)), np.ones(cfg.head_dim, np.float32)) if cfg.qk_norm else None
         self.tokens = st.add(TensorMeta(I32, (R, 1)), np.zeros((R, 1), np.int32))
         self.positions = st.add(TensorMeta(I32, (R, 1)), np.zeros((R, 1), np.int32))
         self.write_index = st.add(TensorMeta(I32, (R,)), np.zeros(R, np.int32))
         self.visible_end = st.add(TensorMeta(I32, (R,)), np.zeros(R, np.int32))
         self.k_cache, self.v_cache = [], []
         for _ in range(cfg.layers):
-            for lst in (self.k_cache, self.v_cache):
-                tid = st.add(TensorMeta(F16, (R, cfg.ctx, cfg.kv_heads, cfg.head_dim)))
+            for lst, dt in ((self.k_cache, cfg.k_dtype), (self.v_cache, cfg.v_dtype)):
+                tid = st.add(TensorMeta(dt, (R, cfg.ctx, cfg.kv_heads, cfg.head_dim), quant_axis=3))
                 ch = st.acquire_mut(tid)
                 self.backend.device_memory.memset(ch.handle, ch.offset, 0, ch.len)
                 lst.append(tid)
@@ -251,12 +265,12 @@ class SyntheticDecoder:
                 StepMatMul(c=self.q, a=self.x_norm, b=w["wq"]),
                 StepMatMul(c=self.k, a=self.x_norm, b=w["wk"]),
                 StepMatMul(c=self.v, a=self.x_norm, b=w["wv"]),
+                *(StepRMSNorm(out=t, x=t, gamma=self.head_gamma, beta=self.head_beta, eps=cfg.eps) for t in (self.q4, self.k4) if cfg.qk_norm),
                 StepRoPE1D(out=self.q4, x=self.q4, positions=self.positions, base_frequency=cfg.rope_base),
                 StepRoPE1D(out=self.k4, x=self.k4, positions=self.positions, base_frequency=cfg.rope_base),
-                StepCast(out=self.k16, x=self.k4, to_dtype=F16),
-                StepCast(out=self.v16, x=self.v4, to_dtype=F16),
-                StepSequenceAppend(cache=self.k_cache[layer], new_kv=self.k16, end_index=self.write_index),
-                StepSequenceAppend(cache=self.v_cache[layer], new_kv=self.v16, end_index=self.write_index),
+                *(step for new, half, cache, dt in ((self.k4, self.k16, self.k_cache[layer], cfg.k_dtype), (self.v4, self.v16, self.v_cache[layer], cfg.v_dtype))
+                  for step in ([StepCast(out=half, x=new, to_dtype=F16), StepSequenceAppend(cache=cache, new_kv=half, end_index=self.write_index)]
+                               if dt == F16 else [StepSequenceAppend(cache=cache, new_kv=new, end_index=self.write_index)])),
                 StepAttention(out=self.attn, q=self.q4, k=self.k_cache[layer], v=self.v_cache[layer],
                               query_positions=self.positions, kv_lengths=self.visible_end, scale=scale,
                               window=AttentionWindow.causal()),
@@ -288,7 +302,10 @@ class SyntheticDecoder:
             steps += [
                 StepMatMul(c=self.qkv, a=self.x_norm, b=w["wqkv"], a_image=ixn),
                 StepRopeKVAppend(q_out=self.q_rot, qkv=self.qkv, positions=self.positions, end_index=self.write_index,
-                                 k_cache=self.k_cache[layer], v_cache=self.v_cache[layer], base_frequency=cfg.rope_base),
+                                 k_cache=self.k_cache[layer], v_cache=self.v_cache[layer], base_frequency=cfg.rope_base) if cfg.plain_cache else
+                StepQKNormRopeAppend(q_out=self.q_rot, qkv=self.qkv, positions=self.positions, end_index=self.write_index,
+                                     k_cache=self.k_cache[layer], v_cache=self.v_cache[layer], base_frequency=cfg.rope_base,
+                                     q_gamma=self.head_gamma, k_gamma=self.head_gamma, eps=cfg.eps),
                 StepAttention(out=self.attn, q=self.q_rot, k=self.k_cache[layer], v=self.v_cache[layer],
                               query_positions=self.positions, kv_lengths=self.visible_end, scale=scale,
                               window=AttentionWindow.causal(), image=iat),

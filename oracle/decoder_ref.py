@@ -46,6 +46,18 @@ class OracleDecoder:
                                         threads=getattr(self, "threads", 0)).reshape(m, n)
         return oracle.matmul_q(self.dt, a.reshape(m, k), self.w[name], m, n, k).reshape(m, n)
 
+    def _append(self, l, k, v, index):
+        """New rows into the caches; a quantized one is kept as the f32 values that its blocks stand for."""
+        for caches, rows, dt in ((self.k_cache, k, getattr(self.cfg, "k_dtype", oracle.F16)), (self.v_cache, v, getattr(self.cfg, "v_dtype", oracle.F16))):
+            if dt in (oracle.Q4_0, oracle.Q8_0):
+                d = rows.shape[-1]
+                rows = oracle.dequant(dt, oracle.quantize(dt, np.ascontiguousarray(rows).reshape(-1, d), 1)).reshape(rows.shape)
+                if caches[l].dtype != np.float32:
+                    caches[l] = caches[l].astype(np.float32)
+            else:
+                rows = oracle.cast_f32_f16(rows)
+            caches[l] = oracle.sequence_append(caches[l], rows, index)
+
     def step(self, tokens, positions):
         cfg, R = self.cfg, self.R
         pos = np.asarray(positions, np.int32).reshape(R, 1)
@@ -64,10 +76,12 @@ class OracleDecoder:
             q = np.ascontiguousarray(q).reshape(R, 1, cfg.heads, cfg.head_dim)
             k = np.ascontiguousarray(k).reshape(R, 1, cfg.kv_heads, cfg.head_dim)
             v = np.ascontiguousarray(v).reshape(R, 1, cfg.kv_heads, cfg.head_dim)
+            if getattr(cfg, "qk_norm", False):
+                one, zero = np.ones(cfg.head_dim, np.float32), np.zeros(cfg.head_dim, np.float32)
+                q, k = (oracle.rms_norm(x.reshape(-1, cfg.head_dim), one, zero, cfg.eps).reshape(x.shape) for x in (q, k))
             q = oracle.rope(q, pos, cfg.rope_base)
             k = oracle.rope(k, pos, cfg.rope_base)
-            self.k_cache[l] = oracle.sequence_append(self.k_cache[l], oracle.cast_f32_f16(k), pos.reshape(R))
-            self.v_cache[l] = oracle.sequence_append(self.v_cache[l], oracle.cast_f32_f16(v), pos.reshape(R))
+            self._append(l, k, v, pos.reshape(R))
             a = oracle.attention(q, self.k_cache[l], self.v_cache[l], scale=1.0 / np.sqrt(cfg.head_dim), positions=pos,
                                  kv_lengths=(pos.reshape(R) + 1).astype(np.int32), right=0)
             o = self._mm(a.reshape(R, cfg.q_width), f"l{l}.wo", cfg.q_width, cfg.hidden)

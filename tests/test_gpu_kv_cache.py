@@ -782,3 +782,87 @@ def test_an_expired_wait_in_the_rows_kernel_is_reported(sess, backend):
         lib.aion_cuda_debug_expire_waits(backend.handle, 0)
     s.execute([step])
     assert np.array_equal(store.read(step.out), want)
+
+
+# ---- the decoder ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("kdt,vdt,norm", [(Q8, Q8, False), (Q8, Q4, True), (Q4, Q4, True), (F16, F16, True)])
+@pytest.mark.parametrize("R", [1, 5])
+def test_decoder_with_quantized_caches_and_normed_heads(backend, R, kdt, vdt, norm, fused):
+    """The synthetic decoder step by step against the same graph of oracle ops, and its recorded program against its steps. The
+    chain re-quantizes its activations before every matmul: 2e-2, as for f16 caches (a code of the cache that falls on the other
+    side of a border moves one value of 256 by a step, less than that)."""
+    from aion_b200.decoder import DecoderConfig, SyntheticDecoder
+    from oracle.decoder_ref import OracleDecoder
+    from tests.test_gpu_decoder import CHAIN_TOL, make_values, rel_l2
+    cfg = DecoderConfig(layers=2, hidden=256, ffn=512, heads=4, kv_heads=2, head_dim=64, vocab=512, ctx=32, k_dtype=kdt, v_dtype=vdt, qk_norm=norm)
+    w, emb = make_values(cfg)
+    dec = SyntheticDecoder(backend, cfg, R, lambda name, k, n: w[name], lambda v0, v1: emb[v0:v1], fused=fused)
+    oracle_dec = OracleDecoder(cfg, R, w, emb)
+    rng = np.random.default_rng(7)
+    try:
+        for t in range(4):
+            tokens, pos = rng.integers(0, cfg.vocab, R).astype(np.int32), np.full(R, t, np.int32)
+            dec.set_inputs(tokens, pos)
+            dec.execute()
+            _, logits, _ = oracle_dec.step(tokens, pos)
+            got = dec.store.read(dec.logits).reshape(R, cfg.vocab)
+            assert rel_l2(got, logits) < CHAIN_TOL
+        dec.record()
+        dec.launch()                                       # the last step again: the same row is written, the same keys are seen
+        assert np.array_equal(dec.store.read(dec.logits).reshape(R, cfg.vocab), got)
+    finally:
+        dec.deinit()
+
+
+@pytest.mark.parametrize("dtype", [Q8, Q4], ids=["q8", "q4"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_writes_the_image_of_its_output(sess, backend, dtype, D):
+    """The activation image next to the output is the one that aion_cuda_act_image makes of it: alone and over a cluster."""
+    from aion_b200.backend import act_image_meta
+    from tests.gpu_util import DevBuf, make_image
+    s, store = sess
+    for T in (40, 1500):
+        q, k, v = inputs([D, T], 3, T, 1, D, 1, 8, Q4, Q8)
+        tid = store.add(act_image_meta(3, 8 * D, dtype))
+        out, _ = run_attention(sess, q, k, v, Q4, Q8, scale=0.1, image=tid)
+        buf = DevBuf(backend, np.ascontiguousarray(out, dtype=np.float32).reshape(-1))
+        want = make_image(backend, dtype, buf, 3, 8 * D)
+        assert np.array_equal(store.read(tid).view(np.uint8), want.read(np.uint8))
+        buf.free(), want.free()
+
+
+@pytest.mark.parametrize("T,L,first", [(1, 1, 7), (3, 2, 50), (5, 9, 2), (16, 4, 100), (17, 4, 2**31 - 21)])
+def test_tiny_rings_and_steps_near_the_last(sess, T, L, first):
+    """Rings of a few rows, and positions up to the largest 32-bit step."""
+    B, H, D = 1, 2, 64
+    q, k, v = inputs([T, L], B, T, H, D, L, 4, Q8, Q4)
+    pos = first + np.arange(L, dtype=np.int64)[None]
+    lens = [int(pos[0, -1]) + 1]
+    for flags in (0, *FORCED):
+        got, _ = run_attention(sess, q, k, v, Q8, Q4, scale=0.1, positions=pos.astype(np.int32), lengths=lens, layout="rolling",
+                               window=AttentionWindow.causal(), flags=flags)
+        check(got, *ref.attention(q, k, v, Q8, Q4, scale=0.1, positions=pos, lengths=lens, rolling=True))
+
+
+def test_two_devices_of_one_gpu_at_once(sess, backend):
+    """Two device objects, each with its stream and scratch, issue attention and appends in turn without waiting: both get what
+    each gets alone."""
+    from aion_b200.backend import CudaBackend
+    other = CudaBackend(0)
+    store2 = DeviceStore(other.device_memory)
+    sess2 = (other.create_session(store2), store2)
+    try:
+        data = [inputs([n], 3, 1100, 2, 128, 1, 8, Q8, Q4) for n in (1, 2)]
+        alone = [run_attention(x, *d, Q8, Q4, scale=0.1) for x, d in zip((sess, sess2), data)]
+        for x, (_, step) in zip((sess, sess2), alone):
+            x[1].write(step.out, np.zeros((3, 1, 8, 128), np.float32))
+        for _ in range(20):
+            for x, (_, step) in zip((sess, sess2), alone):
+                x[0].execute([step])
+        for x, (out, step) in zip((sess, sess2), alone):
+            assert np.array_equal(x[1].read(step.out), out)
+    finally:
+        other.sync()
+        store2.deinit()
+        other.deinit()
