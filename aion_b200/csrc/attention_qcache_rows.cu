@@ -1,19 +1,20 @@
 // `Attention` over a quantized KV cache for many query rows (prompts, several new rows per request): a CTA holds up to 128
-// rows of one kv head, a row being (query position, query head of the group), sixteen to a warp, and streams the keys once
-// for all of them.
+// rows of one kv head, a row being (query position, query head of the group), and streams the keys once for all of them,
+// 64 to a stage, through the tensor cores of the fifth generation.
 //
-//  * S[16 x 64] = Q . C^T and O[16 x D] += P' . V-codes on f16 m16n8k16 with the codes as exact f16 integers (see
-//    attention_qcache.cu): q and P' = p * (V scale) are two f16 terms each, so the tensor pipe does 8 * rows * keys * D
-//    operations for the 4 that f32 attention counts, and half its rate is the ceiling. Dequantized operands for tcgen05
-//    would need two terms of K and V as well (three products each), and 128 x 256 queries in two terms fill the shared
-//    memory that their tiles would need.
-//  * The logits' fragment is the second product's A operand as it stands; only the scale of (key, block) is multiplied in
-//    per block of 32 dimensions, before the split into two terms.
-//  * Four warps turn the raw blocks into fragments of f16 codes, in the order in which the MMAs' lanes take them, and the
-//    scales into f32; eight warps consume them, sixteen rows each. (With every warp unpacking for itself a tensor
-//    instruction came with eight others, and the 1024-row chunk that takes XXX us took 721.) Two buffers of 32 keys lie
-//    between the two sides; raw tiles arrive as TMA boxes of 16 rows. The consumers hold 216 registers, the unpacking
-//    warps 72.
+//  * f32 attention on f16 operands: q, P = exp2(S - max), and the dequantized K and V (code * scale is 19 bits) are two f16
+//    terms each, and each product is the sum of three (lo.hi, hi.lo, hi.hi; what is left out is 2^-22). So the tensor pipe does
+//    6 * 2 * rows * keys * D operations for the 4 * rows * keys * D that f32 attention counts: a third of its rate is the ceiling.
+//  * A row of a cache is brought to a common power of two, so that its largest scale lies in [2^7, 2^8): a small scale next to
+//    a large one of another row loses nothing. The power comes back per key, times the logit and times P.
+//  * Both products take A from tensor memory: q (two terms, D columns) stays there for the whole walk, P overwrites the logits
+//    it is made of. Shared memory holds the two B operands, one 128-byte-swizzled panel per 64 dimensions, K read K-major and V
+//    N-major, so that both are unpacked the same way.
+//  * O of a stage is summed from zero in tensor memory, 64 dimensions at a time in two buffers, and added in f32 registers (the
+//    tensor core cuts its sums off to one side; and the running maximum then costs no trip to tensor memory and back).
+//  * Eight warps do the softmax and hold O (a thread: one row, half of the keys and of every 64 dimensions), six unpack, one
+//    issues the products, one the TMA boxes of 16 rows. The product of the next stage's logits is issued before this stage's
+//    P . V, so that the softmax runs under it.
 //  * A context too long for the few CTAs of a short prompt is cut over a cluster, whose CTAs add up their sums through
 //    distributed shared memory.
 #include <cmath>
@@ -21,6 +22,7 @@
 #include <mutex>
 
 #include "attention_qcache.cuh"
+#include "tcgen05.cuh"
 
 namespace aion {
 
@@ -28,14 +30,19 @@ namespace {
 
 using namespace qcache;
 
-constexpr int RW = 8;                 // consumer warps
-constexpr int PW = 4;                 // unpacking warps
-constexpr int RTHREADS = (RW + PW) * 32;
-constexpr int ROWS = RW * 16;
-constexpr int SUBS = 2;               // tiles of a stage
+constexpr int CW = 8;                 // softmax warps
+constexpr int MMA_WARP = 8, LOAD_WARP = 9, FIRST_UNPACK = 10;
+constexpr int UW = 6;                 // unpacking warps
+constexpr int RTHREADS = 16 * 32;
+constexpr int ROWS = 128;
+constexpr int SUBS = 4;               // tiles of a stage
 constexpr int SK = SUBS * TK;         // keys of a stage
-constexpr int CONSUMER_REGS = 216, UNPACK_REGS = 72;
-static_assert(CONSUMER_REGS * RW * 32 + UNPACK_REGS * PW * 32 <= 168 * RTHREADS, "the registers that the block is launched with");
+constexpr int KRAWS = 3, VRAWS = 2;   // raw stages
+constexpr int SLOTS = 4;              // stages whose exponents and masks are kept
+constexpr int SOFTMAX_REGS = 200, OTHER_REGS = 56;
+static_assert((SOFTMAX_REGS + OTHER_REGS) * (RTHREADS / 2) <= 128 * RTHREADS, "the registers that the block is launched with");
+static_assert(SK == 64 && FIRST_UNPACK + UW == RTHREADS / 32, "a stage is one panel of 64 keys");
+constexpr int PANEL = SK * 128;       // bytes of 64 keys x 64 dimensions of f16
 
 struct RowsGrid {
   uint32_t cluster;      // CTAs that share a unit's keys
@@ -47,29 +54,140 @@ template <int D, bool KQ8, bool VQ8>
 struct RowsGeom {
   using K = RowFmt<D, KQ8>;
   using V = RowFmt<D, VQ8>;
-  static constexpr int NB = D / QK;
-  static constexpr int TILE = TK * (K::PITCH + V::PITCH);
-  static constexpr int STAGE = SUBS * TILE;
-  static constexpr int RAWS = D == 256 ? 1 : 2;                  // raw stages
-  static constexpr int KFRAG = NB * (SK / 8) * 512, VFRAG = NB * SUBS * 1024, FRAG = KFRAG + VFRAG;
-  static constexpr int OFF_QF = 0;                               // uint4 [warp][D / 16][hi, lo][32]; at the end f32 [ROWS][D]
-  static constexpr int QF_BYTES = RW * (D / 16) * 2 * 512;
-  static constexpr int OFF_FRAG = OFF_QF + QF_BYTES;             // uint4 [2][K: block, 8 keys][32], [V: block, 16 keys, half][32]
-  static constexpr int OFF_RAW = OFF_FRAG + 2 * FRAG;
-  static constexpr int OFF_KS = OFF_RAW + RAWS * STAGE;          // f32 [2][block][32]: K scales
-  static constexpr int OFF_VS = OFF_KS + 2 * NB * SK * 4;        // f32 [2][block][32]: V scales, times 2^(29 - E)
-  static constexpr int OFF_CI = OFF_VS + 2 * NB * SK * 4;        // f32 [warp][block][16]: -8 sum q
-  static constexpr int OFF_STATS = OFF_CI + RW * NB * 16 * 4;    // f32 [2][ROWS]: the rows' maxima and weights, for the cluster
-  static constexpr int OFF_ODD = OFF_STATS + 2 * ROWS * 4;       // u32 [2][block]: keys whose V scale is not finite
-  static constexpr int OFF_RVALID = OFF_ODD + 2 * NB * 4;        // uint2 [RAWS][SUBS]: which keys are there, the first of them
-  static constexpr int OFF_VALID = OFF_RVALID + RAWS * SUBS * 8; // the same for the fragments [2][SUBS], then [2] {exponent, any odd}
-  static constexpr int OFF_BARS = OFF_VALID + 2 * SUBS * 8 + 2 * 8;   // raw full [2], fragments full [2], empty [2]
-  static constexpr int OFF_FLAGS = OFF_BARS + 6 * 8;             // bad inputs, gave up, largest V scale, -, first key, key end
-  static constexpr int SMEM = OFF_FLAGS + 32;
-  static_assert(QF_BYTES == ROWS * D * 4 && OFF_RAW % 128 == 0 && SMEM <= 227 * 1024, "shared memory");
+  static constexpr int NP = D / 64;
+  static constexpr int KRAW = SK * K::PITCH, VRAW = SK * V::PITCH;
+  static constexpr int OFF_K = 0;                                // [hi, lo][panel]; first f32 q [ROWS][D], at the end f32 sums
+  static constexpr int OFF_V = OFF_K + 2 * NP * PANEL;           // [hi, lo][panel]
+  static constexpr int OFF_KRAW = OFF_V + 2 * NP * PANEL;
+  static constexpr int OFF_VRAW = OFF_KRAW + KRAWS * KRAW;
+  static constexpr int OFF_KEXP = OFF_VRAW + VRAWS * VRAW;       // f32 [SLOTS][SK]: the keys' powers of two
+  static constexpr int OFF_VEXP = OFF_KEXP + SLOTS * SK * 4;
+  static constexpr int OFF_EX = OFF_VEXP + SLOTS * SK * 4;       // f32 [2][2][ROWS]: maxima (or NaN blocks) of the two halves of a row
+  static constexpr int OFF_STATS = OFF_EX + 4 * ROWS * 4;        // f32 [2][ROWS]: the rows' maxima and weights, for the cluster
+  static constexpr int OFF_VMAX = OFF_STATS + 2 * ROWS * 4;      // u32 [SLOTS][8]: largest V exponent that an unpacking warp met, 256 for a scale that is not finite
+  static constexpr int OFF_VALID = OFF_VMAX + SLOTS * 8 * 4;     // uint2 [SLOTS][SUBS]: which keys are there, the first of them
+  static constexpr int OFF_ODD = OFF_VALID + SLOTS * SUBS * 8;   // u8 [SLOTS][SK]: blocks of a key whose V scale is not finite
+  static constexpr int OFF_PAIR = OFF_ODD + SLOTS * SK;          // u32 [2][2][4]: did the half of the rows meet such a scale?
+  static constexpr int OFF_BARS = OFF_PAIR + 16 * 4;
+  static constexpr int OFF_FLAGS = OFF_BARS + 26 * 8;            // bad inputs, gave up, TMEM, -, first key, key end
+  static constexpr int SMEM = OFF_FLAGS + 32 + 1024;             // (panels begin on 1024 bytes)
+  static_assert(4 * NP * PANEL == ROWS * D * 4 && OFF_KRAW % 128 == 0 && KRAW % 128 == 0 && VRAW % 128 == 0 && SMEM <= 227 * 1024, "shared memory");
+  // tensor memory: columns of 32 bits
+  static constexpr uint32_t T_Q = 0, T_S = D, T_O = D + 2 * 64;
+  static_assert(T_O + 2 * 64 <= 512, "tensor memory");
 };
 
-__device__ __forceinline__ void unpackers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(PW * 32) : "memory"); }
+// D f32, A and B f16, M = 128, N = 64; B K-major, or (bit 16) N-major.
+constexpr uint32_t IDESC_QK = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24), IDESC_PV = IDESC_QK | (1u << 16);
+
+// D[tmem] (+)= A[tmem] . B[smem desc], issued by one thread.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+        "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]),
+        "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]),
+        "=f"(r[30]), "=f"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(CW * 32) : "memory"); }
+// The two warps that hold the halves of the same 32 rows.
+__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory"); }
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)), "l"(*reinterpret_cast<const uint64_t*>(&c)));
+  return *reinterpret_cast<const float2*>(&d);
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// The panels of a stage: lanes are 32 / NP keys x NP panels of 64 dimensions (two blocks), the warps share key groups and
+// the two blocks of a panel.
+template <int D, bool Q8>
+struct Unpack {
+  using F = RowFmt<D, Q8>;
+  static constexpr int NP = D / 64, KPW = 32 / NP, GROUPS = SK / KPW;
+  // Scales of the key's two blocks in this lane's panel and the key's exponent: the largest of its finite scales'.
+  static __device__ __forceinline__ uint32_t scales(const uint8_t* row, uint32_t (&sc)[2]) {
+    sc[0] = *reinterpret_cast<const uint16_t*>(row);
+    sc[1] = *reinterpret_cast<const uint16_t*>(row + F::BB);
+    uint32_t e = 1;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint32_t x = (sc[i] >> 10) & 31;
+      e = x < 31 ? max(e, x) : e;
+    }
+#pragma unroll
+    for (int x = KPW; x < 32; x *= 2) e = max(e, __shfl_xor_sync(FULL, e, x));
+    return e;
+  }
+  // One block of a key: 32 codes times the scale (normed by the key's exponent), as two f16 terms.
+  template <int PAR>
+  static __device__ __forceinline__ void block(const uint8_t* row, uint32_t scale, uint32_t e, uint8_t* hi, uint8_t* lo, uint32_t key) {
+    const float s = half_bits(scale) * pow2f(22 - (int)e);
+    const uint32_t s2 = pack_half2(s, s);
+    constexpr int CODES = Q8 ? 8 : 4, FIRST = Q8 ? 8 : 4;   // words of codes; the word that holds the second block's scale
+    uint32_t w[CODES];
+    {
+      uint32_t raw[CODES + 1];
+#pragma unroll
+      for (int i = 0; i <= CODES; i++) raw[i] = *reinterpret_cast<const uint32_t*>(row + 4 * (i + PAR * FIRST));
+#pragma unroll
+      for (int i = 0; i < CODES; i++) w[i] = PAR ? raw[i + 1] : __byte_perm(raw[i], raw[i + 1], 0x5432);
+    }
+    auto store = [&](int c, const uint32_t (&u)[4]) {   // eight dimensions
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        h[i] = h2_mul(u[i], s2);
+        l[i] = h2_fma(u[i], s2, h[i] ^ 0x80008000u);   // exact: what the rounding left
+      }
+      const uint32_t at = key * 128 + (((PAR * 4 + c) ^ (key & 7)) << 4);
+      *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    };
+    if (Q8) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        uint32_t u[4];
+        unpack_q8(w[2 * c], &u[0], &u[1]);
+        unpack_q8(w[2 * c + 1], &u[2], &u[3]);
+        store(c, u);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)   // a byte's low and high nibble: 1024 + n and 1024 + 16 n
+          u[i] = h2_fma((__byte_perm(w[c], 0, 0x4040 + 0x0101 * i) & 0x00F0000Fu) | 0x64006400u, 0x2C003C00u, 0xD480E408u);
+        store(c, u);
+      }
+    }
+  }
+};
 
 template <int D, bool KQ8, bool VQ8>
 __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const AttnParams p, const RowsGrid rg, const __grid_constant__ CUtensorMap tmap_k,
@@ -77,33 +195,42 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   using G = RowsGeom<D, KQ8, VQ8>;
   using KF = RowFmt<D, KQ8>;
   using VF = RowFmt<D, VQ8>;
-  constexpr int NB = G::NB;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t sbase = ptx::smem_u32(smem);
-  auto lds32 = [&](uint32_t at) { return *reinterpret_cast<const uint32_t*>(smem + at); };
-  auto lds16 = [&](uint32_t at) { return (uint32_t)*reinterpret_cast<const uint16_t*>(smem + at); };
-  auto lds_f2 = [&](uint32_t at) { return *reinterpret_cast<const float2*>(smem + at); };
+  constexpr int NP = G::NP;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t sbase = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (sbase - ptx::smem_u32(smem_raw));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const uint32_t raw_full = sbase + G::OFF_BARS, frag_full = raw_full + 16, frag_empty = raw_full + 32;
+  const uint32_t bars = sbase + G::OFF_BARS;
+  const uint32_t kraw_full = bars, kraw_empty = bars + 24, vraw_full = bars + 48, vraw_empty = bars + 64;   // [3], [3], [2], [2]
+  const uint32_t k_ready = bars + 80, k_free = bars + 88, v_ready = bars + 96, v_free = bars + 104, q_ready = bars + 112, done = bars + 120;
+  const uint32_t s_full = bars + 128, p_ready = bars + 144, o_full = bars + 160, o_free = bars + 176, scaled = bars + 192;   // [2] x 4, [SLOTS]
   volatile uint32_t* flags = reinterpret_cast<uint32_t*>(smem + G::OFF_FLAGS);
-  uint2* raw_valid = reinterpret_cast<uint2*>(smem + G::OFF_RVALID);
-  uint2* valid = reinterpret_cast<uint2*>(smem + G::OFF_VALID);       // [2][SUBS]
-  uint2* summary = valid + 2 * SUBS;                                  // [2]
-  uint32_t* odd = reinterpret_cast<uint32_t*>(smem + G::OFF_ODD);     // [2][NB]
-  const bool consumer = warp < RW;
+  uint2* valid = reinterpret_cast<uint2*>(smem + G::OFF_VALID);
+  const bool softmax = warp < CW;
 
   if (tid == 0) {
+    for (int s = 0; s < KRAWS; s++) ptx::mbar_init(kraw_full + 8 * s, 1), ptx::mbar_init(kraw_empty + 8 * s, UW);
     for (int s = 0; s < 2; s++) {
-      ptx::mbar_init(raw_full + 8 * s, 1);
-      ptx::mbar_init(frag_full + 8 * s, PW);
-      ptx::mbar_init(frag_empty + 8 * s, RW);
+      ptx::mbar_init(vraw_full + 8 * s, 1), ptx::mbar_init(vraw_empty + 8 * s, UW);
+      ptx::mbar_init(s_full + 8 * s, 1), ptx::mbar_init(p_ready + 8 * s, CW);
+      ptx::mbar_init(o_full + 8 * s, 1), ptx::mbar_init(o_free + 8 * s, CW);
     }
-    flags[0] = flags[1] = flags[2] = flags[3] = flags[5] = 0;
+    for (int s = 0; s < SLOTS; s++) ptx::mbar_init(scaled + 8 * s, UW);
+    ptx::mbar_init(k_ready, UW), ptx::mbar_init(k_free, 1), ptx::mbar_init(v_ready, UW), ptx::mbar_init(v_free, 1);
+    ptx::mbar_init(q_ready, CW), ptx::mbar_init(done, 1);
+    flags[0] = flags[1] = flags[5] = 0;
     flags[4] = 0xFFFFFFFFu;
     ptx::fence_barrier_init();
   }
+  for (int i = tid; i < SLOTS * 8; i += RTHREADS) *reinterpret_cast<uint32_t*>(smem + G::OFF_VMAX + 4 * i) = 0;
+  if (warp == MMA_WARP) {
+    tmem_alloc(sbase + G::OFF_FLAGS + 8, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = flags[2];
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
 
@@ -117,30 +244,21 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
     *l = i / group;
     return i < rg.rows ? (b * p.L + *l) * p.Hq + hkv * group + (i - *l * group) : NO_ROW;
   };
-  uint32_t my_row[2], lo[2], hi[2];   // rows g and g + 8 of the warp
-  bool bad = false;
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
+  const int quarter = warp & 3, half = (warp >> 2) & 1;   // of a softmax warp: its 32 rows, its half of the keys and dimensions
+  const uint32_t r = quarter * 32 + lane;
+  uint32_t my_row = NO_ROW, lo = 0, hi = 0, all_lo = 0, all_hi = 0xFFFFFFFFu;
+  if (softmax) {
     uint32_t l;
-    my_row[h] = consumer ? row_of(warp * 16 + g + 8 * h, &l) : NO_ROW;
-    lo[h] = hi[h] = 0;
-    if (my_row[h] != NO_ROW) {
+    my_row = row_of(r, &l);
+    if (my_row != NO_ROW) {
       const KeyRange kr = key_range(p, b, l);
-      bad |= kr.bad;
-      lo[h] = kr.lo, hi[h] = kr.hi;
+      if (kr.bad) flags[0] = 1;
+      lo = all_lo = kr.lo, hi = all_hi = kr.hi;
     }
+    const uint32_t first = __reduce_min_sync(FULL, hi > lo ? lo : 0xFFFFFFFFu), last = __reduce_max_sync(FULL, hi > lo ? hi : 0u);
+    all_lo = __reduce_max_sync(FULL, all_lo), all_hi = __reduce_min_sync(FULL, all_hi);   // what all rows of the warp see
+    if (lane == 0 && last > 0) atomicMin(const_cast<uint32_t*>(flags) + 4, first), atomicMax(const_cast<uint32_t*>(flags) + 5, last);
   }
-  if (bad) flags[0] = 1;
-  // What some row of the warp sees, and what all of its rows see.
-  uint32_t w_lo = 0xFFFFFFFFu, w_hi = 0, w_all_lo = 0, w_all_hi = 0xFFFFFFFFu;
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    if (hi[h] > lo[h]) w_lo = min(w_lo, lo[h]), w_hi = max(w_hi, hi[h]);
-    if (my_row[h] != NO_ROW) w_all_lo = max(w_all_lo, lo[h]), w_all_hi = min(w_all_hi, hi[h]);
-  }
-  w_lo = __reduce_min_sync(FULL, w_lo), w_hi = __reduce_max_sync(FULL, w_hi);
-  w_all_lo = __reduce_max_sync(FULL, w_all_lo), w_all_hi = __reduce_min_sync(FULL, w_all_hi);
-  if (lane == 0 && w_hi > 0) atomicMin(const_cast<uint32_t*>(flags) + 4, w_lo), atomicMax(const_cast<uint32_t*>(flags) + 5, w_hi);
   __syncthreads();
   if (flags[0] && tid == 0) atomicExch(p.fault, FAULT_INVALID_ARGUMENT);
   const uint32_t u_hi = flags[5], u_lo = min(flags[4], u_hi);
@@ -151,484 +269,489 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   const uint32_t my_first = (uint32_t)min((uint64_t)whole.end, whole.first + (uint64_t)rank * per);
   const uint32_t tiles = min(whole.end - my_first, per), stages = (tiles + SUBS - 1) / SUBS;
 
-  float acc[NB][4][4];   // [block][8 dimensions][row g: 2, row g + 8: 2]
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
-  uint32_t e_run = 0;
-
-  if (!consumer) {
-    // ================ raw blocks to fragments ================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(UNPACK_REGS));
-    const int ptid = tid - RW * 32, pwarp = warp - RW;
-    const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;
-    const uint32_t kshift = (hkv * KF::BYTES) & 15, vshift = (hkv * VF::BYTES) & 15;
-    // The first of these threads brings the raw stages; the page numbers of the next one are read a stage ahead.
-    uint32_t seg = my_first / ts.per_seg, in_seg = my_first - seg * ts.per_seg;
-    uint32_t next_seg[SUBS], next_in[SUBS];
-    int32_t next_page[SUBS];
-    auto place = [&](uint32_t stage) {
-#pragma unroll
-      for (int s = 0; s < SUBS; s++) {
-        next_seg[s] = seg, next_in[s] = in_seg, next_page[s] = 0;
-        if (p.page_table && stage * SUBS + s < tiles) next_page[s] = __ldg(p.page_table + (uint64_t)b * p.pages_per_request + seg);
-        if (++in_seg >= ts.per_seg) in_seg = 0, seg++;
-      }
-    };
-    auto issue = [&](uint32_t stage) {
-      const uint32_t st = stage % G::RAWS, bar = raw_full + 8 * st, dst = sbase + G::OFF_RAW + st * G::STAGE;
-      uint32_t count[SUBS], bytes = 0;
-      uint64_t row[SUBS];
-#pragma unroll
-      for (int s = 0; s < SUBS; s++) {
-        count[s] = stage * SUBS + s < tiles ? min((uint32_t)TK, ts.seg_len - next_in[s] * TK) : 0;
-        row[s] = row0 + next_in[s] * TK;
-        if (p.page_table) {
-          if (count[s] && (next_page[s] < 0 || (uint32_t)next_page[s] >= p.pool_pages)) {
-            atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
-            count[s] = 0;
-          }
-          row[s] += (uint64_t)(count[s] ? next_page[s] : 0) * p.page_tokens;
-        }
-        raw_valid[st * SUBS + s] = make_uint2((1u << count[s]) - 1, next_seg[s] * ts.seg_len + next_in[s] * TK);
-        if (count[s]) bytes += G::TILE;
-      }
-      ptx::mbar_arrive_expect_tx(bar, bytes);
-      if (p.drop_first && stage == 0) return;
-#pragma unroll
-      for (int s = 0; s < SUBS; s++)
-        if (count[s]) {
-          ptx::tma_load_2d(dst + s * G::TILE, &tmap_k, (int)((hkv * KF::BYTES) / 16 * 2), (int)row[s], bar);
-          ptx::tma_load_2d(dst + s * G::TILE + TK * KF::PITCH, &tmap_v, (int)((hkv * VF::BYTES) / 16 * 2), (int)row[s], bar);
-        }
-    };
-    if (ptid == 0)
-      for (uint32_t s = 0; s < min(stages, (uint32_t)G::RAWS); s++) place(s), issue(s);
-    if (ptid == 0) place(G::RAWS);
-    const uint32_t first_sel = t ? 0x3210u : 0x5432u, first_sel_v = g ? 0x3210u : 0x5432u;
-    for (uint32_t it = 0; it < stages; it++) {
-      const uint32_t buf = it & 1, raw = G::OFF_RAW + (it % G::RAWS) * G::STAGE, frag = G::OFF_FRAG + buf * G::FRAG + lane * 16;
-      bool ok = ptx::mbar_wait_bounded(raw_full + 8 * (it % G::RAWS), (it / G::RAWS) & 1, p.wait_limit);
-      if (it >= 2) ok = ptx::mbar_wait_bounded(frag_empty + 8 * buf, (it / 2 - 1) & 1, p.wait_limit) && ok;
-      if (!ok) flags[1] = 1;
-      // ---- scales
-      constexpr int PER = (NB * SK + PW * 32 - 1) / (PW * 32);
-      uint32_t vsc[PER], top = 0;
-#pragma unroll
-      for (int j = 0; j < PER; j++) {
-        const uint32_t blk = pwarp + PW * j;   // a warp takes the 32 keys of a block
-        vsc[j] = 0;
-        if (blk >= NB) break;
-        const uint32_t at = raw + (lane / TK) * G::TILE;
-        const float ks = half_bits(lds16(at + kshift + (lane % TK) * KF::PITCH + blk * KF::BB));
-        *reinterpret_cast<float*>(smem + G::OFF_KS + ((buf * NB + blk) * SK + lane) * 4) = ks;
-        vsc[j] = lds16(at + TK * KF::PITCH + vshift + (lane % TK) * VF::PITCH + blk * VF::BB);
-        const uint2 v = raw_valid[(it % G::RAWS) * SUBS + lane / TK];
-        const uint32_t key = v.y + lane % TK;
-        if (!((v.x >> (lane % TK)) & 1) || key < u_lo || key >= u_hi) vsc[j] = 0;   // no row sees it
-        const uint32_t not_finite = __ballot_sync(FULL, (vsc[j] & 0x7FFFu) >= 0x7C00u);
-        if ((vsc[j] & 0x7FFFu) >= 0x7C00u) vsc[j] = 0;
-        if (lane == 0) odd[buf * NB + blk] = not_finite;
-        top = max(top, vsc[j] & 0x7FFFu);
-      }
-      top = __reduce_max_sync(FULL, top);
-      if (lane == 0) atomicMax(const_cast<uint32_t*>(flags) + 2, top);
-      unpackers_sync();
-      if (flags[1]) {
-        if (ptid == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED);
-        for (uint32_t s = it; s < min(stages, it + G::RAWS); s++) ptx::mbar_wait_bounded(raw_full + 8 * (s % G::RAWS), (s / G::RAWS) & 1, p.wait_limit);
-        break;
-      }
-      const uint32_t e_new = flags[2] >> 10;   // the largest exponent so far
-      const float vmul = __uint_as_float((127u + 29u - e_new) << 23);
-#pragma unroll
-      for (int j = 0; j < PER; j++) {
-        const uint32_t blk = pwarp + PW * j;
-        if (blk < NB) *reinterpret_cast<float*>(smem + G::OFF_VS + ((buf * NB + blk) * SK + lane) * 4) = half_bits(vsc[j]) * vmul;
-      }
-      if (ptid == 0) {
-        uint32_t any = 0;
-        for (int i = 0; i < NB; i++) any |= odd[buf * NB + i];
-        summary[buf] = make_uint2(e_new, any);
-        for (int s = 0; s < SUBS; s++) valid[buf * SUBS + s] = raw_valid[(it % G::RAWS) * SUBS + s];
-      }
-      // ---- K: the B operand of 8 keys x 32 dimensions
-      for (int n = pwarp; n < NB * (SK / 8); n += PW) {
-        const uint32_t blk = n / (SK / 8), k = n % (SK / 8);
-        const uint32_t row = raw + kshift + (k >> 1) * G::TILE + ((k & 1) * 8 + g) * KF::PITCH + (blk >> 1) * 2 * KF::BB;
-        uint32_t f[4];
-        if (KQ8) {
-          const uint32_t w0 = blk & 1 ? lds32(row + 36 + 4 * t) : __byte_perm(lds32(row + 4 * t), lds32(row + 32), first_sel);
-          unpack_q8(w0, &f[0], &f[1]);
-          unpack_q8(lds32(row + (blk & 1 ? 52 : 16) + 4 * t), &f[2], &f[3]);
-        } else {
-          unpack_q4_subnormal(blk & 1 ? lds32(row + 20 + 4 * t) : __byte_perm(lds32(row + 4 * t), lds32(row + 16), first_sel), f);
-        }
-        *reinterpret_cast<uint4*>(smem + frag + n * 512) = make_uint4(f[0], f[1], f[2], f[3]);
-      }
-      // ---- V: the B operand of 16 keys x 32 dimensions
-      for (int n = pwarp; n < NB * SUBS; n += PW) {
-        const uint32_t blk = n / SUBS, j = n % SUBS;
-        uint32_t f[4][2];
-#pragma unroll
-        for (int kp = 0; kp < 2; kp++) {
-          const uint32_t row = raw + j * G::TILE + TK * KF::PITCH + vshift + (2 * t + 8 * kp) * VF::PITCH;
-          if (VQ8) {
-            uint32_t x[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const uint32_t pos = row + h * VF::PITCH + (blk >> 1) * 2 * VF::BB;
-              x[h] = (blk & 1 ? lds32(pos + 36 + 4 * g) : __byte_perm(lds32(pos + 4 * g), lds32(pos + 32), first_sel_v)) ^ 0x80808080u;
-            }
-            const uint32_t lo2 = __byte_perm(x[0], x[1], 0x5140), hi2 = __byte_perm(x[0], x[1], 0x7362);
-            f[0][kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4140), 0xE480E480u);
-            f[1][kp] = h2_add(__byte_perm(lo2, 0x64646464u, 0x4342), 0xE480E480u);
-            f[2][kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4140), 0xE480E480u);
-            f[3][kp] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4342), 0xE480E480u);
-          } else {
-            const uint32_t pos = row + blk * VF::BB + 2 + 2 * g;
-            uint32_t x = __byte_perm(lds16(pos), lds16(pos + VF::PITCH), 0x5410);
-            f[0][kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
-            f[1][kp] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
-            x >>= 8;
-            f[2][kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
-            f[3][kp] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
-          }
-        }
-        *reinterpret_cast<uint4*>(smem + frag + G::KFRAG + n * 1024) = make_uint4(f[0][0], f[0][1], f[1][0], f[1][1]);
-        *reinterpret_cast<uint4*>(smem + frag + G::KFRAG + n * 1024 + 512) = make_uint4(f[2][0], f[2][1], f[3][0], f[3][1]);
-      }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(frag_full + 8 * buf);
-      unpackers_sync();   // the raw stage has been read
-      if (ptid == 0 && it + G::RAWS < stages) {
-        issue(it + G::RAWS);
-        place(it + G::RAWS + 1);
-      }
+  // A wait that runs out is reported; the warp then walks on without waiting or working, so that every arrival still comes and
+  // no warp is left at a barrier of a pair.
+  bool dead = false;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (!dead && !__all_sync(FULL, ptx::mbar_wait_bounded(bar, parity & 1, p.wait_limit))) {
+      dead = true;
+      if (lane == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED), flags[1] = 1;
     }
-  } else {
-  // ================ consumers ================
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CONSUMER_REGS));
-  // ---- q as the A operand: rows g and g + 8, two terms, normed by the row's largest value to [2^13, 2^14)
-  const uint32_t qf = G::OFF_QF + warp * ((D / 16) * 1024) + lane * 16;
-  float factor[2];
-  {
-    float up[2] = {0.0f, 0.0f};
-#pragma unroll 1
-    for (int r = 0; r < 16; r++) {
-      uint32_t l;
-      const uint32_t row = row_of(warp * 16 + r, &l);
-      float top = 0.0f;
-      if (row != NO_ROW)
+  };
+  auto arrive = [&](uint32_t bar) {
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar);
+  };
+
+  if (softmax) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
+    float factor;
+    // ---- q into tensor memory: rows whole through shared memory, then normed by their largest value to [2^13, 2^14) and split
+    {
+      float* stage = reinterpret_cast<float*>(smem + G::OFF_K);
+      float* tops = reinterpret_cast<float*>(smem + G::OFF_STATS);
+#pragma unroll 4
+      for (int i = 0; i < ROWS / CW; i++) {
+        const uint32_t row_in = warp * (ROWS / CW) + i;
+        uint32_t l;
+        const uint32_t row = row_of(row_in, &l);
+        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) {
-          const uint64_t at = (uint64_t)row * D + lane + 32 * i;
-          top = fmaxf(top, fabsf(p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at] : __half2float(static_cast<const __half*>(p.q)[at])));
+        for (int j = 0; j < D / 32; j++) {
+          const uint32_t d = lane + 32 * j;
+          float x = 0.0f;
+          if (row != NO_ROW) {
+            const uint64_t at = (uint64_t)row * D + d;
+            x = p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at] : __half2float(static_cast<const __half*>(p.q)[at]);
+          }
+          top = fmaxf(top, fabsf(x));
+          stage[row_in * D + ((((d >> 2) ^ (row_in & 7)) << 2) | (d & 3))] = x;
         }
-      uint32_t e = __reduce_max_sync(FULL, __float_as_uint(top)) >> 23;
+        const uint32_t t = __reduce_max_sync(FULL, __float_as_uint(top));
+        if (lane == 0) tops[row_in] = __uint_as_float(t);
+      }
+      softmax_sync();
+      uint32_t e = __float_as_uint(tops[r]) >> 23;
       if (e == 255) e = 127;
       e = max(e, 40u);
-      if ((r & 7) == g) {
-        const float to_base2 = p.soft_cap > 0.0f ? 1.0f : LOG2E;
-        (r < 8 ? up[0] : up[1]) = __uint_as_float((127u + 13u + 127u - e) << 23);
-        (r < 8 ? factor[0] : factor[1]) = p.scale * __uint_as_float((e - 13u) << 23) * to_base2;
-      }
-    }
+      const float up = __uint_as_float((127u + 13u + 127u - e) << 23);
+      factor = p.scale * __uint_as_float((e - 13u) << 23) * (p.soft_cap > 0.0f ? 1.0f : LOG2E);
+      const uint32_t tq = tmem + ((uint32_t)quarter << 21) + G::T_Q + half * (D / 4);
 #pragma unroll 1
-    for (int blk = 0; blk < NB; blk++) {
-      float part[2] = {0.0f, 0.0f};
+      for (int c = 0; c < D / 64; c++) {   // 32 dimensions
+        uint32_t h[16], l[16];
 #pragma unroll
-      for (int m = 0; m < 2; m++) {
-        uint32_t h4[4], l4[4];
+        for (int i = 0; i < 8; i++) {
+          const uint32_t chunk = half * (D / 8) + c * 8 + i;
+          const float4 x = *reinterpret_cast<const float4*>(stage + r * D + ((chunk ^ (r & 7)) << 2));
+          split2(x.x * up, x.y * up, &h[2 * i], &l[2 * i]);
+          split2(x.z * up, x.w * up, &h[2 * i + 1], &l[2 * i + 1]);
+        }
+        tmem_st16(tq + c * 16, h);
+        tmem_st16(tq + D / 2 + c * 16, l);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      arrive(q_ready);
+    }
+    float acc[NP][32];
 #pragma unroll
-        for (int r = 0; r < 2; r++)
+    for (int q = 0; q < NP; q++)
 #pragma unroll
-          for (int half = 0; half < 2; half++) {   // operand order: (row g, r 0), (row g + 8, r 0), (row g, r 1), (row g + 8, r 1)
-            float x[2];
+      for (int i = 0; i < 32; i++) acc[q][i] = 0.0f;
+    float m_run = -INFINITY, l_run = 0.0f, a_cur = 1.0f, a_next = 1.0f;
+    uint32_t e_run = 0;
+    float* ex = reinterpret_cast<float*>(smem + G::OFF_EX);
+    const uint32_t lane_base = tmem + ((uint32_t)quarter << 21) + half * 32;
+
+    for (uint32_t step = 0; step <= stages; step++) {
+      if (step < stages) {
+        // ---- P of stage `step`
+        const uint32_t it = step, slot = it % SLOTS;
+        wait(scaled + 8 * slot, it / SLOTS);
+        wait(s_full + 8 * (it & 1), it >> 1);
+        tc_fence_after();
+        float s[32];
+        const uint32_t at = lane_base + G::T_S + (it & 1) * 64;
+        tmem_ld32f(at, s);
+        const uint4 v0 = *reinterpret_cast<const uint4*>(smem + G::OFF_VMAX + slot * 32), v1 = *reinterpret_cast<const uint4*>(smem + G::OFF_VMAX + slot * 32 + 16);
+        const uint32_t met = max(max(v0.x & 31, v0.y & 31), max(max(v0.z & 31, v0.w & 31), max(v1.x & 31, v1.y & 31)));
+        const uint32_t e_new = max(e_run, met);
+        uint32_t any_odd = (v0.x | v0.y | v0.z | v0.w | v1.x | v1.y) & 256;
+        bool partial = false;
+        uint32_t there[2], key0[2];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const int dim = KQ8 ? pair_byte(true, blk & 1, t + 4 * m, 2 * r + h) : 2 * pair_byte(false, blk & 1, t, m + 2 * h) + r;
-              x[h] = 0.0f;
-              if (my_row[half] != NO_ROW) {
-                const uint64_t at = (uint64_t)my_row[half] * D + blk * QK + dim;
-                x[h] = p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at] : __half2float(static_cast<const __half*>(p.q)[at]);
+        for (int j = 0; j < 2; j++) {
+          const uint2 v = valid[slot * SUBS + 2 * half + j];
+          there[j] = v.x, key0[j] = v.y;
+          partial |= v.x != 0xFFFFu || v.y < all_lo || v.y + TK > all_hi;
+        }
+        const float4* kexp = reinterpret_cast<const float4*>(smem + G::OFF_KEXP + (slot * SK + half * 32) * 4);
+        const float4* vexp = reinterpret_cast<const float4*>(smem + G::OFF_VEXP + (slot * SK + half * 32) * 4);
+        tmem_ld_wait();
+        float unit = factor;
+        if (p.soft_cap > 0.0f) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float4 k = kexp[i];
+            float x[4] = {s[4 * i] * k.x * factor, s[4 * i + 1] * k.y * factor, s[4 * i + 2] * k.z * factor, s[4 * i + 3] * k.w * factor};
+            cap_logits(x, p.soft_cap, 1.0f / p.soft_cap);
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[4 * i + j] = x[j] * LOG2E;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float4 k = kexp[i];
+            const float2 a = mul2(mul2(make_float2(s[4 * i], s[4 * i + 1]), make_float2(k.x, k.y)), make_float2(unit, unit));
+            const float2 c = mul2(mul2(make_float2(s[4 * i + 2], s[4 * i + 3]), make_float2(k.z, k.w)), make_float2(unit, unit));
+            s[4 * i] = a.x, s[4 * i + 1] = a.y, s[4 * i + 2] = c.x, s[4 * i + 3] = c.y;
+          }
+        }
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            const uint32_t key = key0[i >> 4] + (i & 15);
+            if (!((there[i >> 4] >> (i & 15)) & 1) || key < lo || key >= hi) s[i] = -INFINITY;
+          }
+        }
+        float top[4] = {m_run, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], s[i]);
+        const float mine = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        float* mx = ex + (it & 1) * 2 * ROWS;
+        uint32_t* both = reinterpret_cast<uint32_t*>(smem + G::OFF_PAIR) + (it & 1) * 8 + quarter;
+        mx[half * ROWS + r] = mine;
+        if (lane == 0) both[4 * half] = any_odd;
+        pair_sync(quarter);
+        any_odd = both[0] | both[4];   // (the two warps go the same way, even when one of them has given up waiting)
+        const float m_new = fmaxf(mine, mx[(half ^ 1) * ROWS + r]);
+        float a = m_new > m_run ? ex2(m_run - m_new) : 1.0f;
+        l_run *= a;
+        a_next = a * pow2f((int)e_run - (int)e_new);
+        m_run = m_new, e_run = e_new;
+        // P times the key's V power, over 2^e_run: at most 2^14
+        const float off = 30.0f - (float)e_run - (m_run == -INFINITY ? 0.0f : m_run);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          float2 x = make_float2(s[2 * i], s[2 * i + 1]);
+          add2(x.x, x.y, off, off);
+          x.x = ex2(x.x), x.y = ex2(x.y);
+          add2(sum[i & 1].x, sum[i & 1].y, x.x, x.y);
+          s[2 * i] = x.x, s[2 * i + 1] = x.y;
+        }
+        l_run = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), pow2f((int)e_run - 30), l_run);
+        if (any_odd) {   // a V scale that is not finite: NaN where a row gives weight to its key
+          const uint8_t* odd = smem + G::OFF_ODD + slot * SK + half * 32;
+          uint32_t hit = 0;
+#pragma unroll
+          for (int i = 0; i < 32; i++) hit |= s[i] > 0.0f ? odd[i] : 0u;
+          pair_sync(quarter);   // (the maxima have been read)
+          mx[half * ROWS + r] = __uint_as_float(hit);
+          pair_sync(quarter);
+          hit |= __float_as_uint(mx[(half ^ 1) * ROWS + r]);
+          pair_sync(quarter);
+#pragma unroll
+          for (int q = 0; q < NP; q++)
+            if ((hit >> (2 * q + half)) & 1)
+#pragma unroll
+              for (int i = 0; i < 32; i++) acc[q][i] = NAN;
+        }
+        uint32_t h[16], l[16];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float4 v = vexp[i];
+          const float2 w0 = mul2(make_float2(s[4 * i], s[4 * i + 1]), make_float2(v.x, v.y)), w1 = mul2(make_float2(s[4 * i + 2], s[4 * i + 3]), make_float2(v.z, v.w));
+          split2(w0.x, w0.y, &h[2 * i], &l[2 * i]);
+          split2(w1.x, w1.y, &h[2 * i + 1], &l[2 * i + 1]);
+        }
+        tmem_st16(at, h);
+        tmem_st16(at + 16, l);
+        tmem_st_wait();
+        tc_fence_before();
+        arrive(p_ready + 8 * (it & 1));
+      }
+      if (step > 0) {
+        // ---- O of the stage before
+#pragma unroll
+        for (int q = 0; q < NP; q++) {
+          const uint32_t n = (step - 1) * NP + q;
+          wait(o_full + 8 * (n & 1), n >> 1);
+          tc_fence_after();
+          float o[32];
+          tmem_ld32f(lane_base + G::T_O + (n & 1) * 64, o);
+          tmem_ld_wait();
+          tc_fence_before();
+          arrive(o_free + 8 * (n & 1));
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float2 x = fma2(make_float2(acc[q][2 * i], acc[q][2 * i + 1]), make_float2(a_cur, a_cur), make_float2(o[2 * i], o[2 * i + 1]));
+            acc[q][2 * i] = x.x, acc[q][2 * i + 1] = x.y;
+          }
+        }
+      }
+      a_cur = a_next;
+    }
+
+    // ---- the rows' sums: straight out, or through shared memory to the cluster's others
+    pair_sync(quarter);
+    ex[half * ROWS + r] = l_run;
+    pair_sync(quarter);
+    l_run += ex[(half ^ 1) * ROWS + r];
+    const bool report = !flags[0] && !flags[1];
+    const bool good = l_run > 0.0f && isfinite(l_run);
+    const float back = pow2f((int)e_run - 36);
+    if (rg.cluster == 1) {
+      if (my_row != NO_ROW) {
+        if (!good && hi > lo && half == 0 && report) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
+        const float mul = good ? back * __frcp_rn(l_run) : 0.0f;
+        float* dst = p.out + (uint64_t)my_row * D + half * 32;
+#pragma unroll
+        for (int q = 0; q < NP; q++)
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            *reinterpret_cast<float4*>(dst + q * 64 + 4 * i) = good ? make_float4(acc[q][4 * i] * mul, acc[q][4 * i + 1] * mul, acc[q][4 * i + 2] * mul, acc[q][4 * i + 3] * mul)
+                                                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+    } else {
+      float* res = reinterpret_cast<float*>(smem + G::OFF_K);   // (the last product has been read, so the panels are free)
+      float* stats = reinterpret_cast<float*>(smem + G::OFF_STATS);
+      softmax_sync();
+      if (half == 0) stats[r] = m_run, stats[ROWS + r] = l_run;
+#pragma unroll
+      for (int q = 0; q < NP; q++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const uint32_t chunk = q * 16 + half * 8 + i;
+          *reinterpret_cast<float4*>(res + r * D + ((chunk ^ (r & 7)) << 2)) = make_float4(acc[q][4 * i] * back, acc[q][4 * i + 1] * back, acc[q][4 * i + 2] * back, acc[q][4 * i + 3] * back);
+        }
+      cluster_sync();
+      const uint32_t share = ROWS / rg.cluster, res_addr = sbase + G::OFF_K, stats_addr = sbase + G::OFF_STATS;
+      for (uint32_t i = tid; i < share * (D / 4); i += CW * 32) {
+        const uint32_t rr = rank * share + i / (D / 4), d4 = i % (D / 4);
+        uint32_t l;
+        const uint32_t row = row_of(rr, &l);
+        if (row == NO_ROW) continue;
+        float m[8], w[8], M = -INFINITY, lsum = 0.0f;
+        float4 v[8], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          m[k] = -INFINITY, w[k] = 0.0f, v[k] = o;
+          if (k < (int)rg.cluster) {
+            const uint32_t a = cluster_addr(stats_addr, k);
+            m[k] = ld_cluster_f(a + 4 * rr), w[k] = ld_cluster_f(a + 4 * (ROWS + rr));
+            v[k] = ld_cluster_f4(cluster_addr(res_addr, k) + (rr * D + ((d4 ^ (rr & 7)) << 2)) * 4);
+          }
+          M = fmaxf(M, m[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const float f = m[k] == -INFINITY ? 0.0f : ex2(m[k] - M);
+          o.x += v[k].x * f, o.y += v[k].y * f, o.z += v[k].z * f, o.w += v[k].w * f;
+          lsum += w[k] * f;
+        }
+        const bool fine = lsum > 0.0f && isfinite(lsum);
+        if (!fine && d4 == 0 && report) {
+          const KeyRange kr = key_range(p, b, l);
+          if (kr.hi > kr.lo) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
+        }
+        const float inv = fine ? __frcp_rn(lsum) : 0.0f;
+        *reinterpret_cast<float4*>(p.out + (uint64_t)row * D + 4 * d4) = fine ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      __syncwarp();
+      cluster_sync();   // no CTA leaves before the others have read its sums
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    if (warp == MMA_WARP) {
+      // ================ the products ================
+      wait(q_ready, 0);
+      auto logits = [&](uint32_t it) {
+        wait(k_ready, it);
+        tc_fence_after();
+        if (!dead && lane == 0) {
+          const uint64_t kh = smem_desc_sw128(sbase + G::OFF_K), kl = smem_desc_sw128(sbase + G::OFF_K + NP * PANEL);
+          const uint32_t d = tmem + G::T_S + (it & 1) * 64, qh = tmem + G::T_Q, ql = qh + D / 2;
+#pragma unroll 1
+          for (int j = 0; j < 3; j++) {
+            const uint32_t a = j == 0 ? ql : qh;
+            const uint64_t bd = j == 1 ? kl : kh;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ks++) umma_f16_ts(d, a + 8 * ks, bd + (ks >> 2) * (PANEL >> 4) + (ks & 3) * 2, IDESC_QK, j > 0 || ks > 0);
+          }
+          umma_commit(s_full + 8 * (it & 1));
+          umma_commit(k_free);
+        }
+        __syncwarp();
+      };
+      if (stages > 0) logits(0);
+      for (uint32_t it = 0; it < stages; it++) {
+        if (it + 1 < stages) logits(it + 1);
+        wait(v_ready, it);
+        wait(p_ready + 8 * (it & 1), it >> 1);
+        for (int q = 0; q < NP; q++) {
+          const uint32_t n = it * NP + q;
+          if (n >= 2) wait(o_free + 8 * (n & 1), (n >> 1) - 1);
+          tc_fence_after();
+          if (!dead && lane == 0) {
+            const uint64_t vh = smem_desc_sw128(sbase + G::OFF_V + q * PANEL), vl = vh + NP * (PANEL >> 4);
+            const uint32_t d = tmem + G::T_O + (n & 1) * 64, ph = tmem + G::T_S + (it & 1) * 64;
+#pragma unroll
+            for (int j = 0; j < 3; j++)
+#pragma unroll
+              for (int ks = 0; ks < SK / 16; ks++)   // 16 keys: eight columns of P, two groups of eight rows of V
+                umma_f16_ts(d, ph + (ks >> 1) * 32 + (ks & 1) * 8 + (j == 0 ? 16 : 0), (j == 1 ? vl : vh) + ks * (2048 >> 4), IDESC_PV, j > 0 || ks > 0);
+            umma_commit(o_full + 8 * (n & 1));
+            if (q == NP - 1) umma_commit(v_free);
+          }
+          __syncwarp();
+        }
+      }
+      if (lane == 0) umma_commit(done);
+      ptx::mbar_wait_bounded(done, 0, p.wait_limit);
+    } else if (warp == LOAD_WARP) {
+      // ================ raw stages ================
+      if (lane == 0) {
+        const uint64_t row0 = p.page_table ? 0 : (uint64_t)b * p.T;
+        uint32_t seg = my_first / ts.per_seg, in_seg = my_first - seg * ts.per_seg;
+        int32_t page = 0;
+        auto lookup = [&](uint32_t s, uint32_t tile) {   // the page of the next tile, read a tile ahead
+          page = p.page_table && tile < tiles ? __ldg(p.page_table + (uint64_t)b * p.pages_per_request + s) : 0;
+        };
+        lookup(seg, 0);
+        // A slot is armed again only when it has been read AND its own bytes have come: warps that gave up waiting for them
+        // arrive all the same, and a second arrival in a phase that still waits for bytes is an error of the barrier.
+        auto reusable = [&](uint32_t full, uint32_t empty, uint32_t use) {
+          return use == 0 || (ptx::mbar_wait_bounded(empty, (use - 1) & 1, p.wait_limit) && ptx::mbar_wait_bounded(full, (use - 1) & 1, p.wait_limit));
+        };
+        bool gone = false;
+        uint32_t k_issued = 0, v_issued = 0;
+        for (uint32_t it = 0; it < stages && !gone; it++) {
+          uint32_t count[SUBS], key[SUBS], bytes_k = 0, bytes_v = 0;
+          uint64_t row[SUBS];
+#pragma unroll
+          for (int s = 0; s < SUBS; s++) {
+            const uint32_t tile = it * SUBS + s;
+            count[s] = tile < tiles ? min((uint32_t)TK, ts.seg_len - in_seg * TK) : 0;
+            row[s] = row0 + in_seg * TK;
+            key[s] = seg * ts.seg_len + in_seg * TK;
+            if (p.page_table) {
+              if (count[s] && (page < 0 || (uint32_t)page >= p.pool_pages)) {
+                atomicExch(p.fault, FAULT_INVALID_ARGUMENT);   // a page outside the pool: its keys are left out
+                count[s] = 0;
               }
-              x[h] = x[h] * up[half] * (!KQ8 && r ? 0.0625f : 1.0f);
+              row[s] += (uint64_t)(count[s] ? page : 0) * p.page_tokens;
             }
-            split2(x[0], x[1], &h4[2 * r + half], &l4[2 * r + half]);
-            if (!KQ8) {
-              const float2 a = __half22float2(*reinterpret_cast<__half2*>(&h4[2 * r + half])), c = __half22float2(*reinterpret_cast<__half2*>(&l4[2 * r + half]));
-              part[half] += ((a.x + c.x) + (a.y + c.y)) * (r ? 16.0f : 1.0f);
+            if (++in_seg >= ts.per_seg) in_seg = 0, seg++, lookup(seg, tile + 1);
+            if (count[s]) bytes_k += TK * KF::PITCH, bytes_v += TK * VF::PITCH;
+          }
+          const uint32_t ks = it % KRAWS, vs = it % VRAWS, kbar = kraw_full + 8 * ks, vbar = vraw_full + 8 * vs;
+          gone = !reusable(kbar, kraw_empty + 8 * ks, it / KRAWS);
+          if (gone) break;
+          ptx::mbar_arrive_expect_tx(kbar, bytes_k);
+          const bool drop = p.drop_first && it == 0;
+          if (!drop)
+#pragma unroll
+            for (int s = 0; s < SUBS; s++)
+              if (count[s]) ptx::tma_load_2d(sbase + G::OFF_KRAW + ks * G::KRAW + s * (TK * KF::PITCH), &tmap_k, (int)((hkv * KF::BYTES) / 16 * 2), (int)row[s], kbar);
+          gone = !reusable(vbar, vraw_empty + 8 * vs, it / VRAWS);
+          k_issued = it + 1;
+          if (gone) break;
+#pragma unroll
+          for (int s = 0; s < SUBS; s++) valid[(it % SLOTS) * SUBS + s] = make_uint2((1u << count[s]) - 1, key[s]);
+          ptx::mbar_arrive_expect_tx(vbar, bytes_v);
+          v_issued = it + 1;
+          if (!drop)
+#pragma unroll
+            for (int s = 0; s < SUBS; s++)
+              if (count[s]) ptx::tma_load_2d(sbase + G::OFF_VRAW + vs * G::VRAW + s * (TK * VF::PITCH), &tmap_v, (int)((hkv * VF::BYTES) / 16 * 2), (int)row[s], vbar);
+        }
+        if (gone) atomicExch(p.fault, FAULT_WAIT_EXPIRED), flags[1] = 1;
+        // No copy is in flight when the block ends.
+        for (uint32_t it = k_issued > KRAWS ? k_issued - KRAWS : 0; it < k_issued; it++) ptx::mbar_wait_bounded(kraw_full + 8 * (it % KRAWS), (it / KRAWS) & 1, p.wait_limit);
+        for (uint32_t it = v_issued > VRAWS ? v_issued - VRAWS : 0; it < v_issued; it++) ptx::mbar_wait_bounded(vraw_full + 8 * (it % VRAWS), (it / VRAWS) & 1, p.wait_limit);
+      }
+      __syncwarp();
+    } else {
+      // ================ raw blocks to operands ================
+      const uint32_t uw = warp - FIRST_UNPACK;
+      const uint32_t kshift = (hkv * KF::BYTES) & 15, vshift = (hkv * VF::BYTES) & 15;
+      using UK = Unpack<D, KQ8>;
+      using UV = Unpack<D, VQ8>;
+      constexpr int KPW = UK::KPW, GROUPS = UK::GROUPS;
+      const uint32_t in_group = lane % KPW, panel = lane / KPW;
+      wait(q_ready, 0);   // (q passed through the panels)
+      auto keys = [&](uint32_t it) {
+        wait(kraw_full + 8 * (it % KRAWS), it / KRAWS);
+        if (it > 0) wait(k_free, it - 1);
+        if (!dead) {
+          const uint8_t* raw = smem + G::OFF_KRAW + (it % KRAWS) * G::KRAW + kshift + panel * 2 * KF::BB;
+          uint8_t* kh = smem + G::OFF_K + panel * PANEL;
+          for (uint32_t u = uw; u < 2 * GROUPS; u += UW) {
+            const uint32_t key = (u >> 1) * KPW + in_group;
+            const uint8_t* row = raw + key * KF::PITCH;
+            uint32_t sc[2];
+            const uint32_t e = UK::scales(row, sc);
+            if (u & 1) {
+              UK::template block<1>(row, sc[1], e, kh, kh + NP * PANEL, key);
+            } else {
+              UK::template block<0>(row, sc[0], e, kh, kh + NP * PANEL, key);
+              if (panel == 0) *reinterpret_cast<float*>(smem + G::OFF_KEXP + ((it % SLOTS) * SK + key) * 4) = pow2f((int)e - 22);
             }
           }
-        *reinterpret_cast<uint4*>(smem + qf + (2 * blk + m) * 1024) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
-        *reinterpret_cast<uint4*>(smem + qf + (2 * blk + m) * 1024 + 512) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
-      }
-      if (!KQ8) {
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-          part[half] += __shfl_xor_sync(FULL, part[half], 1);
-          part[half] += __shfl_xor_sync(FULL, part[half], 2);
-          if (t == 0) *reinterpret_cast<float*>(smem + G::OFF_CI + ((warp * NB + blk) * 16 + g + 8 * half) * 4) = part[half] * (-8.0f * 5.9604644775390625e-8f);
+          ptx::fence_proxy_async();
         }
+        arrive(k_ready);
+        arrive(kraw_empty + 8 * (it % KRAWS));
+      };
+      // Is the key there, and does a row of the block see it?
+      auto seen = [&](uint32_t it, uint32_t key) {
+        const uint2 v = valid[(it % SLOTS) * SUBS + key / TK];
+        const uint32_t at = v.y + key % TK;
+        return ((v.x >> (key % TK)) & 1) && at >= u_lo && at < u_hi;
+      };
+      auto exponents = [&](uint32_t it) {
+        wait(vraw_full + 8 * (it % VRAWS), it / VRAWS);
+        if (!dead) {
+          const uint8_t* raw = smem + G::OFF_VRAW + (it % VRAWS) * G::VRAW + vshift + panel * 2 * VF::BB;
+          uint32_t top = 0, any = 0;
+          for (uint32_t u = uw; u < GROUPS; u += UW) {
+            const uint32_t key = u * KPW + in_group;
+            uint32_t sc[2];
+            const uint32_t e = UV::scales(raw + key * VF::PITCH, sc);
+            const bool on = seen(it, key);
+            uint32_t odd = 0;
+            if (on) odd = ((sc[0] & 0x7C00u) == 0x7C00u ? 1u : 0u) << (2 * panel) | ((sc[1] & 0x7C00u) == 0x7C00u ? 2u : 0u) << (2 * panel);
+#pragma unroll
+            for (int x = KPW; x < 32; x *= 2) odd |= __shfl_xor_sync(FULL, odd, x);
+            if (panel == 0) {
+              *reinterpret_cast<float*>(smem + G::OFF_VEXP + ((it % SLOTS) * SK + key) * 4) = pow2f((int)e - 16);
+              smem[G::OFF_ODD + (it % SLOTS) * SK + key] = (uint8_t)odd;
+            }
+            top = max(top, on ? e : 0u);
+            any |= odd;
+          }
+          top = __reduce_max_sync(FULL, top) | (__any_sync(FULL, any != 0) ? 256u : 0u);
+          if (lane == 0) *reinterpret_cast<uint32_t*>(smem + G::OFF_VMAX + ((it % SLOTS) * 8 + uw) * 4) = top;
+        }
+        arrive(scaled + 8 * (it % SLOTS));
+      };
+      auto values = [&](uint32_t it) {
+        if (it > 0) wait(v_free, it - 1);
+        if (!dead) {
+          const uint8_t* raw = smem + G::OFF_VRAW + (it % VRAWS) * G::VRAW + vshift + panel * 2 * VF::BB;
+          uint8_t* vh = smem + G::OFF_V + panel * PANEL;
+          for (uint32_t u = uw; u < 2 * GROUPS; u += UW) {
+            const uint32_t key = (u >> 1) * KPW + in_group;
+            const uint8_t* row = raw + key * VF::PITCH;
+            uint32_t sc[2];
+            const uint32_t e = UV::scales(row, sc);
+            uint32_t mine = u & 1 ? sc[1] : sc[0];
+            if (!seen(it, key) || (mine & 0x7C00u) == 0x7C00u) mine = 0;
+            if (u & 1) UV::template block<1>(row, mine, e, vh, vh + NP * PANEL, key);
+            else UV::template block<0>(row, mine, e, vh, vh + NP * PANEL, key);
+          }
+          ptx::fence_proxy_async();
+        }
+        arrive(v_ready);
+        arrive(vraw_empty + 8 * (it % VRAWS));
+      };
+      if (stages > 0) keys(0), exponents(0), values(0);
+      for (uint32_t it = 1; it < stages; it++) {
+        keys(it), exponents(it);
+        if (it > 1) values(it - 1);
       }
+      if (stages > 1) values(stages - 1);
+    }
+    if (rg.cluster > 1) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
     }
   }
-  __syncwarp();
-
-#pragma unroll
-  for (int i = 0; i < NB; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) acc[i][j][e] = 0.0f;
-
-  for (uint32_t it = 0; it < stages; it++) {
-    const uint32_t buf = it & 1, frag = G::OFF_FRAG + buf * G::FRAG + lane * 16;
-    if (!__all_sync(FULL, ptx::mbar_wait_bounded(frag_full + 8 * buf, (it >> 1) & 1, p.wait_limit))) {
-      if (lane == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED), flags[1] = 1;
-      break;
-    }
-    const uint32_t e_new = summary[buf].x, any_odd = summary[buf].y;
-    // Does some row of this warp see a key of the stage, and do all of them see all?
-    bool some = false, partial = false;
-    uint32_t key0[SUBS], there[SUBS];
-#pragma unroll
-    for (int s = 0; s < SUBS; s++) {
-      const uint2 v = valid[buf * SUBS + s];
-      there[s] = v.x, key0[s] = v.y;
-      some |= v.x && v.y < w_hi && v.y + TK > w_lo;
-      partial |= v.x != 0xFFFFu || v.y < w_all_lo || v.y + TK > w_all_hi;
-    }
-    if (some) {
-
-    // ---- S: rows g and g + 8, keys 8n + 2t and 8n + 2t + 1
-    float s[SK / 8][4];
-#pragma unroll
-    for (int n = 0; n < SK / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-    for (int blk = 0; blk < NB; blk++) {
-      uint4 qh[2], ql[2];
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-        qh[m] = *reinterpret_cast<const uint4*>(smem + qf + (2 * blk + m) * 1024);
-        ql[m] = *reinterpret_cast<const uint4*>(smem + qf + (2 * blk + m) * 1024 + 512);
-      }
-      float ci[2] = {0.0f, 0.0f};
-      if (!KQ8)
-#pragma unroll
-        for (int half = 0; half < 2; half++) ci[half] = *reinterpret_cast<const float*>(smem + G::OFF_CI + ((warp * NB + blk) * 16 + g + 8 * half) * 4);
-      // (Step by step over all keys: neighbouring MMAs are independent.)
-      uint4 f[SK / 8];
-      float c[SK / 8][4];
-#pragma unroll
-      for (int n = 0; n < SK / 8; n++) {
-        f[n] = *reinterpret_cast<const uint4*>(smem + frag + (blk * (SK / 8) + n) * 512);
-        mma_f16_from(c[n], ql[0].x, ql[0].y, ql[0].z, ql[0].w, f[n].x, f[n].y, ci[0], ci[0], ci[1], ci[1]);
-      }
-#pragma unroll
-      for (int n = 0; n < SK / 8; n++) mma_f16_from(c[n], ql[1].x, ql[1].y, ql[1].z, ql[1].w, f[n].z, f[n].w, c[n][0], c[n][1], c[n][2], c[n][3]);
-#pragma unroll
-      for (int n = 0; n < SK / 8; n++) mma_f16_from(c[n], qh[0].x, qh[0].y, qh[0].z, qh[0].w, f[n].x, f[n].y, c[n][0], c[n][1], c[n][2], c[n][3]);
-#pragma unroll
-      for (int n = 0; n < SK / 8; n++) mma_f16_from(c[n], qh[1].x, qh[1].y, qh[1].z, qh[1].w, f[n].z, f[n].w, c[n][0], c[n][1], c[n][2], c[n][3]);
-#pragma unroll
-      for (int n = 0; n < SK / 8; n++) {
-        const float2 sc = lds_f2(G::OFF_KS + ((buf * NB + blk) * SK + 8 * n + 2 * t) * 4);
-        s[n][0] = fmaf(sc.x, c[n][0], s[n][0]);
-        s[n][1] = fmaf(sc.y, c[n][1], s[n][1]);
-        s[n][2] = fmaf(sc.x, c[n][2], s[n][2]);
-        s[n][3] = fmaf(sc.y, c[n][3], s[n][3]);
-      }
-    }
-    // ---- softmax
-    float m_new[2] = {m_run[0], m_run[1]}, unit[2] = {factor[0], factor[1]};
-    if (!KQ8) {   // the codes' 2^24
-#pragma unroll
-      for (int n = 0; n < SK / 8; n++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[n][e] *= 16777216.0f;
-    }
-    if (p.soft_cap > 0.0f) {
-#pragma unroll
-      for (int n = 0; n < SK / 8; n++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[n][e] *= factor[e >> 1];
-        cap_logits(s[n], p.soft_cap, 1.0f / p.soft_cap);
-      }
-      unit[0] = unit[1] = LOG2E;
-    }
-#pragma unroll
-    for (int n = 0; n < SK / 8; n++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float y = s[n][e] * unit[e >> 1];
-        if (partial) {
-          const uint32_t k = (n & 1) * 8 + 2 * t + (e & 1), key = key0[n >> 1] + k;
-          if (!((there[n >> 1] >> k) & 1) || key < lo[e >> 1] || key >= hi[e >> 1]) y = -INFINITY;
-        }
-        s[n][e] = y;
-        m_new[e >> 1] = fmaxf(m_new[e >> 1], y);
-      }
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      m_new[h] = fmaxf(m_new[h], __shfl_xor_sync(FULL, m_new[h], 1));
-      m_new[h] = fmaxf(m_new[h], __shfl_xor_sync(FULL, m_new[h], 2));
-    }
-    if (__any_sync(FULL, m_new[0] > m_run[0] || m_new[1] > m_run[1] || e_new > e_run)) {
-      const float down = __uint_as_float((127u + e_run - e_new) << 23);
-      float a[2];
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        a[h] = m_new[h] > m_run[h] ? ex2(m_run[h] - m_new[h]) : 1.0f;
-        l_run[h] *= a[h];
-        a[h] *= down;
-        m_run[h] = m_new[h];
-      }
-      e_run = e_new;
-#pragma unroll
-      for (int i = 0; i < NB; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j][0] *= a[0], acc[i][j][1] *= a[0], acc[i][j][2] *= a[1], acc[i][j][3] *= a[1];
-    }
-    const float safe[2] = {m_run[0] == -INFINITY ? 0.0f : m_run[0], m_run[1] == -INFINITY ? 0.0f : m_run[1]};
-#pragma unroll
-    for (int n = 0; n < SK / 8; n++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        s[n][e] = ex2(s[n][e] - safe[e >> 1]);
-        l_run[e >> 1] += s[n][e];
-      }
-
-    // ---- O += P' . V
-#pragma unroll
-    for (int blk = 0; blk < NB; blk++) {
-      // (Summed from zero and added in f32: the tensor core cuts its sums off to one side.)
-      float o[4][4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < SUBS; j++) {
-        uint32_t ah[4], al[4];
-#pragma unroll
-        for (int kp = 0; kp < 2; kp++) {
-          const float2 v = lds_f2(G::OFF_VS + ((buf * NB + blk) * SK + TK * j + 2 * t + 8 * kp) * 4);
-          const float2 w0 = mul2(make_float2(s[2 * j + kp][0], s[2 * j + kp][1]), v), w1 = mul2(make_float2(s[2 * j + kp][2], s[2 * j + kp][3]), v);
-          split2(w0.x, w0.y, &ah[2 * kp], &al[2 * kp]);
-          split2(w1.x, w1.y, &ah[2 * kp + 1], &al[2 * kp + 1]);
-        }
-        const uint4 f0 = *reinterpret_cast<const uint4*>(smem + frag + G::KFRAG + (blk * SUBS + j) * 1024);
-        const uint4 f1 = *reinterpret_cast<const uint4*>(smem + frag + G::KFRAG + (blk * SUBS + j) * 1024 + 512);
-        const uint32_t bf[4][2] = {{f0.x, f0.y}, {f0.z, f0.w}, {f1.x, f1.y}, {f1.z, f1.w}};
-#pragma unroll
-        for (int i = 0; i < 4; i++) mma_f16_from(o[i], al[0], al[1], al[2], al[3], bf[i][0], bf[i][1], o[i][0], o[i][1], o[i][2], o[i][3]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) mma_f16_from(o[i], ah[0], ah[1], ah[2], ah[3], bf[i][0], bf[i][1], o[i][0], o[i][1], o[i][2], o[i][3]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        add2(acc[blk][i][0], acc[blk][i][1], o[i][0], o[i][1]), add2(acc[blk][i][2], acc[blk][i][3], o[i][2], o[i][3]);
-    }
-    if (any_odd) {   // a V scale that is not finite: NaN where a row gives weight to its key
-#pragma unroll
-      for (int blk = 0; blk < NB; blk++) {
-        const uint32_t which = odd[buf * NB + blk];
-        bool met[2] = {false, false};
-#pragma unroll
-        for (int n = 0; n < SK / 8; n++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) met[e >> 1] |= ((which >> (8 * n + 2 * t + (e & 1))) & 1) && s[n][e] > 0.0f;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t who = __ballot_sync(FULL, met[h]);
-          const float add = (who >> (4 * g)) & 15 ? NAN : 0.0f;
-#pragma unroll
-          for (int i = 0; i < 4; i++) acc[blk][i][2 * h] += add, acc[blk][i][2 * h + 1] += add;
-        }
-      }
-    }
-    }
-    __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(frag_empty + 8 * buf);   // the fragments have been read
-  }
-
-  // ---- the rows' sums: straight out, or through shared memory to the cluster's others
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    l_run[h] += __shfl_xor_sync(FULL, l_run[h], 1);
-    l_run[h] += __shfl_xor_sync(FULL, l_run[h], 2);
-  }
-  const float back = __uint_as_float((127u + e_run - 29u) << 23);
-  const bool report = !flags[0] && !flags[1];
-  float* res = reinterpret_cast<float*>(smem + G::OFF_QF);
-  float* stats = reinterpret_cast<float*>(smem + G::OFF_STATS);
-  __syncwarp();   // (a warp's sums take the place of its own queries)
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    const uint32_t r = warp * 16 + g + 8 * h;
-    const bool good = l_run[h] > 0.0f && isfinite(l_run[h]);
-    float mul = back;
-    float* dst = res + r * D;
-    if (rg.cluster == 1) {
-      if (my_row[h] == NO_ROW) continue;
-      if (!good && hi[h] > lo[h] && report) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
-      mul = good ? back * __frcp_rn(l_run[h]) : 0.0f;
-      dst = p.out + (uint64_t)my_row[h] * D;
-    } else if (t == 0) {
-      stats[r] = m_run[h], stats[ROWS + r] = l_run[h];
-    }
-#pragma unroll
-    for (int blk = 0; blk < NB; blk++)
-#pragma unroll
-      for (int c = 0; c < 2; c++) {   // dimensions of the column group 2t + c
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = rg.cluster == 1 && !good ? 0.0f : acc[blk][i][2 * h + c] * mul;
-        float* at = dst + blk * QK;
-        if (VQ8) {
-          const int d0 = pair_byte(true, blk & 1, 2 * t + c, 0), d2 = pair_byte(true, blk & 1, 2 * t + c, 2);
-          *reinterpret_cast<float2*>(at + d0) = make_float2(v[0], v[1]);
-          *reinterpret_cast<float2*>(at + d2) = make_float2(v[2], v[3]);
-        } else {
-          *reinterpret_cast<float4*>(at + 4 * (2 * t + c)) = make_float4(v[0], v[1], v[2], v[3]);
-        }
-      }
-  }
-  }   // consumers
-  if (rg.cluster == 1) return;
-  const bool report = !flags[0] && !flags[1];
-  cluster_sync();
-  const uint32_t share = ROWS / rg.cluster, res_addr = sbase + G::OFF_QF, stats_addr = sbase + G::OFF_STATS;
-  for (uint32_t i = tid; i < share * (D / 4); i += RTHREADS) {
-    const uint32_t r = rank * share + i / (D / 4), d4 = i % (D / 4);
-    uint32_t l;
-    const uint32_t row = row_of(r, &l);
-    if (row == NO_ROW) continue;
-    float m[8], w[8], M = -INFINITY, lsum = 0.0f;
-    float4 v[8], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-      m[k] = -INFINITY, w[k] = 0.0f, v[k] = o;
-      if (k < (int)rg.cluster) {
-        const uint32_t a = cluster_addr(stats_addr, k);
-        m[k] = ld_cluster_f(a + 4 * r), w[k] = ld_cluster_f(a + 4 * (ROWS + r));
-        v[k] = ld_cluster_f4(cluster_addr(res_addr, k) + (r * D + 4 * d4) * 4);
-      }
-      M = fmaxf(M, m[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const float f = m[k] == -INFINITY ? 0.0f : ex2(m[k] - M);
-      o.x += v[k].x * f, o.y += v[k].y * f, o.z += v[k].z * f, o.w += v[k].w * f;
-      lsum += w[k] * f;
-    }
-    const bool good = lsum > 0.0f && isfinite(lsum);
-    if (!good && d4 == 0 && report) {
-      const KeyRange kr = key_range(p, b, l);
-      if (kr.hi > kr.lo) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
-    }
-    const float inv = good ? __frcp_rn(lsum) : 0.0f;
-    *reinterpret_cast<float4*>(p.out + (uint64_t)row * D + 4 * d4) = good ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  }
-  cluster_sync();   // no CTA leaves before the others have read its sums
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
 template <int D, bool KQ8, bool VQ8>
