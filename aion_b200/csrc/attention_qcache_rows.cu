@@ -62,14 +62,16 @@ struct RowsGeom {
   static constexpr int OFF_VRAW = OFF_KRAW + KRAWS * KRAW;
   static constexpr int OFF_KEXP = OFF_VRAW + VRAWS * VRAW;       // f32 [SLOTS][SK]: the keys' powers of two
   static constexpr int OFF_VEXP = OFF_KEXP + SLOTS * SK * 4;
-  static constexpr int OFF_EX = OFF_VEXP + SLOTS * SK * 4;       // f32 [2][2][ROWS]: maxima (or NaN blocks) of the two halves of a row
+  static constexpr int OFF_KSC = OFF_VEXP + SLOTS * SK * 4;      // f16 [2][SK][blocks]: the scales, normed
+  static constexpr int OFF_VSC = OFF_KSC + 2 * SK * NP * 4;      // f16 [3][SK][blocks]
+  static constexpr int OFF_EX = OFF_VSC + 3 * SK * NP * 4;       // f32 [2][2][ROWS]: maxima (or NaN blocks) of the two halves of a row
   static constexpr int OFF_STATS = OFF_EX + 4 * ROWS * 4;        // f32 [2][ROWS]: the rows' maxima and weights, for the cluster
   static constexpr int OFF_VMAX = OFF_STATS + 2 * ROWS * 4;      // u32 [SLOTS][8]: largest V exponent that an unpacking warp met, 256 for a scale that is not finite
   static constexpr int OFF_VALID = OFF_VMAX + SLOTS * 8 * 4;     // uint2 [SLOTS][SUBS]: which keys are there, the first of them
   static constexpr int OFF_ODD = OFF_VALID + SLOTS * SUBS * 8;   // u8 [SLOTS][SK]: blocks of a key whose V scale is not finite
   static constexpr int OFF_PAIR = OFF_ODD + SLOTS * SK;          // u32 [2][2][4]: did the half of the rows meet such a scale?
   static constexpr int OFF_BARS = OFF_PAIR + 16 * 4;
-  static constexpr int OFF_FLAGS = OFF_BARS + 26 * 8;            // bad inputs, gave up, TMEM, -, first key, key end
+  static constexpr int OFF_FLAGS = OFF_BARS + 28 * 8;             // bad inputs, gave up, TMEM, -, first key, key end
   static constexpr int SMEM = OFF_FLAGS + 32 + 1024;             // (panels begin on 1024 bytes)
   static_assert(4 * NP * PANEL == ROWS * D * 4 && OFF_KRAW % 128 == 0 && KRAW % 128 == 0 && VRAW % 128 == 0 && SMEM <= 227 * 1024, "shared memory");
   // tensor memory: columns of 32 bits
@@ -80,12 +82,20 @@ struct RowsGeom {
 // D f32, A and B f16, M = 128, N = 64; B K-major, or (bit 16) N-major.
 constexpr uint32_t IDESC_QK = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24), IDESC_PV = IDESC_QK | (1u << 16);
 
-// D[tmem] (+)= A[tmem] . B[smem desc], issued by one thread.
+// D[tmem] (+)= A[tmem] . B[smem desc]. The whole warp comes here and one elected thread, always the same, issues: so the
+// operands stay in uniform registers and an instruction is issued in the 32 clocks that it takes. (Inside a branch of one
+// thread 49 clocks each, and 102 with descriptors that a loop chooses.)
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_elected(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xFFFFFFFF;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld32f(uint32_t taddr, float (&r)[32]) {
@@ -107,12 +117,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(CW * 32) : "memory"); }
+__device__ __forceinline__ void unpack_sync() { asm volatile("bar.sync 6, %0;" ::"n"(UW * 32) : "memory"); }
 // The two warps that hold the halves of the same 32 rows.
 __device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory"); }
 __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
+}
+__device__ __forceinline__ uint32_t h2_rest(uint32_t a, uint32_t b, uint32_t c) {   // a * b - c
+  const __half2 d = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), __hneg2(*reinterpret_cast<__half2*>(&c)));
+  return *reinterpret_cast<const uint32_t*>(&d);
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   uint64_t d;
@@ -143,11 +158,15 @@ struct Unpack {
     for (int x = KPW; x < 32; x *= 2) e = max(e, __shfl_xor_sync(FULL, e, x));
     return e;
   }
-  // One block of a key: 32 codes times the scale (normed by the key's exponent), as two f16 terms.
+  // The two scales in units of 2^(e - 22).
+  static __device__ __forceinline__ uint32_t normed(const uint32_t (&sc)[2], uint32_t e) {
+    const float up = pow2f(22 - (int)e);
+    return pack_half2(half_bits(sc[0]) * up, half_bits(sc[1]) * up);
+  }
+  // One block of a key: 32 codes times its (normed) scale, as two f16 terms.
   template <int PAR>
-  static __device__ __forceinline__ void block(const uint8_t* row, uint32_t scale, uint32_t e, uint8_t* hi, uint8_t* lo, uint32_t key) {
-    const float s = half_bits(scale) * pow2f(22 - (int)e);
-    const uint32_t s2 = pack_half2(s, s);
+  static __device__ __forceinline__ void block(const uint8_t* row, uint32_t pair, uint8_t* hi, uint8_t* lo, uint32_t key) {
+    const uint32_t s2 = __byte_perm(pair, 0, PAR ? 0x3232 : 0x1010);
     constexpr int CODES = Q8 ? 8 : 4, FIRST = Q8 ? 8 : 4;   // words of codes; the word that holds the second block's scale
     uint32_t w[CODES];
     {
@@ -162,7 +181,7 @@ struct Unpack {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         h[i] = h2_mul(u[i], s2);
-        l[i] = h2_fma(u[i], s2, h[i] ^ 0x80008000u);   // exact: what the rounding left
+        l[i] = h2_rest(u[i], s2, h[i]);   // exact: what the rounding left
       }
       const uint32_t at = key * 128 + (((PAR * 4 + c) ^ (key & 7)) << 4);
       *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -202,8 +221,8 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t bars = sbase + G::OFF_BARS;
   const uint32_t kraw_full = bars, kraw_empty = bars + 24, vraw_full = bars + 48, vraw_empty = bars + 64;   // [3], [3], [2], [2]
-  const uint32_t k_ready = bars + 80, k_free = bars + 88, v_ready = bars + 96, v_free = bars + 104, q_ready = bars + 112, done = bars + 120;
-  const uint32_t s_full = bars + 128, p_ready = bars + 144, o_full = bars + 160, o_free = bars + 176, scaled = bars + 192;   // [2] x 4, [SLOTS]
+  const uint32_t k_ready = bars + 80, k_free = bars + 88, v_free = bars + 96, q_ready = bars + 104, done = bars + 112;
+  const uint32_t s_full = bars + 120, p_ready = bars + 136, o_full = bars + 152, o_free = bars + 168, scaled = bars + 184;   // [2] x 4, [SLOTS]
   volatile uint32_t* flags = reinterpret_cast<uint32_t*>(smem + G::OFF_FLAGS);
   uint2* valid = reinterpret_cast<uint2*>(smem + G::OFF_VALID);
   const bool softmax = warp < CW;
@@ -212,11 +231,11 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
     for (int s = 0; s < KRAWS; s++) ptx::mbar_init(kraw_full + 8 * s, 1), ptx::mbar_init(kraw_empty + 8 * s, UW);
     for (int s = 0; s < 2; s++) {
       ptx::mbar_init(vraw_full + 8 * s, 1), ptx::mbar_init(vraw_empty + 8 * s, UW);
-      ptx::mbar_init(s_full + 8 * s, 1), ptx::mbar_init(p_ready + 8 * s, CW);
+      ptx::mbar_init(s_full + 8 * s, 1), ptx::mbar_init(p_ready + 8 * s, CW + UW);
       ptx::mbar_init(o_full + 8 * s, 1), ptx::mbar_init(o_free + 8 * s, CW);
     }
     for (int s = 0; s < SLOTS; s++) ptx::mbar_init(scaled + 8 * s, UW);
-    ptx::mbar_init(k_ready, UW), ptx::mbar_init(k_free, 1), ptx::mbar_init(v_ready, UW), ptx::mbar_init(v_free, 1);
+    ptx::mbar_init(k_ready, UW), ptx::mbar_init(k_free, 1), ptx::mbar_init(v_free, 1);
     ptx::mbar_init(q_ready, CW), ptx::mbar_init(done, 1);
     flags[0] = flags[1] = flags[5] = 0;
     flags[4] = 0xFFFFFFFFu;
@@ -339,15 +358,15 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
     for (int q = 0; q < NP; q++)
 #pragma unroll
       for (int i = 0; i < 32; i++) acc[q][i] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f, a_cur = 1.0f, a_next = 1.0f;
+    float m_run = -INFINITY, l_run = 0.0f, a_cur = 1.0f;
     uint32_t e_run = 0;
     float* ex = reinterpret_cast<float*>(smem + G::OFF_EX);
     const uint32_t lane_base = tmem + ((uint32_t)quarter << 21) + half * 32;
 
-    for (uint32_t step = 0; step <= stages; step++) {
-      if (step < stages) {
-        // ---- P of stage `step`
-        const uint32_t it = step, slot = it % SLOTS;
+    for (uint32_t it = 0; it < stages; it++) {
+      {
+        // ---- P, while the next stage's logits are made
+        const uint32_t slot = it % SLOTS;
         wait(scaled + 8 * slot, it / SLOTS);
         wait(s_full + 8 * (it & 1), it >> 1);
         tc_fence_after();
@@ -408,7 +427,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         const float m_new = fmaxf(mine, mx[(half ^ 1) * ROWS + r]);
         float a = m_new > m_run ? ex2(m_run - m_new) : 1.0f;
         l_run *= a;
-        a_next = a * pow2f((int)e_run - (int)e_new);
+        a_cur = a * pow2f((int)e_run - (int)e_new);
         m_run = m_new, e_run = e_new;
         // P times the key's V power, over 2^e_run: at most 2^14
         const float off = 30.0f - (float)e_run - (m_run == -INFINITY ? 0.0f : m_run);
@@ -452,11 +471,11 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         tc_fence_before();
         arrive(p_ready + 8 * (it & 1));
       }
-      if (step > 0) {
-        // ---- O of the stage before
+      {
+        // ---- O, panel by panel as it comes
 #pragma unroll
         for (int q = 0; q < NP; q++) {
-          const uint32_t n = (step - 1) * NP + q;
+          const uint32_t n = it * NP + q;
           wait(o_full + 8 * (n & 1), n >> 1);
           tc_fence_after();
           float o[32];
@@ -471,7 +490,6 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           }
         }
       }
-      a_cur = a_next;
     }
 
     // ---- the rows' sums: straight out, or through shared memory to the cluster's others
@@ -547,49 +565,50 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
     if (warp == MMA_WARP) {
       // ================ the products ================
       wait(q_ready, 0);
+      const uint32_t t0 = __reduce_max_sync(FULL, tmem), rounds = __reduce_max_sync(FULL, stages);   // (uniform registers)
+      const uint64_t kh = smem_desc_sw128(sbase + G::OFF_K), kl = kh + NP * (PANEL >> 4);
+      const uint64_t vh = smem_desc_sw128(sbase + G::OFF_V), vl = vh + NP * (PANEL >> 4);
       auto logits = [&](uint32_t it) {
         wait(k_ready, it);
         tc_fence_after();
-        if (!dead && lane == 0) {
-          const uint64_t kh = smem_desc_sw128(sbase + G::OFF_K), kl = smem_desc_sw128(sbase + G::OFF_K + NP * PANEL);
-          const uint32_t d = tmem + G::T_S + (it & 1) * 64, qh = tmem + G::T_Q, ql = qh + D / 2;
+        {
+          const uint32_t d = t0 + G::T_S + (it & 1) * 64, qh = t0 + G::T_Q, ql = qh + D / 2;
+          // (Panels in a loop: spelled out, their descriptors are all kept, most of them in local memory.)
+          auto product = [&](uint32_t a, uint64_t bd, uint32_t more) {
 #pragma unroll 1
-          for (int j = 0; j < 3; j++) {
-            const uint32_t a = j == 0 ? ql : qh;
-            const uint64_t bd = j == 1 ? kl : kh;
+            for (int q = 0; q < NP; q++)
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ks++) umma_f16_ts(d, a + 8 * ks, bd + (ks >> 2) * (PANEL >> 4) + (ks & 3) * 2, IDESC_QK, j > 0 || ks > 0);
-          }
-          umma_commit(s_full + 8 * (it & 1));
-          umma_commit(k_free);
+              for (int ks = 0; ks < 4; ks++) umma_f16_ts(d, a + 32 * q + 8 * ks, bd + q * (PANEL >> 4) + 2 * ks, IDESC_QK, more | (uint32_t)(q + ks));
+          };
+          product(ql, kh, 0), product(qh, kl, 1), product(qh, kh, 1);
+          umma_commit_elected(s_full + 8 * (it & 1));
+          umma_commit_elected(k_free);
         }
-        __syncwarp();
       };
-      if (stages > 0) logits(0);
-      for (uint32_t it = 0; it < stages; it++) {
-        if (it + 1 < stages) logits(it + 1);
-        wait(v_ready, it);
-        wait(p_ready + 8 * (it & 1), it >> 1);
+      if (rounds > 0) logits(0);
+      for (uint32_t it = 0; it < rounds; it++) {
+        if (it + 1 < rounds) logits(it + 1);
+        wait(p_ready + 8 * (it & 1), it >> 1);   // P and V
+#pragma unroll 1
         for (int q = 0; q < NP; q++) {
           const uint32_t n = it * NP + q;
           if (n >= 2) wait(o_free + 8 * (n & 1), (n >> 1) - 1);
           tc_fence_after();
-          if (!dead && lane == 0) {
-            const uint64_t vh = smem_desc_sw128(sbase + G::OFF_V + q * PANEL), vl = vh + NP * (PANEL >> 4);
-            const uint32_t d = tmem + G::T_O + (n & 1) * 64, ph = tmem + G::T_S + (it & 1) * 64;
+          {
+            const uint32_t d = t0 + G::T_O + (n & 1) * 64, ph = t0 + G::T_S + (it & 1) * 64;
 #pragma unroll
             for (int j = 0; j < 3; j++)
 #pragma unroll
               for (int ks = 0; ks < SK / 16; ks++)   // 16 keys: eight columns of P, two groups of eight rows of V
-                umma_f16_ts(d, ph + (ks >> 1) * 32 + (ks & 1) * 8 + (j == 0 ? 16 : 0), (j == 1 ? vl : vh) + ks * (2048 >> 4), IDESC_PV, j > 0 || ks > 0);
-            umma_commit(o_full + 8 * (n & 1));
-            if (q == NP - 1) umma_commit(v_free);
+                umma_f16_ts(d, ph + (ks >> 1) * 32 + (ks & 1) * 8 + (j == 0 ? 16 : 0), (j == 1 ? vl : vh) + q * (PANEL >> 4) + ks * (2048 >> 4), IDESC_PV, j > 0 || ks > 0);
+            umma_commit_elected(o_full + 8 * (n & 1));
+            if (q == NP - 1) umma_commit_elected(v_free);
           }
-          __syncwarp();
         }
       }
-      if (lane == 0) umma_commit(done);
+      umma_commit_elected(done);
       ptx::mbar_wait_bounded(done, 0, p.wait_limit);
+      __syncwarp();
     } else if (warp == LOAD_WARP) {
       // ================ raw stages ================
       if (lane == 0) {
@@ -662,49 +681,43 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       constexpr int KPW = UK::KPW, GROUPS = UK::GROUPS;
       const uint32_t in_group = lane % KPW, panel = lane / KPW;
       wait(q_ready, 0);   // (q passed through the panels)
-      auto keys = [&](uint32_t it) {
-        wait(kraw_full + 8 * (it % KRAWS), it / KRAWS);
-        if (it > 0) wait(k_free, it - 1);
-        if (!dead) {
-          const uint8_t* raw = smem + G::OFF_KRAW + (it % KRAWS) * G::KRAW + kshift + panel * 2 * KF::BB;
-          uint8_t* kh = smem + G::OFF_K + panel * PANEL;
-          for (uint32_t u = uw; u < 2 * GROUPS; u += UW) {
-            const uint32_t key = (u >> 1) * KPW + in_group;
-            const uint8_t* row = raw + key * KF::PITCH;
-            uint32_t sc[2];
-            const uint32_t e = UK::scales(row, sc);
-            if (u & 1) {
-              UK::template block<1>(row, sc[1], e, kh, kh + NP * PANEL, key);
-            } else {
-              UK::template block<0>(row, sc[0], e, kh, kh + NP * PANEL, key);
-              if (panel == 0) *reinterpret_cast<float*>(smem + G::OFF_KEXP + ((it % SLOTS) * SK + key) * 4) = pow2f((int)e - 22);
-            }
-          }
-          ptx::fence_proxy_async();
-        }
-        arrive(k_ready);
-        arrive(kraw_empty + 8 * (it % KRAWS));
-      };
       // Is the key there, and does a row of the block see it?
       auto seen = [&](uint32_t it, uint32_t key) {
         const uint2 v = valid[(it % SLOTS) * SUBS + key / TK];
         const uint32_t at = v.y + key % TK;
         return ((v.x >> (key % TK)) & 1) && at >= u_lo && at < u_hi;
       };
-      auto exponents = [&](uint32_t it) {
-        wait(vraw_full + 8 * (it % VRAWS), it / VRAWS);
-        if (!dead) {
-          const uint8_t* raw = smem + G::OFF_VRAW + (it % VRAWS) * G::VRAW + vshift + panel * 2 * VF::BB;
-          uint32_t top = 0, any = 0;
+      auto key_scales = [&](uint32_t it) {
+        wait(kraw_full + 8 * (it % KRAWS), it / KRAWS);
+        if (!dead)
+#pragma unroll 1
           for (uint32_t u = uw; u < GROUPS; u += UW) {
             const uint32_t key = u * KPW + in_group;
             uint32_t sc[2];
-            const uint32_t e = UV::scales(raw + key * VF::PITCH, sc);
+            const uint32_t e = UK::scales(smem + G::OFF_KRAW + (it % KRAWS) * G::KRAW + kshift + panel * 2 * KF::BB + key * KF::PITCH, sc);
+            *reinterpret_cast<uint32_t*>(smem + G::OFF_KSC + ((it & 1) * SK * NP + key * NP + panel) * 4) = UK::normed(sc, e);
+            if (panel == 0) *reinterpret_cast<float*>(smem + G::OFF_KEXP + ((it % SLOTS) * SK + key) * 4) = pow2f((int)e - 22);
+          }
+        unpack_sync();   // (every warp comes here, also one that has given up)
+      };
+      auto value_scales = [&](uint32_t it) {
+        wait(vraw_full + 8 * (it % VRAWS), it / VRAWS);
+        if (!dead) {
+          uint32_t top = 0, any = 0;
+#pragma unroll 1
+          for (uint32_t u = uw; u < GROUPS; u += UW) {
+            const uint32_t key = u * KPW + in_group;
+            uint32_t sc[2], odd = 0;
+            const uint32_t e = UV::scales(smem + G::OFF_VRAW + (it % VRAWS) * G::VRAW + vshift + panel * 2 * VF::BB + key * VF::PITCH, sc);
             const bool on = seen(it, key);
-            uint32_t odd = 0;
-            if (on) odd = ((sc[0] & 0x7C00u) == 0x7C00u ? 1u : 0u) << (2 * panel) | ((sc[1] & 0x7C00u) == 0x7C00u ? 2u : 0u) << (2 * panel);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              if (on && (sc[i] & 0x7C00u) == 0x7C00u) odd |= (1u << i) << (2 * panel);
+              if (!on || (sc[i] & 0x7C00u) == 0x7C00u) sc[i] = 0;
+            }
 #pragma unroll
             for (int x = KPW; x < 32; x *= 2) odd |= __shfl_xor_sync(FULL, odd, x);
+            *reinterpret_cast<uint32_t*>(smem + G::OFF_VSC + ((it % 3) * SK * NP + key * NP + panel) * 4) = UV::normed(sc, e);
             if (panel == 0) {
               *reinterpret_cast<float*>(smem + G::OFF_VEXP + ((it % SLOTS) * SK + key) * 4) = pow2f((int)e - 16);
               smem[G::OFF_ODD + (it % SLOTS) * SK + key] = (uint8_t)odd;
@@ -717,32 +730,50 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         }
         arrive(scaled + 8 * (it % SLOTS));
       };
+      auto keys = [&](uint32_t it) {
+        if (it > 0) wait(k_free, it - 1);
+        if (!dead) {
+          const uint8_t* raw = smem + G::OFF_KRAW + (it % KRAWS) * G::KRAW + kshift + panel * 2 * KF::BB;
+          const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + G::OFF_KSC) + (it & 1) * SK * NP + panel;
+          uint8_t* kh = smem + G::OFF_K + panel * PANEL;
+#pragma unroll 1
+          for (uint32_t u = uw; u < 2 * GROUPS; u += UW) {
+            const uint32_t key = (u >> 1) * KPW + in_group;
+            if (u & 1) UK::template block<1>(raw + key * KF::PITCH, sc[key * NP], kh, kh + NP * PANEL, key);
+            else UK::template block<0>(raw + key * KF::PITCH, sc[key * NP], kh, kh + NP * PANEL, key);
+          }
+          ptx::fence_proxy_async();
+        }
+        arrive(k_ready);
+        arrive(kraw_empty + 8 * (it % KRAWS));
+      };
       auto values = [&](uint32_t it) {
         if (it > 0) wait(v_free, it - 1);
         if (!dead) {
           const uint8_t* raw = smem + G::OFF_VRAW + (it % VRAWS) * G::VRAW + vshift + panel * 2 * VF::BB;
+          const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + G::OFF_VSC) + (it % 3) * SK * NP + panel;
           uint8_t* vh = smem + G::OFF_V + panel * PANEL;
+#pragma unroll 1
           for (uint32_t u = uw; u < 2 * GROUPS; u += UW) {
             const uint32_t key = (u >> 1) * KPW + in_group;
-            const uint8_t* row = raw + key * VF::PITCH;
-            uint32_t sc[2];
-            const uint32_t e = UV::scales(row, sc);
-            uint32_t mine = u & 1 ? sc[1] : sc[0];
-            if (!seen(it, key) || (mine & 0x7C00u) == 0x7C00u) mine = 0;
-            if (u & 1) UV::template block<1>(row, mine, e, vh, vh + NP * PANEL, key);
-            else UV::template block<0>(row, mine, e, vh, vh + NP * PANEL, key);
+            if (u & 1) UV::template block<1>(raw + key * VF::PITCH, sc[key * NP], vh, vh + NP * PANEL, key);
+            else UV::template block<0>(raw + key * VF::PITCH, sc[key * NP], vh, vh + NP * PANEL, key);
           }
           ptx::fence_proxy_async();
         }
-        arrive(v_ready);
+        arrive(p_ready + 8 * (it & 1));
         arrive(vraw_empty + 8 * (it % VRAWS));
       };
-      if (stages > 0) keys(0), exponents(0), values(0);
-      for (uint32_t it = 1; it < stages; it++) {
-        keys(it), exponents(it);
-        if (it > 1) values(it - 1);
+      for (uint32_t it = 0; it <= stages; it++) {
+        if (it < stages) {
+          key_scales(it);
+          keys(it);
+          value_scales(it);
+        } else {
+          unpack_sync();
+        }
+        if (it > 0) values(it - 1);
       }
-      if (stages > 1) values(stages - 1);
     }
     if (rg.cluster > 1) {
       __syncwarp();
