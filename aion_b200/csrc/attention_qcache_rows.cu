@@ -115,6 +115,18 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+        "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(CW * 32) : "memory"); }
 __device__ __forceinline__ void unpack_sync() { asm volatile("bar.sync 6, %0;" ::"n"(UW * 32) : "memory"); }
@@ -292,7 +304,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   // no warp is left at a barrier of a pair.
   bool dead = false;
   auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (!dead && !__all_sync(FULL, ptx::mbar_wait_bounded(bar, parity & 1, p.wait_limit))) {
+    if (!dead && !__all_sync(FULL, ptx::mbar_try_wait_spin(bar, parity & 1) || ptx::mbar_wait_bounded(bar, parity & 1, p.wait_limit))) {
       dead = true;
       if (lane == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED), flags[1] = 1;
     }
@@ -358,25 +370,50 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
     for (int q = 0; q < NP; q++)
 #pragma unroll
       for (int i = 0; i < 32; i++) acc[q][i] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f, a_cur = 1.0f;
+    float m_run = -INFINITY, l_run = 0.0f;
     uint32_t e_run = 0;
     float* ex = reinterpret_cast<float*>(smem + G::OFF_EX);
     const uint32_t lane_base = tmem + ((uint32_t)quarter << 21) + half * 32;
 
-    for (uint32_t it = 0; it < stages; it++) {
-      {
-        // ---- P, while the next stage's logits are made
-        const uint32_t slot = it % SLOTS;
+    // O of a stage, 64 dimensions: the other half of the warps takes the other 32.
+    float a_of = 1.0f;   // what the sums so far are worth in units of that stage
+    auto drain = [&](uint32_t it, int q, float (&sums)[32]) {
+      const uint32_t n = it * NP + q;
+      wait(o_full + 8 * (n & 1), n >> 1);
+      tc_fence_after();
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        float o[16];
+        tmem_ld16f(lane_base + G::T_O + (n & 1) * 64 + j * 16, o);
+        tmem_ld_wait();
+        if (j == 1) {
+          tc_fence_before();
+          arrive(o_free + 8 * (n & 1));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float2 x = fma2(make_float2(sums[16 * j + 2 * i], sums[16 * j + 2 * i + 1]), make_float2(a_of, a_of), make_float2(o[2 * i], o[2 * i + 1]));
+          sums[16 * j + 2 * i] = x.x, sums[16 * j + 2 * i + 1] = x.y;
+        }
+      }
+    };
+    // P of stage `it`, in four steps, and between them O of the stage before, panel by panel as it comes.
+    for (uint32_t it = 0; it <= stages; it++) {
+      const bool more = it < stages, prev = it > 0;
+      const uint32_t slot = it % SLOTS, at = lane_base + G::T_S + (it & 1) * 64;
+      float s[32];
+      float a_next = 1.0f;
+      float* mx = ex + (it & 1) * 2 * ROWS;
+      uint32_t any_odd = 0;
+      if (more) {   // logits, the running maximum
         wait(scaled + 8 * slot, it / SLOTS);
         wait(s_full + 8 * (it & 1), it >> 1);
         tc_fence_after();
-        float s[32];
-        const uint32_t at = lane_base + G::T_S + (it & 1) * 64;
         tmem_ld32f(at, s);
         const uint4 v0 = *reinterpret_cast<const uint4*>(smem + G::OFF_VMAX + slot * 32), v1 = *reinterpret_cast<const uint4*>(smem + G::OFF_VMAX + slot * 32 + 16);
         const uint32_t met = max(max(v0.x & 31, v0.y & 31), max(max(v0.z & 31, v0.w & 31), max(v1.x & 31, v1.y & 31)));
         const uint32_t e_new = max(e_run, met);
-        uint32_t any_odd = (v0.x | v0.y | v0.z | v0.w | v1.x | v1.y) & 256;
+        any_odd = (v0.x | v0.y | v0.z | v0.w | v1.x | v1.y) & 256;
         bool partial = false;
         uint32_t there[2], key0[2];
 #pragma unroll
@@ -386,9 +423,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           partial |= v.x != 0xFFFFu || v.y < all_lo || v.y + TK > all_hi;
         }
         const float4* kexp = reinterpret_cast<const float4*>(smem + G::OFF_KEXP + (slot * SK + half * 32) * 4);
-        const float4* vexp = reinterpret_cast<const float4*>(smem + G::OFF_VEXP + (slot * SK + half * 32) * 4);
         tmem_ld_wait();
-        float unit = factor;
         if (p.soft_cap > 0.0f) {
 #pragma unroll
           for (int i = 0; i < 8; i++) {
@@ -402,8 +437,8 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             const float4 k = kexp[i];
-            const float2 a = mul2(mul2(make_float2(s[4 * i], s[4 * i + 1]), make_float2(k.x, k.y)), make_float2(unit, unit));
-            const float2 c = mul2(mul2(make_float2(s[4 * i + 2], s[4 * i + 3]), make_float2(k.z, k.w)), make_float2(unit, unit));
+            const float2 a = mul2(mul2(make_float2(s[4 * i], s[4 * i + 1]), make_float2(k.x, k.y)), make_float2(factor, factor));
+            const float2 c = mul2(mul2(make_float2(s[4 * i + 2], s[4 * i + 3]), make_float2(k.z, k.w)), make_float2(factor, factor));
             s[4 * i] = a.x, s[4 * i + 1] = a.y, s[4 * i + 2] = c.x, s[4 * i + 3] = c.y;
           }
         }
@@ -418,18 +453,19 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
 #pragma unroll
         for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], s[i]);
         const float mine = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        float* mx = ex + (it & 1) * 2 * ROWS;
         uint32_t* both = reinterpret_cast<uint32_t*>(smem + G::OFF_PAIR) + (it & 1) * 8 + quarter;
         mx[half * ROWS + r] = mine;
         if (lane == 0) both[4 * half] = any_odd;
         pair_sync(quarter);
         any_odd = both[0] | both[4];   // (the two warps go the same way, even when one of them has given up waiting)
         const float m_new = fmaxf(mine, mx[(half ^ 1) * ROWS + r]);
-        float a = m_new > m_run ? ex2(m_run - m_new) : 1.0f;
+        const float a = m_new > m_run ? ex2(m_run - m_new) : 1.0f;
         l_run *= a;
-        a_cur = a * pow2f((int)e_run - (int)e_new);
+        a_next = a * pow2f((int)e_run - (int)e_new);
         m_run = m_new, e_run = e_new;
-        // P times the key's V power, over 2^e_run: at most 2^14
+      }
+      if (prev) drain(it - 1, 0, acc[0]);
+      if (more) {   // weights, in units in which the largest product with a V power is at most 2^14
         const float off = 30.0f - (float)e_run - (m_run == -INFINITY ? 0.0f : m_run);
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -441,55 +477,48 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           s[2 * i] = x.x, s[2 * i + 1] = x.y;
         }
         l_run = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), pow2f((int)e_run - 30), l_run);
-        if (any_odd) {   // a V scale that is not finite: NaN where a row gives weight to its key
-          const uint8_t* odd = smem + G::OFF_ODD + slot * SK + half * 32;
-          uint32_t hit = 0;
-#pragma unroll
-          for (int i = 0; i < 32; i++) hit |= s[i] > 0.0f ? odd[i] : 0u;
-          pair_sync(quarter);   // (the maxima have been read)
-          mx[half * ROWS + r] = __uint_as_float(hit);
-          pair_sync(quarter);
-          hit |= __float_as_uint(mx[(half ^ 1) * ROWS + r]);
-          pair_sync(quarter);
-#pragma unroll
-          for (int q = 0; q < NP; q++)
-            if ((hit >> (2 * q + half)) & 1)
-#pragma unroll
-              for (int i = 0; i < 32; i++) acc[q][i] = NAN;
-        }
-        uint32_t h[16], l[16];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float4 v = vexp[i];
-          const float2 w0 = mul2(make_float2(s[4 * i], s[4 * i + 1]), make_float2(v.x, v.y)), w1 = mul2(make_float2(s[4 * i + 2], s[4 * i + 3]), make_float2(v.z, v.w));
-          split2(w0.x, w0.y, &h[2 * i], &l[2 * i]);
-          split2(w1.x, w1.y, &h[2 * i + 1], &l[2 * i + 1]);
-        }
-        tmem_st16(at, h);
-        tmem_st16(at + 16, l);
-        tmem_st_wait();
-        tc_fence_before();
-        arrive(p_ready + 8 * (it & 1));
       }
-      {
-        // ---- O, panel by panel as it comes
+      if (NP > 1 && prev) drain(it - 1, 1, acc[1 % NP]);
+      if (any_odd) {   // a V scale that is not finite: NaN where a row gives weight to its key
+        const uint8_t* odd = smem + G::OFF_ODD + slot * SK + half * 32;
+        uint32_t hit = 0;
 #pragma unroll
-        for (int q = 0; q < NP; q++) {
-          const uint32_t n = it * NP + q;
-          wait(o_full + 8 * (n & 1), n >> 1);
-          tc_fence_after();
-          float o[32];
-          tmem_ld32f(lane_base + G::T_O + (n & 1) * 64, o);
-          tmem_ld_wait();
-          tc_fence_before();
-          arrive(o_free + 8 * (n & 1));
+        for (int i = 0; i < 32; i++) hit |= s[i] > 0.0f ? odd[i] : 0u;
+        pair_sync(quarter);   // (the maxima have been read)
+        mx[half * ROWS + r] = __uint_as_float(hit);
+        pair_sync(quarter);
+        hit |= __float_as_uint(mx[(half ^ 1) * ROWS + r]);
+        pair_sync(quarter);
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float2 x = fma2(make_float2(acc[q][2 * i], acc[q][2 * i + 1]), make_float2(a_cur, a_cur), make_float2(o[2 * i], o[2 * i + 1]));
-            acc[q][2 * i] = x.x, acc[q][2 * i + 1] = x.y;
+        for (int q = 0; q < NP; q++)
+          if ((hit >> (2 * q + half)) & 1)
+#pragma unroll
+            for (int i = 0; i < 32; i++) acc[q][i] = NAN;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; j++) {   // two terms of the products, over the logits: 16 keys are eight columns
+        if (more) {
+          const float4* vexp = reinterpret_cast<const float4*>(smem + G::OFF_VEXP + (slot * SK + half * 32 + j * 16) * 4);
+          uint32_t h[8], l[8];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float4 v = vexp[i];
+            const float* x = s + 16 * j + 4 * i;
+            const float2 w0 = mul2(make_float2(x[0], x[1]), make_float2(v.x, v.y)), w1 = mul2(make_float2(x[2], x[3]), make_float2(v.z, v.w));
+            split2(w0.x, w0.y, &h[2 * i], &l[2 * i]);
+            split2(w1.x, w1.y, &h[2 * i + 1], &l[2 * i + 1]);
+          }
+          tmem_st8(at + 8 * j, h);
+          tmem_st8(at + 16 + 8 * j, l);
+          if (j == 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            arrive(p_ready + 8 * (it & 1));
           }
         }
+        if (NP > 2 + j && prev) drain(it - 1, 2 + j, acc[(2 + j) % NP]);
       }
+      a_of = a_next;
     }
 
     // ---- the rows' sums: straight out, or through shared memory to the cluster's others
