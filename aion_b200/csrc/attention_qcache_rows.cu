@@ -464,7 +464,10 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         a_next = a * pow2f((int)e_run - (int)e_new);
         m_run = m_new, e_run = e_new;
       }
-      if (prev) drain(it - 1, 0, acc[0]);
+      if (prev) {
+        drain(it - 1, 0, acc[0]);
+        if (NP > 1) drain(it - 1, 1, acc[1 % NP]);
+      }
       if (more) {   // weights, in units in which the largest product with a V power is at most 2^14
         const float off = 30.0f - (float)e_run - (m_run == -INFINITY ? 0.0f : m_run);
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -478,7 +481,6 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         }
         l_run = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), pow2f((int)e_run - 30), l_run);
       }
-      if (NP > 1 && prev) drain(it - 1, 1, acc[1 % NP]);
       if (any_odd) {   // a V scale that is not finite: NaN where a row gives weight to its key
         const uint8_t* odd = smem + G::OFF_ODD + slot * SK + half * 32;
         uint32_t hit = 0;
@@ -516,7 +518,10 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
             arrive(p_ready + 8 * (it & 1));
           }
         }
-        if (NP > 2 + j && prev) drain(it - 1, 2 + j, acc[(2 + j) % NP]);
+      }
+      if (NP > 2 && prev) {
+        drain(it - 1, 2, acc[2 % NP]);
+        drain(it - 1, 3, acc[3 % NP]);
       }
       a_of = a_next;
     }
