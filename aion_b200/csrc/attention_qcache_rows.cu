@@ -66,7 +66,8 @@ struct RowsGeom {
   static constexpr int OFF_VSC = OFF_KSC + 2 * SK * NP * 4;      // f16 [3][SK][blocks]
   static constexpr int OFF_EX = OFF_VSC + 3 * SK * NP * 4;       // f32 [2][2][ROWS]: maxima (or NaN blocks) of the two halves of a row
   static constexpr int OFF_STATS = OFF_EX + 4 * ROWS * 4;        // f32 [2][ROWS]: the rows' maxima and weights, for the cluster
-  static constexpr int OFF_VMAX = OFF_STATS + 2 * ROWS * 4;      // u32 [SLOTS][8]: largest V exponent that an unpacking warp met, 256 for a scale that is not finite
+  static constexpr int OFF_ROWS = OFF_STATS + 2 * ROWS * 4;      // u32 [ROWS]: a row's place in q and out
+  static constexpr int OFF_VMAX = OFF_ROWS + ROWS * 4;      // u32 [SLOTS][8]: largest V exponent that an unpacking warp met, 256 for a scale that is not finite
   static constexpr int OFF_VALID = OFF_VMAX + SLOTS * 8 * 4;     // uint2 [SLOTS][SUBS]: which keys are there, the first of them
   static constexpr int OFF_ODD = OFF_VALID + SLOTS * SUBS * 8;   // u8 [SLOTS][SK]: blocks of a key whose V scale is not finite
   static constexpr int OFF_PAIR = OFF_ODD + SLOTS * SK;          // u32 [2][2][4]: did the half of the rows meet such a scale?
@@ -277,10 +278,12 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   };
   const int quarter = warp & 3, half = (warp >> 2) & 1;   // of a softmax warp: its 32 rows, its half of the keys and dimensions
   const uint32_t r = quarter * 32 + lane;
+  uint32_t* rows = reinterpret_cast<uint32_t*>(smem + G::OFF_ROWS);
   uint32_t my_row = NO_ROW, lo = 0, hi = 0, all_lo = 0, all_hi = 0xFFFFFFFFu;
   if (softmax) {
     uint32_t l;
     my_row = row_of(r, &l);
+    if (half == 0) rows[r] = my_row;
     if (my_row != NO_ROW) {
       const KeyRange kr = key_range(p, b, l);
       if (kr.bad) flags[0] = 1;
@@ -321,25 +324,37 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
     {
       float* stage = reinterpret_cast<float*>(smem + G::OFF_K);
       float* tops = reinterpret_cast<float*>(smem + G::OFF_STATS);
-#pragma unroll 4
-      for (int i = 0; i < ROWS / CW; i++) {
-        const uint32_t row_in = warp * (ROWS / CW) + i;
-        uint32_t l;
-        const uint32_t row = row_of(row_in, &l);
-        float top = 0.0f;
+#pragma unroll 1
+      for (int i0 = 0; i0 < ROWS / CW; i0 += 8) {   // (eight rows' loads at once)
+        float x[8][D / 32];
 #pragma unroll
-        for (int j = 0; j < D / 32; j++) {
-          const uint32_t d = lane + 32 * j;
-          float x = 0.0f;
-          if (row != NO_ROW) {
-            const uint64_t at = (uint64_t)row * D + d;
-            x = p.q_dtype == AION_CUDA_DTYPE_F32 ? static_cast<const float*>(p.q)[at] : __half2float(static_cast<const __half*>(p.q)[at]);
+        for (int i = 0; i < 8; i++) {
+          const uint32_t row = rows[warp * (ROWS / CW) + i0 + i];
+          const uint64_t at = (uint64_t)row * D + lane;
+          if (row == NO_ROW) {
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) x[i][j] = 0.0f;
+          } else if (p.q_dtype == AION_CUDA_DTYPE_F32) {
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) x[i][j] = __ldg(static_cast<const float*>(p.q) + at + 32 * j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) x[i][j] = __half2float(__ldg(static_cast<const __half*>(p.q) + at + 32 * j));
           }
-          top = fmaxf(top, fabsf(x));
-          stage[row_in * D + ((((d >> 2) ^ (row_in & 7)) << 2) | (d & 3))] = x;
         }
-        const uint32_t t = __reduce_max_sync(FULL, __float_as_uint(top));
-        if (lane == 0) tops[row_in] = __uint_as_float(t);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const uint32_t row_in = warp * (ROWS / CW) + i0 + i;
+          float top = 0.0f;
+#pragma unroll
+          for (int j = 0; j < D / 32; j++) {
+            const uint32_t d = lane + 32 * j;
+            top = fmaxf(top, fabsf(x[i][j]));
+            stage[row_in * D + ((((d >> 2) ^ (row_in & 7)) << 2) | (d & 3))] = x[i][j];
+          }
+          const uint32_t t = __reduce_max_sync(FULL, __float_as_uint(top));
+          if (lane == 0) tops[row_in] = __uint_as_float(t);
+        }
       }
       softmax_sync();
       uint32_t e = __float_as_uint(tops[r]) >> 23;
@@ -526,74 +541,95 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       a_of = a_next;
     }
 
-    // ---- the rows' sums: straight out, or through shared memory to the cluster's others
+    // ---- the rows' sums, through shared memory: a row is written whole, and a cluster's CTAs add up theirs, each for its share
+    // of the rows
     pair_sync(quarter);
     ex[half * ROWS + r] = l_run;
     pair_sync(quarter);
     l_run += ex[(half ^ 1) * ROWS + r];
     const bool report = !flags[0] && !flags[1];
-    const bool good = l_run > 0.0f && isfinite(l_run);
     const float back = pow2f((int)e_run - 36);
-    if (rg.cluster == 1) {
-      if (my_row != NO_ROW) {
-        if (!good && hi > lo && half == 0 && report) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
-        const float mul = good ? back * __frcp_rn(l_run) : 0.0f;
-        float* dst = p.out + (uint64_t)my_row * D + half * 32;
+    float* res = reinterpret_cast<float*>(smem + G::OFF_K);   // (the last product has been read, so the panels are free)
+    float* stats = reinterpret_cast<float*>(smem + G::OFF_STATS);
+    float* weight = reinterpret_cast<float*>(smem + G::OFF_KRAW);   // [8][ROWS]: what a CTA's sums count in a row
+    softmax_sync();
+    if (half == 0) stats[r] = m_run, stats[ROWS + r] = l_run;
 #pragma unroll
-        for (int q = 0; q < NP; q++)
+    for (int q = 0; q < NP; q++)
 #pragma unroll
-          for (int i = 0; i < 8; i++)
-            *reinterpret_cast<float4*>(dst + q * 64 + 4 * i) = good ? make_float4(acc[q][4 * i] * mul, acc[q][4 * i + 1] * mul, acc[q][4 * i + 2] * mul, acc[q][4 * i + 3] * mul)
-                                                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int i = 0; i < 8; i++) {
+        const uint32_t chunk = q * 16 + half * 8 + i;
+        *reinterpret_cast<float4*>(res + r * D + ((chunk ^ (r & 7)) << 2)) = make_float4(acc[q][4 * i] * back, acc[q][4 * i + 1] * back, acc[q][4 * i + 2] * back, acc[q][4 * i + 3] * back);
       }
-    } else {
-      float* res = reinterpret_cast<float*>(smem + G::OFF_K);   // (the last product has been read, so the panels are free)
-      float* stats = reinterpret_cast<float*>(smem + G::OFF_STATS);
-      softmax_sync();
-      if (half == 0) stats[r] = m_run, stats[ROWS + r] = l_run;
+    if (rg.cluster == 1) softmax_sync();
+    else cluster_sync();
+    const uint32_t share = ROWS / rg.cluster, res_addr = sbase + G::OFF_K, stats_addr = sbase + G::OFF_STATS;
+    for (uint32_t i = tid; i < share; i += CW * 32) {
+      const uint32_t rr = rank * share + i;
+      float m[8], w[8], M = -INFINITY, lsum = 0.0f;
 #pragma unroll
-      for (int q = 0; q < NP; q++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const uint32_t chunk = q * 16 + half * 8 + i;
-          *reinterpret_cast<float4*>(res + r * D + ((chunk ^ (r & 7)) << 2)) = make_float4(acc[q][4 * i] * back, acc[q][4 * i + 1] * back, acc[q][4 * i + 2] * back, acc[q][4 * i + 3] * back);
+      for (int k = 0; k < 8; k++) {
+        m[k] = -INFINITY, w[k] = 0.0f;
+        if (k < (int)rg.cluster) {
+          const uint32_t a = cluster_addr(stats_addr, k);
+          m[k] = ld_cluster_f(a + 4 * rr), w[k] = ld_cluster_f(a + 4 * (ROWS + rr));
         }
-      cluster_sync();
-      const uint32_t share = ROWS / rg.cluster, res_addr = sbase + G::OFF_K, stats_addr = sbase + G::OFF_STATS;
-      for (uint32_t i = tid; i < share * (D / 4); i += CW * 32) {
-        const uint32_t rr = rank * share + i / (D / 4), d4 = i % (D / 4);
-        uint32_t l;
-        const uint32_t row = row_of(rr, &l);
-        if (row == NO_ROW) continue;
-        float m[8], w[8], M = -INFINITY, lsum = 0.0f;
-        float4 v[8], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          m[k] = -INFINITY, w[k] = 0.0f, v[k] = o;
-          if (k < (int)rg.cluster) {
-            const uint32_t a = cluster_addr(stats_addr, k);
-            m[k] = ld_cluster_f(a + 4 * rr), w[k] = ld_cluster_f(a + 4 * (ROWS + rr));
-            v[k] = ld_cluster_f4(cluster_addr(res_addr, k) + (rr * D + ((d4 ^ (rr & 7)) << 2)) * 4);
-          }
-          M = fmaxf(M, m[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const float f = m[k] == -INFINITY ? 0.0f : ex2(m[k] - M);
-          o.x += v[k].x * f, o.y += v[k].y * f, o.z += v[k].z * f, o.w += v[k].w * f;
-          lsum += w[k] * f;
-        }
-        const bool fine = lsum > 0.0f && isfinite(lsum);
-        if (!fine && d4 == 0 && report) {
-          const KeyRange kr = key_range(p, b, l);
-          if (kr.hi > kr.lo) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
-        }
-        const float inv = fine ? __frcp_rn(lsum) : 0.0f;
-        *reinterpret_cast<float4*>(p.out + (uint64_t)row * D + 4 * d4) = fine ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        M = fmaxf(M, m[k]);
       }
-      __syncwarp();
-      cluster_sync();   // no CTA leaves before the others have read its sums
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        m[k] = m[k] == -INFINITY ? 0.0f : ex2(m[k] - M);
+        lsum += w[k] * m[k];
+      }
+      const bool good = lsum > 0.0f && isfinite(lsum);
+      const float inv = good ? __frcp_rn(lsum) : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (k < (int)rg.cluster) weight[k * ROWS + i] = good ? m[k] * inv : 0.0f;
+      uint32_t l;
+      if (!good && report && row_of(rr, &l) != NO_ROW) {
+        const KeyRange kr = key_range(p, b, l);
+        if (kr.hi > kr.lo) atomicCAS(p.fault, FAULT_NONE, FAULT_NONFINITE);
+      }
     }
+    softmax_sync();
+    constexpr int LPR = D < 128 ? D / 4 : 32, VPL = D / 4 / LPR, RPI = CW * 32 / LPR, BATCH = 8 / VPL;   // lanes of a row, rows at once
+    const uint32_t d4 = lane % LPR;
+    for (uint32_t i0 = warp * (32 / LPR) + lane / LPR; i0 < share; i0 += BATCH * RPI) {
+      float4 o[BATCH][VPL];
+#pragma unroll
+      for (int j = 0; j < BATCH; j++)
+#pragma unroll
+        for (int c = 0; c < VPL; c++) o[j][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+      for (uint32_t k = 0; k < rg.cluster; k++) {
+        const uint32_t from = cluster_addr(res_addr, k);
+        float4 v[BATCH][VPL];
+#pragma unroll
+        for (int j = 0; j < BATCH; j++)
+#pragma unroll
+          for (int c = 0; c < VPL; c++) {
+            const uint32_t rr = rank * share + min(i0 + j * RPI, share - 1);
+            v[j][c] = ld_cluster_f4(from + rr * (D * 4) + (((d4 + 32 * c) ^ (rr & 7)) << 4));
+          }
+#pragma unroll
+        for (int j = 0; j < BATCH; j++) {
+          const float f = weight[k * ROWS + min(i0 + j * RPI, share - 1)];
+#pragma unroll
+          for (int c = 0; c < VPL; c++)   // (sums without weight may be anything)
+            if (f != 0.0f) o[j][c].x += v[j][c].x * f, o[j][c].y += v[j][c].y * f, o[j][c].z += v[j][c].z * f, o[j][c].w += v[j][c].w * f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < BATCH; j++) {
+        const uint32_t i = i0 + j * RPI, row = i < share ? rows[rank * share + i] : NO_ROW;
+        if (row != NO_ROW)
+#pragma unroll
+          for (int c = 0; c < VPL; c++) *reinterpret_cast<float4*>(p.out + (uint64_t)row * D + 4 * (d4 + 32 * c)) = o[j][c];
+      }
+    }
+    __syncwarp();
+    if (rg.cluster > 1) cluster_sync();   // no CTA leaves before the others have read its sums
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
     if (warp == MMA_WARP) {
@@ -714,7 +750,6 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       using UV = Unpack<D, VQ8>;
       constexpr int KPW = UK::KPW, GROUPS = UK::GROUPS;
       const uint32_t in_group = lane % KPW, panel = lane / KPW;
-      wait(q_ready, 0);   // (q passed through the panels)
       // Is the key there, and does a row of the block see it?
       auto seen = [&](uint32_t it, uint32_t key) {
         const uint2 v = valid[(it % SLOTS) * SUBS + key / TK];
@@ -766,6 +801,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       };
       auto keys = [&](uint32_t it) {
         if (it > 0) wait(k_free, it - 1);
+        else wait(q_ready, 0);   // (q passed through the panels)
         if (!dead) {
           const uint8_t* raw = smem + G::OFF_KRAW + (it % KRAWS) * G::KRAW + kshift + panel * 2 * KF::BB;
           const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + G::OFF_KSC) + (it & 1) * SK * NP + panel;
@@ -856,11 +892,11 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap&
   const uint64_t units = (uint64_t)p.B * rg.row_blocks * p.Hkv;
   // One CTA an SM. The keys are cut over as many CTAs as finish soonest in rounds of what the device holds at once
   // (clusters of eight fit only where a group of SMs has as many free), four stages each at least; a cluster's sums
-  // cost about as much as eight stages.
+  // cost less than a stage.
   rg.cluster = 1;
   double best = 1e30;
   for (uint32_t c = 1, i = 0; c <= 8 && max_keys >= (uint64_t)c * (c > 1 ? 4 : 0) * SK; c *= 2, i++) {
-    const double cost = std::ceil((double)units / held[i]) * (std::ceil((double)max_keys / (c * SK)) + 4.0 + (c > 1 ? 8.0 : 0.0));
+    const double cost = std::ceil((double)units / held[i]) * (std::ceil((double)max_keys / (c * SK)) + 4.0 + (c > 1 ? 1.0 : 0.0));
     if (cost < best) best = cost, rg.cluster = c;
   }
   if (units * rg.cluster > 0x7FFFFFFFull) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
