@@ -83,14 +83,19 @@ struct RowsGeom {
 // D f32, A and B f16, M = 128, N = 64; B K-major, or (bit 16) N-major.
 constexpr uint32_t IDESC_QK = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24), IDESC_PV = IDESC_QK | (1u << 16);
 
-// D[tmem] (+)= A[tmem] . B[smem desc]. The whole warp comes here and one elected thread, always the same, issues: so the
-// operands stay in uniform registers and an instruction is issued in the 32 clocks that it takes. (Inside a branch of one
-// thread 49 clocks each, and 102 with descriptors that a loop chooses.)
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] . B[smem desc], four steps of K = 16: A eight columns further each (the third and fourth SKIP more), B
+// STEP units of its descriptor. The whole warp comes here and one elected thread, always the same, issues: so the operands stay
+// in uniform registers and an instruction is issued in the 32 clocks that it takes. (Inside a branch of one thread 49 clocks each.)
+template <int SKIP, int STEP>
+__device__ __forceinline__ void umma_f16_ts4(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\telect.sync _|e, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, %5;\n\tadd.u32 a3, %1, %6;\n\tadd.u64 b1, %2, %7;\n\tadd.u64 b2, %2, %8;\n\tadd.u64 b3, %2, %9;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(16 + SKIP), "n"(24 + SKIP), "n"(STEP), "n"(2 * STEP), "n"(3 * STEP)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit_elected(uint32_t bar) {
@@ -176,19 +181,22 @@ struct Unpack {
     const float up = pow2f(22 - (int)e);
     return pack_half2(half_bits(sc[0]) * up, half_bits(sc[1]) * up);
   }
-  // One block of a key: 32 codes times its (normed) scale, as two f16 terms.
-  template <int PAR>
-  static __device__ __forceinline__ void block(const uint8_t* row, uint32_t pair, uint8_t* hi, uint8_t* lo, uint32_t key) {
-    const uint32_t s2 = __byte_perm(pair, 0, PAR ? 0x3232 : 0x1010);
-    constexpr int CODES = Q8 ? 8 : 4, FIRST = Q8 ? 8 : 4;   // words of codes; the word that holds the second block's scale
+  // One block of a key (the panel's first or second): 32 codes times its (normed) scale, as two f16 terms. `row` is where the
+  // panel's bytes begin. (One code for both: the loop's instructions have to stay in the cache, see the kernel.)
+  static __device__ __forceinline__ void block(const uint8_t* row, uint32_t second, uint32_t pair, uint8_t* hi, uint8_t* lo, uint32_t key) {
+    const uint32_t s2 = __byte_perm(pair, 0, second ? 0x3232 : 0x1010);
+    constexpr int CODES = Q8 ? 8 : 4;   // words of codes; the second block's begin in the middle of the word before
     uint32_t w[CODES];
     {
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(row) + (second ? CODES : 0);
+      const uint32_t sel = second ? 0x7654 : 0x5432;
       uint32_t raw[CODES + 1];
 #pragma unroll
-      for (int i = 0; i <= CODES; i++) raw[i] = *reinterpret_cast<const uint32_t*>(row + 4 * (i + PAR * FIRST));
+      for (int i = 0; i <= CODES; i++) raw[i] = words[i];
 #pragma unroll
-      for (int i = 0; i < CODES; i++) w[i] = PAR ? raw[i + 1] : __byte_perm(raw[i], raw[i + 1], 0x5432);
+      for (int i = 0; i < CODES; i++) w[i] = __byte_perm(raw[i], raw[i + 1], sel);
     }
+    const uint32_t first = (second * 4) ^ (key & 7);
     auto store = [&](int c, const uint32_t (&u)[4]) {   // eight dimensions
       uint32_t h[4], l[4];
 #pragma unroll
@@ -196,7 +204,7 @@ struct Unpack {
         h[i] = h2_mul(u[i], s2);
         l[i] = h2_rest(u[i], s2, h[i]);   // exact: what the rounding left
       }
-      const uint32_t at = key * 128 + (((PAR * 4 + c) ^ (key & 7)) << 4);
+      const uint32_t at = key * 128 + ((first ^ c) << 4);
       *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
       *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
     };
@@ -643,14 +651,13 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         tc_fence_after();
         {
           const uint32_t d = t0 + G::T_S + (it & 1) * 64, qh = t0 + G::T_Q, ql = qh + D / 2;
-          // (Panels in a loop: spelled out, their descriptors are all kept, most of them in local memory.)
-          auto product = [&](uint32_t a, uint64_t bd, uint32_t more) {
 #pragma unroll 1
-            for (int q = 0; q < NP; q++)
-#pragma unroll
-              for (int ks = 0; ks < 4; ks++) umma_f16_ts(d, a + 32 * q + 8 * ks, bd + q * (PANEL >> 4) + 2 * ks, IDESC_QK, more | (uint32_t)(q + ks));
-          };
-          product(ql, kh, 0), product(qh, kl, 1), product(qh, kh, 1);
+          for (int j = 0; j < 3; j++) {   // lo.hi, hi.lo, hi.hi
+            const uint32_t a = j == 0 ? ql : qh;
+            const uint64_t bd = j == 1 ? kl : kh;
+#pragma unroll 1
+            for (int q = 0; q < NP; q++) umma_f16_ts4<0, 2>(d, a + 32 * q, bd + q * (PANEL >> 4), IDESC_QK, j | q);
+          }
           umma_commit_elected(s_full + 8 * (it & 1));
           umma_commit_elected(k_free);
         }
@@ -666,11 +673,9 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           tc_fence_after();
           {
             const uint32_t d = t0 + G::T_O + (n & 1) * 64, ph = t0 + G::T_S + (it & 1) * 64;
-#pragma unroll
-            for (int j = 0; j < 3; j++)
-#pragma unroll
-              for (int ks = 0; ks < SK / 16; ks++)   // 16 keys: eight columns of P, two groups of eight rows of V
-                umma_f16_ts(d, ph + (ks >> 1) * 32 + (ks & 1) * 8 + (j == 0 ? 16 : 0), (j == 1 ? vl : vh) + q * (PANEL >> 4) + ks * (2048 >> 4), IDESC_PV, j > 0 || ks > 0);
+#pragma unroll 1
+            for (int j = 0; j < 3; j++)   // 16 keys: eight columns of P, two groups of eight rows of V
+              umma_f16_ts4<16, (2048 >> 4)>(d, ph + (j == 0 ? 16 : 0), (j == 1 ? vl : vh) + q * (PANEL >> 4), IDESC_PV, j);
             umma_commit_elected(o_full + 8 * (n & 1));
             if (q == NP - 1) umma_commit_elected(v_free);
           }
@@ -767,7 +772,6 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
             *reinterpret_cast<uint32_t*>(smem + G::OFF_KSC + ((it & 1) * SK * NP + key * NP + panel) * 4) = UK::normed(sc, e);
             if (panel == 0) *reinterpret_cast<float*>(smem + G::OFF_KEXP + ((it % SLOTS) * SK + key) * 4) = pow2f((int)e - 22);
           }
-        unpack_sync();   // (every warp comes here, also one that has given up)
       };
       auto value_scales = [&](uint32_t it) {
         wait(vraw_full + 8 * (it % VRAWS), it / VRAWS);
@@ -799,50 +803,37 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         }
         arrive(scaled + 8 * (it % SLOTS));
       };
-      auto keys = [&](uint32_t it) {
-        if (it > 0) wait(k_free, it - 1);
-        else wait(q_ready, 0);   // (q passed through the panels)
-        if (!dead) {
-          const uint8_t* raw = smem + G::OFF_KRAW + (it % KRAWS) * G::KRAW + kshift + panel * 2 * KF::BB;
-          const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + G::OFF_KSC) + (it & 1) * SK * NP + panel;
-          uint8_t* kh = smem + G::OFF_K + panel * PANEL;
-#pragma unroll 1
-          for (uint32_t u = uw; u < 2 * GROUPS; u += UW) {
-            const uint32_t key = (u >> 1) * KPW + in_group;
-            if (u & 1) UK::template block<1>(raw + key * KF::PITCH, sc[key * NP], kh, kh + NP * PANEL, key);
-            else UK::template block<0>(raw + key * KF::PITCH, sc[key * NP], kh, kh + NP * PANEL, key);
-          }
-          ptx::fence_proxy_async();
-        }
-        arrive(k_ready);
-        arrive(kraw_empty + 8 * (it % KRAWS));
-      };
-      auto values = [&](uint32_t it) {
-        if (it > 0) wait(v_free, it - 1);
-        if (!dead) {
-          const uint8_t* raw = smem + G::OFF_VRAW + (it % VRAWS) * G::VRAW + vshift + panel * 2 * VF::BB;
-          const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + G::OFF_VSC) + (it % 3) * SK * NP + panel;
-          uint8_t* vh = smem + G::OFF_V + panel * PANEL;
-#pragma unroll 1
-          for (uint32_t u = uw; u < 2 * GROUPS; u += UW) {
-            const uint32_t key = (u >> 1) * KPW + in_group;
-            if (u & 1) UV::template block<1>(raw + key * VF::PITCH, sc[key * NP], vh, vh + NP * PANEL, key);
-            else UV::template block<0>(raw + key * VF::PITCH, sc[key * NP], vh, vh + NP * PANEL, key);
-          }
-          ptx::fence_proxy_async();
-        }
-        arrive(p_ready + 8 * (it & 1));
-        arrive(vraw_empty + 8 * (it % VRAWS));
-      };
       for (uint32_t it = 0; it <= stages; it++) {
-        if (it < stages) {
-          key_scales(it);
-          keys(it);
-          value_scales(it);
-        } else {
-          unpack_sync();
+#pragma unroll 1
+        for (uint32_t v = 0; v < 2; v++) {   // K of this stage, V of the one before
+          const uint32_t st = it - v;
+          if (v == 0) {
+            if (it < stages) key_scales(it);
+            unpack_sync();   // (every warp comes here, also one that has given up)
+            if (it == stages) continue;
+            if (it == 0) wait(q_ready, 0);   // (q passed through the panels)
+          } else {
+            if (it < stages) value_scales(it);
+            if (it == 0) break;
+          }
+          if (st > 0) wait(v ? v_free : k_free, st - 1);
+          if (!dead) {
+            const uint8_t* raw = smem + (v ? G::OFF_VRAW + (st % VRAWS) * G::VRAW + vshift + panel * 2 * VF::BB
+                                           : G::OFF_KRAW + (st % KRAWS) * G::KRAW + kshift + panel * 2 * KF::BB);
+            const uint32_t* sc = reinterpret_cast<const uint32_t*>(smem + (v ? G::OFF_VSC : G::OFF_KSC)) + (v ? st % 3 : st & 1) * SK * NP + panel;
+            uint8_t* hi = smem + (v ? G::OFF_V : G::OFF_K) + panel * PANEL;
+            const uint32_t pitch = v ? VF::PITCH : KF::PITCH;
+#pragma unroll 1
+            for (uint32_t u = uw; u < 2 * GROUPS; u += UW) {
+              const uint32_t key = (u >> 1) * KPW + in_group;
+              if (KQ8 == VQ8 || v == 0) UK::block(raw + key * pitch, u & 1, sc[key * NP], hi, hi + NP * PANEL, key);
+              else UV::block(raw + key * pitch, u & 1, sc[key * NP], hi, hi + NP * PANEL, key);
+            }
+            ptx::fence_proxy_async();
+          }
+          arrive(v ? p_ready + 8 * (st & 1) : k_ready);
+          arrive(v ? vraw_empty + 8 * (st % VRAWS) : kraw_empty + 8 * (st % KRAWS));
         }
-        if (it > 0) values(it - 1);
       }
     }
     if (rg.cluster > 1) {
