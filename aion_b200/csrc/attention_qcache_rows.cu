@@ -311,14 +311,14 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   const uint32_t my_first = (uint32_t)min((uint64_t)whole.end, whole.first + (uint64_t)rank * per);
   const uint32_t tiles = min(whole.end - my_first, per), stages = (tiles + SUBS - 1) / SUBS;
 
-  // A wait that runs out is reported; the warp then walks on without waiting or working, so that every arrival still comes and
+  // A wait that runs out is reported at the end; the warp then walks on without waiting or working, so that every arrival still comes and
   // no warp is left at a barrier of a pair.
   bool dead = false;
   auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (!dead && !__all_sync(FULL, ptx::mbar_try_wait_spin(bar, parity & 1) || ptx::mbar_wait_bounded(bar, parity & 1, p.wait_limit))) {
-      dead = true;
-      if (lane == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED), flags[1] = 1;
-    }
+    for (uint32_t i = 0; !dead && !__all_sync(FULL, ptx::mbar_try_wait_spin(bar, parity & 1)); i++) dead = (i >> 4) >= p.wait_limit;   // (short polls)
+  };
+  auto report_wait = [&]() {
+    if (dead && lane == 0) atomicExch(p.fault, FAULT_WAIT_EXPIRED), flags[1] = 1;
   };
   auto arrive = [&](uint32_t bar) {
     __syncwarp();
@@ -551,6 +551,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
 
     // ---- the rows' sums, through shared memory: a row is written whole, and a cluster's CTAs add up theirs, each for its share
     // of the rows
+    report_wait();
     pair_sync(quarter);
     ex[half * ROWS + r] = l_run;
     pair_sync(quarter);
@@ -681,6 +682,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           }
         }
       }
+      report_wait();
       umma_commit_elected(done);
       ptx::mbar_wait_bounded(done, 0, p.wait_limit);
       __syncwarp();
@@ -835,6 +837,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           arrive(v ? vraw_empty + 8 * (st % VRAWS) : kraw_empty + 8 * (st % KRAWS));
         }
       }
+      report_wait();
     }
     if (rg.cluster > 1) {
       __syncwarp();
