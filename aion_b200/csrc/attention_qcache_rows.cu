@@ -229,7 +229,7 @@ struct Unpack {
   }
 };
 
-template <int D, bool KQ8, bool VQ8>
+template <int D, bool KQ8, bool VQ8, bool CAP>
 __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const AttnParams p, const RowsGrid rg, const __grid_constant__ CUtensorMap tmap_k,
                                                                       const __grid_constant__ CUtensorMap tmap_v) {
   using G = RowsGeom<D, KQ8, VQ8>;
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
       if (e == 255) e = 127;
       e = max(e, 40u);
       const float up = __uint_as_float((127u + 13u + 127u - e) << 23);
-      factor = p.scale * __uint_as_float((e - 13u) << 23) * (p.soft_cap > 0.0f ? 1.0f : LOG2E);
+      factor = p.scale * __uint_as_float((e - 13u) << 23) * (CAP ? 1.0f : LOG2E);
       const uint32_t tq = tmem + ((uint32_t)quarter << 21) + G::T_Q + half * (D / 4);
 #pragma unroll 1
       for (int c = 0; c < D / 64; c++) {   // 32 dimensions
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         }
         const float4* kexp = reinterpret_cast<const float4*>(smem + G::OFF_KEXP + (slot * SK + half * 32) * 4);
         tmem_ld_wait();
-        if (p.soft_cap > 0.0f) {
+        if (CAP) {
 #pragma unroll
           for (int i = 0; i < 8; i++) {
             const float4 k = kexp[i];
@@ -849,10 +849,10 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-template <int D, bool KQ8, bool VQ8>
+template <int D, bool KQ8, bool VQ8, bool CAP>
 int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, uint64_t max_keys) {
   using G = RowsGeom<D, KQ8, VQ8>;
-  auto kernel = attn_qcache_rows_kernel<D, KQ8, VQ8>;
+  auto kernel = attn_qcache_rows_kernel<D, KQ8, VQ8, CAP>;
   // Clusters of 1, 2, 4 and 8 CTAs that the device holds at once; worked out once per device and instantiation.
   uint32_t held[4];
   {
@@ -915,15 +915,20 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap&
 
 int32_t attention_qcache_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, uint64_t max_keys) {
   const bool kq8 = p.k_dtype == AION_CUDA_DTYPE_Q8_0, vq8 = p.v_dtype == AION_CUDA_DTYPE_Q8_0;
-#define AION_QROWS(D)                                                                                                                  \
-  if (kq8) return vq8 ? launch_rows<D, true, true>(dev, p, tk, tv, max_keys) : launch_rows<D, true, false>(dev, p, tk, tv, max_keys); \
-  return vq8 ? launch_rows<D, false, true>(dev, p, tk, tv, max_keys) : launch_rows<D, false, false>(dev, p, tk, tv, max_keys);
+  // (A soft cap in a kernel of its own: its instructions in the loop cost the others 20 us of 177.)
+#define AION_QROWS_AS(D, K, V) return p.soft_cap > 0.0f ? launch_rows<D, K, V, true>(dev, p, tk, tv, max_keys) : launch_rows<D, K, V, false>(dev, p, tk, tv, max_keys);
+#define AION_QROWS(D)                                          \
+  if (kq8 && vq8) AION_QROWS_AS(D, true, true)                 \
+  if (kq8) AION_QROWS_AS(D, true, false)                       \
+  if (vq8) AION_QROWS_AS(D, false, true)                       \
+  AION_QROWS_AS(D, false, false)
   switch (p.Dk) {
     case 64: AION_QROWS(64)
     case 128: AION_QROWS(128)
     default: AION_QROWS(256)
   }
 #undef AION_QROWS
+#undef AION_QROWS_AS
 }
 
 }  // namespace aion
