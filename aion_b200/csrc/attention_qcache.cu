@@ -1007,17 +1007,18 @@ int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p, uint32_t fla
     const uint64_t span = (uint64_t)(p.win_chunk ? p.win_chunk : 1) + p.win_left + p.win_right + p.pos_per_tile;
     if (p.win_left != AION_CUDA_WINDOW_UNBOUNDED && p.win_right != AION_CUDA_WINDOW_UNBOUNDED && span < max_keys) max_keys = span;
     // Few columns at a time or 128 rows: by what each would cost. A unit of eight columns passes a key in 16, 24 or 31 ns
-    // (D = 64, 128, 256) with all resident CTAs at work, after 8 us; a unit of 128 rows in 48, 66 or 160 ns, after 15 us.
-    // (8 heads over 4 kv heads of 256: 256 rows of one request over 2048 keys 73 us by columns, 132 us by rows; of eight
-    // requests over 4096 keys 885 and 624 us. 16 over 4 of 64: 61 and 40, 614 and 395 us.)
+    // (D = 64, 128, 256) with all resident CTAs at work, after 8 us; a unit of 128 rows in 25, 34 or 51 ns, after 8, 10 or
+    // 15 us and 1.1 us for each CTA of a cluster. (8 heads over 4 kv heads of 256: 32 positions of one request over 2048 keys
+    // 17 us by columns, 40 us by rows; of eight requests over 4096 keys 129 and 72 us, 256 positions 839 and 231 us. 16 over 4
+    // of 64: 16 and 23, 112 and 40, 617 and 233 us.)
     const int size = p.Dk == 64 ? 0 : p.Dk == 128 ? 1 : 2;
-    constexpr double column_ns[3] = {16.0, 24.0, 31.0}, row_ns[3] = {48.0, 66.0, 160.0};
+    constexpr double column_ns[3] = {16.0, 24.0, 31.0}, row_ns[3] = {25.0, 34.0, 51.0}, row_start[3] = {8.0, 10.0, 15.0};
     const double sms = (double)dev->sm_count, keys = (double)max_keys;
     const double columns_us = 8.0 + 1e-3 * column_ns[size] * keys * std::max(1.0 / 8.0, (double)units / (sms * (p.Dk == 256 ? 2.0 : 3.0)));
     const uint64_t blocks = (uint64_t)p.B * p.Hkv * (((uint64_t)p.L * group + 127) / 128);
     double rows_us = 1e30;
     for (uint64_t cluster = 1; cluster <= 8; cluster *= 2)
-      rows_us = std::min(rows_us, 15.0 + 1e-3 * row_ns[size] * keys / (double)cluster * std::ceil((double)(blocks * cluster) / (sms * (cluster > 2 ? 0.85 : 1.0))));
+      rows_us = std::min(rows_us, row_start[size] + (cluster > 1 ? 1.1 * (double)cluster : 0.0) + 1e-3 * row_ns[size] * keys / (double)cluster * std::ceil((double)(blocks * cluster) / (sms * (cluster > 2 ? 0.85 : 1.0))));
     const bool rows_kernel = !p.image && p.L > 1 && !(flags & AION_CUDA_ATTENTION_ROW_UNITS) && ((flags & AION_CUDA_ATTENTION_BLOCKS) || rows_us < columns_us);
 #define AION_QCACHE(D)                                                                                     \
   if (kq8) return vq8 ? launch_decode<D, true, true>(dev, p, max_keys, rows_kernel) : launch_decode<D, true, false>(dev, p, max_keys, rows_kernel); \

@@ -17,6 +17,13 @@
 //    P . V, so that the softmax runs under it.
 //  * A context too long for the few CTAs of a short prompt is cut over a cluster, whose CTAs add up their sums through
 //    distributed shared memory.
+//
+// 1024 rows against 8192 keys, 8 heads over 4 kv heads of 256, q8_0: 222 us, 289 TFLOP/s of the 4 * rows * keys * D that attention
+// counts (the products alone would take 103 us of a loop of 207); a causal prompt of 4096 tokens 217 us, 316 TFLOP/s; 32 over 8
+// heads of 128 538 us, 239 TFLOP/s. (On m16n8k16, eight warps of sixteen rows that held all in registers: 616, 596 and 1129 us.)
+// What bounds it: the hand-overs between the roles of a stage, and how fast instructions come. The loop is straight code of four
+// kinds, more than the cache of an SM holds when written without care: spelled-out products (their descriptors went to local
+// memory), waits with a report in each, a copy of the unpacking per block and operand cost 378 us against these 222.
 #include <cmath>
 #include <cstdlib>
 #include <mutex>
@@ -39,8 +46,10 @@ constexpr int SUBS = 4;               // tiles of a stage
 constexpr int SK = SUBS * TK;         // keys of a stage
 constexpr int KRAWS = 3, VRAWS = 2;   // raw stages
 constexpr int SLOTS = 4;              // stages whose exponents and masks are kept
-constexpr int SOFTMAX_REGS = 200, OTHER_REGS = 56;
-static_assert((SOFTMAX_REGS + OTHER_REGS) * (RTHREADS / 2) <= 128 * RTHREADS, "the registers that the block is launched with");
+// Registers of a softmax warp's thread and of the others'; they add up to what the block is launched with, 128 each. (Heads of
+// 256, whose sums alone take 128: 221 us, with 192 and 64 226; heads of 128: 157 and 152 us.)
+constexpr int softmax_regs(int d) { return d == 256 ? 200 : 192; }
+constexpr int other_regs(int d) { return 256 - softmax_regs(d); }
 static_assert(SK == 64 && FIRST_UNPACK + UW == RTHREADS / 32, "a stage is one panel of 64 keys");
 constexpr int PANEL = SK * 128;       // bytes of 64 keys x 64 dimensions of f16
 
@@ -326,7 +335,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   };
 
   if (softmax) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(softmax_regs(D)));
     float factor;
     // ---- q into tensor memory: rows whole through shared memory, then normed by their largest value to [2^13, 2^14) and split
     {
@@ -640,7 +649,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
     __syncwarp();
     if (rg.cluster > 1) cluster_sync();   // no CTA leaves before the others have read its sums
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(other_regs(D)));
     if (warp == MMA_WARP) {
       // ================ the products ================
       wait(q_ready, 0);
@@ -886,11 +895,11 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap&
   const uint64_t units = (uint64_t)p.B * rg.row_blocks * p.Hkv;
   // One CTA an SM. The keys are cut over as many CTAs as finish soonest in rounds of what the device holds at once
   // (clusters of eight fit only where a group of SMs has as many free), four stages each at least; a cluster's sums
-  // cost less than a stage.
+  // cost a third of a stage for each of them.
   rg.cluster = 1;
   double best = 1e30;
   for (uint32_t c = 1, i = 0; c <= 8 && max_keys >= (uint64_t)c * (c > 1 ? 4 : 0) * SK; c *= 2, i++) {
-    const double cost = std::ceil((double)units / held[i]) * (std::ceil((double)max_keys / (c * SK)) + 4.0 + (c > 1 ? 1.0 : 0.0));
+    const double cost = std::ceil((double)units / held[i]) * (std::ceil((double)max_keys / (c * SK)) + 4.0 + (c > 1 ? 0.35 * c : 0.0));
     if (cost < best) best = cost, rg.cluster = c;
   }
   if (units * rg.cluster > 0x7FFFFFFFull) return fail(AION_CUDA_UNSUPPORTED, "attention: too many rows");
