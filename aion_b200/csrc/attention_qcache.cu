@@ -141,7 +141,8 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
 //  * S^T[16 keys x 8] = C . Q^T on f16 m16n8k16: the codes are exact in f16, q is two f16 terms (22 bits, normed
 //    by the column's largest value), and the products of one block of 32 dimensions are scaled by the block's
 //    scale in f32. q4_0 codes enter as the subnormals n * 2^-24 that a nibble IS in the low bits of an f16 (one
-//    AND per two codes); their offset of 8 is the accumulator's initial value, -8 sum q.
+//    AND per two codes); their offset of 8, -8 sum q, is added in f32 behind the products (as the accumulator's initial
+//    value it made every one of them lose the low bits that its size cuts off: twice the error of the outputs).
 //  * The logits are transposed by movmatrix (two 16-bit halves each), so a lane holds one column's logits of the
 //    keys that it needs as the B operand of the second product.
 //  * O^T[D x 8] += V-codes^T . P'^T, P' = p * scale of (key, block) in f32, again two f16 terms. P' is scaled by
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   for (int j = 0; j < (NB + WARPS - 1) / WARPS; j++) {
     const int blk = warp + j * WARPS;
     if (blk < NB) {
-      float part = 0.0f;
+      double part = 0.0;   // (eight times its error comes on every logit: not in f32)
 #pragma unroll
       for (int m = 0; m < 2; m++) {
         uint32_t hl[2][2];
@@ -480,7 +481,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
           split2(x[0], x[1], &hl[0][r], &hl[1][r]);
           if (!KQ8) {
             const float2 a = __half22float2(*reinterpret_cast<__half2*>(&hl[0][r])), c = __half22float2(*reinterpret_cast<__half2*>(&hl[1][r]));
-            part += ((a.x + c.x) + (a.y + c.y)) * (r ? 16.0f : 1.0f);
+            part += (((double)a.x + (double)c.x) + ((double)a.y + (double)c.y)) * (r ? 16.0 : 1.0);
           }
         }
         made[j][m] = make_uint4(hl[0][0], hl[0][1], hl[1][0], hl[1][1]);
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
       if (!KQ8) {
         part += __shfl_xor_sync(FULL, part, 1);
         part += __shfl_xor_sync(FULL, part, 2);
-        if (t == 0) ci[blk * 2 * COLS + g / 2 * 4 + g % 2] = ci[blk * 2 * COLS + g / 2 * 4 + g % 2 + 2] = part * (-8.0f * 5.9604644775390625e-8f);   // -8 * 2^-24
+        if (t == 0) ci[blk * 2 * COLS + g / 2 * 4 + g % 2] = ci[blk * 2 * COLS + g / 2 * 4 + g % 2 + 2] = (float)(part * (-8.0 * 5.9604644775390625e-8));   // -8 * 2^-24
       }
     }
   }
@@ -624,10 +625,11 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
         for (int k = 0; k < 2; k++) {
           const int q = 2 * k;
           float c[4];
-          mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], ql[q][0], ql[q][1], init[k].x, init[k].y, init[k].z, init[k].w);
+          mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], ql[q][0], ql[q][1], 0.0f, 0.0f, 0.0f, 0.0f);
           mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], ql[q + 1][0], ql[q + 1][1], c[0], c[1], c[2], c[3]);
           mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], qh[q][0], qh[q][1], c[0], c[1], c[2], c[3]);
           mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], qh[q + 1][0], qh[q + 1][1], c[0], c[1], c[2], c[3]);
+          if (!KQ8) add2(c[0], c[1], init[k].x, init[k].y), add2(c[2], c[3], init[k].z, init[k].w);
           s[j][0] = fmaf(sl[k], c[0], s[j][0]);
           s[j][1] = fmaf(sl[k], c[1], s[j][1]);
           s[j][2] = fmaf(sh[k], c[2], s[j][2]);

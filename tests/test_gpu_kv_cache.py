@@ -845,6 +845,42 @@ def test_tiny_rings_and_steps_near_the_last(sess, T, L, first):
         check(got, *ref.attention(q, k, v, Q8, Q4, scale=0.1, positions=pos, lengths=lens, rolling=True))
 
 
+@pytest.mark.parametrize("D,kdt,vdt", [(64, Q8, Q4), (128, Q4, Q4), (128, Q8, Q8), (256, Q4, Q8), (256, Q8, Q8)])
+@pytest.mark.parametrize("layout,page", [("plain", 0), ("paged", 40), ("rolling", 0)])
+def test_rows_kernel_over_many_stages(sess, D, kdt, vdt, layout, page):
+    """As many units as SMs, so that a CTA walks a whole context of eleven stages alone: every ring of stages comes round."""
+    B, T, H, L = 20, 700, 8, 2
+    q, k, v = inputs([D, kdt, 5], B, T, H, D, L, H, kdt, vdt)
+    lens = [T - 31 * b for b in range(B)]
+    if layout == "rolling":
+        lens = [n + 500 for n in lens]
+    pos = np.array([[n - L + i for i in range(L)] for n in lens], dtype=np.int32)
+    got, _ = run_attention(sess, q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, layout=layout, page=page,
+                           window=AttentionWindow.causal(), flags=capi.ATTENTION_BLOCKS)
+    check(got, *ref.attention(q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, rolling=layout == "rolling"))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_scales_of_zero_and_below_are_refused(sess, scale):
+    q, k, v = inputs([11], 2, 150, 1, 128, 3, 4, Q8, Q4)
+    with pytest.raises(BackendError) as e:
+        run_attention(sess, q, k, v, Q8, Q4, scale=scale)
+    assert e.value.name == "InvalidArgument"
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 65504.0])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_what_a_row_of_a_block_does_not_see_does_not_reach_it(sess, bad, D):
+    """The rows kernel: a K row of NaN, infinite or huge scales leaves the rows before it (causal) as they are."""
+    B, T, H, L = 1, 90, 1, 12
+    q, k, v = inputs([3], B, T, H, D, L, 8, Q8, Q8)
+    pos = np.arange(70, 70 + L, dtype=np.int32)[None]
+    want, bound = ref.attention(q, k, v, Q8, Q8, scale=0.1, positions=pos, lengths=[T])
+    k.reshape(B, T, H, D // 32, 34)[0, 76, :, :, :2] = np.frombuffer(np.float16(bad).tobytes(), np.uint8)
+    got, _ = run_attention(sess_quiet(sess), q, k, v, Q8, Q8, scale=0.1, positions=pos, lengths=[T], window=AttentionWindow.causal(), flags=capi.ATTENTION_BLOCKS)
+    check(got[:, :6], want[:, :6], bound[:, :6])
+
+
 def test_two_devices_of_one_gpu_at_once(sess, backend):
     """Two device objects, each with its stream and scratch, issue attention and appends in turn without waiting: both get what
     each gets alone."""
