@@ -908,6 +908,8 @@ class CudaSession:
                                     ld_qkv=xm.row_stride, t_cap=T, eps=s.eps, base_frequency=s.base_frequency,
                                     scale_factor=s.scale_factor, proportion=s.rope_proportion, k_dtype=km.dtype, v_dtype=vm.dtype,
                                     rolling=self._policy(s.k_cache, what), **ops, **paging)
+        if self._policy(s.v_cache, what) != rec.rolling:
+            raise BackendError(capi.INVALID_ARGUMENT, f"{what}: one of the caches is a ring, the other is not")
         _check(self._lib.aion_cuda_qk_norm_rope_append(self.backend._h, C.byref(rec)))
 
     def _gather_rows(self, s: StepGatherRows) -> None:

@@ -702,6 +702,9 @@ int32_t aion_cuda_sequence_read(AionCudaDevice* dev, const AionCudaSequenceRead*
   const uintptr_t cache_align = s->dtype == AION_CUDA_DTYPE_F32 ? 3 : 1;
   if ((reinterpret_cast<uintptr_t>(cache) & cache_align) || (reinterpret_cast<uintptr_t>(out) & (ob - 1)))
     return fail(AION_CUDA_INVALID_ARGUMENT, "%s: misaligned operand", what);
+  const uint64_t out_bytes = s->batch * s->out_len * row_values * ob, all_bytes = cache_bytes(s->dtype, rows * row_values);
+  if (reinterpret_cast<uintptr_t>(out) < reinterpret_cast<uintptr_t>(cache) + all_bytes && reinterpret_cast<uintptr_t>(cache) < reinterpret_cast<uintptr_t>(out) + out_bytes)
+    return fail(AION_CUDA_INVALID_ARGUMENT, "%s: out overlaps the cache", what);
   if (ob == 4) return launch_read(dev, s, reinterpret_cast<float*>(out), cache, start, lengths, g);
   return launch_read(dev, s, reinterpret_cast<__half*>(out), cache, start, lengths, g);
 }
@@ -749,6 +752,14 @@ int32_t aion_cuda_qk_norm_rope_append(AionCudaDevice* dev, const AionCudaQKNormR
                          reinterpret_cast<uintptr_t>(p.k_gamma);
   if ((f32s & 3) || ((reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache)) & 1))
     return fail(AION_CUDA_INVALID_ARGUMENT, "%s: misaligned operand", what);
+  // What one warp writes no other may read or write: K and V are two caches, q_out is not the projection.
+  auto overlap = [](const void* a, uint64_t na, const void* b, uint64_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + nb && y < x + na;
+  };
+  if (overlap(p.k_cache, cache_bytes(s->k_dtype, cache_rows * row_values), p.v_cache, cache_bytes(s->v_dtype, cache_rows * row_values)) ||
+      overlap(p.q_out, rows * s->h_q * d * sizeof(float), p.qkv, ((rows - 1) * ld + width) * sizeof(float)))
+    return fail(AION_CUDA_INVALID_ARGUMENT, "%s: operands overlap", what);
   p.len = (uint32_t)s->len, p.h_q = (uint32_t)s->h_q, p.h_kv = (uint32_t)s->h_kv, p.d = (uint32_t)d;
   p.ld = ld;
   p.rope_pairs = pf > (float)(d / 2) ? (uint32_t)(d / 2) : (uint32_t)pf;

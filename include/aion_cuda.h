@@ -522,9 +522,9 @@ AION_CUDA_API int32_t aion_cuda_rope_kv_append(AionCudaDevice* dev, const AionCu
  *   v_dtype, each f16, q8_0 or q4_0: rows end_index[b] + l receive RoPE(norm(k)) and v.
  * Range rules, rolling and pages as in aion_cuda_sequence_append, except that q_out is written
  * for every row. A head whose mean square is not finite is reported by the next aion_cuda_sync /
- * aion_cuda_d2h (nothing of that head is written). q_out must not overlap qkv. Of more new rows
- * than a ring holds, the last t_cap stay. head_dim even, at most 1024, a multiple of 32 for a
- * quantized cache.
+ * aion_cuda_d2h (nothing of that head is written). q_out must not overlap qkv, nor k_cache
+ * v_cache. Of more new rows than a ring holds, the last t_cap stay. head_dim even, at most 1024,
+ * a multiple of 32 for a quantized cache.
  * Results equal RMSNorm, RoPE1D, Cast and SequenceAppend in sequence, up to the norm's statistic. */
 typedef struct AionCudaQKNormRopeAppend AionCudaQKNormRopeAppend;
 struct AionCudaQKNormRopeAppend {

@@ -860,6 +860,23 @@ def test_rows_kernel_over_many_stages(sess, D, kdt, vdt, layout, page):
     check(got, *ref.attention(q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, rolling=layout == "rolling"))
 
 
+def test_operands_that_overlap_are_refused(sess):
+    """One cache for K and V, an output inside what is read."""
+    s, store = sess
+    cache, other = (put_cache(store, np.zeros((1, 8, 1, 2 * 34), np.uint8), Q8, 64) for _ in range(2))
+    big = store.add(TensorMeta(F32, (1, 8, 1, 64)))
+    qkv = put(store, np.zeros((1, 1, 192), np.float32), F32)
+    q, pos, end = store.add(TensorMeta(F32, (1, 1, 1, 64))), put(store, np.zeros((1, 1), np.int32), I32), put(store, np.zeros(1, np.int32), I32)
+    bind = lambda tid, meta: store.bind(meta, store.acquire_const(tid))
+    rope = dict(q_out=q, qkv=qkv, positions=pos, end_index=end, k_cache=cache, v_cache=other, base_frequency=1e4)
+    s.execute([StepQKNormRopeAppend(**rope)])
+    for step in (StepQKNormRopeAppend(**{**rope, "v_cache": cache}), StepQKNormRopeAppend(**{**rope, "q_out": bind(qkv, TensorMeta(F32, (1, 1, 1, 64)))}),
+                 StepSequenceRead(out=big, cache=bind(big, TensorMeta(Q8, (1, 8, 1, 64), quant_axis=3)))):
+        with pytest.raises(BackendError) as e:
+            s.execute([step])
+        assert e.value.name == "InvalidArgument"
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1])
 def test_scales_of_zero_and_below_are_refused(sess, scale):
     q, k, v = inputs([11], 2, 150, 1, 128, 3, 4, Q8, Q4)

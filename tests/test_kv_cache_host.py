@@ -162,13 +162,13 @@ def test_session_refuses_reads_and_fused_appends():
     s, t = _session(cache=_cache(), bad_axis=_cache(axis=1), out=TensorMeta(F32, (2, 5, 2, 64)), wide=TensorMeta(F32, (2, 5, 3, 64)),
                     index=TensorMeta(I32, (2,)), index3=TensorMeta(I32, (3,)), table=TensorMeta(I32, (3, 4)), q=TensorMeta(F32, (2, 1, 4, 64)),
                     qkv=TensorMeta(F32, (2, 1, 8 * 64)), short=TensorMeta(F32, (2, 1, 7 * 64)), pos=TensorMeta(I32, (2, 1)),
-                    gamma=TensorMeta(F32, (64,)), gamma32=TensorMeta(F32, (32,)), half=TensorMeta(F16, (2, 64, 2, 32)))
+                    gamma=TensorMeta(F32, (64,)), gamma32=TensorMeta(F32, (32,)), half=TensorMeta(F16, (2, 64, 2, 32)), ring=_cache(policy="rolling"))
     read = lambda **kw: StepSequenceRead(**{**dict(out=t["out"], cache=t["cache"]), **kw})
     rope = lambda **kw: StepQKNormRopeAppend(**{**dict(q_out=t["q"], qkv=t["qkv"], positions=t["pos"], end_index=t["index"], k_cache=t["cache"],
                                                        v_cache=t["cache"], base_frequency=1e4, q_gamma=t["gamma"]), **kw})
     attn = lambda **kw: StepAttention(**{**dict(out=t["q"], q=t["q"], k=t["cache"], v=t["cache"]), **kw})
     for step in (read(cache=t["bad_axis"]), read(out=t["wide"]), read(start_index=t["index3"]), read(lengths=t["gamma"]), read(page_table=t["table"]),
-                 rope(k_cache=t["bad_axis"]), rope(qkv=t["short"]), rope(q_gamma=t["gamma32"]), rope(end_index=t["index3"]), rope(v_cache=t["half"]),
+                 rope(k_cache=t["bad_axis"]), rope(qkv=t["short"]), rope(q_gamma=t["gamma32"]), rope(end_index=t["index3"]), rope(v_cache=t["half"]), rope(v_cache=t["ring"]), rope(k_cache=t["ring"]),
                  rope(positions=t["index"]), attn(k=t["bad_axis"]), attn(v=t["bad_axis"])):
         with pytest.raises(BackendError):
             s.execute([step])
