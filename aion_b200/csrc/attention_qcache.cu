@@ -142,7 +142,7 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
 //    by the column's largest value), and the products of one block of 32 dimensions are scaled by the block's
 //    scale in f32. q4_0 codes enter as the subnormals n * 2^-24 that a nibble IS in the low bits of an f16 (one
 //    AND per two codes); their offset of 8, -8 sum q, is added in f32 behind the products (as the accumulator's initial
-//    value it made every one of them lose the low bits that its size cuts off: twice the error of the outputs).
+//    value it would cost each of them the low bits that its size cuts off; the addition does not show in the time).
 //  * The logits are transposed by movmatrix (two 16-bit halves each), so a lane holds one column's logits of the
 //    keys that it needs as the B operand of the second product.
 //  * O^T[D x 8] += V-codes^T . P'^T, P' = p * scale of (key, block) in f32, again two f16 terms. P' is scaled by
