@@ -12,17 +12,12 @@
 #include <mutex>
 
 #include "attention_qcache.cuh"
-#include "cache_geom.cuh"
 
 namespace aion {
 
 namespace {
 
 using namespace qcache;
-
-__device__ __forceinline__ CacheGeom geom_of(const AttnParams& p) {
-  return CacheGeom{p.page_table, p.T, p.page_tokens, p.pages_per_request, p.pool_pages, p.rolling};
-}
 
 template <bool Q8>
 __device__ __forceinline__ float block_value(const uint8_t* row, uint32_t e) {
@@ -257,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   __syncthreads();
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
-  const TileSpace ts = tile_space(p);
+  const TileSpace ts = tile_space(geom_of(p));
   // ---- this cluster's unit, and its place among the unit's clusters
   const uint32_t cluster = blockIdx.x / dg.cluster, rank = blockIdx.x - cluster * dg.cluster;
   uint32_t row_unit = cluster / dg.per_row, in_row = cluster - row_unit * dg.per_row, split = 0, nsplit = 1;
@@ -387,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   };
   auto issue = [&](uint32_t n) {
     const uint32_t stage = n % G::NST;
-    uint32_t count = tile_of(n) < tiles ? min((uint32_t)TK, ts.seg_len - in_seg * TK) : 0;   // keys of the tile
+    uint32_t count = tile_of(n) < tiles ? tile_rows(ts, in_seg) : 0;   // keys of the tile
     uint64_t row = count ? row0 + in_seg * TK : 0;
     if (p.page_table) {
       if (count && (next_page < 0 || (uint32_t)next_page >= p.pool_pages)) {

@@ -3,12 +3,13 @@
 #pragma once
 
 #include "attention_device.cuh"
+#include "cache_geom.cuh"
 
 namespace aion {
 namespace qcache {
 
 constexpr uint32_t FULL = 0xFFFFFFFFu;
-constexpr int TK = 16;              // keys of a tile
+constexpr int TK = TILE_KEYS;       // keys of a tile
 
 template <int D, bool Q8>
 struct RowFmt {
@@ -40,26 +41,8 @@ __device__ __forceinline__ float ld_cluster_f(uint32_t a) {
 }
 __device__ __forceinline__ void st_cluster_u32(uint32_t a, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 
-// Tiles are cut so that none straddles a page or the end of a ring: a segment (a page, a lap of the ring, or the
-// whole contiguous cache) is cut into tiles of TK keys, the last of which may be shorter.
-struct TileSpace {
-  uint32_t seg_len, per_seg;
-};
-__device__ __forceinline__ TileSpace tile_space(const AttnParams& p) {
-  const uint32_t len = p.page_table ? p.page_tokens : p.rolling ? p.T : 0x7FFFFFFFu;
-  return TileSpace{len, len / TK + (len % TK != 0)};
-}
-__device__ __forceinline__ uint32_t tile_at(const TileSpace& ts, uint32_t key) {
-  const uint32_t seg = key / ts.seg_len;
-  return seg * ts.per_seg + (key - seg * ts.seg_len) / TK;
-}
-// Tiles [first, end) hold the keys that the columns of (request b, positions from l0 on) see together.
-struct TileRange {
-  uint32_t first, end;
-};
-__device__ __forceinline__ TileRange tiles_of_keys(const TileSpace& ts, uint32_t lo, uint32_t hi) {
-  if (hi <= lo) return TileRange{0, 0};
-  return TileRange{tile_at(ts, lo), tile_at(ts, hi - 1) + 1};
+__device__ __forceinline__ CacheGeom geom_of(const AttnParams& p) {
+  return CacheGeom{p.page_table, p.T, p.page_tokens, p.pages_per_request, p.pool_pages, p.rolling};
 }
 __device__ __forceinline__ uint32_t movm(uint32_t a) {
   uint32_t d;

@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
   __syncthreads();
   if (flags[0] && tid == 0) atomicExch(p.fault, FAULT_INVALID_ARGUMENT);
   const uint32_t u_hi = flags[5], u_lo = min(flags[4], u_hi);
-  const TileSpace ts = tile_space(p);
+  const TileSpace ts = tile_space(geom_of(p));
   const TileRange whole = tiles_of_keys(ts, u_lo, u_hi);
   uint32_t per = (whole.end - whole.first + rg.cluster - 1) / rg.cluster;
   per = (per + SUBS - 1) / SUBS * SUBS;
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
 #pragma unroll
           for (int s = 0; s < SUBS; s++) {
             const uint32_t tile = it * SUBS + s;
-            count[s] = tile < tiles ? min((uint32_t)TK, ts.seg_len - in_seg * TK) : 0;
+            count[s] = tile < tiles ? tile_rows(ts, in_seg) : 0;
             row[s] = row0 + in_seg * TK;
             key[s] = seg * ts.seg_len + in_seg * TK;
             if (p.page_table) {

@@ -60,4 +60,33 @@ CACHE_FN ReadSpan read_span(const CacheGeom& g, const int32_t* start, const int3
   return s;
 }
 
+// The attention kernels copy a context in tiles of TILE_KEYS rows, cut so that none straddles a page or the end of a request's
+// rows: a segment (a page, a lap of the ring, or the whole contiguous cache) is cut into tiles of TILE_KEYS keys, the last of
+// which may be shorter.
+constexpr uint32_t TILE_KEYS = 16;
+struct TileSpace {
+  uint32_t seg_len, per_seg;
+};
+CACHE_FN TileSpace tile_space(const CacheGeom& g) {
+  const uint32_t len = g.table ? g.page_tokens : g.t_cap;
+  return TileSpace{len, len / TILE_KEYS + (len % TILE_KEYS != 0)};
+}
+CACHE_FN uint32_t tile_at(const TileSpace& ts, uint32_t key) {
+  const uint32_t seg = key / ts.seg_len;
+  return seg * ts.per_seg + (key - seg * ts.seg_len) / TILE_KEYS;
+}
+// Rows of a segment's tile: no copy may take more.
+CACHE_FN uint32_t tile_rows(const TileSpace& ts, uint32_t in_seg) {
+  const uint32_t left = ts.seg_len - in_seg * TILE_KEYS;
+  return left < TILE_KEYS ? left : TILE_KEYS;
+}
+// Tiles [first, end) hold the keys [lo, hi).
+struct TileRange {
+  uint32_t first, end;
+};
+CACHE_FN TileRange tiles_of_keys(const TileSpace& ts, uint32_t lo, uint32_t hi) {
+  if (hi <= lo) return TileRange{0, 0};
+  return TileRange{tile_at(ts, lo), tile_at(ts, hi - 1) + 1};
+}
+
 }  // namespace aion

@@ -250,3 +250,49 @@ def test_every_row_the_kernels_name_is_the_right_one(tmp_path):
         want += _expected(t_cap, page, table.tolist(), pool, kind == 1, e, s, length, n)
     got = subprocess.run([str(exe)], input="\n".join(text), capture_output=True, text=True, check=True).stdout.splitlines()
     assert [[int(x) for x in line.split()] for line in got] == want
+
+
+TILES = r"""
+#include <cstdio>
+#include "%s/aion_b200/csrc/cache_geom.cuh"
+using namespace aion;
+int main() {
+  // stdin: t_cap page rolling lo hi; out: segment, first row in it and rows of every tile that holds keys [lo, hi)
+  unsigned t_cap, page, rolling, lo, hi;
+  while (scanf("%%u %%u %%u %%u %%u", &t_cap, &page, &rolling, &lo, &hi) == 5) {
+    static int32_t table[1];
+    const TileSpace ts = tile_space(CacheGeom{page ? table : nullptr, t_cap, page, page ? (t_cap + page - 1) / page : 0, 1, rolling});
+    const TileRange r = tiles_of_keys(ts, lo, hi);
+    for (unsigned tile = r.first; tile < r.end; tile++) {
+      const unsigned seg = tile / ts.per_seg, in_seg = tile - seg * ts.per_seg;
+      printf("%%u %%u %%u ", seg, in_seg * TILE_KEYS, tile_rows(ts, in_seg));
+    }
+    printf("\n");
+  }
+}
+"""
+
+
+def test_no_tile_of_attention_reaches_beyond_its_page_ring_or_cache(tmp_path):
+    """Every tile that the attention kernels copy lies within its segment's rows (a page, a lap of the ring, the request's rows of a
+    contiguous cache, whatever its length), and the tiles of a range of keys hold each of them once, in order."""
+    src = tmp_path / "tiles.cpp"
+    src.write_text(TILES % ROOT)
+    exe = tmp_path / "tiles"
+    subprocess.run(["g++", "-std=c++17", "-fsanitize=undefined,address", "-o", str(exe), str(src)], check=True)
+    cases = []
+    for t_cap in (1, 2, 15, 16, 17, 31, 33, 90, 96, 700):
+        for page, rolling in ((0, 0), (0, 1), (1, 0), (5, 0), (16, 0), (40, 0), (2**31 - 1, 0)):
+            seg_len = page or t_cap
+            cases += [(t_cap, page, rolling, lo, hi, seg_len) for lo in (0, 1, t_cap // 2, t_cap - 1) for hi in (lo, lo + 1, t_cap)]
+            if rolling:
+                cases += [(t_cap, page, 1, 5 * t_cap + 3, 6 * t_cap + 3, t_cap), (t_cap, page, 1, 2**31 - 1 - t_cap, 2**31 - 1, t_cap)]
+    text = "\n".join(" ".join(map(str, c[:5])) for c in cases)
+    out = subprocess.run([str(exe)], input=text, capture_output=True, text=True, check=True).stdout.split("\n")
+    for (t_cap, page, rolling, lo, hi, seg_len), line in zip(cases, out):
+        v = [int(x) for x in line.split()]
+        keys = []
+        for seg, first, rows in zip(v[::3], v[1::3], v[2::3]):
+            assert 0 < rows <= 16 and first + rows <= seg_len, (t_cap, page, rolling, lo, hi, seg, first, rows)
+            keys += range(seg * seg_len + first, seg * seg_len + first + rows)
+        assert keys == sorted(set(keys)) and set(range(lo, hi)) <= set(keys), (t_cap, page, rolling, lo, hi)
