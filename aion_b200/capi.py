@@ -74,6 +74,7 @@ class MatMulNT(C.Structure):
 ATTENTION_GENERIC = 1
 ATTENTION_ROW_UNITS = 2
 ATTENTION_BLOCKS = 4
+QCACHE_KERNEL_ANY, QCACHE_KERNEL_COLUMNS, QCACHE_KERNEL_COLUMNS_BOXES, QCACHE_KERNEL_ROWS = 1, 2, 3, 4
 
 
 class Attention(C.Structure):
@@ -186,6 +187,7 @@ SIGNATURES = {
     "aion_cuda_program_launch": (C.c_int32, [_DEV, C.c_void_p]),
     "aion_cuda_program_destroy": (None, [_DEV, C.c_void_p]),
     "aion_cuda_debug_expire_waits": (C.c_int32, [_DEV, C.c_int32]),
+    "aion_cuda_debug_qcache_kernel": (C.c_int32, [_DEV, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),
     "aion_cuda_last_error": (C.c_int32, [C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t)]),
     "aion_cuda_memory_model": (C.c_int32, [_DEV]),
     "aion_cuda_max_binding_bytes": (C.c_uint64, [_DEV]),

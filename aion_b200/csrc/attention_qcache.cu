@@ -121,6 +121,7 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
   const size_t smem = (p.Dk + ROW_WARPS * (p.Dv + 2)) * sizeof(float);
   attn_qcache_row_kernel<KQ8, VQ8><<<p.B * p.L * p.Hq, ROW_WARPS * 32, smem, dev->stream>>>(p);
   AION_CUDA_TRY(cudaGetLastError());
+  dev->debug_qcache = {AION_CUDA_QCACHE_KERNEL_ANY, 1u, 0u};
   return AION_CUDA_OK;
 }
 
@@ -958,6 +959,7 @@ int32_t launch_decode_as(AionCudaDevice* dev, AttnParams& p, const CUtensorMap& 
   static const bool no_pdl_main = std::getenv("AION_CUDA_NO_PDL_MAIN") != nullptr;  // tuning only
   cfg.numAttrs = no_pdl_main ? 1 : 2;
   AION_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, dg, tk, tv));
+  dev->debug_qcache = {TMA ? AION_CUDA_QCACHE_KERNEL_COLUMNS_BOXES : AION_CUDA_QCACHE_KERNEL_COLUMNS, dg.cluster, dg.dealt};
   return AION_CUDA_OK;
 }
 

@@ -917,6 +917,7 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap&
   static const bool no_pdl_main = std::getenv("AION_CUDA_NO_PDL_MAIN") != nullptr;  // tuning only
   cfg.numAttrs = no_pdl_main ? 1 : 2;
   AION_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p, rg, tk, tv));
+  dev->debug_qcache = {AION_CUDA_QCACHE_KERNEL_ROWS, rg.cluster, 0u};
   return AION_CUDA_OK;
 }
 

@@ -92,6 +92,10 @@ struct AionCudaDevice {
   // Test hook (aion_cuda_debug_expire_waits): matmul launches leave out a copy and poll briefly,
   // so that a bounded wait runs out and the fault path can be observed.
   bool debug_expire_waits = false;
+  // What the last attention over a quantized cache launched (aion_cuda_debug_qcache_kernel).
+  struct {
+    uint32_t kernel = 0, cluster = 0, dealt = 0;
+  } debug_qcache;
 
   // Tensor maps (TMA descriptors) already encoded for this device, keyed by view geometry.
   struct TmapCache;

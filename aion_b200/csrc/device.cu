@@ -503,6 +503,14 @@ int32_t aion_cuda_debug_expire_waits(AionCudaDevice* dev, int32_t on) {
   return AION_CUDA_OK;
 }
 
+int32_t aion_cuda_debug_qcache_kernel(const AionCudaDevice* dev, uint32_t* kernel, uint32_t* cluster, uint32_t* dealt) {
+  if (!dev) return fail(AION_CUDA_INVALID_ARGUMENT, "debug_qcache_kernel: null device");
+  if (kernel) *kernel = dev->debug_qcache.kernel;
+  if (cluster) *cluster = dev->debug_qcache.cluster;
+  if (dealt) *dealt = dev->debug_qcache.dealt;
+  return AION_CUDA_OK;
+}
+
 int32_t aion_cuda_last_error(char* buf, size_t cap, size_t* len) {
   const std::string& s = g_last_error;
   if (len) *len = s.size();

@@ -134,6 +134,14 @@ AION_CUDA_API void aion_cuda_program_destroy(AionCudaDevice* dev, AionCudaProgra
  * and poll a few hundred times instead of a million, so that exactly this happens within
  * milliseconds (the result of such a matmul is meaningless). For tests of the fault path. */
 AION_CUDA_API int32_t aion_cuda_debug_expire_waits(AionCudaDevice* dev, int32_t on);
+/* Test hook, no counterpart in the reference: which kernel the last aion_cuda_attention over quantized
+ * K / V launched on this device (0: none yet), how many CTAs share the keys of a unit, and whether the
+ * clusters were dealt out by the keys of the requests. A result pointer may be NULL. */
+#define AION_CUDA_QCACHE_KERNEL_ANY 1u           /* any head size, one CTA per row */
+#define AION_CUDA_QCACHE_KERNEL_COLUMNS 2u       /* columns of eight, rows copied in pieces */
+#define AION_CUDA_QCACHE_KERNEL_COLUMNS_BOXES 3u /* columns of eight, rows copied in TMA boxes */
+#define AION_CUDA_QCACHE_KERNEL_ROWS 4u          /* blocks of 128 rows */
+AION_CUDA_API int32_t aion_cuda_debug_qcache_kernel(const AionCudaDevice* dev, uint32_t* kernel, uint32_t* cluster, uint32_t* dealt);
 /* Per-thread diagnostic text of the last failing call on this thread
  * (aion src/aion/diagnostic.zig:8-44; include/aion.h:117-140). Copies at most `cap`
  * bytes, NUL-terminates when cap > 0, stores the full length in *len when non-NULL. */
@@ -336,7 +344,11 @@ typedef struct AionCudaAttention {
  * aion_cuda_qk_norm_rope_append write. Everything above holds for them (a page table may then have
  * any positive page_tokens). Keys and values are used as code x scale, logits and sums are f32: the
  * result is that of f32 attention over the dequantized cache. A page number outside the pool is
- * reported like a bad length, and its keys are left out. */
+ * reported like a bad length, and its keys are left out.
+ * Which kernel works: heads of 64, 128 and 256 (d_k = d_v) go by columns of eight or, where that is
+ * cheaper, by blocks of 128 rows. ROW_UNITS takes columns. BLOCKS takes rows where they can be taken:
+ * l_q > 1, no image, and K and V at 16-byte addresses with rows (h_kv heads) of whole 16 bytes; other
+ * operands go by columns, as without the flag. (aion_cuda_debug_qcache_kernel says which ran.) */
 
 AION_CUDA_API int32_t aion_cuda_attention(AionCudaDevice* dev, const AionCudaAttention* step);
 

@@ -1,0 +1,161 @@
+"""Attention over quantized caches: every path of its kernels, each test sure of the kernel that it ran."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from aion_b200 import capi
+from aion_b200.backend import AttentionWindow
+from tests import kv_cache_ref as ref
+from tests.kv_cache_ref import Q4, Q8
+from tests.test_gpu_kv_cache import ALL, NAMES, inputs, run_attention, sess, sess_quiet  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+ROWS, COLUMNS, BOXES, ANY = capi.QCACHE_KERNEL_ROWS, capi.QCACHE_KERNEL_COLUMNS, capi.QCACHE_KERNEL_COLUMNS_BOXES, capi.QCACHE_KERNEL_ANY
+IDS = [f"{NAMES[a]}{NAMES[b]}" for a, b in ALL]
+
+
+def launched(backend):
+    """(kernel, CTAs of a cluster, dealt) of the last attention."""
+    v = [C.c_uint32() for _ in range(3)]
+    assert backend._lib.aion_cuda_debug_qcache_kernel(backend.handle, *(C.byref(x) for x in v)) == capi.OK
+    return tuple(x.value for x in v)
+
+
+def within(got, want, bound):
+    """No further from the 64-bit result than f32 arithmetic may be (kv_cache_ref.attention)."""
+    assert np.isfinite(got).all()
+    over = np.abs(got - want) - bound
+    assert (over <= 0).all(), f"{(over > 0).sum()} of {over.size} beyond the bound, worst by {over.max():g}"
+
+
+def causal(lens, L):
+    return np.array([[max(0, n - L) + i for i in range(L)] for n in lens], dtype=np.int32)
+
+
+@pytest.mark.parametrize("kdt,vdt", ALL, ids=IDS)
+@pytest.mark.parametrize("D,H,Hq", [(64, 4, 8), (128, 2, 8), (256, 1, 4)])
+@pytest.mark.parametrize("layout,page", [("plain", 0), ("paged", 40), ("rolling", 0)])
+@pytest.mark.parametrize("L,T,cluster", [(20, 600, 2), (7, 1100, 4), (3, 2100, 8)])
+def test_rows_share_the_keys_of_a_cluster(sess, backend, kdt, vdt, D, H, Hq, layout, page, L, T, cluster):
+    """Few blocks of rows over many keys: the CTAs of a cluster add up their sums; one request has no keys, and one so few that
+    most of its CTAs have none."""
+    lens = [T, 0, 70] if layout != "rolling" else [3 * T + 5, 0, 70]
+    B = len(lens)
+    q, k, v = inputs([D, L, kdt], B, T, H, D, L, Hq, kdt, vdt)
+    pos = causal(lens, L)
+    got, _ = run_attention(sess, q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, layout=layout, page=page,
+                           window=AttentionWindow.causal(), flags=capi.ATTENTION_BLOCKS)
+    assert launched(backend) == (ROWS, cluster, 0)
+    within(got, *ref.attention(q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, rolling=layout == "rolling"))
+    assert not got[1].any()
+
+
+@pytest.mark.parametrize("kdt,vdt", ALL, ids=IDS)
+@pytest.mark.parametrize("L,Hq,H,D", [(9, 28, 4, 64), (130, 4, 4, 64), (33, 8, 4, 128), (50, 6, 2, 256)])
+@pytest.mark.parametrize("layout,page", [("plain", 0), ("paged", 24), ("rolling", 0)])
+@pytest.mark.parametrize("cap", [0.0, 25.0])
+def test_rows_with_windows_and_caps(sess, backend, L, Hq, H, D, layout, page, kdt, vdt, cap):
+    B, T = 2, 300
+    q, k, v = inputs([L, D, kdt], B, T, H, D, L, Hq, kdt, vdt)
+    lens = [711, 300] if layout == "rolling" else [300, 137]
+    pos = causal(lens, L)
+    got, _ = run_attention(sess, q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, layout=layout, page=page,
+                           window=AttentionWindow(left=150, right=0), cap=cap, flags=capi.ATTENTION_BLOCKS)
+    assert launched(backend)[0] == ROWS
+    within(got, *ref.attention(q, k, v, kdt, vdt, scale=D ** -0.5, positions=pos, lengths=lens, rolling=layout == "rolling", left=150, cap=cap))
+
+
+@pytest.mark.parametrize("T,L,first", [(1, 1, 7), (3, 2, 50), (5, 9, 2), (16, 4, 100), (17, 4, 2**31 - 21)])
+@pytest.mark.parametrize("flags,kernel", [(capi.ATTENTION_ROW_UNITS, BOXES), (capi.ATTENTION_BLOCKS, ROWS)], ids=["columns", "rows"])
+def test_tiny_rings_and_late_steps_in_boxes(sess, backend, T, L, first, flags, kernel):
+    B, H, D = 1, 4, 64
+    q, k, v = inputs([T, L], B, T, H, D, L, 8, Q8, Q4)
+    pos = first + np.arange(L, dtype=np.int64)[None]
+    lens = [int(pos[0, -1]) + 1]
+    got, _ = run_attention(sess, q, k, v, Q8, Q4, scale=0.1, positions=pos.astype(np.int32), lengths=lens, layout="rolling",
+                           window=AttentionWindow.causal(), flags=flags)
+    assert launched(backend)[0] == (kernel if L > 1 else BOXES)
+    within(got, *ref.attention(q, k, v, Q8, Q4, scale=0.1, positions=pos, lengths=lens, rolling=True))
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("D,H,vdt", [(64, 4, Q8), (128, 2, Q4), (256, 1, Q8)])
+@pytest.mark.parametrize("T,cluster", [(90, 1), (1100, 4)])
+@pytest.mark.parametrize("flags,kernel", [(capi.ATTENTION_ROW_UNITS, BOXES), (capi.ATTENTION_BLOCKS, ROWS)], ids=["columns", "rows"])
+def test_v_scales_that_are_not_finite_spoil_their_own_block(sess, backend, bad, D, H, vdt, T, cluster, flags, kernel):
+    """One V scale of NaN or an infinity, in the last block of the last head: the rows that see its key have no finite value in the
+    block's 32 dimensions and their true values elsewhere; rows that do not see it, and other heads, are clean."""
+    B, L, Hq, at = 1, 12, 2 * H, T - 15
+    q, k, v = inputs([5], B, T, H, D, L, Hq, Q8, vdt)
+    pos = np.arange(T - 20, T - 20 + L, dtype=np.int32)[None]
+    kw = dict(scale=0.1, positions=pos, lengths=[T])
+    want, bound = ref.attention(q, k, v, Q8, vdt, **kw)
+    v.reshape(B, T, H, D // 32, -1)[0, at, -1, -1, :2] = np.frombuffer(np.float16(bad).tobytes(), np.uint8)
+    got, _ = run_attention(sess, q, k, v, Q8, vdt, window=AttentionWindow.causal(), flags=flags, **kw)
+    assert launched(backend)[0] == kernel
+    if kernel == ROWS:
+        assert launched(backend)[1] == cluster
+    clean = np.ones(got.shape, bool)
+    clean[:, 5:, Hq - Hq // H:, D - 32:] = False
+    assert not np.isfinite(got[~clean]).any()
+    assert (np.abs(got - want)[clean] <= bound[clean]).all()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 65504.0])
+@pytest.mark.parametrize("D,H", [(64, 4), (128, 2), (256, 1)])
+@pytest.mark.parametrize("flags,kernel", [(capi.ATTENTION_ROW_UNITS, BOXES), (capi.ATTENTION_BLOCKS, ROWS)], ids=["columns", "rows"])
+def test_key_rows_that_only_later_rows_see(sess, backend, bad, D, H, flags, kernel):
+    """A key row of NaN, infinite or huge scales: the rows before it (causal) are those of a clean cache."""
+    B, T, L = 1, 90, 12
+    q, k, v = inputs([3], B, T, H, D, L, 8 * H, Q8, Q8)
+    pos = np.arange(70, 70 + L, dtype=np.int32)[None]
+    want, bound = ref.attention(q, k, v, Q8, Q8, scale=0.1, positions=pos, lengths=[T])
+    k.reshape(B, T, H, D // 32, 34)[0, 76, :, :, :2] = np.frombuffer(np.float16(bad).tobytes(), np.uint8)
+    got, _ = run_attention(sess_quiet(sess), q, k, v, Q8, Q8, scale=0.1, positions=pos, lengths=[T], window=AttentionWindow.causal(), flags=flags)
+    assert launched(backend)[0] == kernel
+    within(got[:, :6], want[:, :6], bound[:, :6])
+
+
+@pytest.mark.parametrize("D,H,kernel", [(64, 1, COLUMNS), (128, 1, COLUMNS), (256, 1, BOXES)])
+@pytest.mark.parametrize("L", [1, 2])
+def test_a_single_unit_with_more_keys_than_a_cluster_walks(sess, backend, D, H, kernel, L):
+    """Dealt clusters: their sums meet in global memory, and the last of them to arrive adds them up, the same way every time."""
+    T = 6000
+    q, k, v = inputs([D, L], 1, T, H, D, L, 4, Q8, Q4)
+    pos = causal([T], L)
+    kw = dict(scale=D ** -0.5, positions=pos, lengths=[T], window=AttentionWindow.causal(), flags=capi.ATTENTION_ROW_UNITS)
+    got, step = run_attention(sess, q, k, v, Q8, Q4, **kw)
+    assert launched(backend) == (kernel, 8, 1)
+    within(got, *ref.attention(q, k, v, Q8, Q4, scale=D ** -0.5, positions=pos, lengths=[T]))
+    for _ in range(3):
+        sess[1].write(step.out, np.zeros(q.shape, np.float32))
+        sess[0].execute([step])
+        assert np.array_equal(sess[1].read(step.out), got)
+
+
+@pytest.mark.parametrize("kdt,vdt", [(Q8, Q4), (Q4, Q8)])
+@pytest.mark.parametrize("H,kernel", [(4, BOXES), (3, COLUMNS)])
+@pytest.mark.parametrize("layout,page", [("plain", 0), ("paged", 1000)])
+def test_long_uneven_requests_are_dealt_by_their_keys(sess, backend, kdt, vdt, H, kernel, layout, page):
+    """Many tiles for each warp, and requests from none to all of the context."""
+    B, D, L, T = 8, 64, 1, 24000 if H == 4 else 32000
+    lens = [T, 0, 1, T // 2, 16, T - 1, T // 3, 5000]
+    q, k, v = inputs([H, kdt], B, T, H, D, L, 2 * H, kdt, vdt)
+    pos = causal(lens, L)
+    got, _ = run_attention(sess, q, k, v, kdt, vdt, scale=0.125, positions=pos, lengths=lens, layout=layout, page=page, window=AttentionWindow.causal())
+    ran = launched(backend)
+    assert ran[0] == kernel and ran[2] == 1
+    within(got, *ref.attention(q, k, v, kdt, vdt, scale=0.125, positions=pos, lengths=lens))
+    assert not got[1].any()
+
+
+def test_the_forced_kernels_that_operands_allow(sess, backend):
+    """Which kernel runs: ATTENTION_BLOCKS holds where rows are whole 16 bytes and more than one position is asked for, else columns do
+    the work; other head sizes are any-shape."""
+    for L, D, H, flags, kernel in ((2, 128, 2, capi.ATTENTION_BLOCKS, ROWS), (2, 128, 1, capi.ATTENTION_BLOCKS, COLUMNS), (1, 128, 2, capi.ATTENTION_BLOCKS, BOXES),
+                                   (2, 128, 2, capi.ATTENTION_ROW_UNITS, BOXES), (2, 128, 2, capi.ATTENTION_GENERIC, ANY), (2, 96, 2, capi.ATTENTION_BLOCKS, ANY)):
+        q, k, v = inputs([L, D], 1, 50, H, D, L, 4, Q8, Q8)
+        got, _ = run_attention(sess, q, k, v, Q8, Q8, scale=0.1, flags=flags)
+        assert launched(backend)[0] == kernel, (L, D, H, flags)
+        within(got, *ref.attention(q, k, v, Q8, Q8, scale=0.1, positions=np.zeros((1, L), int), lengths=[50], right=capi.WINDOW_UNBOUNDED))
