@@ -136,9 +136,9 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
 //
 //  * S^T[16 keys x 8] = C . Q^T on f16 m16n8k16: the codes are exact in f16, q is two f16 terms (22 bits, normed
 //    by the column's largest value), and the products of one block of 32 dimensions are scaled by the block's
-//    scale in f32. q4_0 codes enter as the subnormals n * 2^-24 that a nibble IS in the low bits of an f16 (one
-//    AND per two codes); their offset of 8, -8 sum q, is added in f32 behind the products (as the accumulator's initial
-//    value it would cost each of them the low bits that its size cuts off; the addition does not show in the time).
+//    scale in f32. q4_0 codes are made the normal numbers n - 8: as the subnormals n * 2^-24 that a nibble IS in the low
+//    bits of an f16 they would need no arithmetic, but a tensor core aligns its products by the exponent fields, where a
+//    subnormal counts as 2^-14, and cuts the low bits of q off.
 //  * The logits are transposed by movmatrix (two 16-bit halves each), so a lane holds one column's logits of the
 //    keys that it needs as the B operand of the second product.
 //  * O^T[D x 8] += V-codes^T . P'^T, P' = p * scale of (key, block) in f32, again two f16 terms. P' is scaled by
@@ -176,8 +176,7 @@ struct DecodeGeom {
   static_assert(NST >= 2 && WARPS * WS * 4 <= RING, "ring");
   static constexpr int OFF_VS = RING;                                        // f32 [warp][block][keys of an iteration]: V scales
   static constexpr int OFF_Q = OFF_VS + WARPS * (D / QK) * TK * TPI * 4;     // uint4 [D / 16][32]: Q fragments; first f32 [8][D]: q
-  static constexpr int OFF_CI = OFF_Q + COLS * D * 4;                        // float4 [block][4]: -8 sum q of columns 2t, 2t + 1, twice
-  static constexpr int OFF_META = OFF_CI + D / QK * COLS * 8;                // per column: row, first key, key end, output row, head, factor
+  static constexpr int OFF_META = OFF_Q + COLS * D * 4;                      // per column: row, first key, key end, output row, head, factor
   static constexpr int OFF_VALID = OFF_META + COLS * 24;                     // per warp and stage: which keys are there, the first of them
   static constexpr int OFF_BARS = OFF_VALID + WARPS * NST * 8;               // per warp and stage: the copies' barrier
   static constexpr int OFF_FLAGS = OFF_BARS + WARPS * NST * 8;
@@ -241,7 +240,6 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   uint32_t* col_head = col_orow + COLS;
   float* col_factor = reinterpret_cast<float*>(col_head + COLS);
   float* qs = reinterpret_cast<float*>(smem + G::OFF_Q);
-  float* ci = reinterpret_cast<float*>(smem + G::OFF_CI);
   int* flags = reinterpret_cast<int*>(smem + G::OFF_FLAGS);   // [0] bad inputs, [1] last cluster of the unit
 
   const uint32_t bars = sbase + G::OFF_BARS + warp * (G::NST * 8);
@@ -436,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     }
   }
 
-  // ---- q: normed by the column's largest value to [2^13, 2^14), and the sums that offset q4_0 codes
+  // ---- q: normed by the column's largest value to [2^13, 2^14)
 #pragma unroll
   for (int j = 0; j < COLS / WARPS; j++) {
     const int c = warp + j * WARPS;
@@ -452,15 +450,13 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     if (lane == 0) col_factor[c] = p.scale * __uint_as_float((e - 13u) << 23);
   }
   __syncthreads();
-  // Q^T as the B operand: this lane's column g, the dimensions of word t. Where a q4_0 code enters times 16, q
-  // enters by 16 less.
+  // Q^T as the B operand: this lane's column g, the dimensions of word t.
   // Every warp makes a part of the fragments for all.
   uint4 made[NB / WARPS > 0 ? NB / WARPS : 1][2];
 #pragma unroll
   for (int j = 0; j < (NB + WARPS - 1) / WARPS; j++) {
     const int blk = warp + j * WARPS;
     if (blk < NB) {
-      double part = 0.0;   // (eight times its error comes on every logit: not in f32)
 #pragma unroll
       for (int m = 0; m < 2; m++) {
         uint32_t hl[2][2];
@@ -472,20 +468,11 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
             int dim;
             if (KQ8) dim = pair_byte(true, blk & 1, t + 4 * m, 2 * r + h);
             else dim = 2 * pair_byte(false, blk & 1, t, m + 2 * h) + r;      // nibbles (2m + r, 2m + r + 4): bytes m, m + 2
-            x[h] = qs[g * D + blk * QK + dim] * (!KQ8 && r ? 0.0625f : 1.0f);
+            x[h] = qs[g * D + blk * QK + dim];
           }
           split2(x[0], x[1], &hl[0][r], &hl[1][r]);
-          if (!KQ8) {
-            const float2 a = __half22float2(*reinterpret_cast<__half2*>(&hl[0][r])), c = __half22float2(*reinterpret_cast<__half2*>(&hl[1][r]));
-            part += (((double)a.x + (double)c.x) + ((double)a.y + (double)c.y)) * (r ? 16.0 : 1.0);
-          }
         }
         made[j][m] = make_uint4(hl[0][0], hl[0][1], hl[1][0], hl[1][1]);
-      }
-      if (!KQ8) {
-        part += __shfl_xor_sync(FULL, part, 1);
-        part += __shfl_xor_sync(FULL, part, 2);
-        if (t == 0) ci[blk * 2 * COLS + g / 2 * 4 + g % 2] = ci[blk * 2 * COLS + g / 2 * 4 + g % 2 + 2] = (float)(part * (-8.0 * 5.9604644775390625e-8));   // -8 * 2^-24
       }
     }
   }
@@ -591,9 +578,6 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
         const uint4 f = qfrag[(4 * pr + i) * 32 + lane];
         qh[i][0] = f.x, qh[i][1] = f.y, ql[i][0] = f.z, ql[i][1] = f.w;
       }
-      float4 init[2];
-#pragma unroll
-      for (int k = 0; k < 2; k++) init[k] = KQ8 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(ci + (2 * pr + k) * 2 * COLS + 4 * t);
 #pragma unroll
       for (int j = 0; j < TPI; j++) {
         uint32_t a[2][2][4];                   // [block of the pair][MMA][operand]
@@ -610,9 +594,9 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
             unpack_q8(lds32(row + 52 + 4 * t), &a[1][1][half], &a[1][1][2 + half]);
           } else {
             uint32_t u[4];
-            unpack_q4_subnormal(first, u);
+            unpack_q4(first, u);
             a[0][0][half] = u[0], a[0][0][2 + half] = u[1], a[0][1][half] = u[2], a[0][1][2 + half] = u[3];
-            unpack_q4_subnormal(lds32(row + 20 + 4 * t), u);
+            unpack_q4(lds32(row + 20 + 4 * t), u);
             a[1][0][half] = u[0], a[1][0][2 + half] = u[1], a[1][1][half] = u[2], a[1][1][2 + half] = u[3];
           }
           (half ? sh : sl)[0] = half_bits(w0 & 0xFFFFu), (half ? sh : sl)[1] = half_bits(wm >> 16);
@@ -625,7 +609,6 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
           mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], ql[q + 1][0], ql[q + 1][1], c[0], c[1], c[2], c[3]);
           mma_f16_from(c, a[k][0][0], a[k][0][1], a[k][0][2], a[k][0][3], qh[q][0], qh[q][1], c[0], c[1], c[2], c[3]);
           mma_f16_from(c, a[k][1][0], a[k][1][1], a[k][1][2], a[k][1][3], qh[q + 1][0], qh[q + 1][1], c[0], c[1], c[2], c[3]);
-          if (!KQ8) add2(c[0], c[1], init[k].x, init[k].y), add2(c[2], c[3], init[k].z, init[k].w);
           s[j][0] = fmaf(sl[k], c[0], s[j][0]);
           s[j][1] = fmaf(sl[k], c[1], s[j][1]);
           s[j][2] = fmaf(sh[k], c[2], s[j][2]);
@@ -639,9 +622,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
     for (int j = 0; j < TPI; j++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        float x0 = s[j][2 * h], x1 = s[j][2 * h + 1];
-        if (!KQ8) x0 *= 16777216.0f, x1 *= 16777216.0f;   // the codes' 2^24
-        const uint32_t u = __float_as_uint(x0 * f0), w = __float_as_uint(x1 * f1);
+        const uint32_t u = __float_as_uint(s[j][2 * h] * f0), w = __float_as_uint(s[j][2 * h + 1] * f1);
         const uint32_t low = movm(__byte_perm(u, w, 0x5410)), high = movm(__byte_perm(u, w, 0x7632));
         y[4 * j + 2 * h] = __uint_as_float(__byte_perm(low, high, 0x5410));
         y[4 * j + 2 * h + 1] = __uint_as_float(__byte_perm(low, high, 0x7632));
@@ -709,13 +690,9 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
               a[j][1][2 * kp + 1] = h2_add(__byte_perm(hi2, 0x64646464u, 0x4342), 0xE480E480u);
             } else {
               const uint32_t pos = row + blk * VF::BB + 2 + 2 * g;
-              uint32_t x = __byte_perm(lds16(pos), lds16(pos + VF::PITCH), 0x5410);
-              // 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n: both leave n - 8 exactly
-              a[j][0][2 * kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
-              a[j][0][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
-              x >>= 8;
-              a[j][1][2 * kp] = h2_add((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
-              a[j][1][2 * kp + 1] = h2_fma((x & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+              uint32_t u[4];
+              unpack_q4(__byte_perm(lds16(pos), lds16(pos + VF::PITCH), 0x5410), u);
+              a[j][0][2 * kp] = u[0], a[j][0][2 * kp + 1] = u[1], a[j][1][2 * kp] = u[2], a[j][1][2 * kp + 1] = u[3];
             }
           }
         }

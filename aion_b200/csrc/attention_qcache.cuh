@@ -128,12 +128,13 @@ __host__ __device__ constexpr int pair_byte(bool q8, bool second, int u, int j) 
   return second ? 4 * u + j : u ? 4 * u - 2 + j : j < 2 ? j : n - 4 + j;
 }
 
-__device__ __forceinline__ void unpack_q4_subnormal(uint32_t w, uint32_t (&x)[4]) {
-  x[0] = w & 0x000F000Fu;        // n * 2^-24
-  x[1] = w & 0x00F000F0u;        // n * 2^-20
+// 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n: both leave n - 8 exactly.
+__device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t (&x)[4]) {
+  x[0] = h2_add((w & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+  x[1] = h2_fma((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
   w >>= 8;
-  x[2] = w & 0x000F000Fu;
-  x[3] = w & 0x00F000F0u;
+  x[2] = h2_add((w & 0x000F000Fu) | 0x64006400u, 0xE408E408u);
+  x[3] = h2_fma((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
 }
 __device__ __forceinline__ void unpack_q8(uint32_t w, uint32_t* r0, uint32_t* r1) {
   w ^= 0x80808080u;

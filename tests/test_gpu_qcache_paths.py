@@ -159,3 +159,42 @@ def test_the_forced_kernels_that_operands_allow(sess, backend):
         got, _ = run_attention(sess, q, k, v, Q8, Q8, scale=0.1, flags=flags)
         assert launched(backend)[0] == kernel, (L, D, H, flags)
         within(got, *ref.attention(q, k, v, Q8, Q8, scale=0.1, positions=np.zeros((1, L), int), lengths=[50], right=capi.WINDOW_UNBOUNDED))
+
+
+# ---- precision: inputs whose f32 evaluation is exact but for a few known roundings --------------------------------------------
+KERNELS = [("columns", capi.ATTENTION_ROW_UNITS, BOXES), ("rows", capi.ATTENTION_BLOCKS, ROWS)]
+FORCED = dict(argvalues=[(f, k) for _, f, k in KERNELS], ids=[n for n, _, _ in KERNELS])
+
+
+def blocks(dtype, codes, scales):
+    """Stored rows from whole-number codes [..., D] and f16 scales [..., D / 32]."""
+    codes = np.asarray(codes).reshape(*np.shape(codes)[:-1], -1, 32)
+    head = np.asarray(scales, np.float16)[..., None].view(np.uint8)
+    if dtype == Q8:
+        body = codes.astype(np.int8).view(np.uint8)
+    else:
+        n = (codes + 8).astype(np.uint8)
+        body = n[..., 0::2] | n[..., 1::2] << 4
+    return np.concatenate([np.broadcast_to(head, (*body.shape[:-1], 2)), body], -1).reshape(*codes.shape[:-2], -1)
+
+
+@pytest.mark.parametrize("flags,kernel", **FORCED)
+@pytest.mark.parametrize("D,H", [(64, 4), (128, 2), (256, 1)])
+@pytest.mark.parametrize("kdt", [Q8, Q4], ids=["q8", "q4"])
+def test_logits_keep_the_low_bits_of_the_queries(sess, backend, kdt, D, H, flags, kernel):
+    """q = (1 + 2^-18, 1) and keys (7, -7) S and (-7, 7) S in two dimensions of a block, S = 2^12: every product is exact in f32 and so is
+    their sum, +-7 * 2^-6, so the weights' quotient is known. Beyond two roundings of the logit's move to base 2 only exp2 (2^-22),
+    the weights' two f16 terms (2^-23) and the sums and the quotient of two weights (4 * 2^-24) round: below 2^-20 of values of size one."""
+    L, T = 2, 32
+    q = np.zeros((1, L, H, D), np.float32)
+    q[..., 33], q[..., 50] = 1 + 2.0 ** -18, 1.0
+    codes = np.zeros((1, T, H, D))
+    codes[0, 0::2, :, 33], codes[0, 0::2, :, 50] = 7, -7
+    codes[0, 1::2, :, 33], codes[0, 1::2, :, 50] = -7, 7
+    k = blocks(kdt, codes, np.full((1, T, H, D // 32), 2.0 ** 12))
+    sign = np.where(np.arange(T) % 2 == 0, 1, -1)[None, :, None, None]
+    v = blocks(Q8, np.broadcast_to(sign * 64, codes.shape), np.full((1, T, H, D // 32), 1 / 64))
+    got, _ = run_attention(sess, q, k, v, kdt, Q8, scale=1.0, flags=flags)
+    assert launched(backend)[0] == kernel
+    want = np.tanh(7 * 2.0 ** 12 * 2.0 ** -18)
+    assert np.abs(got - want).max() <= 2.0 ** -20
