@@ -500,8 +500,8 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
         drain(it - 1, 0, acc[0]);
         if (NP > 1) drain(it - 1, 1, acc[1 % NP]);
       }
-      if (more) {   // weights, in units in which the largest product with a V power is at most 2^14
-        const float off = 30.0f - (float)e_run - (m_run == -INFINITY ? 0.0f : m_run);
+      if (more) {   // weights
+        const float off = m_run == -INFINITY ? 0.0f : -m_run;
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           add2(sum[i & 1].x, sum[i & 1].y, x.x, x.y);
           s[2 * i] = x.x, s[2 * i + 1] = x.y;
         }
-        l_run = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), pow2f((int)e_run - 30), l_run);
+        l_run += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       if (any_odd) {   // a V scale that is not finite: NaN where a row gives weight to its key
         const uint8_t* odd = smem + G::OFF_ODD + slot * SK + half * 32;
@@ -532,13 +532,16 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
 #pragma unroll
       for (int j = 0; j < 2; j++) {   // two terms of the products, over the logits: 16 keys are eight columns
         if (more) {
+          // Units in which the largest product with a V power is at most 2^14. (A factor: in exp2's argument the power would
+          // leave the weight's last bits no room.)
+          const float2 unit = make_float2(pow2f(30 - (int)e_run), pow2f(30 - (int)e_run));
           const float4* vexp = reinterpret_cast<const float4*>(smem + G::OFF_VEXP + (slot * SK + half * 32 + j * 16) * 4);
           uint32_t h[8], l[8];
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const float4 v = vexp[i];
             const float* x = s + 16 * j + 4 * i;
-            const float2 w0 = mul2(make_float2(x[0], x[1]), make_float2(v.x, v.y)), w1 = mul2(make_float2(x[2], x[3]), make_float2(v.z, v.w));
+            const float2 w0 = mul2(make_float2(x[0], x[1]), mul2(make_float2(v.x, v.y), unit)), w1 = mul2(make_float2(x[2], x[3]), mul2(make_float2(v.z, v.w), unit));
             split2(w0.x, w0.y, &h[2 * i], &l[2 * i]);
             split2(w1.x, w1.y, &h[2 * i + 1], &l[2 * i + 1]);
           }

@@ -198,3 +198,28 @@ def test_logits_keep_the_low_bits_of_the_queries(sess, backend, kdt, D, H, flags
     assert launched(backend)[0] == kernel
     want = np.tanh(7 * 2.0 ** 12 * 2.0 ** -18)
     assert np.abs(got - want).max() <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("flags,kernel", **FORCED)
+@pytest.mark.parametrize("vscale", [2.0 ** -13, 1.0, 2.0 ** 13])
+def test_weights_are_exact_to_the_last_bits_whatever_the_values_size(sess, backend, vscale, flags, kernel):
+    """Two keys, one with V = 0: out / v = w / (1 + w) with w = exp(-x), x in [0, 1/2). In f32: x to base 2 rounds three times
+    (2^-24 x each), the difference once, exp2 is good to 2^-22, the weights' two f16 terms to 2^-23, sum, quotient and product round
+    once each. As independent errors, uniform over these bounds, their root mean square is below
+    sqrt(3 * 0.5^2 + 1 + 16 + 4 + 3) / sqrt(3) * 2^-24 = 2.9 * 2^-24, times 1 / (1 + w) <= 0.63."""
+    L, H, D, Hq = 256, 2, 128, 2
+    rng = np.random.default_rng(17)
+    x = rng.integers(1, 2 ** 10, (1, L, Hq)).astype(np.float32) * 2.0 ** -11
+    q = np.zeros((1, L, Hq, D), np.float32)
+    q[..., 5] = x
+    codes = np.zeros((1, 2, H, D))
+    codes[0, 1, :, 5] = -1
+    k = blocks(Q8, codes, np.ones((1, 2, H, D // 32)))
+    vc = np.zeros((1, 2, H, D))
+    vc[0, 1] = 64
+    v = blocks(Q8, vc, np.full((1, 2, H, D // 32), vscale))
+    got, _ = run_attention(sess, q, k, v, Q8, Q8, scale=1.0, flags=flags)
+    assert launched(backend)[0] == kernel
+    w = np.exp(-x.astype(np.float64))[..., None]
+    rel = got / (64 * vscale) / (w / (1 + w)) - 1
+    assert np.sqrt((rel[..., 0] ** 2).mean()) <= 0.63 * 2.9 * 2.0 ** -24
