@@ -141,9 +141,11 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p) {
 //    subnormal counts as 2^-14, and cuts the low bits of q off.
 //  * The logits are transposed by movmatrix (two 16-bit halves each), so a lane holds one column's logits of the
 //    keys that it needs as the B operand of the second product.
-//  * O^T[D x 8] += V-codes^T . P'^T, P' = p * scale of (key, block) in f32, again two f16 terms. P' is scaled by
-//    a power of two that follows the largest V scale met so far: without it small V scales would push the terms
-//    into f16's subnormals. The accumulators are moved over when that power or a column's maximum grows.
+//  * O^T[D x 8] += V-codes^T . P'^T, P' = p * scale of (key, block) in f32, again two f16 terms, the
+//    second one times 2^11 with a sum of its own. P' is scaled by a power of two that follows the largest V scale
+//    met so far: it is below 2^15, and where keys or columns differ in size the second term still has eleven bits when the
+//    first one is down to f16's subnormals (23 bits of a P' down to 2^-29 of the largest). The accumulators are moved over
+//    when that power or a column's maximum grows.
 //  * The context of a unit (one kv head's columns) is cut over clusters of up to eight CTAs. A cluster's sums meet
 //    through distributed shared memory, every CTA adding up its share of the outputs; only units that several
 //    clusters work on leave partial sums in global memory, for the last of them to arrive. (With one ticket per
@@ -672,7 +674,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
           for (int kp = 0; kp < 2; kp++) {
             const float2 v = lds_f2(vs + (blk * KI + j * TK + 2 * t + 8 * kp) * 4);
             const float2 w = mul2(make_float2(y[4 * j + 2 * kp], y[4 * j + 2 * kp + 1]), v);
-            split2(w.x, w.y, &bh[j][kp], &blw[j][kp]);
+            split2_scaled(w.x, w.y, &bh[j][kp], &blw[j][kp]);
             const uint32_t row = at[j] + TK * KF::PITCH + vshift + (2 * t + 8 * kp) * VF::PITCH;
             if (VQ8) {
               uint32_t x[2];
@@ -700,13 +702,16 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
         // keys that adds up. So an iteration is summed from zero and added in f32.
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-          float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ol[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int j = 0; j < TPI; j++) mma_f16_from(o, a[j][m][0], a[j][m][1], a[j][m][2], a[j][m][3], blw[j][0], blw[j][1], o[0], o[1], o[2], o[3]);
+          for (int j = 0; j < TPI; j++) mma_f16_from(ol, a[j][m][0], a[j][m][1], a[j][m][2], a[j][m][3], blw[j][0], blw[j][1], ol[0], ol[1], ol[2], ol[3]);
 #pragma unroll
           for (int j = 0; j < TPI; j++) mma_f16_from(o, a[j][m][0], a[j][m][1], a[j][m][2], a[j][m][3], bh[j][0], bh[j][1], o[0], o[1], o[2], o[3]);
-          add2(acc[2 * blk + m][0], acc[2 * blk + m][1], o[0], o[1]);
-          add2(acc[2 * blk + m][2], acc[2 * blk + m][3], o[2], o[3]);
+          constexpr float down = 1.0f / LO_SCALE;
+          const float2 x = fma2(make_float2(ol[0], ol[1]), make_float2(down, down), make_float2(o[0], o[1]));
+          const float2 z = fma2(make_float2(ol[2], ol[3]), make_float2(down, down), make_float2(o[2], o[3]));
+          add2(acc[2 * blk + m][0], acc[2 * blk + m][1], x.x, x.y);
+          add2(acc[2 * blk + m][2], acc[2 * blk + m][3], z.x, z.y);
         }
       }
     if (weird) {

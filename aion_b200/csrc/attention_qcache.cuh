@@ -83,6 +83,19 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
   *hi = h;
   *lo = pack_half2(la, lb);
 }
+// The same with the second term times 2^11, for weights: they reach down to where f16 has no more bits (a small weight, or small
+// values beside large ones), and so scaled the second term keeps eleven bits where the first one has none left. Together they are
+// good to 2^-23 of x down to 2^-14, and to 2^-37 below that. Its products have a sum of their own.
+constexpr float LO_SCALE = 2048.0f;
+__device__ __forceinline__ void split2_scaled(float a, float b, uint32_t* hi, uint32_t* lo) {
+  const uint32_t h = pack_half2(a, b);
+  float la, lb;   // 2^11 x - 2^11 hi
+  asm("{.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xE800;\n\tfma.rn.f32.f16 %0, l, m, %3;\n\tfma.rn.f32.f16 %1, h, m, %4;\n\t}"
+      : "=f"(la), "=f"(lb)
+      : "r"(h), "f"(a * LO_SCALE), "f"(b * LO_SCALE));
+  *hi = h;
+  *lo = pack_half2(la, lb);
+}
 
 // cap * tanh(x / cap) of N logits. Up to |x| = cap, where capped logits mostly lie, tanh is the sixth convergent of
 // Lambert's continued fraction z / (1 + z^2 / (3 + z^2 / (5 + ...))), whose error at z = 1 is 7e-10; beyond it tanhf.
@@ -109,6 +122,13 @@ __device__ __forceinline__ void cap_logits(float (&x)[N], float cap, float inv_c
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)), "l"(*reinterpret_cast<const uint64_t*>(&c)));
   return *reinterpret_cast<const float2*>(&d);
 }
 __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {

@@ -5,6 +5,8 @@
 //  * f32 attention on f16 operands: q, P = exp2(S - max), and the dequantized K and V (code * scale is 19 bits) are two f16
 //    terms each, and each product is the sum of three (lo.hi, hi.lo, hi.hi; what is left out is 2^-22). So the tensor pipe does
 //    6 * 2 * rows * keys * D operations for the 4 * rows * keys * D that f32 attention counts: a third of its rate is the ceiling.
+//    P's second term is held times 2^11 and scaled back as the sum goes on (scale-input-d): the power of two that P is normed by
+//    follows the largest V scale that any row of the block sees, and so a weight on a small V keeps its 23 bits down to 2^-28 of it.
 //  * A row of a cache is brought to a common power of two, so that its largest scale lies in [2^7, 2^8): a small scale next to
 //    a large one of another row loses nothing. The power comes back per key, times the logit and times P.
 //  * Both products take A from tensor memory: q (two terms, D columns) stays there for the whole walk, P overwrites the logits
@@ -95,16 +97,17 @@ constexpr uint32_t IDESC_QK = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 2
 // D[tmem] (+)= A[tmem] . B[smem desc], four steps of K = 16: A eight columns further each (the third and fourth SKIP more), B
 // STEP units of its descriptor. The whole warp comes here and one elected thread, always the same, issues: so the operands stay
 // in uniform registers and an instruction is issued in the 32 clocks that it takes. (Inside a branch of one thread 49 clocks each.)
-template <int SKIP, int STEP>
+// What D holds before is worth 2^-DOWN of it.
+template <int SKIP, int STEP, int DOWN = 0>
 __device__ __forceinline__ void umma_f16_ts4(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p, e;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\telect.sync _|e, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, %5;\n\tadd.u32 a3, %1, %6;\n\tadd.u64 b1, %2, %7;\n\tadd.u64 b2, %2, %8;\n\tadd.u64 b3, %2, %9;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, %10;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, 1;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, 1;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, 1;\n\t}" ::"r"(d),
-      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(16 + SKIP), "n"(24 + SKIP), "n"(STEP), "n"(2 * STEP), "n"(3 * STEP)
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(16 + SKIP), "n"(24 + SKIP), "n"(STEP), "n"(2 * STEP), "n"(3 * STEP), "n"(DOWN)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit_elected(uint32_t bar) {
@@ -155,13 +158,6 @@ __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t h2_rest(uint32_t a, uint32_t b, uint32_t c) {   // a * b - c
   const __half2 d = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), __hneg2(*reinterpret_cast<__half2*>(&c)));
   return *reinterpret_cast<const uint32_t*>(&d);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)), "l"(*reinterpret_cast<const uint64_t*>(&c)));
-  return *reinterpret_cast<const float2*>(&d);
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
@@ -542,8 +538,8 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
             const float4 v = vexp[i];
             const float* x = s + 16 * j + 4 * i;
             const float2 w0 = mul2(make_float2(x[0], x[1]), mul2(make_float2(v.x, v.y), unit)), w1 = mul2(make_float2(x[2], x[3]), mul2(make_float2(v.z, v.w), unit));
-            split2(w0.x, w0.y, &h[2 * i], &l[2 * i]);
-            split2(w1.x, w1.y, &h[2 * i + 1], &l[2 * i + 1]);
+            split2_scaled(w0.x, w0.y, &h[2 * i], &l[2 * i]);
+            split2_scaled(w1.x, w1.y, &h[2 * i + 1], &l[2 * i + 1]);
           }
           tmem_st8(at + 8 * j, h);
           tmem_st8(at + 16 + 8 * j, l);
@@ -686,9 +682,11 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           tc_fence_after();
           {
             const uint32_t d = t0 + G::T_O + (n & 1) * 64, ph = t0 + G::T_S + (it & 1) * 64;
-#pragma unroll 1
-            for (int j = 0; j < 3; j++)   // 16 keys: eight columns of P, two groups of eight rows of V
-              umma_f16_ts4<16, (2048 >> 4)>(d, ph + (j == 0 ? 16 : 0), (j == 1 ? vl : vh) + q * (PANEL >> 4), IDESC_PV, j);
+            // 16 keys: eight columns of P, two groups of eight rows of V. P's second term is times 2^11.
+            static_assert(LO_SCALE == 2048.0f, "2^11");
+            umma_f16_ts4<16, (2048 >> 4)>(d, ph + 16, vh + q * (PANEL >> 4), IDESC_PV, 0);
+            umma_f16_ts4<16, (2048 >> 4), 11>(d, ph, vl + q * (PANEL >> 4), IDESC_PV, 1);
+            umma_f16_ts4<16, (2048 >> 4)>(d, ph, vh + q * (PANEL >> 4), IDESC_PV, 1);
             umma_commit_elected(o_full + 8 * (n & 1));
             if (q == NP - 1) umma_commit_elected(v_free);
           }

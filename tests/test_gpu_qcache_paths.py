@@ -223,3 +223,55 @@ def test_weights_are_exact_to_the_last_bits_whatever_the_values_size(sess, backe
     w = np.exp(-x.astype(np.float64))[..., None]
     rel = got / (64 * vscale) / (w / (1 + w)) - 1
     assert np.sqrt((rel[..., 0] ** 2).mean()) <= 0.63 * 2.9 * 2.0 ** -24
+
+
+def spread_case(rng, kdt, vdt, T, L, H, D, Hq):
+    """Queries of one dimension, keys that are whole numbers there: a logit is one exact product, in [-1, 1]."""
+    q = np.zeros((1, L, Hq, D), np.float32)
+    q[..., 5] = 2.0 ** -3
+    codes = np.zeros((1, T, H, D))
+    codes[..., 5] = rng.integers(-7, 8, (1, T, H))
+    vc = rng.integers(-7, 8, (1, T, H, D))
+    return q, codes, vc
+
+
+def spread_bound(w, values, ymax):
+    """The weights' errors (the logit's move to base 2 and the difference: 5 * 2^-24 of the largest logit, exp2 2^-22, two f16 terms
+    2^-22) count twice (sum and quotient), sums of N terms N + 16 roundings, each of them times sum w |v| / sum w."""
+    mean_abs = w @ np.abs(values) / w.sum()
+    return (2 * (5 * ymax * 2.0 ** -24 + 2.0 ** -21) + (len(w) + 16) * 2.0 ** -24) * mean_abs
+
+
+@pytest.mark.parametrize("flags,kernel", **FORCED)
+@pytest.mark.parametrize("vdt", [Q8, Q4], ids=["q8", "q4"])
+@pytest.mark.parametrize("D,H", [(64, 4), (128, 2), (256, 1)])
+@pytest.mark.parametrize("small", [2.0 ** -4, 2.0 ** -9, 2.0 ** -14])
+@pytest.mark.parametrize("seen", [False, True])
+def test_a_huge_value_row_costs_the_others_nothing(sess, backend, D, H, vdt, small, seen, flags, kernel):
+    """One key's V has scales of 65504, the others' are `small`: rows that do not see the key (causal), and rows that give it a weight
+    of e^-100, keep f32's precision in what they make of the others."""
+    L, T, at = 12, 60, 45
+    rng = np.random.default_rng([D, vdt])
+    q, codes, vc = spread_case(rng, Q8, vdt, T, L, H, D, 2 * H)
+    if seen:
+        q[..., 6], codes[0, at, :, 6] = 2.0 ** -3, -100
+        codes[0, at, :, 5] = 0
+        q[..., 6] *= 8.0
+    pos = np.arange(at - 6, at - 6 + L, dtype=np.int32)[None] if not seen else np.full((1, L), T - 1, np.int32)
+    k = blocks(Q8, codes, np.ones((1, T, H, D // 32)))
+    vs = np.full((1, T, H, D // 32), small) * (1 + rng.integers(0, 512, (1, T, H, D // 32)) / 1024)
+    vs[0, at] = 65504
+    vs = vs.astype(np.float16)
+    v = blocks(vdt, vc, vs)
+    got, _ = run_attention(sess, q, k, v, Q8, vdt, scale=1.0, positions=pos, lengths=[T], window=AttentionWindow.causal(), flags=flags, spoil_rows=False)
+    assert launched(backend)[0] == kernel
+    vals = ref.unpack(vdt, v)
+    for l in range(L):
+        n = int(pos[0, l]) + 1
+        if not seen and n > at:
+            continue
+        for h in range(2 * H):
+            y = codes[0, :n, h // 2] @ q[0, l, h].astype(np.float64)
+            w = np.exp(y - y.max())
+            want, bound = w @ vals[0, :n, h // 2] / w.sum(), spread_bound(w, vals[0, :n, h // 2], 1.0)
+            assert (np.abs(got[0, l, h] - want) <= bound).all(), (l, h, np.abs(got[0, l, h] - want).max(), bound.max())
