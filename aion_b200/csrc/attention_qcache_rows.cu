@@ -7,8 +7,10 @@
 //    6 * 2 * rows * keys * D operations for the 4 * rows * keys * D that f32 attention counts: a third of its rate is the ceiling.
 //    P's second term is held times 2^11 and scaled back as the sum goes on (scale-input-d): the power of two that P is normed by
 //    follows the largest V scale that any row of the block sees, and so a weight on a small V keeps its 23 bits down to 2^-28 of it.
-//  * A row of a cache is brought to a common power of two, so that its largest scale lies in [2^7, 2^8): a small scale next to
-//    a large one of another row loses nothing. The power comes back per key, times the logit and times P.
+//  * A row of a cache is brought to a common power of two, so that its largest scale lies in [2^14, 2^15), and its codes count
+//    1/128 each: a scale next to a larger one of its row is exact over 28 powers of two, and one next to another row's
+//    loses nothing at all. Code times scale is exact down to 2^-21 of the row's largest scale, below that good to 2^-32 of
+//    it. The power comes back per key, times the logit and times P.
 //  * Both products take A from tensor memory: q (two terms, D columns) stays there for the whole walk, P overwrites the logits
 //    it is made of. Shared memory holds the two B operands, one 128-byte-swizzled panel per 64 dimensions, K read K-major and V
 //    N-major, so that both are unpacked the same way.
@@ -181,12 +183,12 @@ struct Unpack {
     for (int x = KPW; x < 32; x *= 2) e = max(e, __shfl_xor_sync(FULL, e, x));
     return e;
   }
-  // The two scales in units of 2^(e - 22).
+  // The two scales in units of 2^(e - 29).
   static __device__ __forceinline__ uint32_t normed(const uint32_t (&sc)[2], uint32_t e) {
-    const float up = pow2f(22 - (int)e);
+    const float up = pow2f(29 - (int)e);
     return pack_half2(half_bits(sc[0]) * up, half_bits(sc[1]) * up);
   }
-  // One block of a key (the panel's first or second): 32 codes times its (normed) scale, as two f16 terms. `row` is where the
+  // One block of a key (the panel's first or second): 32 codes, 1/128 each, times its (normed) scale, as two f16 terms. `row` is where the
   // panel's bytes begin. (One code for both: the loop's instructions have to stay in the cache, see the kernel.)
   static __device__ __forceinline__ void block(const uint8_t* row, uint32_t second, uint32_t pair, uint8_t* hi, uint8_t* lo, uint32_t key) {
     const uint32_t s2 = __byte_perm(pair, 0, second ? 0x3232 : 0x1010);
@@ -217,8 +219,12 @@ struct Unpack {
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         uint32_t u[4];
-        unpack_q8(w[2 * c], &u[0], &u[1]);
-        unpack_q8(w[2 * c + 1], &u[2], &u[3]);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {   // 0x6400 | (n + 128) is 1152 + n: 9 + n / 128
+          const uint32_t x = w[2 * c + i] ^ 0x80808080u;
+          u[2 * i] = h2_fma(__byte_perm(x, 0x64646464u, 0x4140), 0x20002000u, 0xC880C880u);
+          u[2 * i + 1] = h2_fma(__byte_perm(x, 0x64646464u, 0x4342), 0x20002000u, 0xC880C880u);
+        }
         store(c, u);
       }
     } else {
@@ -226,8 +232,8 @@ struct Unpack {
       for (int c = 0; c < 4; c++) {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++)   // a byte's low and high nibble: 1024 + n and 1024 + 16 n
-          u[i] = h2_fma((__byte_perm(w[c], 0, 0x4040 + 0x0101 * i) & 0x00F0000Fu) | 0x64006400u, 0x2C003C00u, 0xD480E408u);
+        for (int i = 0; i < 4; i++)   // a byte's low and high nibble, 1024 + n and 1024 + 16 n: 8 + n / 128 and 1/2 + n / 128
+          u[i] = h2_fma((__byte_perm(w[c], 0, 0x4040 + 0x0101 * i) & 0x00F0000Fu) | 0x64006400u, 0x10002000u, 0xB880C808u);
         store(c, u);
       }
     }

@@ -342,8 +342,10 @@ typedef struct AionCudaAttention {
 /* Quantized K / V: k_dtype and v_dtype may be AION_CUDA_DTYPE_Q8_0 or AION_CUDA_DTYPE_Q4_0, each of
  * its own (both quantized, or neither): the caches that aion_cuda_sequence_append and
  * aion_cuda_qk_norm_rope_append write. Everything above holds for them (a page table may then have
- * any positive page_tokens). Keys and values are used as code x scale, logits and sums are f32: the
- * result is that of f32 attention over the dequantized cache. A page number outside the pool is
+ * any positive page_tokens). Keys and values are used as code x scale, logits and sums are f32, queries
+ * (against the largest of their row) and weights are good to 22 bits: the result is as close as that of
+ * f32 attention over the dequantized cache. Where blocks of rows are taken, a value is good to 2^-32 of
+ * the largest scale in its head row, if not to 22 bits. A page number outside the pool is
  * reported like a bad length, and its keys are left out.
  * Which kernel works: heads of 64, 128 and 256 (d_k = d_v) go by columns of eight or, where that is
  * cheaper, by blocks of 128 rows. ROW_UNITS takes columns. BLOCKS takes rows where they can be taken:

@@ -275,3 +275,32 @@ def test_a_huge_value_row_costs_the_others_nothing(sess, backend, D, H, vdt, sma
             w = np.exp(y - y.max())
             want, bound = w @ vals[0, :n, h // 2] / w.sum(), spread_bound(w, vals[0, :n, h // 2], 1.0)
             assert (np.abs(got[0, l, h] - want) <= bound).all(), (l, h, np.abs(got[0, l, h] - want).max(), bound.max())
+
+
+@pytest.mark.parametrize("flags,kernel", **FORCED)
+@pytest.mark.parametrize("vdt", [Q8, Q4], ids=["q8", "q4"])
+@pytest.mark.parametrize("D,H", [(64, 4), (128, 2), (256, 1)])
+@pytest.mark.parametrize("ratio", [2.0 ** 8, 2.0 ** 16, 2.0 ** 24])
+def test_a_huge_block_costs_the_others_of_its_rows_little(sess, backend, D, H, vdt, ratio, flags, kernel):
+    """The scales of one block of every V row are `ratio` times the others': these keep f32's precision. The rows kernel holds a value as
+    two f16 terms of which the row's largest scale is at most 2^15 of 128 codes: half of f16's last bit, 2^-25, is 2^-32 of that scale."""
+    L, T = 3, 50
+    rng = np.random.default_rng([D, vdt, 1])
+    q, codes, vc = spread_case(rng, Q8, vdt, T, L, H, D, 2 * H)
+    if vdt == Q8:
+        vc = rng.integers(-127, 128, vc.shape)
+    k = blocks(Q8, codes, np.ones((1, T, H, D // 32)))
+    vs = 2.0 ** -10 * (1 + rng.integers(0, 512, (1, T, H, D // 32)) / 1024)
+    vs[..., -1] *= ratio
+    v = blocks(vdt, vc, vs)
+    got, _ = run_attention(sess, q, k, v, Q8, vdt, scale=1.0, flags=flags)
+    assert launched(backend)[0] == kernel
+    vals = ref.unpack(vdt, v)
+    for l in range(L):
+        for h in range(2 * H):
+            y = codes[0, :, h // 2] @ q[0, l, h].astype(np.float64)
+            w = np.exp(y - y.max())
+            want, bound = w @ vals[0, :, h // 2] / w.sum(), spread_bound(w, vals[0, :, h // 2], 1.0)
+            if kernel == ROWS:
+                bound = bound + 2.0 ** -32 * vs[0, :, h // 2].max()
+            assert (np.abs(got[0, l, h] - want) <= bound).all(), (l, h, np.abs(got[0, l, h] - want).max(), bound.max())
