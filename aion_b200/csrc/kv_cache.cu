@@ -7,6 +7,7 @@
 // launch and one trip to memory the small ones.
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "cache_geom.cuh"
 #include "common.cuh"
@@ -588,6 +589,26 @@ int32_t cache_geom(uint64_t batch, uint64_t t_cap, uint32_t rolling, const AionC
   return AION_CUDA_OK;
 }
 
+// A stretch of device memory that a step reads or writes; p null: an operand that is absent.
+struct Span {
+  const void* p;
+  uint64_t bytes;
+};
+// What one warp writes no other may read or write: no written operand overlaps another one, read or written.
+int32_t check_apart(const char* what, std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  auto overlap = [](const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
+  };
+  for (const Span& w : written) {
+    for (const Span& o : written)
+      if (&o != &w && overlap(w, o)) return fail(AION_CUDA_INVALID_ARGUMENT, "%s: operands overlap", what);
+    for (const Span& o : read)
+      if (overlap(w, o)) return fail(AION_CUDA_INVALID_ARGUMENT, "%s: operands overlap", what);
+  }
+  return AION_CUDA_OK;
+}
+
 unsigned blocks_for(const AionCudaDevice* dev, uint64_t items, unsigned per_block) {
   const uint64_t want = ceil_div(items, (uint64_t)per_block), cap = (uint64_t)dev->sm_count * 16;
   return (unsigned)(want < cap ? want : cap);
@@ -653,7 +674,6 @@ int32_t append_quantized(AionCudaDevice* dev, const AionCudaSequenceAppend* s) {
   if (int32_t st = cache_geom(s->batch, s->t_cap, s->rolling, s->page_table, s->page_tokens, s->pool_pages, what, &g, &rows)) return st;
   const uint64_t row_values = s->heads * s->head_dim;
   if (rows > (1ull << 40) / row_values * 64 || s->batch * s->new_len > (1ull << 31)) return fail(AION_CUDA_UNSUPPORTED, "%s: shape beyond what the kernels index", what);
-  if (int32_t st = dev->make_current()) return st;
   uint8_t *cache, *nk;
   const int32_t* idx;
   if (int32_t st = resolve(s->cache, cache_bytes(s->dtype, rows * row_values), "sequence_append.cache", &cache)) return st;
@@ -662,6 +682,10 @@ int32_t append_quantized(AionCudaDevice* dev, const AionCudaSequenceAppend* s) {
   if (int32_t st = resolve(s->end_index, s->batch * sizeof(int32_t), "sequence_append.end_index", &idx)) return st;
   if ((reinterpret_cast<uintptr_t>(cache) & 1) || (reinterpret_cast<uintptr_t>(nk) & (eb - 1)))
     return fail(AION_CUDA_INVALID_ARGUMENT, "%s: misaligned operand", what);
+  if (int32_t st = check_apart(what, {{cache, cache_bytes(s->dtype, rows * row_values)}},
+                               {{nk, s->batch * s->new_len * row_values * eb}, {idx, s->batch * sizeof(int32_t)}, {g.table, s->batch * g.pages_per_request * sizeof(int32_t)}}))
+    return st;
+  if (int32_t st = dev->make_current()) return st;
   if (eb == 4) return launch_append(dev, s, cache, reinterpret_cast<const float*>(nk), idx, g);
   return launch_append(dev, s, cache, reinterpret_cast<const __half*>(nk), idx, g);
 }
@@ -689,7 +713,6 @@ int32_t aion_cuda_sequence_read(AionCudaDevice* dev, const AionCudaSequenceRead*
   if (int32_t st = cache_geom(s->batch, s->t_cap, s->rolling, s->page_table, s->page_tokens, s->pool_pages, what, &g, &rows)) return st;
   const uint64_t row_values = s->heads * s->head_dim;
   if (rows > (1ull << 40) / row_values * 64 || s->batch * s->out_len > (1ull << 31)) return fail(AION_CUDA_UNSUPPORTED, "%s: shape beyond what the kernels index", what);
-  if (int32_t st = dev->make_current()) return st;
   uint8_t *out, *cache;
   const int32_t *start = nullptr, *lengths = nullptr;
   const uint64_t ob = s->out_dtype == AION_CUDA_DTYPE_F32 ? 4 : 2;
@@ -702,9 +725,11 @@ int32_t aion_cuda_sequence_read(AionCudaDevice* dev, const AionCudaSequenceRead*
   const uintptr_t cache_align = s->dtype == AION_CUDA_DTYPE_F32 ? 3 : 1;
   if ((reinterpret_cast<uintptr_t>(cache) & cache_align) || (reinterpret_cast<uintptr_t>(out) & (ob - 1)))
     return fail(AION_CUDA_INVALID_ARGUMENT, "%s: misaligned operand", what);
-  const uint64_t out_bytes = s->batch * s->out_len * row_values * ob, all_bytes = cache_bytes(s->dtype, rows * row_values);
-  if (reinterpret_cast<uintptr_t>(out) < reinterpret_cast<uintptr_t>(cache) + all_bytes && reinterpret_cast<uintptr_t>(cache) < reinterpret_cast<uintptr_t>(out) + out_bytes)
-    return fail(AION_CUDA_INVALID_ARGUMENT, "%s: out overlaps the cache", what);
+  const uint64_t per_request = s->batch * sizeof(int32_t);
+  if (int32_t st = check_apart(what, {{out, s->batch * s->out_len * row_values * ob}},
+                               {{cache, cache_bytes(s->dtype, rows * row_values)}, {start, per_request}, {lengths, per_request}, {g.table, per_request * g.pages_per_request}}))
+    return st;
+  if (int32_t st = dev->make_current()) return st;
   if (ob == 4) return launch_read(dev, s, reinterpret_cast<float*>(out), cache, start, lengths, g);
   return launch_read(dev, s, reinterpret_cast<__half*>(out), cache, start, lengths, g);
 }
@@ -734,7 +759,6 @@ int32_t aion_cuda_qk_norm_rope_append(AionCudaDevice* dev, const AionCudaQKNormR
   if (int32_t st = cache_geom(s->batch, s->t_cap, s->rolling, s->page_table, s->page_tokens, s->pool_pages, what, &p.geom, &cache_rows)) return st;
   const uint64_t row_values = s->h_kv * d, rows = s->batch * s->len;
   if (row_values && cache_rows > (1ull << 40) / row_values * 64) return fail(AION_CUDA_UNSUPPORTED, "%s: shape beyond what the kernels index", what);
-  if (int32_t st = dev->make_current()) return st;
   if (s->h_q)
     if (int32_t st = resolve(s->q_out, rows * s->h_q * d * sizeof(float), "qk_norm_rope_append.q_out", &p.q_out)) return st;
   if (int32_t st = resolve(s->qkv, ((rows - 1) * ld + width) * sizeof(float), "qk_norm_rope_append.qkv", &p.qkv)) return st;
@@ -752,14 +776,14 @@ int32_t aion_cuda_qk_norm_rope_append(AionCudaDevice* dev, const AionCudaQKNormR
                          reinterpret_cast<uintptr_t>(p.k_gamma);
   if ((f32s & 3) || ((reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache)) & 1))
     return fail(AION_CUDA_INVALID_ARGUMENT, "%s: misaligned operand", what);
-  // What one warp writes no other may read or write: K and V are two caches, q_out is not the projection.
-  auto overlap = [](const void* a, uint64_t na, const void* b, uint64_t nb) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return a && b && x < y + nb && y < x + na;
-  };
-  if (overlap(p.k_cache, cache_bytes(s->k_dtype, cache_rows * row_values), p.v_cache, cache_bytes(s->v_dtype, cache_rows * row_values)) ||
-      overlap(p.q_out, rows * s->h_q * d * sizeof(float), p.qkv, ((rows - 1) * ld + width) * sizeof(float)))
-    return fail(AION_CUDA_INVALID_ARGUMENT, "%s: operands overlap", what);
+  if (int32_t st = check_apart(what,
+                               {{p.k_cache, cache_bytes(s->k_dtype, cache_rows * row_values)}, {p.v_cache, cache_bytes(s->v_dtype, cache_rows * row_values)},
+                                {p.q_out, rows * s->h_q * d * sizeof(float)}},
+                               {{p.qkv, ((rows - 1) * ld + width) * sizeof(float)}, {p.q_gamma, d * sizeof(float)}, {p.k_gamma, d * sizeof(float)},
+                                {p.positions, rows * sizeof(int32_t)}, {p.end_index, s->batch * sizeof(int32_t)},
+                                {p.geom.table, s->batch * p.geom.pages_per_request * sizeof(int32_t)}}))
+    return st;
+  if (int32_t st = dev->make_current()) return st;
   p.len = (uint32_t)s->len, p.h_q = (uint32_t)s->h_q, p.h_kv = (uint32_t)s->h_kv, p.d = (uint32_t)d;
   p.ld = ld;
   p.rope_pairs = pf > (float)(d / 2) ? (uint32_t)(d / 2) : (uint32_t)pf;

@@ -447,7 +447,7 @@ AION_CUDA_API int32_t aion_cuda_sequence_append(AionCudaDevice* dev, const AionC
  *  - aion_cuda_sequence_append with such a dtype quantizes new_kv [B, Ln, H, D] (new_dtype) as it
  *    is written: the blocks are those that aion_cuda_quantize makes of the rows. page_tokens may be
  *    any positive number. An f16 or f32 cache ignores new_dtype: its rows have the cache's type.
- *    Of more new rows than a ring holds, the last T stay.
+ *    Of more new rows than a ring holds, the last T stay. The cache must not overlap what is read.
  *  - aion_cuda_sequence_read gives logical steps back as values:
  *      out [B, out_len, H, D] (out_dtype f32 or f16), row t of request b = step start_index[b] + t.
  *    lengths i32 [B] says how many logical steps each request has (absent: t_cap): steps
@@ -456,7 +456,7 @@ AION_CUDA_API int32_t aion_cuda_sequence_append(AionCudaDevice* dev, const AionC
  *    code x scale, exact in f32 (aion_cuda_dequantize) and rounded once to f16.
  *    A negative start or length, a length beyond a plain or paged cache, or a page number outside
  *    the pool is reported by the next aion_cuda_sync / aion_cuda_d2h; the rows it concerns become
- *    zeros. Pages without a step that is read are not looked up. out must not overlap the cache. */
+ *    zeros. Pages without a step that is read are not looked up. out must not overlap what is read. */
 typedef struct AionCudaSequenceRead AionCudaSequenceRead;
 struct AionCudaSequenceRead {
   AionCudaOperand out, cache;
@@ -536,8 +536,8 @@ AION_CUDA_API int32_t aion_cuda_rope_kv_append(AionCudaDevice* dev, const AionCu
  *   v_dtype, each f16, q8_0 or q4_0: rows end_index[b] + l receive RoPE(norm(k)) and v.
  * Range rules, rolling and pages as in aion_cuda_sequence_append, except that q_out is written
  * for every row. A head whose mean square is not finite is reported by the next aion_cuda_sync /
- * aion_cuda_d2h (nothing of that head is written). q_out must not overlap qkv, nor k_cache
- * v_cache. Of more new rows than a ring holds, the last t_cap stay. head_dim even, at most 1024,
+ * aion_cuda_d2h (nothing of that head is written). q_out, k_cache and v_cache must not overlap
+ * each other, nor anything that is read. Of more new rows than a ring holds, the last t_cap stay. head_dim even, at most 1024,
  * a multiple of 32 for a quantized cache.
  * Results equal RMSNorm, RoPE1D, Cast and SequenceAppend in sequence, up to the norm's statistic. */
 typedef struct AionCudaQKNormRopeAppend AionCudaQKNormRopeAppend;

@@ -296,3 +296,29 @@ def test_no_tile_of_attention_reaches_beyond_its_page_ring_or_cache(tmp_path):
             assert 0 < rows <= 16 and first + rows <= seg_len, (t_cap, page, rolling, lo, hi, seg, first, rows)
             keys += range(seg * seg_len + first, seg * seg_len + first + rows)
         assert keys == sorted(set(keys)) and set(range(lo, hi)) <= set(keys), (t_cap, page, rolling, lo, hi)
+
+
+# ---- operands that overlap ----------------------------------------------------------------------
+def _apart(**kw):
+    """Operands of their own, a gigabyte apart, but for those that `kw` places: name=(other's name, bytes into it)."""
+    def place(names):
+        at = {n: (i + 1) << 30 for i, n in enumerate(names)}
+        for n, (other, off) in kw.items():
+            at[n] = at[other] + off
+        return {n: capi.Operand(at[n], 0, 1 << 29) for n in names}
+    return place
+
+
+@pytest.mark.parametrize("fn,make,names,case", [
+    *[("aion_cuda_sequence_append", _append, ("cache", "new_kv", "end_index"), {n: ("cache", off)})
+      for n, off in (("new_kv", 0), ("new_kv", 2 * 64 * 2 * 68 - 4), ("end_index", 8))],
+    ("aion_cuda_sequence_append", _append, ("cache", "new_kv", "end_index"), {"cache": ("new_kv", 2 * 2 * 64 * 4 - 2)}),
+    *[("aion_cuda_sequence_read", _read, ("out", "cache", "start_index", "lengths"), {n: ("out", 4)}) for n in ("start_index", "lengths")],
+    ("aion_cuda_sequence_read", _read, ("out", "cache", "start_index", "lengths"), {"cache": ("out", 2 * 3 * 2 * 64 * 4 - 4)}),
+    *[("aion_cuda_qk_norm_rope_append", _rope, ("q_out", "qkv", "q_gamma", "k_gamma", "positions", "end_index", "k_cache", "v_cache"), {a: (b, 0)})
+      for a, b in (("k_cache", "qkv"), ("v_cache", "qkv"), ("k_cache", "q_out"), ("q_out", "v_cache"), ("q_out", "qkv"), ("v_cache", "k_cache"),
+                   ("q_gamma", "q_out"), ("positions", "k_cache"), ("end_index", "v_cache"))],
+])
+def test_operands_that_overlap_are_refused_before_any_cuda_call(fn, make, names, case):
+    got, message = _call(fn, make(**_apart(**case)(names)))
+    assert got == INV and "overlap" in message, (got, message)
