@@ -37,7 +37,7 @@ from typing import Callable, Optional
 import numpy as np
 
 from . import capi
-from .backend import (AttentionWindow, Chunk, CudaBackend, CudaSession, DeviceStore, StepArgMax, StepAttention, StepCast,
+from .backend import (AttentionWindow, BackendError, Chunk, CudaBackend, CudaSession, DeviceStore, StepArgMax, StepAttention, StepCast,
                       StepElemwiseBinary, StepGatherRows, StepMatMul, StepRMSNorm, StepRMSNormPair, StepRoPE1D,
                       StepRopeKVAppend, StepSequenceAppend, StepQKNormRopeAppend, TensorMeta, _check, act_image_meta)
 
@@ -57,16 +57,26 @@ class DecoderConfig:
     eps: float = 1e-6
     rope_base: float = 10000.0
     weight_dtype: int = Q4
-    # KV cache: f16, or q8_0 / q4_0 blocks (53 % and 28 % of its bytes); K and V each of their own type.
+    # KV cache: f16, or q8_0 / q4_0 blocks (53 % and 28 % of its bytes), then K and V each of their own type.
     k_dtype: int = F16
     v_dtype: int = F16
     # RMSNorm of every query and key head (gamma = 1) before the rotation.
     qk_norm: bool = False
 
     @property
+    def quantized_cache(self) -> bool:
+        """q8_0 or q4_0 caches. Attention reads both quantized, or neither."""
+        quantized = self.k_dtype in (Q4, Q8)
+        if quantized != (self.v_dtype in (Q4, Q8)):
+            raise BackendError(capi.UNSUPPORTED, "decoder: K and V are both quantized, or neither")
+        if quantized and self.head_dim % 32:
+            raise BackendError(capi.UNSUPPORTED, f"decoder: a quantized cache needs heads of whole 32-blocks, got {self.head_dim}")
+        return quantized
+
+    @property
     def plain_cache(self) -> bool:
         """f16 caches and heads without a norm: `StepRopeKVAppend`; else `StepQKNormRopeAppend`."""
-        return self.k_dtype == F16 and self.v_dtype == F16 and not self.qk_norm
+        return not self.quantized_cache and not self.qk_norm
 
     @property
     def q_width(self) -> int:
@@ -113,6 +123,8 @@ class SyntheticDecoder:
     def __init__(self, backend: CudaBackend, cfg: DecoderConfig, requests: int,
                  weight_values: Callable[[str, int, int], object], embedding_values: Callable[[int, int], object],
                  store: Optional[DeviceStore] = None, fused: bool = True, images: bool = True):
+        if not cfg.quantized_cache and fused and (cfg.k_dtype, cfg.v_dtype) != (F16, F16):
+            raise BackendError(capi.UNSUPPORTED, "decoder: the fused steps append to f16, q8_0 or q4_0 caches")
         self.backend, self.cfg, self.requests, self.fused = backend, cfg, requests, fused
         # Images ride on the fused steps and on rows the register-resident norm kernel takes.
         self.images = bool(images and fused and cfg.hidden % 32 == 0 and cfg.hidden <= 4096 and cfg.ffn % 32 == 0

@@ -322,3 +322,12 @@ def _apart(**kw):
 def test_operands_that_overlap_are_refused_before_any_cuda_call(fn, make, names, case):
     got, message = _call(fn, make(**_apart(**case)(names)))
     assert got == INV and "overlap" in message, (got, message)
+
+
+@pytest.mark.parametrize("kw", [dict(k_dtype=Q8), dict(v_dtype=Q4), dict(k_dtype=F16, v_dtype=Q8, qk_norm=True), dict(k_dtype=Q8, v_dtype=Q8, head_dim=48),
+                                dict(k_dtype=F32, v_dtype=F32), dict(k_dtype=F32, v_dtype=F16)], ids=str)
+def test_a_decoder_whose_caches_attention_cannot_read_is_refused_when_it_is_built(kw):
+    from aion_b200.decoder import DecoderConfig, SyntheticDecoder
+    with pytest.raises(BackendError) as e:
+        SyntheticDecoder(_Backend(), DecoderConfig(layers=1, **kw), 1, None, None)
+    assert e.value.name == "Unsupported"
