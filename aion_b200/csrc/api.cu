@@ -334,9 +334,8 @@ int32_t aion_cuda_attention(AionCudaDevice* dev, const AionCudaAttention* s) {
     return fail(AION_CUDA_INVALID_ARGUMENT, "attention: %llu query heads over %llu kv heads", (unsigned long long)s->h_q,
                 (unsigned long long)s->h_kv);
   if (s->t_cap == 0) return fail(AION_CUDA_INVALID_ARGUMENT, "attention: empty K/V");
-  if (s->batch * s->l_q * s->h_q == 0) return AION_CUDA_OK;
+  if (s->batch == 0 || s->l_q == 0) return AION_CUDA_OK;
   if (s->d_k == 0 || s->d_v == 0) return fail(AION_CUDA_INVALID_ARGUMENT, "attention: zero head dimension");
-  if (int32_t st = dev->make_current()) return st;
   return attention_launch(dev, s);
 }
 

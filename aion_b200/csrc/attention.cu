@@ -742,7 +742,8 @@ int32_t launch_decode(AionCudaDevice* dev, const AttnParams& p, uint32_t units) 
 int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
   AttnParams p{};
   const uint64_t B = s->batch, L = s->l_q, Hq = s->h_q, Hkv = s->h_kv, Dk = s->d_k, Dv = s->d_v, T = s->t_cap;
-  if (B > 0x7FFFFFFF || L > 0x7FFFFFFF || Hq > 65535 || Dk > 65535 || Dv > 65535 || T > 0x7FFFFFFF || B * L * Hq > 0x7FFFFFFF)
+  // (Checked factor by factor: no product here or below passes 64 bits.)
+  if (B > 0x7FFFFFFF || L > 0x7FFFFFFF || Hq > 65535 || Dk > 65535 || Dv > 65535 || T > 0x7FFFFFFF || B * L > 0x7FFFFFFF || B * L * Hq > 0x7FFFFFFF)
     return fail(AION_CUDA_UNSUPPORTED, "attention: a dimension is beyond what the kernels index");
   auto esz = [](uint32_t dt) { return dt == AION_CUDA_DTYPE_F32 ? 4u : 2u; };
   auto is_quant = [](uint32_t dt) { return dt == AION_CUDA_DTYPE_Q8_0 || dt == AION_CUDA_DTYPE_Q4_0; };
@@ -759,12 +760,13 @@ int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
       return fail(AION_CUDA_INVALID_ARGUMENT, "attention: page_tokens %llu", (unsigned long long)page_tokens);
     if (!quant && (page_tokens == 0 || page_tokens % KT != 0 || page_tokens > (1u << 20)))
       return fail(AION_CUDA_INVALID_ARGUMENT, "attention: page_tokens %llu must be a positive multiple of %d", (unsigned long long)page_tokens, KT);
-    if (pool_pages == 0 || pool_pages * page_tokens > 0x7FFFFFFFull)
-      return fail(AION_CUDA_INVALID_ARGUMENT, "attention: pool of %llu pages", (unsigned long long)pool_pages);
+    if (pool_pages == 0 || pool_pages > 0x7FFFFFFFull || page_tokens > 0x7FFFFFFFull || pool_pages * page_tokens > 0x7FFFFFFFull)
+      return fail(AION_CUDA_INVALID_ARGUMENT, "attention: pool of %llu pages of %llu tokens", (unsigned long long)pool_pages, (unsigned long long)page_tokens);
     if (s->rolling) return fail(AION_CUDA_UNSUPPORTED, "attention: a rolling cache cannot be paged");
     pages_per_request = (T + page_tokens - 1) / page_tokens;
   }
   const uint64_t kv_rows = paged ? pool_pages * page_tokens : B * T;
+  if (kv_rows > (1ull << 60) / (Hkv * (Dk + Dv))) return fail(AION_CUDA_UNSUPPORTED, "attention: a dimension is beyond what the kernels index");
   const uint8_t *q, *k, *v;
   float* out;
   if (int32_t st = resolve(s->q, B * L * Hq * Dk * esz(s->q_dtype), "attention.q", &q)) return st;
@@ -818,6 +820,7 @@ int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
     if (reinterpret_cast<uintptr_t>(p.image) & 15) return fail(AION_CUDA_INVALID_ARGUMENT, "attention.image: the image must be 16-byte aligned");
     p.image_dtype = s->image_dtype;
   }
+  if (int32_t st = dev->make_current()) return st;
   if (quant) return attention_qcache_launch(dev, p, s->flags);
   if (tensor_path) {
     const uint32_t group = p.Hq / p.Hkv;

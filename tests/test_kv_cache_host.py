@@ -331,3 +331,17 @@ def test_a_decoder_whose_caches_attention_cannot_read_is_refused_when_it_is_buil
     with pytest.raises(BackendError) as e:
         SyntheticDecoder(_Backend(), DecoderConfig(layers=1, **kw), 1, None, None)
     assert e.value.name == "Unsupported"
+
+
+@pytest.mark.parametrize("rec,status", [
+    (_attn(batch=1 << 30, l_q=1 << 30, h_q=16, h_kv=16), UNS),                                        # 2^64 rows: no rows modulo 2^64
+    (_attn(batch=274177, l_q=1, h_q=1 << 40, h_kv=1), UNS),
+    (_attn(k_dtype=F16, v_dtype=F16, batch=1 << 29, t_cap=(1 << 31) - 1, h_q=1, h_kv=1, d_k=128, d_v=128), UNS),
+    (_attn(batch=1 << 29, t_cap=(1 << 31) - 1, h_q=1, h_kv=1), UNS),
+    (_attn(page_table=OP, page_tokens=1 << 20, pool_pages=(1 << 44) + 1), INV),                       # 2^64 + 2^20 rows
+    (_attn(page_table=OP, page_tokens=0, pool_pages=2), INV),
+    (_attn(page_table=OP, page_tokens=1 << 30, pool_pages=2), INV),
+])
+def test_attention_refuses_sizes_whose_products_wrap(rec, status):
+    got, message = _call("aion_cuda_attention", rec)
+    assert got == status and "attention" in message, (got, message)
