@@ -756,8 +756,7 @@ int32_t attention_launch(AionCudaDevice* dev, const AionCudaAttention* s) {
   const uint64_t page_tokens = s->page_tokens, pool_pages = s->pool_pages;
   uint64_t pages_per_request = 0;
   if (paged) {
-    if (quant && (page_tokens == 0 || page_tokens > (1u << 20)))
-      return fail(AION_CUDA_INVALID_ARGUMENT, "attention: page_tokens %llu", (unsigned long long)page_tokens);
+    if (quant && page_tokens == 0) return fail(AION_CUDA_INVALID_ARGUMENT, "attention: page_tokens must be positive");
     if (!quant && (page_tokens == 0 || page_tokens % KT != 0 || page_tokens > (1u << 20)))
       return fail(AION_CUDA_INVALID_ARGUMENT, "attention: page_tokens %llu must be a positive multiple of %d", (unsigned long long)page_tokens, KT);
     if (pool_pages == 0 || pool_pages > 0x7FFFFFFFull || page_tokens > 0x7FFFFFFFull || pool_pages * page_tokens > 0x7FFFFFFFull)

@@ -304,3 +304,29 @@ def test_a_huge_block_costs_the_others_of_its_rows_little(sess, backend, D, H, v
             if kernel == ROWS:
                 bound = bound + 2.0 ** -32 * vs[0, :, h // 2].max()
             assert (np.abs(got[0, l, h] - want) <= bound).all(), (l, h, np.abs(got[0, l, h] - want).max(), bound.max())
+
+
+@pytest.mark.parametrize("L", [1, 3])
+def test_pages_of_more_than_a_million_tokens(sess, backend, L):
+    """A page may hold any number of tokens: two requests, each in a page of its own."""
+    import torch
+
+    from aion_b200.backend import Chunk, StepAttention, TensorMeta
+    s, store = sess
+    D, H, page, T = 64, 4, 1_100_003, 700
+    q, k, v = inputs([L], 2, T, H, D, L, 8, Q4, Q4)
+    tids, pools = [], []
+    for x in (k, v):
+        pool = torch.zeros((2, page, x[0, 0].size), dtype=torch.uint8, device="cuda")
+        for b in range(2):
+            pool[1 - b, :T] = torch.from_numpy(x[b].reshape(T, -1)).cuda()
+        tids.append(store.bind(TensorMeta(Q4, (2, page, H, D), quant_axis=3), Chunk(pool.data_ptr(), 0, pool.numel())))
+        pools.append(pool)
+    torch.cuda.synchronize()
+    lens, pos = [T, 123], causal([T, 123], L)
+    put = lambda a: store.add(TensorMeta(capi.DTYPE_I32, a.shape), a)
+    tq, to = store.add(TensorMeta(capi.DTYPE_F32, q.shape), q), store.add(TensorMeta(capi.DTYPE_F32, q.shape))
+    s.execute([StepAttention(out=to, q=tq, k=tids[0], v=tids[1], scale=0.125, query_positions=put(pos), kv_lengths=put(np.array(lens, np.int32)),
+                             window=AttentionWindow.causal(), page_table=put(np.array([[1], [0]], np.int32)), flags=capi.ATTENTION_BLOCKS)])
+    within(store.read(to), *ref.attention(q, k, v, Q4, Q4, scale=0.125, positions=pos, lengths=lens))
+    assert launched(backend)[0] == (ROWS if L > 1 else BOXES)
