@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   float* all = reinterpret_cast<float*>(smem);
   {
     float* mb = all + warp * G::WS;
-    // 2^(E - 29) in two exact steps: the product of the whole range would leave f32 for E = 0
+    // 2^(E - 29): exact, but where the sum itself is below f32's normal range
     const float back = __uint_as_float((127u + e_run - 29u) << 23);
 #pragma unroll
     for (int blk = 0; blk < NB; blk++)
@@ -990,8 +990,8 @@ int32_t attention_qcache_launch(AionCudaDevice* dev, AttnParams& p, uint32_t fla
     // Few columns at a time or 128 rows: by what each would cost. A unit of eight columns passes a key in 16, 24 or 31 ns
     // (D = 64, 128, 256) with all resident CTAs at work, after 8 us; a unit of 128 rows in 25, 34 or 51 ns, after 8, 10 or
     // 15 us and 1.1 us for each CTA of a cluster. (8 heads over 4 kv heads of 256: 32 positions of one request over 2048 keys
-    // 17 us by columns, 40 us by rows; of eight requests over 4096 keys 129 and 72 us, 256 positions 839 and 231 us. 16 over 4
-    // of 64: 16 and 23, 112 and 40, 617 and 233 us.)
+    // 17 us by columns, 40 us by rows; of eight requests over 4096 keys 130 and 72 us, 256 positions 846 and 231 us. 16 over 4
+    // of 64: 16 and 23, 112 and 40, 616 and 232 us.)
     const int size = p.Dk == 64 ? 0 : p.Dk == 128 ? 1 : 2;
     constexpr double column_ns[3] = {16.0, 24.0, 31.0}, row_ns[3] = {25.0, 34.0, 51.0}, row_start[3] = {8.0, 10.0, 15.0};
     const double sms = (double)dev->sm_count, keys = (double)max_keys;

@@ -22,9 +22,9 @@
 //  * A context too long for the few CTAs of a short prompt is cut over a cluster, whose CTAs add up their sums through
 //    distributed shared memory.
 //
-// 1024 rows against 8192 keys, 8 heads over 4 kv heads of 256, q8_0: 222 us, 289 TFLOP/s of the 4 * rows * keys * D that attention
-// counts (the products alone would take 103 us of a loop of 207); a causal prompt of 4096 tokens 217 us, 316 TFLOP/s; 32 over 8
-// heads of 128 538 us, 239 TFLOP/s. (On m16n8k16, eight warps of sixteen rows that held all in registers: 616, 596 and 1129 us.)
+// 1024 rows against 8192 keys, 8 heads over 4 kv heads of 256, q8_0: 224 us, 288 TFLOP/s of the 4 * rows * keys * D that attention
+// counts (the products alone take 118 us at 1634 TFLOP/s); a causal prompt of 4096 tokens 218 us, 315 TFLOP/s; 32 over 8
+// heads of 128 552 us, 233 TFLOP/s. (On m16n8k16, eight warps of sixteen rows that held all in registers: 616, 596 and 1129 us.)
 // What bounds it: the hand-overs between the roles of a stage; the tensor pipe is active 48 % of the cycles (59 % on the busiest
 // SM). The loop is straight code of four kinds and has to fit the instruction cache: with the products spelled out (their
 // descriptors went to local memory), a report in every wait and the unpacking once per block and operand it took 378 us.
@@ -51,7 +51,7 @@ constexpr int SK = SUBS * TK;         // keys of a stage
 constexpr int KRAWS = 3, VRAWS = 2;   // raw stages
 constexpr int SLOTS = 4;              // stages whose exponents and masks are kept
 // Registers of a softmax warp's thread and of the others'; they add up to what the block is launched with, 128 each. (Heads of
-// 256, whose sums alone take 128: 221 us, with 192 and 64 226; heads of 128: 157 and 152 us.)
+// 256, whose sums alone take 128, were 2 % slower with 192 and 64, heads of 128 3 % faster.)
 constexpr int softmax_regs(int d) { return d == 256 ? 200 : 192; }
 constexpr int other_regs(int d) { return 256 - softmax_regs(d); }
 static_assert(SK == 64 && FIRST_UNPACK + UW == RTHREADS / 32, "a stage is one panel of 64 keys");
@@ -932,7 +932,7 @@ int32_t launch_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap&
 
 int32_t attention_qcache_rows(AionCudaDevice* dev, const AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv, uint64_t max_keys) {
   const bool kq8 = p.k_dtype == AION_CUDA_DTYPE_Q8_0, vq8 = p.v_dtype == AION_CUDA_DTYPE_Q8_0;
-  // (A soft cap in a kernel of its own: its instructions in the loop cost the others 20 us of 177.)
+  // (A soft cap in a kernel of its own: its instructions in the loop cost the others 11 %.)
 #define AION_QROWS_AS(D, K, V) return p.soft_cap > 0.0f ? launch_rows<D, K, V, true>(dev, p, tk, tv, max_keys) : launch_rows<D, K, V, false>(dev, p, tk, tv, max_keys);
 #define AION_QROWS(D)                                          \
   if (kq8 && vq8) AION_QROWS_AS(D, true, true)                 \
