@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(THREADS, DecodeGeom<D, KQ8, VQ8>::CTAS) attn_q
   }
   __syncthreads();
   // With a soft cap the logits are wanted first; else they go straight to base 2.
-  const float to_base2 = p.soft_cap > 0.0f ? 1.0f : LOG2E, inv_cap = p.soft_cap > 0.0f ? 1.0f / p.soft_cap : 0.0f;
+  const float to_base2 = p.soft_cap > 0.0f ? 1.0f : LOG2E, inv_cap = p.soft_cap > 0.0f ? inverse_cap(p.soft_cap) : 0.0f;
   const float f0 = col_factor[2 * t] * to_base2, f1 = col_factor[2 * t + 1] * to_base2;
   const uint32_t lo_g = col_lo[g], hi_g = col_hi[g];
 

@@ -100,6 +100,8 @@ __device__ __forceinline__ void split2_scaled(float a, float b, uint32_t* hi, ui
 // cap * tanh(x / cap) of N logits. Up to |x| = cap, where capped logits mostly lie, tanh is the sixth convergent of
 // Lambert's continued fraction z / (1 + z^2 / (3 + z^2 / (5 + ...))), whose error at z = 1 is 7e-10; beyond it tanhf.
 // (Five rows over a ring of 1023 keys: 18 us, with tanhf throughout 25.)
+// (1 / cap of a cap below f32's normal range is held at f32's largest number: a logit of zero stays one.)
+__device__ __forceinline__ float inverse_cap(float cap) { return fminf(1.0f / cap, FLT_MAX); }
 template <int N>
 __device__ __forceinline__ void cap_logits(float (&x)[N], float cap, float inv_cap) {
   float top = 0.0f;

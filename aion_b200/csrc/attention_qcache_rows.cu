@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) attn_qcache_rows_kernel(const Att
           for (int i = 0; i < 8; i++) {
             const float4 k = kexp[i];
             float x[4] = {s[4 * i] * k.x * factor, s[4 * i + 1] * k.y * factor, s[4 * i + 2] * k.z * factor, s[4 * i + 3] * k.w * factor};
-            cap_logits(x, p.soft_cap, 1.0f / p.soft_cap);
+            cap_logits(x, p.soft_cap, inverse_cap(p.soft_cap));
 #pragma unroll
             for (int j = 0; j < 4; j++) s[4 * i + j] = x[j] * LOG2E;
           }

@@ -330,3 +330,24 @@ def test_pages_of_more_than_a_million_tokens(sess, backend, L):
                              window=AttentionWindow.causal(), page_table=put(np.array([[1], [0]], np.int32)), flags=capi.ATTENTION_BLOCKS)])
     within(store.read(to), *ref.attention(q, k, v, Q4, Q4, scale=0.125, positions=pos, lengths=lens))
     assert launched(backend)[0] == (ROWS if L > 1 else BOXES)
+
+
+@pytest.mark.parametrize("flags,kernel", [*[(f, k) for _, f, k in KERNELS], (capi.ATTENTION_GENERIC, ANY)], ids=["columns", "rows", "any"])
+@pytest.mark.parametrize("cap", [1e-45, 1e-40, 1e-38, 1e30])
+def test_soft_caps_near_the_ends_of_f32(sess, backend, cap, flags, kernel):
+    """A cap that f32 holds as a subnormal number: all logits are zero beside any value of V, those of a query of zeros too. One far
+    above the logits changes nothing."""
+    T, H, D, L = 40, 2, 128, 3
+    q, k, v = inputs([2], 1, T, H, D, L, 4, Q8, Q4)
+    q[:, 0] = 0.0
+    got, _ = run_attention(sess, q, k, v, Q8, Q4, scale=0.1, cap=cap, flags=flags)
+    assert launched(backend)[0] == kernel
+    kw = dict(positions=np.zeros((1, L), int), lengths=[T], right=capi.WINDOW_UNBOUNDED)
+    want, bound = ref.attention(q, k, v, Q8, Q4, scale=0.1, **kw)
+    if cap < 1:
+        want, bound = ref.attention(0 * q, k, v, Q8, Q4, scale=0.1, **kw)
+    else:
+        # the division and the tanh of a small number: 2^-21 of a logit, which counts twice
+        top = 0.1 * np.abs(np.einsum("lhd,thd->lht", q[0].astype(np.float64), np.repeat(ref.unpack(Q8, k)[0], 2, 1))).max()
+        bound = bound + 2.0 ** -20 * top * np.abs(ref.unpack(Q4, v)).max()
+    within(got, want, bound)
